@@ -409,6 +409,123 @@ int pbx_self_speculative_generate(pbx_model *m, const int32_t *prompt, int n_pro
                                   const int32_t *eos_ids, int n_eos, int batched_verify,
                                   int32_t *out_tokens, int *n_out, pbx_spec_stats *stats);
 
+/* ---- paged 8-bit KV cache ------------------------------------------------
+ * A KV cache that many sequences share, for callers that run several requests
+ * through one resident model (no reference counterpart: the reference holds
+ * one sequence in f32).  The pool has n_pages pages of page_tokens positions
+ * (of every layer); a sequence holds whole pages, handed out by the library as
+ * it grows.  Keys and values are int8 codes with one f32 scale s for each
+ * block of PBX_KV_BLOCK positions of a sequence, each KV head, keys and values
+ * apart:
+ *   s = max |x| / 127 over the block's rows, rounded to f32,
+ *   code = x / s rounded half to even, and the value it stands for is code * s.
+ * Rows appended to a block that already holds some raise s where their own
+ * maximum asks for it (it never falls); the earlier codes c are then rounded
+ * again, c * s_old / s_new.  Quotients and rotated values are taken in 64 bits,
+ * so codes do not depend on the batch that appends a row, only on which rows
+ * of a block arrive together.  A scale below 2^-120 is held as 0 (the block
+ * reads as zeros); a block that got a NaN or an infinite value reads as NaN.
+ */
+typedef struct pbx_kv pbx_kv;
+typedef struct pbx_kv_batch pbx_kv_batch;
+
+#define PBX_KV_BLOCK 32  /* positions that share a scale */
+
+/* Position rotation of queries and keys: none, of adjacent dims (2i, 2i + 1)
+ * as pbx_model rotates (llama.js:159-191), or of dims (i, i + rope_dim / 2).
+ * Pair i turns by the angle pos / rope_scale * rope_theta^(-2i / rope_dim) /
+ * rope_factors[i], evaluated in 64 bits; dims from rope_dim on are copied. */
+#define PBX_ROPE_NONE   0
+#define PBX_ROPE_PAIRS  1
+#define PBX_ROPE_HALVES 2
+
+typedef struct pbx_kv_config {
+  int32_t n_layers, n_heads, n_kv_heads; /* n_kv_heads divides n_heads          */
+  int32_t head_dim;      /* 32..256, a multiple of 4                            */
+  int32_t page_tokens;   /* 32, 64, 128, 256, 512 or 1024                       */
+  int32_t n_pages;
+  int32_t max_seqs;      /* sequence ids are 0..max_seqs - 1                    */
+  int32_t max_seq;       /* positions of one sequence, at most 2^20             */
+  int32_t rope_style;    /* PBX_ROPE_*                                          */
+  int32_t rope_dim;      /* leading dims that turn: a multiple of 4, 0: head_dim */
+  double rope_theta;     /* > 0                                                 */
+  double rope_scale;     /* > 0: positions are divided by it (1: as they are)   */
+  const float *rope_factors; /* [rope_dim / 2] or NULL (all 1); > 0; copied     */
+} pbx_kv_config;
+
+int pbx_kv_create(pbx_ctx *ctx, const pbx_kv_config *cfg, pbx_kv **out);
+/* Frees the cache and every batch of it. */
+int pbx_kv_free(pbx_kv *kv);
+int pbx_kv_info(const pbx_kv *kv, int *free_pages, size_t *device_bytes);
+/* Positions that a sequence holds; and dropping those from n_tokens on (0: the
+ * whole sequence), which gives back the pages they leave empty.  Batches that
+ * were set over dropped positions are refused from then on. */
+int pbx_kv_length(const pbx_kv *kv, int seq, int *n_tokens);
+int pbx_kv_truncate(pbx_kv *kv, int seq, int n_tokens);
+
+/* A batch: counts[i] rows of sequence seqs[i] (none twice) at the positions
+ * starts[i].., packed in this order (all rows of a sequence side by side).
+ * pbx_kv_batch_set lengthens a sequence to hold its rows, with pages from the
+ * pool (PBX_ENOMEM, and nothing changed, when it has too few); starts[i] is at
+ * most its length, and starts == NULL means each sequence's end.  counts[i] may
+ * be 0.  The set-up is made once and used by every layer's calls below; it waits
+ * for no GPU work but the previous set-up of the same batch.  The three calls
+ * enqueue on the context's stream; of one batch they use the same workspace, so
+ * work captured from one batch into graphs is replayed on one stream at a time.
+ * A batch whose calls were captured keeps its rows (set refuses, PBX_EINVAL):
+ * a replay runs over the same positions, which the sequences must still hold,
+ * and the batch lives as long as the graph.
+ */
+int pbx_kv_batch_create(pbx_kv *kv, pbx_kv_batch **out);
+int pbx_kv_batch_free(pbx_kv_batch *b);
+int pbx_kv_batch_set(pbx_kv_batch *b, int n_seqs, const int32_t *seqs,
+                     const int32_t *starts, const int32_t *counts);
+int pbx_kv_batch_rows(const pbx_kv_batch *b, int *n_rows);
+
+/* Rotates the batch's queries and keys by their positions and appends its keys
+ * and values to layer `layer`.  Rows are f32 [n_heads | n_kv_heads][head_dim],
+ * *_stride floats apart (a multiple of 4; 0: packed); addresses are 16-byte
+ * aligned.  The rotated queries go to dQout, which may be dQ itself (dQ and
+ * dQout both NULL: keys and values only).  The rows must be the last of their
+ * sequences. */
+int pbx_kv_append_dev(pbx_kv_batch *b, int layer, const float *dQ, int64_t q_stride,
+                      const float *dK, int64_t k_stride, const float *dV, int64_t v_stride,
+                      float *dQout, int64_t qout_stride);
+/* Attention of the batch's (rotated) query rows over layer `layer` of their
+ * sequences: head h of a row at position p sees KV head h / (n_heads /
+ * n_kv_heads) at positions 0..p.  scale: of the products (0: 1 /
+ * sqrt(head_dim)).  Rows as above; dOut [n_rows][n_heads][head_dim].  Values
+ * are used as they stand in the cache, everything else in 22 bits or more; the
+ * result of a row does not depend on the other rows' values. */
+int pbx_kv_attention_dev(pbx_kv_batch *b, int layer, const float *dQ, int64_t q_stride,
+                         float scale, float *dOut, int64_t out_stride);
+/* The batch's rows of the cache as the values they stand for, f32 [n_rows]
+ * [n_kv_heads][head_dim] (either may be NULL). */
+int pbx_kv_read_dev(pbx_kv_batch *b, int layer, float *dK, int64_t k_stride, float *dV,
+                    int64_t v_stride);
+
+/* ---- log probabilities -----------------------------------------------------
+ * Of `rows` rows of f32 logits [vocab], `stride` floats apart (0: vocab):
+ *   dLogp[r]     log softmax at dTargets[r] (NaN for a target outside the
+ *                vocabulary); NULL, like dTargets, to leave it out
+ *   dEntropy[r]  -sum p log p, in nats; or NULL
+ *   dTopIds, dTopLogp [rows][top]: the `top` (0..PBX_LOGPROBS_TOP_MAX, at most
+ *                vocab) most likely tokens in order, equal logits by the lower
+ *                index, and their log probabilities; either NULL to leave it out
+ * A logit of -inf is a token that cannot be chosen (log probability -inf, no
+ * entropy).  A row with a NaN or +inf logit, or with nothing but -inf, has no
+ * distribution: NaN log probabilities and entropy, top tokens -1.
+ * Only enqueues on the context's stream.  work: device memory of the size that
+ * pbx_logprobs_workspace gives (it may be 0), 16-byte aligned, any content,
+ * for this call alone until it has run.  No reference counterpart: the
+ * reference samples on the host (llama.js:394-442). */
+#define PBX_LOGPROBS_TOP_MAX 32
+int pbx_logprobs_workspace(pbx_ctx *ctx, int64_t rows, int64_t vocab, int top, size_t *bytes);
+int pbx_logprobs_dev(pbx_ctx *ctx, const float *dLogits, int64_t stride, int64_t rows,
+                     int64_t vocab, const int32_t *dTargets, int top, float *dLogp,
+                     float *dEntropy, int32_t *dTopIds, float *dTopLogp, void *work,
+                     size_t work_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,254 @@
+// pbx_logprobs.hip -- log probabilities of given tokens, entropy and the most
+// likely tokens of rows of logits.
+//
+// With m = max x, S = sum e^(x - m) and T = sum e^(x - m) (x - m) of a row:
+//   log p_t = x_t - m - log S,  entropy = log S - T / S
+// in one pass over the row: (m, S, T) join with those of other elements as
+//   S = S1 e^(m1 - m) + S2 e^(m2 - m),  T = sum (Ti + (mi - m) Si) e^(mi - m).
+
+#include "pbx_gemv_impl.h"
+
+using namespace pbx;
+
+namespace {
+
+// The maximum before any element: finite, so differences need no special case
+// (an element of -inf adds nothing; a row of nothing else keeps S == 0).
+constexpr float LOWEST = -3.402823466e38f;
+constexpr int LP_T = 512;      // threads of a part
+constexpr int LP_SHARE = 64;   // float4 groups a thread takes at most
+constexpr int LP_TOP = 32;
+
+struct Sums {
+  float m, s, t;
+};
+
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504f); }
+// e^d is 0 from -104 on; the bound keeps products with 0 finite
+__device__ __forceinline__ float bounded(float d) { return fmaxf(d, -200.f); }
+
+__device__ __forceinline__ Sums moved(Sums a, float m) {  // to the larger maximum m
+  const float d = bounded(a.m - m), f = exp_of(d);
+  return {m, a.s * f, fmaf(d, a.s, a.t) * f};
+}
+__device__ __forceinline__ Sums joined(Sums a, Sums b) {
+  const float m = fmaxf(a.m, b.m);
+  a = moved(a, m);
+  b = moved(b, m);
+  return {m, a.s + b.s, a.t + b.t};
+}
+
+// Larger logits have larger keys, equal ones the lower index.
+__device__ __forceinline__ uint64_t key_of(float x, unsigned i) {
+  const unsigned u = __float_as_uint(x + 0.f);  // -0 as 0
+  return (uint64_t)(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (0xFFFFFFFFu - i);
+}
+__device__ __forceinline__ float key_value(uint64_t k) {
+  const unsigned u = (unsigned)(k >> 32);
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+
+__device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int mask) {
+  const unsigned lo = (unsigned)__shfl_xor((int)(unsigned)v, mask, 64);
+  const unsigned hi = (unsigned)__shfl_xor((int)(unsigned)(v >> 32), mask, 64);
+  return (uint64_t)hi << 32 | lo;
+}
+// One step of a bitonic network: the lane whose partner bit is clear keeps the
+// larger value.
+__device__ __forceinline__ uint64_t exchange(uint64_t v, int mask, int lane, int bit) {
+  const uint64_t o = shfl_xor_u64(v, mask);
+  return ((lane & bit) == 0) == (o > v) ? o : v;
+}
+// A wave's 64 keys in descending order.
+__device__ __forceinline__ uint64_t sort_wave(uint64_t v, int lane) {
+#pragma unroll
+  for (int k = 2; k <= 64; k *= 2) {
+    v = exchange(v, k - 1, lane, k / 2);  // against the mirrored half
+#pragma unroll
+    for (int j = k / 4; j >= 1; j /= 2) v = exchange(v, j, lane, j);
+  }
+  return v;
+}
+// The 64 largest of two descending lists, in descending order.
+__device__ __forceinline__ uint64_t merge_wave(uint64_t a, uint64_t b, int lane) {
+  const uint64_t o = shfl_xor_u64(b, 63);
+  uint64_t v = o > a ? o : a;
+#pragma unroll
+  for (int j = 32; j >= 1; j /= 2) v = exchange(v, j, lane, j);
+  return v;
+}
+
+// The 64 largest keys of W waves' descending lists, in wave 0.
+template <int W>
+__device__ __forceinline__ uint64_t merge_waves(uint64_t v, uint64_t (*buf)[64], int wave, int lane) {
+#pragma unroll
+  for (int h = W / 2; h >= 1; h /= 2) {
+    if (wave >= h && wave < 2 * h) buf[wave][lane] = v;
+    __syncthreads();
+    if (wave < h) v = merge_wave(v, buf[wave + h][lane], lane);
+    __syncthreads();
+  }
+  return v;
+}
+
+template <int W>
+__device__ __forceinline__ Sums join_waves(Sums a, float (*buf)[3], int wave, int lane) {
+#pragma unroll
+  for (int off = 32; off >= 1; off /= 2)
+    a = joined(a, {__shfl_xor(a.m, off, 64), __shfl_xor(a.s, off, 64), __shfl_xor(a.t, off, 64)});
+  if (lane == 0) {
+    buf[wave][0] = a.m;
+    buf[wave][1] = a.s;
+    buf[wave][2] = a.t;
+  }
+  __syncthreads();
+  a = {buf[0][0], buf[0][1], buf[0][2]};
+#pragma unroll
+  for (int w = 1; w < W; ++w) a = joined(a, {buf[w][0], buf[w][1], buf[w][2]});
+  return a;
+}
+
+struct Out {
+  const int *targets;
+  float *logp, *entropy;
+  int *top_ids;
+  float *top_logp;
+};
+
+// The answers for row `row` of x from its sums and (lane i) i-th largest key.
+__device__ __forceinline__ void answer(const Out &o, int64_t row, const float *x, int vocab, int top, Sums a,
+                                       uint64_t key, int lane) {
+  const bool none = !(a.s > 0.f && a.s < INFINITY);  // no distribution
+  const float ls = logf(a.s), nan = __uint_as_float(0x7fc00000u);
+  if (lane == 0) {
+    if (o.logp) {
+      const int t = o.targets[row];
+      o.logp[row] = none || t < 0 || t >= vocab ? nan : x[t] - a.m - ls;
+    }
+    if (o.entropy) o.entropy[row] = none ? nan : ls - a.t / a.s;
+  }
+  if (lane < top) {
+    if (o.top_ids) o.top_ids[row * top + lane] = none ? -1 : (int)(0xFFFFFFFFu - (unsigned)key);
+    if (o.top_logp) o.top_logp[row * top + lane] = none ? nan : key_value(key) - a.m - ls;
+  }
+}
+
+// The group of four elements that start at i (aligned to 16 bytes; i < 0 or
+// i + 3 >= vocab at a row's ends: absent ones as -inf).
+__device__ __forceinline__ float4 group_at(const float *x, int i, int vocab) {
+  if (i >= 0 && i + 3 < vocab) return *reinterpret_cast<const float4 *>(x + i);
+  float v[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = i + e >= 0 && i + e < vocab ? x[i + e] : -INFINITY;
+  return make_float4(v[0], v[1], v[2], v[3]);
+}
+
+}  // namespace
+
+// Workgroup (part, row): the row's 16-byte groups in `parts` pieces of at most
+// LP_SHARE groups a thread.  A thread keeps its sums and its first largest
+// group; the `top` threads with the largest ones hold the piece's `top` largest
+// elements among them (those threads' maxima alone are `top` elements as large),
+// so only their groups, read again, are looked through.
+extern "C" __global__ void __launch_bounds__(LP_T)
+pbx_logprobs_part(const float *logits, int64_t stride, int vocab, int parts, int top, Out out, float *sums,
+                  uint64_t *keys) {
+  constexpr int W = LP_T / 64;
+  __shared__ float sbuf[W][3];
+  __shared__ uint64_t kbuf[W][64];
+  __shared__ int chosen[LP_TOP];
+  __shared__ int count, n_chosen;
+  __shared__ uint64_t limit;
+  __shared__ uint64_t list[LP_TOP * LP_SHARE * 4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = blockIdx.x / parts;
+  const int part = (int)(blockIdx.x % parts);
+  const float *x = logits + row * stride;
+  const int skew = (int)((uintptr_t)x / 4 & 3);  // elements of the first group before the row
+  const int groups = (int)(((int64_t)vocab + skew + 3) / 4);
+  const int g0 = (int)((int64_t)groups * part / parts), g1 = (int)((int64_t)groups * (part + 1) / parts);
+  Sums a = {LOWEST, 0.f, 0.f};
+  float best = -INFINITY;
+  int at = -1;
+  for (int g = g0 + tid; g < g1; g += LP_T) {
+    const float4 v = group_at(x, 4 * g - skew, vocab);
+    const float top4 = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+    if (top4 > best || at < 0) {
+      best = top4;
+      at = g;
+    }
+    if (top4 > a.m) a = moved(a, top4);
+    const float d[4] = {v.x - a.m, v.y - a.m, v.z - a.m, v.w - a.m};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float p = exp_of(d[e]);
+      a.s += p;
+      a.t = fmaf(p, bounded(d[e]), a.t);
+    }
+  }
+  a = join_waves<W>(a, sbuf, wave, lane);
+  uint64_t key = 0;
+  if (top) {
+    const uint64_t mine = at < 0 ? 0 : key_of(best, (unsigned)at);
+    key = merge_waves<W>(sort_wave(mine, lane), kbuf, wave, lane);
+    if (tid == top - 1) limit = key;
+    if (tid == 0) count = n_chosen = 0;
+    __syncthreads();
+    if (mine && mine >= limit) chosen[atomicAdd(&n_chosen, 1)] = tid;
+    __syncthreads();
+    // a group's key is at most those of its largest elements, which have its value
+    const float floor_value = limit ? key_value(limit) : -INFINITY;
+    const int share = (g1 - g0 + LP_T - 1) / LP_T, n = n_chosen * share;
+    for (int i = tid; i < n; i += LP_T) {
+      const int g = g0 + chosen[i / share] + i % share * LP_T;
+      if (g >= g1) continue;
+      const int i0 = 4 * g - skew;
+      const float4 v = group_at(x, i0, vocab);
+      const float u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i0 + e >= 0 && i0 + e < vocab && u[e] >= floor_value)
+          list[atomicAdd(&count, 1)] = key_of(u[e], (unsigned)(i0 + e));
+    }
+    __syncthreads();
+    key = 0;
+    for (int i = 64 * wave; i < count; i += LP_T)
+      key = merge_wave(key, sort_wave(i + lane < count ? list[i + lane] : 0, lane), lane);
+    key = merge_waves<W>(key, kbuf, wave, lane);
+  }
+  if (wave) return;
+  if (parts == 1) {
+    answer(out, row, x, vocab, top, a, key, lane);
+    return;
+  }
+  if (lane == 0) {
+    sums[3 * blockIdx.x] = a.m;
+    sums[3 * blockIdx.x + 1] = a.s;
+    sums[3 * blockIdx.x + 2] = a.t;
+  }
+  if (lane < top) keys[blockIdx.x * (int64_t)top + lane] = key;
+}
+
+// A row's parts put together: one workgroup of four waves a row.
+extern "C" __global__ void __launch_bounds__(256)
+pbx_logprobs_join(const float *logits, int64_t stride, int vocab, int parts, int top, Out out, const float *sums,
+                  const uint64_t *keys) {
+  __shared__ float sbuf[4][3];
+  __shared__ uint64_t kbuf[4][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t row = blockIdx.x;
+  Sums a = {LOWEST, 0.f, 0.f};
+  for (int i = tid; i < parts; i += 256) {
+    const float *s = sums + 3 * (row * parts + i);
+    a = joined(a, {s[0], s[1], s[2]});
+  }
+  a = join_waves<4>(a, sbuf, wave, lane);
+  uint64_t key = 0;
+  if (top) {
+    const int n = parts * top;
+    for (int i = 64 * wave; i < n; i += 256)
+      key = merge_wave(key, sort_wave(i + lane < n ? keys[row * n + i + lane] : 0, lane), lane);
+    key = merge_waves<4>(key, kbuf, wave, lane);
+  }
+  if (!wave) answer(out, row, logits + row * stride, vocab, top, a, key, lane);
+}

@@ -126,6 +126,7 @@ struct pbx_ctx {
   void *h_stage[2] = {nullptr, nullptr};
   size_t h_stage_cap[2] = {0, 0};
   void *models = nullptr;  // decode-step models owned by this context
+  void *kvs = nullptr;     // paged KV caches owned by this context
   // this device's copy of the library's static device array (pbx_scratch.hip),
   // the workspace of pbx_linear_dev_noalloc; null when the lookup failed
   void *scratch = nullptr;
@@ -199,6 +200,7 @@ int pbx_gemm_launch(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M,
 // Bytes of one GGUF row of K elements (0 for an unknown type).
 size_t pbx_type_row_bytes(int type, int64_t K);
 void pbx_model_release_all(pbx_ctx *c);
+void pbx_kv_release_all(pbx_ctx *c);
 int pbx_model_clear_range(pbx_model *m, int from, int to);
 // pbx_model_generate with every step stopping after the first max_layers
 // layers (0: all); the self-speculative draft.

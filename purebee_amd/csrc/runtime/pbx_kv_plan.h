@@ -1,0 +1,216 @@
+// pbx_kv_plan.h -- the paged KV cache's bookkeeping on the host: which pages a
+// sequence holds, and the work lists of a batch that the kernels of pbx_kv.hip
+// run over.  No HIP calls, so every page id and index that reaches a kernel
+// can be checked without a GPU.
+#ifndef PBX_KV_PLAN_H
+#define PBX_KV_PLAN_H
+
+#include <stdint.h>
+#include <stdio.h>
+
+#include <algorithm>
+#include <string>
+#include <vector>
+
+#include "pbx.h"
+
+struct kv_seq {
+  int len = 0;
+  std::vector<int32_t> pages;
+};
+
+struct kv_pages {
+  int page_tokens = 0, max_seq = 0;
+  std::vector<int32_t> free_list;  // handed out from the back
+  std::vector<kv_seq> seqs;
+
+  void init(int page_tokens_, int n_pages, int max_seqs, int max_seq_) {
+    page_tokens = page_tokens_;
+    max_seq = max_seq_;
+    free_list.resize(n_pages);
+    for (int i = 0; i < n_pages; ++i) free_list[i] = n_pages - 1 - i;
+    seqs.assign(max_seqs, kv_seq());
+  }
+  int pages_of(int tokens) const { return (int)(((int64_t)tokens + page_tokens - 1) / page_tokens); }
+
+  int truncate(int seq, int n, std::string *why) {
+    char buf[160];
+    if (seq < 0 || seq >= (int)seqs.size()) {
+      snprintf(buf, sizeof buf, "sequence %d outside [0, %d)", seq, (int)seqs.size());
+    } else if (n < 0 || n > seqs[seq].len) {
+      snprintf(buf, sizeof buf, "sequence %d holds %d positions, not %d", seq, seqs[seq].len, n);
+    } else {
+      kv_seq &s = seqs[seq];
+      s.len = n;
+      while ((int)s.pages.size() > pages_of(n)) {
+        free_list.push_back(s.pages.back());
+        s.pages.pop_back();
+      }
+      return PBX_OK;
+    }
+    *why = buf;
+    return PBX_EINVAL;
+  }
+};
+
+// One block of PBX_KV_BLOCK positions that a batch's rows touch (append, read).
+struct kv_block_item {
+  int32_t page, sub;    // the page and the block's place in it
+  int32_t pos0;         // the block's first position
+  int32_t start, count; // the sequence's rows of the batch: positions and
+  int32_t row0;         // first packed row
+  int32_t pad[2];
+};
+// Query rows 16 tile .. of a sequence ((row, head of the KV group) pairs, the
+// head fastest) over its blocks blk0..blk1 - 1.
+struct kv_attn_item {
+  int32_t start, count, row0;
+  int32_t tile;
+  int32_t blk0, blk1;
+  int32_t tab;   // the sequence's page ids, from here on in the page table
+  int32_t slot;  // partial result to write, or -1: the only item of its rows
+};
+// The partial results of one tile: slots slot .. slot + n - 1.
+struct kv_join_item {
+  int32_t count, row0, tile;
+  int32_t slot, n;
+  int32_t pad[3];
+};
+
+struct kv_batch_plan {
+  int n_rows = 0;
+  bool last = true;  // the rows are the last of their sequences
+  std::vector<int32_t> seqs, starts, counts;
+  // work lists, in the order they lie in device memory
+  std::vector<kv_block_item> blocks;
+  std::vector<kv_attn_item> attn;
+  std::vector<kv_join_item> joins;
+  std::vector<int32_t> row_pos;  // position of every packed row
+  std::vector<int32_t> table;    // page ids, sequence by sequence
+  int n_slots = 0;
+};
+
+// Checks a batch and, if it holds, takes its pages and fills the plan; refused
+// batches change nothing.
+inline int kv_plan_rows(kv_pages *kv, int n, const int32_t *seqs, const int32_t *starts,
+                        const int32_t *counts, kv_batch_plan *p, std::string *why) {
+  char buf[200];
+  std::vector<char> seen(kv->seqs.size(), 0);
+  int64_t rows = 0, need = 0;
+  for (int i = 0; i < n; ++i) {
+    const int s = seqs[i];
+    buf[0] = 0;
+    if (s < 0 || s >= (int)kv->seqs.size()) {
+      snprintf(buf, sizeof buf, "sequence %d outside [0, %d)", s, (int)kv->seqs.size());
+    } else if (seen[s]) {
+      snprintf(buf, sizeof buf, "sequence %d twice in one batch", s);
+    } else if (counts[i] < 0) {
+      snprintf(buf, sizeof buf, "sequence %d: %d rows", s, counts[i]);
+    } else {
+      const int len = kv->seqs[s].len, at = starts ? starts[i] : len;
+      if (at < 0 || at > len)
+        snprintf(buf, sizeof buf, "sequence %d holds %d positions: rows cannot start at %d", s, len, at);
+      else if ((int64_t)at + counts[i] > kv->max_seq)
+        snprintf(buf, sizeof buf, "sequence %d: positions [%d, %lld) exceed max_seq %d", s, at,
+                 (long long)at + counts[i], kv->max_seq);
+      else
+        need += std::max(0, kv->pages_of(at + counts[i]) - (int)kv->seqs[s].pages.size());
+    }
+    if (buf[0]) {
+      *why = buf;
+      return PBX_EINVAL;
+    }
+    seen[s] = 1;
+    rows += counts[i];
+  }
+  if (rows > (1 << 26)) {
+    snprintf(buf, sizeof buf, "%lld rows in one batch", (long long)rows);
+    *why = buf;
+    return PBX_ENOTSUP;
+  }
+  if (need > (int64_t)kv->free_list.size()) {
+    snprintf(buf, sizeof buf, "%lld pages wanted, %d free", (long long)need, (int)kv->free_list.size());
+    *why = buf;
+    return PBX_ENOMEM;
+  }
+  kv_batch_plan q;
+  for (int i = 0; i < n; ++i) {
+    kv_seq &s = kv->seqs[seqs[i]];
+    q.seqs.push_back(seqs[i]);
+    q.starts.push_back(starts ? starts[i] : s.len);
+    q.counts.push_back(counts[i]);
+    s.pages.reserve(kv->pages_of(q.starts[i] + counts[i]));
+  }
+  q.n_rows = (int)rows;
+  q.row_pos.reserve(rows);
+  // nothing below allocates on behalf of a sequence: the pages change hands whole
+  for (int i = 0; i < n; ++i) {
+    kv_seq &s = kv->seqs[seqs[i]];
+    const int end = q.starts[i] + counts[i];
+    while ((int)s.pages.size() < kv->pages_of(end)) {
+      s.pages.push_back(kv->free_list.back());
+      kv->free_list.pop_back();
+    }
+    s.len = std::max(s.len, end);
+  }
+  std::swap(*p, q);
+  return PBX_OK;
+}
+
+// The work lists of a planned batch: `groups` = n_heads / n_kv_heads query
+// heads a KV head, `kv_heads` KV heads (each item runs once per KV head),
+// `want` workgroups that fill the GPU.
+inline void kv_plan_work(const kv_pages &kv, int groups, int kv_heads, int want, kv_batch_plan *p) {
+  const int n = (int)p->seqs.size();
+  p->blocks.clear();
+  p->attn.clear();
+  p->joins.clear();
+  p->row_pos.clear();
+  p->table.clear();
+  p->n_slots = 0;
+  p->last = true;
+  int64_t total = 0;  // blocks that the tiles visit
+  auto tiles_of = [&](int i) { return (int)(((int64_t)p->counts[i] * groups + 15) / 16); };
+  auto blocks_of = [&](int i, int tile) {  // visible to the tile's last row
+    const int64_t last = std::min<int64_t>((int64_t)p->counts[i] * groups, 16 * ((int64_t)tile + 1)) - 1;
+    return (int)((p->starts[i] + last / groups) / PBX_KV_BLOCK + 1);
+  };
+  for (int i = 0; i < n; ++i)
+    for (int t = 0; t < tiles_of(i); ++t) total += blocks_of(i, t);
+  // an item: at least 8 blocks (two a wave), and about `want` workgroups in all
+  const int64_t chunk = std::max<int64_t>(8, (total * kv_heads + want - 1) / want);
+  int row0 = 0;
+  for (int i = 0; i < n; ++i) {
+    const kv_seq &s = kv.seqs[p->seqs[i]];
+    const int start = p->starts[i], count = p->counts[i], tab = (int)p->table.size();
+    if (!count) continue;
+    if (start + count != s.len) p->last = false;
+    const int used = kv.pages_of(start + count);
+    p->table.insert(p->table.end(), s.pages.begin(), s.pages.begin() + used);
+    const int per_page = kv.page_tokens / PBX_KV_BLOCK;
+    for (int b = start / PBX_KV_BLOCK; b * PBX_KV_BLOCK < start + count; ++b)
+      p->blocks.push_back({s.pages[b / per_page], b % per_page, b * PBX_KV_BLOCK, start, count, row0, {0, 0}});
+    for (int t = 0; t < count; ++t) p->row_pos.push_back(start + t);
+    for (int t = 0; t < tiles_of(i); ++t) {
+      const int nb = blocks_of(i, t);
+      const int parts = (int)((nb + chunk - 1) / chunk);
+      for (int k = 0; k < parts; ++k)
+        p->attn.push_back({start, count, row0, t, (int)((int64_t)nb * k / parts),
+                           (int)((int64_t)nb * (k + 1) / parts), tab, parts > 1 ? p->n_slots + k : -1});
+      if (parts > 1) {
+        p->joins.push_back({count, row0, t, p->n_slots, parts, {0, 0, 0}});
+        p->n_slots += parts;
+      }
+    }
+    row0 += count;
+  }
+}
+
+// Whether the batch has rows of sequence seq from position n on.
+inline bool kv_plan_reaches(const kv_batch_plan &p, int seq, int n) {
+  for (size_t i = 0; i < p.seqs.size(); ++i)
+    if (p.seqs[i] == seq) return p.counts[i] && p.starts[i] + p.counts[i] > n;
+  return false;
+}
+
+#endif

@@ -45,7 +45,16 @@ EXPORTS = (
     "pbx_gguf_open", "pbx_gguf_close", "pbx_gguf_info", "pbx_gguf_tensor_info",
     "pbx_gguf_find_tensor", "pbx_gguf_get_int", "pbx_gguf_get_float", "pbx_gguf_get_string",
     "pbx_gguf_get_array", "pbx_gguf_model_config", "pbx_model_load_gguf",
+    "pbx_kv_create", "pbx_kv_free", "pbx_kv_info", "pbx_kv_length", "pbx_kv_truncate",
+    "pbx_kv_batch_create", "pbx_kv_batch_free", "pbx_kv_batch_set", "pbx_kv_batch_rows",
+    "pbx_kv_append_dev", "pbx_kv_attention_dev", "pbx_kv_read_dev",
+    "pbx_logprobs_workspace", "pbx_logprobs_dev",
 )
+
+# Position rotations of a KvCache (PBX_ROPE_*).
+ROPE = {"none": 0, "pairs": 1, "halves": 2}
+KV_BLOCK = 32          # PBX_KV_BLOCK
+LOGPROBS_TOP_MAX = 32  # PBX_LOGPROBS_TOP_MAX
 
 # Tensor ids of pbx_model_set_tensor (GGUF tensor names, gguf.js:378-410).
 T_TOKEN_EMBD, T_OUTPUT, T_OUTPUT_NORM, T_ATTN_NORM, T_FFN_NORM = 0, 1, 2, 3, 4
@@ -70,6 +79,14 @@ class SpecStats(ctypes.Structure):
     _fields_ = [("rounds", ctypes.c_int32), ("drafted", ctypes.c_int32),
                 ("accepted", ctypes.c_int32), ("prefill_ms", ctypes.c_double),
                 ("decode_ms", ctypes.c_double)]
+
+
+class KvConfig(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "n_layers", "n_heads", "n_kv_heads", "head_dim", "page_tokens", "n_pages", "max_seqs",
+        "max_seq", "rope_style", "rope_dim")] + \
+        [("rope_theta", ctypes.c_double), ("rope_scale", ctypes.c_double),
+         ("rope_factors", ctypes.c_void_p)]
 
 
 class PbxError(RuntimeError):
@@ -185,6 +202,25 @@ def load_library():
                                                 ctypes.POINTER(ctypes.c_double),
                                                 ctypes.POINTER(ctypes.c_double),
                                                 ctypes.POINTER(ctypes.c_int)]),
+        "pbx_kv_create": (ctypes.c_int, [_vp, ctypes.POINTER(KvConfig), ctypes.POINTER(_vp)]),
+        "pbx_kv_free": (ctypes.c_int, [_vp]),
+        "pbx_kv_info": (ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_int),
+                                       ctypes.POINTER(ctypes.c_size_t)]),
+        "pbx_kv_length": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.POINTER(ctypes.c_int)]),
+        "pbx_kv_truncate": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int]),
+        "pbx_kv_batch_create": (ctypes.c_int, [_vp, ctypes.POINTER(_vp)]),
+        "pbx_kv_batch_free": (ctypes.c_int, [_vp]),
+        "pbx_kv_batch_set": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _vp]),
+        "pbx_kv_batch_rows": (ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_int)]),
+        "pbx_kv_append_dev": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _i64, _vp, _i64, _vp, _i64,
+                                             _vp, _i64]),
+        "pbx_kv_attention_dev": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _i64, ctypes.c_float, _vp,
+                                                _i64]),
+        "pbx_kv_read_dev": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _i64, _vp, _i64]),
+        "pbx_logprobs_workspace": (ctypes.c_int, [_vp, _i64, _i64, ctypes.c_int,
+                                                  ctypes.POINTER(ctypes.c_size_t)]),
+        "pbx_logprobs_dev": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i64, _vp, ctypes.c_int, _vp, _vp,
+                                            _vp, _vp, _vp, ctypes.c_size_t]),
         "pbx_speculative_generate": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, ctypes.c_int,
                                                     ctypes.c_int, _vp, ctypes.c_int, ctypes.c_int,
                                                     _vp, ctypes.POINTER(ctypes.c_int),
@@ -390,6 +426,19 @@ class Context:
         self._call("pbx_dequant", self._p, w.ptr, out.ctypes.data)
         return out
 
+    def logprobs_workspace(self, rows, vocab, top):
+        """Bytes of device workspace that logprobs_dev needs for these sizes."""
+        b = ctypes.c_size_t()
+        self._call("pbx_logprobs_workspace", self._p, rows, vocab, top, ctypes.byref(b))
+        return b.value
+
+    def logprobs_dev(self, dLogits, rows, vocab, dTargets, top, dLogp, dEntropy, dTopIds, dTopLogp,
+                     dWork=None, work_bytes=0, stride=0):
+        """pbx_logprobs_dev: log probabilities of dTargets, entropy and the `top`
+        most likely tokens of rows of f32 logits on the device."""
+        self._call("pbx_logprobs_dev", self._p, dLogits, stride, rows, vocab, dTargets, top, dLogp,
+                   dEntropy, dTopIds, dTopLogp, dWork, work_bytes)
+
     def alloc(self, nbytes):
         return DeviceBuffer(self, nbytes)
 
@@ -418,6 +467,118 @@ class Context:
         self._call("pbx_bench_linear_graph" if graph else "pbx_bench_linear", self._p, n, W, X, Y,
                    M, reps, ctypes.byref(ms))
         return ms.value
+
+
+def _i32(a):
+    return np.ascontiguousarray(list(a), np.int32)
+
+
+class KvCache:
+    """A paged 8-bit KV cache that many sequences share (pbx_kv_*): n_pages pages
+    of page_tokens positions, sequence ids 0..max_seqs - 1."""
+
+    def __init__(self, ctx, n_layers, n_heads, n_kv_heads, head_dim, n_pages, max_seqs, max_seq,
+                 page_tokens=64, rope="pairs", rope_dim=0, rope_theta=10000.0, rope_scale=1.0,
+                 rope_factors=None):
+        self.ctx = ctx
+        self._kv = None
+        f = None if rope_factors is None else np.ascontiguousarray(rope_factors, np.float32)
+        style = ROPE[rope]
+        if f is not None and style and f.size != (rope_dim or head_dim) // 2:
+            raise ValueError(f"{f.size} rope_factors for {(rope_dim or head_dim) // 2} pairs")
+        self.cfg = KvConfig(n_layers, n_heads, n_kv_heads, head_dim, page_tokens, n_pages, max_seqs,
+                            max_seq, style, rope_dim, rope_theta, rope_scale,
+                            None if f is None else f.ctypes.data)
+        p = _vp()
+        ctx._call("pbx_kv_create", ctx._p, ctypes.byref(self.cfg), ctypes.byref(p))
+        self.cfg.rope_factors = None
+        self._kv = p.value
+
+    @property
+    def _ptr(self):
+        # None, which the library refuses, once the cache or its context is gone
+        return self._kv if self.ctx._p else None
+
+    def batch(self, seqs, counts, starts=None):
+        """A KvBatch set to counts[i] rows of sequence seqs[i], at starts[i].. or
+        (None) at the sequences' ends."""
+        b = KvBatch(self)
+        try:
+            return b.set(seqs, counts, starts)
+        except PbxError:
+            b.free()
+            raise
+
+    def info(self):
+        n, b = ctypes.c_int(), ctypes.c_size_t()
+        self.ctx._call("pbx_kv_info", self._ptr, ctypes.byref(n), ctypes.byref(b))
+        return {"free_pages": n.value, "device_bytes": b.value}
+
+    def length(self, seq):
+        n = ctypes.c_int()
+        self.ctx._call("pbx_kv_length", self._ptr, seq, ctypes.byref(n))
+        return n.value
+
+    def truncate(self, seq, n_tokens=0):
+        """Drop the positions from n_tokens on, and the pages they leave empty."""
+        self.ctx._call("pbx_kv_truncate", self._ptr, seq, n_tokens)
+
+    def free(self):
+        """Frees the cache and its batches."""
+        if self._ptr:
+            self.ctx._call("pbx_kv_free", self._ptr)
+        self._kv = None
+
+
+class KvBatch:
+    """Rows of a KvCache's sequences, packed (pbx_kv_batch_*); the *_dev calls
+    take device addresses and enqueue on the context's stream.  Strides are in
+    floats (0: packed rows)."""
+
+    def __init__(self, cache):
+        self.cache, self.ctx = cache, cache.ctx
+        self._b = None
+        p = _vp()
+        self.ctx._call("pbx_kv_batch_create", cache._ptr, ctypes.byref(p))
+        self._b = p.value
+
+    @property
+    def _ptr(self):
+        # a freed cache has freed its batches
+        return self._b if self.cache._ptr else None
+
+    def set(self, seqs, counts, starts=None):
+        s, c = _i32(seqs), _i32(counts)
+        a = None if starts is None else _i32(starts)
+        if len(c) != len(s) or (a is not None and len(a) != len(s)):
+            raise ValueError("seqs, counts and starts of different length")
+        self.ctx._call("pbx_kv_batch_set", self._ptr, len(s), s.ctypes.data,
+                       None if a is None else a.ctypes.data, c.ctypes.data)
+        return self
+
+    @property
+    def rows(self):
+        n = ctypes.c_int()
+        self.ctx._call("pbx_kv_batch_rows", self._ptr, ctypes.byref(n))
+        return n.value
+
+    def append_dev(self, layer, dQ, dK, dV, dQout, q_stride=0, k_stride=0, v_stride=0, qout_stride=0):
+        """Rotate queries (into dQout) and keys, append keys and values."""
+        self.ctx._call("pbx_kv_append_dev", self._ptr, layer, dQ, q_stride, dK, k_stride, dV, v_stride,
+                       dQout, qout_stride)
+
+    def attention_dev(self, layer, dQ, dOut, scale=0.0, q_stride=0, out_stride=0):
+        """Causal attention of the batch's rotated query rows over the cache."""
+        self.ctx._call("pbx_kv_attention_dev", self._ptr, layer, dQ, q_stride, scale, dOut, out_stride)
+
+    def read_dev(self, layer, dK, dV, k_stride=0, v_stride=0):
+        """The batch's rows of the cache as the f32 values they stand for."""
+        self.ctx._call("pbx_kv_read_dev", self._ptr, layer, dK, k_stride, dV, v_stride)
+
+    def free(self):
+        if self._ptr:
+            self.ctx._call("pbx_kv_batch_free", self._ptr)
+        self._b = None
 
 
 class GGUF:
