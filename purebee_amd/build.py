@@ -23,9 +23,10 @@ ARCH = "gfx950"
 # Packed-FP32 VALU forms are kept out of every code object.
 HIP_FLAGS = ["-O3", "-std=c++17", f"--offload-arch={ARCH}",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-# Per-file additions: the GEMM keeps MFMA accumulators in VGPRs, so the
-# per-block scale FMAs read them without v_accvgpr moves.
-KERNEL_FLAGS = {"pbx_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+# Per-file additions: the GEMM and the cache's attention keep MFMA accumulators
+# in VGPRs, so the per-block scale FMAs read them without v_accvgpr moves.
+KERNEL_FLAGS = {"pbx_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+                "pbx_kv.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 HOST_FLAGS = ["-O2", "-g", "-fPIC", "-std=c++17", "-Wall", "-Wextra", "-Wno-unused-parameter",
               "-D__HIP_PLATFORM_AMD__"]
 

@@ -30,15 +30,12 @@ struct KvRope {
   const double *table;  // [position][dim / 2][cos, sin]
   int style, dim;       // PBX_ROPE_*
 };
-// kv_block_item, kv_attn_item and kv_join_item of pbx_kv_plan.h
+// kv_block_item and kv_attn_item of pbx_kv_plan.h
 struct BlockItem {
   int page, sub, pos0, start, count, row0, pad[2];
 };
 struct AttnItem {
-  int start, count, row0, tile, blk0, blk1, tab, slot;
-};
-struct JoinItem {
-  int count, row0, tile, slot, n, pad[3];
+  int start, count, row0, tile, blk0, blk1, tab, part, parts, slot, join, pad, pages[4];
 };
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -286,210 +283,389 @@ constexpr float NONE = -1e38f;
 // 22 bits of them down to 2^-15 of the row's largest, and some down to 2^-36.
 constexpr float LIFT = 12.f;
 
-// One row's state while it travels between waves or workgroups: maximum (in
-// powers of two), sum and weighted values.
-//
-// Attention: workgroup (item, KV head), four waves that take the item's blocks
-// in turn.  A wave holds 16 query rows (token, head of the group) as the columns
-// of its products: scores S = K Q^T of 32 keys (two 16-key tiles), a softmax
-// step whose maxima and sums stay within a column (lanes c, c + 16, c + 32,
-// c + 48), and O^T += V^T P^T with P taken from the score registers as they lie.
-// Codes are exact in fp16; queries (divided by a power of two near the row's
-// largest) and probabilities enter as fp16 pairs, two products each, summed in
-// f32.  The block's key scale joins the row's factor, its value scale weighs the
-// block's products as they are added up.
+// A block's codes as a wave loads them, and its scales.
 template <int HDP>
+struct Keys {
+  uintx4 pair[2][HDP / 64 ? HDP / 64 : 1];  // [16-key tile][64 dims]
+  uintx2 rest[2];                           // the last 32 dims of an odd HDP / 32
+};
+template <int HDP>
+struct Values {
+  uintx4 w[HDP / 32];
+};
+
+template <int HDP>
+__device__ __forceinline__ void load_keys(Keys<HDP> &k, const uint8_t *kb, int c, int g) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+#pragma unroll
+    for (int p = 0; p < HDP / 64; ++p)
+      k.pair[t][p] = *reinterpret_cast<const uintx4 *>(kb + p * (BLK * 64) + (16 * t + c) * 64 + 16 * g);
+    if constexpr (HDP / 32 % 2)
+      k.rest[t] = *reinterpret_cast<const uintx2 *>(kb + HDP / 64 * (BLK * 64) + (16 * t + c) * 32 + 8 * g);
+  }
+}
+template <int HDP>
+__device__ __forceinline__ void load_values(Values<HDP> &v, const uint8_t *vb, int c, int g) {
+#pragma unroll
+  for (int i = 0; i < HDP / 32; ++i) v.w[i] = *reinterpret_cast<const uintx4 *>(vb + i * 1024 + c * 64 + 16 * g);
+}
+
+// A constant that the compiler cannot see through.
+__device__ __forceinline__ float opaque(float x) {
+  asm("" : "+s"(x));
+  return x;
+}
+
+// hi = fp16(x), lo = fp16(x - hi) of 8 values: a packed conversion for two, and a
+// mixed-precision fma each, which a visible -1 would be taken out of (three
+// instructions then).
+__device__ __forceinline__ void split8(const float x[8], float minus_one, half8 &hi, half8 &lo) {
+  typedef float float2t __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float2t v = {x[e], x[e + 1]};
+    const half2t h = __builtin_convertvector(v, half2t);
+    hi[e] = h[0];
+    hi[e + 1] = h[1];
+    lo[e] = (_Float16)fmaf((float)h[0], minus_one, x[e]);
+    lo[e + 1] = (_Float16)fmaf((float)h[1], minus_one, x[e + 1]);
+  }
+}
+
+// Partial results cross workgroups (and XCDs, whose L2 caches do not see each
+// other's lines) inside a launch: stores and loads at the device's coherence
+// point, 8 bytes each.
+__device__ __forceinline__ void put2(float *p, float x, float y) {
+  const uint64_t v = (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x);
+  __hip_atomic_store(reinterpret_cast<uint64_t *>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get2(const float *p) {
+  const uint64_t v =
+      __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__uint_as_float((unsigned)v), __uint_as_float((unsigned)(v >> 32)));
+}
+
+// Attention: workgroup (item, KV head), four waves that take the item's blocks
+// in turn.  A wave holds NQ tiles of 16 query rows (token, head of the group),
+// each as the columns of its products: scores S = K Q^T of 32 keys (two 16-key
+// tiles), a softmax step whose maxima and sums stay within a column (lanes c,
+// c + 16, c + 32, c + 48), and O^T += V^T P^T with P taken from the score
+// registers as they lie.  Codes are exact in fp16; queries (divided by a power
+// of two near the row's largest) and probabilities enter as fp16 pairs, two
+// products each, summed in f32.  The block's key scale joins the row's factor,
+// its value scale weighs the block's products as they are added up.
+// A block's keys are fetched while the one before goes through its softmax, its
+// values while the next scores are computed; no LDS until the waves' states are
+// put together.  Where a tile's blocks are split over several workgroups, the
+// one that finishes last puts their states together, in the order of the keys.
+template <int HDP, int NQ, int KW>
 __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items, const int *table, const float *Q,
-                                          int64_t qs, float scale, float *O, int64_t os, float *part) {
+                                          int64_t qs, float scale, float *O, int64_t os, float *part,
+                                          unsigned *arrived) {
   constexpr int HC = HDP / 32, PAIRS = HDP / 64, DT = HDP / 16;
-  __shared__ __attribute__((aligned(16))) float mrg[2][DT * 64 * 4];
-  __shared__ float mrg_ml[4][2][16];
-  const AttnItem it = items[blockIdx.x / a.kv_heads];
+  constexpr int U = NQ * 4 / KW;        // 16-row tiles of the workgroup
+  constexpr int UNIT = 16 * (HDP + 2);  // floats of 16 rows' partial state
+  constexpr int MERGED = KW > 1 ? 4 : 1;
+  __shared__ __attribute__((aligned(16))) float mrg[MERGED][NQ * DT][256];
+  __shared__ float mrg_m[4][NQ][16], mrg_l[4][NQ][16];
+  __shared__ unsigned order;
+  const AttnItem &it = items[blockIdx.x / a.kv_heads];
   const int head = (int)(blockIdx.x % a.kv_heads);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-  const int r = it.tile * 16 + c, tok = r / a.groups;
-  const bool live = tok < it.count;
-  const int pos = live ? it.start + tok : -1;
-  const int64_t row = (int64_t)it.row0 + tok;
-  const int qhead = head * a.groups + r % a.groups;
-  half8 qh[HC], ql[HC];
-  float factor;  // of the products: the row's power of two, scale, log2(e)
-  {
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int blk0 = it.blk0, blk1 = it.blk1, start = it.start, count = it.count, tile = it.tile;
+  const int sub_mask = (1 << a.page_shift) - 1;
+  auto codes_at = [&](int page, int b) {
+    return a.codes + block_index(a, page, head, b & sub_mask) * (2 * BLK * HDP);
+  };
+  auto scales_at = [&](int page, int b) {
+    return *reinterpret_cast<const float2 *>(a.scales + 2 * block_index(a, page, head, b & sub_mask));
+  };
+  // wave (qw, kw): query tiles qw NQ .., blocks b0, b0 + KW, ..: page ids one a lane, 64 at a time; the
+  // first one's comes with the item
+  const int qw = wave / KW, kw = wave % KW;
+  const int rows = min(16 * U, count * a.groups - tile * 16 * U);  // that are there
+  // (with all keys in one wave, those that its rows see)
+  const int seen = KW > 1 ? blk1
+                          : min(blk1, (start + (tile * 16 * U + min(rows, 16 * NQ * (qw + 1)) - 1) / a.groups) / BLK + 1);
+  const int first_pos = start + (tile * 16 * U + 16 * NQ * qw) / a.groups;  // of the wave's rows
+  const int b0 = blk0 + kw;
+  const int n = 16 * NQ * qw < rows ? (seen - b0 + KW - 1) / KW : 0;  // <= 0: none
+  auto pages_from = [&](int i) {
+    return table[it.tab + (min(b0 + KW * (i + lane), blk1 - 1) >> a.page_shift)];
+  };
+  // the larger of two raw products is their median with infinity: fmaxf puts a
+  // canonicalising move before each (of numbers; a NaN travels with the sums)
+  const float inf = opaque(INFINITY), minus_one = opaque(-1.f);
+  Keys<HDP> kr;
+  Values<HDP> vr;
+  float2 sc = make_float2(0.f, 0.f);
+  int pages = 0;
+  if (n > 0) {
+    const int j = (b0 >> a.page_shift) - (blk0 >> a.page_shift);
+    const int page = j == 0 ? it.pages[0] : j == 1 ? it.pages[1] : j == 2 ? it.pages[2] : it.pages[3];
+    const uint8_t *p = codes_at(page, b0);
+    load_keys<HDP>(kr, p, c, g);
+    load_values<HDP>(vr, p + BLK * HDP, c, g);
+    sc = scales_at(page, b0);
+    pages = pages_from(0);
+  }
+  half8 qh[NQ][HC], ql[NQ][HC];
+  float factor[NQ];  // of the products: the row's power of two, scale, log2(e)
+  int pos[NQ];
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) {
+    const int r = (tile * U + qw * NQ + q) * 16 + c, tok = r / a.groups;
+    const bool live = tok < count;
+    pos[q] = live ? start + tok : -1;
+    // (rows past the end load the last one's: no load waits behind a branch)
+    const float *src = Q + ((int64_t)it.row0 + min(tok, count - 1)) * qs +
+                       (int64_t)(head * a.groups + r % a.groups) * a.head_dim;
     float x[HC][8];
-    const float *q = Q + row * qs + (int64_t)qhead * a.head_dim;
     unsigned peak = 0;
 #pragma unroll
     for (int i = 0; i < HC; ++i)
 #pragma unroll
       for (int e = 0; e < 8; e += 4) {
         const int d = i < 2 * PAIRS ? 64 * (i >> 1) + 16 * g + 8 * (i & 1) + e : 32 * i + 8 * g + e;
-        const float4 v = live && d < a.head_dim ? *reinterpret_cast<const float4 *>(q + d)
-                                                : make_float4(0.f, 0.f, 0.f, 0.f);
-        x[i][e] = v.x; x[i][e + 1] = v.y; x[i][e + 2] = v.z; x[i][e + 3] = v.w;
+        const bool in = live && d < a.head_dim;
+        const float4 v = *reinterpret_cast<const float4 *>(src + min(d, a.head_dim - 4));
+        x[i][e] = in ? v.x : 0.f; x[i][e + 1] = in ? v.y : 0.f;
+        x[i][e + 2] = in ? v.z : 0.f; x[i][e + 3] = in ? v.w : 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) peak = max(peak, __float_as_uint(x[i][e + k]) & 0x7fffffffu);
       }
     peak = max(peak, (unsigned)__shfl_xor((int)peak, 16, 64));
     peak = max(peak, (unsigned)__shfl_xor((int)peak, 32, 64));
     const unsigned ex = min(max(peak >> 23, 1u), 253u);
-    const float down = __uint_as_float((254u - ex) << 23);  // 2^(127 - ex)
-    factor = __uint_as_float(ex << 23) * scale * 1.44269504f;
+    // 2^(127 - ex), with scale's sign so that the factor keeps the scores' order
+    const float down = copysignf(__uint_as_float((254u - ex) << 23), scale);
+    factor[q] = __uint_as_float(ex << 23) * (fabsf(scale) * 1.44269504f);
 #pragma unroll
-    for (int i = 0; i < HC; ++i)
+    for (int i = 0; i < HC; ++i) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y = x[i][e] * down;
-        const _Float16 h = (_Float16)y;
-        qh[i][e] = h;
-        ql[i][e] = (_Float16)(y - (float)h);
-      }
+      for (int e = 0; e < 8; ++e) x[i][e] *= down;
+      split8(x[i], minus_one, qh[q][i], ql[q][i]);
+    }
   }
   const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
-  floatx4 acc[DT];
+  floatx4 acc[NQ][DT];
+  float m[NQ], l[NQ];
 #pragma unroll
-  for (int i = 0; i < DT; ++i) acc[i] = zero;
-  float m = NONE, l = 0.f;
-  for (int b = it.blk0 + wave; b < it.blk1; b += 4) {
-    const int page = table[it.tab + (b >> a.page_shift)];
-    const int64_t bi = block_index(a, page, head, b & ((1 << a.page_shift) - 1));
-    const uint8_t *kb = a.codes + bi * (2 * BLK * HDP), *vb = kb + BLK * HDP;
-    const float2 sc = *reinterpret_cast<const float2 *>(a.scales + 2 * bi);
-    floatx4 s[2] = {zero, zero};
+  for (int q = 0; q < NQ; ++q) {
+    m[q] = NONE;
+    l[q] = 0.f;
+#pragma unroll
+    for (int i = 0; i < DT; ++i) acc[q][i] = zero;
+  }
+  for (int i = 0; i < n; ++i) {
+    const int b = b0 + KW * i;
+    const bool more = i + 1 < n;
+    if (((i + 1) & 63) == 0 && more) pages = pages_from(i + 1);
+    const int page = __builtin_amdgcn_readlane(pages, (i + 1) & 63);
+    const uint8_t *next = codes_at(more ? page : 0, more ? b + KW : 0);
+    floatx4 s[NQ][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
-      for (int p = 0; p < PAIRS; ++p) {
-        const uintx4 w = *reinterpret_cast<const uintx4 *>(kb + p * (BLK * 64) + (16 * t + c) * 64 + 16 * g);
-        const half8 k0 = halves(w[0], w[1]), k1 = halves(w[2], w[3]);
-        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[2 * p], s[t], 0, 0, 0);
-        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[2 * p], s[t], 0, 0, 0);
-        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[2 * p + 1], s[t], 0, 0, 0);
-        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql[2 * p + 1], s[t], 0, 0, 0);
-      }
-      if constexpr (HC % 2) {
-        const uintx2 w = *reinterpret_cast<const uintx2 *>(kb + PAIRS * (BLK * 64) + (16 * t + c) * 32 + 8 * g);
-        const half8 k0 = halves(w[0], w[1]);
-        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[HC - 1], s[t], 0, 0, 0);
-        s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[HC - 1], s[t], 0, 0, 0);
+      for (int q = 0; q < NQ; ++q) s[q][t] = zero;
+#pragma unroll
+      for (int p = 0; p < HC; ++p) {
+        half8 k;
+        if (p < 2 * PAIRS)
+          k = halves(kr.pair[t][p / 2][2 * (p & 1)], kr.pair[t][p / 2][2 * (p & 1) + 1]);
+        else
+          k = halves(kr.rest[t][0], kr.rest[t][1]);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) s[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[q][p], s[q][t], 0, 0, 0);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) s[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[q][p], s[q][t], 0, 0, 0);
       }
     }
-    const float f = factor * sc.x;
-    float x[8], mx = NONE;
-    const int p0 = b * BLK + 4 * g;
-    const bool whole = b * BLK + BLK - 1 <= it.start;  // every live row sees the block
+    if (more) load_keys<HDP>(kr, next, c, g);
+    half8 ph[NQ], pl[NQ];
+    float al[NQ], sv[NQ];
+    bool moved = false;
+    const bool whole = b * BLK + BLK - 1 <= first_pos;  // every live row sees the block
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int p = p0 + 16 * (e >> 2) + (e & 3);
-      x[e] = s[e >> 2][e & 3] * f;
-      if (!whole && p > pos) x[e] = NONE;
-      mx = fmaxf(mx, x[e]);
-    }
-    mx = pair_max<32>(pair_max<16>(mx));
-    const float mn = fmaxf(m, mx);
-    const float al = __builtin_amdgcn_exp2f(m - mn);
-    const float base = mn == NONE ? 0.f : mn - LIFT;
-    float sum = 0.f;
-    half8 ph, pl;
+    for (int q = 0; q < NQ; ++q) {
+      // never 0, so that masked scores stay -inf (a block of zeros has scale 0)
+      float f = factor[q] * sc.x;
+      f = f < 1e-30f ? 1e-30f : f;
+      sv[q] = sc.y;
+      if (!whole) {
+        // a row that sees nothing of the block takes nothing of its scales either
+        const bool none = b * BLK > pos[q];
+        f = none ? 1e-30f : f;
+        sv[q] = none ? 0.f : sv[q];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float p = __builtin_amdgcn_exp2f(x[e] - base);
-      sum += p;
-      const _Float16 h = (_Float16)p;
-      ph[e] = h;
-      pl[e] = (_Float16)(p - (float)h);
-    }
-    l = fmaf(l, al, sum);  // of this lane's keys: the column's sum is taken at the end
-    m = mn;
-#pragma unroll
-    for (int i = 0; i < HC; ++i) {
-      const uintx4 w = *reinterpret_cast<const uintx4 *>(vb + i * 1024 + c * 64 + 16 * g);
-      const half8 v0 = halves(w[0], w[1]), v1 = halves(w[2], w[3]);
-      floatx4 d0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph, zero, 0, 0, 0);
-      floatx4 d1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph, zero, 0, 0, 0);
-      d0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl, d0, 0, 0, 0);
-      d1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl, d1, 0, 0, 0);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        acc[2 * i][e] = fmaf(d0[e], sc.y, acc[2 * i][e] * al);
-        acc[2 * i + 1][e] = fmaf(d1[e], sc.y, acc[2 * i + 1][e] * al);
+        for (int e = 0; e < 8; ++e)
+          if (b * BLK + 4 * g + 16 * (e >> 2) + (e & 3) > pos[q]) s[q][e >> 2][e & 3] = -INFINITY;
       }
+      float mx = s[q][0][0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) mx = __builtin_amdgcn_fmed3f(mx, s[q][e >> 2][e & 3], inf);
+      mx = pair_max<32>(pair_max<16>(mx));
+      const float mn = fmaxf(m[q], mx * f);
+      al[q] = __builtin_amdgcn_exp2f(m[q] - mn);
+      moved = moved || mn != m[q];
+      const float base = mn - LIFT;
+      float p[8], sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(fmaf(s[q][e >> 2][e & 3], f, -base));
+        sum += p[e];
+      }
+      split8(p, minus_one, ph[q], pl[q]);
+      l[q] = fmaf(l[q], al[q], sum);  // of this lane's keys: the column's sum is taken at the end
+      m[q] = mn;
+    }
+    if (__any(moved)) {
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[q][d] *= al[q];
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const half8 v = halves(vr.w[d / 2][2 * (d & 1)], vr.w[d / 2][2 * (d & 1) + 1]);
+      floatx4 o[NQ];
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) o[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[q], zero, 0, 0, 0);
+#pragma unroll
+      for (int q = 0; q < NQ; ++q) o[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[q], o[q], 0, 0, 0);
+#pragma unroll
+      for (int q = 0; q < NQ; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[q][d][e] = fmaf(o[q][e], sv[q], acc[q][d][e]);
+    }
+    if (more) {
+      load_values<HDP>(vr, next + BLK * HDP, c, g);
+      sc = scales_at(page, b + KW);
     }
   }
-  l = pair_sum<32>(pair_sum<16>(l));
-  // the waves' states: one maximum, then the sums, waves 2 and 3 into 0 and 1,
-  // 1 into 0
-  if (g == 0) mrg_ml[wave][0][c] = m;
+#pragma unroll
+  for (int q = 0; q < NQ; ++q) l[q] = pair_sum<32>(pair_sum<16>(l[q]));
+  if constexpr (KW > 1) {
+    // the states of the waves with the same rows put together: one maximum, then
+    // the sums, each wave a share of the 16 x 16 output tiles
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+      if (g == 0) mrg_m[wave][q][c] = m[q];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      float M = mrg_m[qw * KW][q][c];
+#pragma unroll
+      for (int w = 1; w < KW; ++w) M = fmaxf(M, mrg_m[qw * KW + w][q][c]);
+      const float f = __builtin_amdgcn_exp2f(m[q] - M);
+      if (g == 0) mrg_l[wave][q][c] = l[q] * f;
+      m[q] = M;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+        *reinterpret_cast<floatx4 *>(&mrg[wave][q * DT + d][4 * lane]) = acc[q][d] * f;
+    }
+    __syncthreads();
+  }
+  float *mine = part + ((int64_t)(it.slot + it.part * U) * a.kv_heads + head * U) * UNIT;
+#pragma unroll
+  for (int u = 0; u < NQ * DT; ++u) {
+    if (u % KW != kw) continue;
+    const int q = u / DT, d = 16 * (u % DT) + 4 * g, r = 16 * (qw * NQ + q) + c;
+    floatx4 o;
+    float sum;
+    if constexpr (KW > 1) {
+      o = zero;
+      sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        o += *reinterpret_cast<const floatx4 *>(&mrg[qw * KW + w][u][4 * lane]);
+        sum += mrg_l[qw * KW + w][q][c];
+      }
+    } else {
+      o = acc[q][u % DT];
+      sum = l[q];
+    }
+    if (r >= rows) continue;
+    if (it.parts > 1) {
+      float *p = mine + (qw * NQ + q) * UNIT;
+      put2(p + c * HDP + d, o[0], o[1]);
+      put2(p + c * HDP + d + 2, o[2], o[3]);
+      if (u % DT == 0 && g == 0) put2(p + 16 * HDP + 2 * c, m[q], sum);
+    } else if (d < a.head_dim) {
+      const float inv = 1.f / sum;
+      const int t = tile * 16 * U + r;
+      *reinterpret_cast<float4 *>(O + ((int64_t)it.row0 + t / a.groups) * os +
+                                  (int64_t)(head * a.groups + t % a.groups) * a.head_dim + d) =
+          make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    }
+  }
+  if (it.parts == 1) return;
+  // this part's state is at the coherence point before its workgroup counts
+  // itself in; the workgroup that completes the count reads the others' from there
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  float M = mrg_ml[0][0][c];
-#pragma unroll
-  for (int w = 1; w < 4; ++w) M = fmaxf(M, mrg_ml[w][0][c]);
-  const float al = __builtin_amdgcn_exp2f(m - M);
-  l *= al;
-  if (g == 0) mrg_ml[wave][1][c] = l;
-#pragma unroll
-  for (int i = 0; i < DT; ++i) acc[i] *= al;
-#pragma unroll
-  for (int half = 2; half >= 1; half /= 2) {
-    if (wave >= half && wave < 2 * half)
-#pragma unroll
-      for (int i = 0; i < DT; ++i)
-        *reinterpret_cast<floatx4 *>(&mrg[wave - half][(i * 64 + lane) * 4]) = acc[i];
-    __syncthreads();
-    if (wave < half)
-#pragma unroll
-      for (int i = 0; i < DT; ++i) acc[i] += *reinterpret_cast<const floatx4 *>(&mrg[wave][(i * 64 + lane) * 4]);
-    __syncthreads();
-  }
-  if (wave) return;
-  l = mrg_ml[0][1][c] + mrg_ml[1][1][c] + mrg_ml[2][1][c] + mrg_ml[3][1][c];
-  if (it.slot < 0) {
-    if (!live) return;
-    const float inv = 1.f / l;
-    float *o = O + row * os + (int64_t)qhead * a.head_dim;
-#pragma unroll
-    for (int i = 0; i < DT; ++i)
-      if (16 * i + 4 * g < a.head_dim)
-        *reinterpret_cast<float4 *>(o + 16 * i + 4 * g) =
-            make_float4(acc[i][0] * inv, acc[i][1] * inv, acc[i][2] * inv, acc[i][3] * inv);
-    return;
-  }
-  float *p = part + ((int64_t)it.slot * a.kv_heads + head) * (16 * (HDP + 2));
-#pragma unroll
-  for (int i = 0; i < DT; ++i)
-    *reinterpret_cast<floatx4 *>(p + c * HDP + 16 * i + 4 * g) = acc[i];
-  if (g == 0) {
-    p[16 * HDP + c] = M;
-    p[16 * HDP + 16 + c] = l;
-  }
-}
-
-// Split rows: workgroup (tile, KV head) adds up the tile's partial states in
-// the order of their keys.
-template <int HDP>
-__device__ __forceinline__ void join_body(const KvArgs &a, const JoinItem *items, const float *part, float *O,
-                                          int64_t os) {
-  const JoinItem it = items[blockIdx.x / a.kv_heads];
-  const int head = (int)(blockIdx.x % a.kv_heads);
-  const int64_t step = (int64_t)a.kv_heads * (16 * (HDP + 2));
-  const float *p = part + ((int64_t)it.slot * a.kv_heads + head) * (16 * (HDP + 2));
-  for (int i = threadIdx.x; i < 16 * HDP / 4; i += 256) {
-    const int c = i / (HDP / 4), d = 4 * (i % (HDP / 4));
-    const int r = it.tile * 16 + c, tok = r / a.groups;
-    if (tok >= it.count || d >= a.head_dim) continue;
-    float M = NONE, l = 0.f;
-    for (int k = 0; k < it.n; ++k) M = fmaxf(M, p[k * step + 16 * HDP + c]);
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < it.n; ++k) {
-      const float f = __builtin_amdgcn_exp2f(p[k * step + 16 * HDP + c] - M);
-      const float4 v = *reinterpret_cast<const float4 *>(p + k * step + c * HDP + d);
-      l = fmaf(p[k * step + 16 * HDP + 16 + c], f, l);
-      o.x = fmaf(v.x, f, o.x); o.y = fmaf(v.y, f, o.y);
-      o.z = fmaf(v.z, f, o.z); o.w = fmaf(v.w, f, o.w);
+  if (threadIdx.x == 0)
+    order = __hip_atomic_fetch_add(&arrived[it.join * a.kv_heads + head], 1u, __ATOMIC_RELAXED,
+                                   __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (order != (unsigned)it.parts - 1) return;
+  if (threadIdx.x == 0)
+    __hip_atomic_store(&arrived[it.join * a.kv_heads + head], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const int64_t step = (int64_t)a.kv_heads * U * UNIT;  // from part to part
+  const float *first = part + ((int64_t)it.slot * a.kv_heads + head * U) * UNIT;
+  // unit: four dims of a row; the parts in `ways` shares where there are few units
+  const int units = rows * (HDP / 4);
+  const int ways = units >= 256 ? 1 : units >= 128 ? 2 : 4;  // at least 64 units
+  __shared__ __attribute__((aligned(16))) float shares[256][8];
+  for (int u0 = 0; u0 < units; u0 += 256 / ways) {
+    const int u = u0 + (int)threadIdx.x / ways, way = (int)threadIdx.x % ways;
+    const int r = u / (HDP / 4), d = 4 * (u % (HDP / 4));
+    float M = NONE, sum = 0.f;
+    floatx4 o = zero;
+    if (u < units) {
+      const float *p = first + (r >> 4) * UNIT;
+      const int rr = r & 15;
+#pragma unroll 4
+      for (int k = way; k < it.parts; k += ways) {
+        const float2 ml = get2(p + k * step + 16 * HDP + 2 * rr);
+        const float2 x = get2(p + k * step + rr * HDP + d), y = get2(p + k * step + rr * HDP + d + 2);
+        const float mn = fmaxf(M, ml.x);
+        const float f = __builtin_amdgcn_exp2f(M - mn), h = __builtin_amdgcn_exp2f(ml.x - mn);
+        M = mn;
+        sum = fmaf(ml.y, h, sum * f);
+        o[0] = fmaf(x.x, h, o[0] * f);
+        o[1] = fmaf(x.y, h, o[1] * f);
+        o[2] = fmaf(y.x, h, o[2] * f);
+        o[3] = fmaf(y.y, h, o[3] * f);
+      }
     }
-    const float inv = 1.f / l;
-    *reinterpret_cast<float4 *>(O + ((int64_t)it.row0 + tok) * os +
-                                (int64_t)(head * a.groups + r % a.groups) * a.head_dim + d) =
-        make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    if (ways > 1) {  // (one pass: the units fit)
+      __syncthreads();
+      float *s = shares[threadIdx.x];
+      *reinterpret_cast<floatx4 *>(s) = o;
+      s[4] = M;
+      s[5] = sum;
+      __syncthreads();
+      if (way) continue;
+      for (int w = 1; w < ways; ++w) {
+        const float *t = s + 8 * w;
+        const float mn = fmaxf(M, t[4]);
+        const float f = __builtin_amdgcn_exp2f(M - mn), h = __builtin_amdgcn_exp2f(t[4] - mn);
+        M = mn;
+        sum = fmaf(t[5], h, sum * f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(t[e], h, o[e] * f);
+      }
+    }
+    if (u < units && d < a.head_dim) {
+      const float inv = 1.f / sum;
+      const int t = tile * 16 * U + r;
+      *reinterpret_cast<float4 *>(O + ((int64_t)it.row0 + t / a.groups) * os +
+                                  (int64_t)(head * a.groups + t % a.groups) * a.head_dim + d) =
+          make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    }
   }
 }
 
@@ -516,15 +692,13 @@ pbx_kv_rope_table(const double *freq, double *table, int half, int64_t n) {
   extern "C" __global__ void __launch_bounds__(256)                                                                \
       pbx_kv_read_##HDP(KvArgs a, const BlockItem *items, float *K, int64_t ks, float *V, int64_t vs) {            \
     read_body<HDP>(a, items, K, ks, V, vs);                                                                        \
-  }                                                                                                                \
-  extern "C" __global__ void __launch_bounds__(256)                                                                \
-      pbx_kv_attn_##HDP(KvArgs a, const AttnItem *items, const int *table, const float *Q, int64_t qs,             \
-                        float scale, float *O, int64_t os, float *part) {                                          \
-    attn_body<HDP>(a, items, table, Q, qs, scale, O, os, part);                                                    \
-  }                                                                                                                \
-  extern "C" __global__ void __launch_bounds__(256)                                                                \
-      pbx_kv_join_##HDP(KvArgs a, const JoinItem *items, const float *part, float *O, int64_t os) {                \
-    join_body<HDP>(a, items, part, O, os);                                                                         \
+  }
+#define PBX_KV_ATTN(HDP, U, NQ, KW, WAVES)                                                                         \
+  extern "C" __global__ void __launch_bounds__(256, WAVES)                                                         \
+      pbx_kv_attn_##HDP##_##U(KvArgs a, const AttnItem *items, const int *table, const float *Q, int64_t qs,       \
+                              float scale, float *O, int64_t os, float *part, unsigned *arrived) {                 \
+    static_assert(U == NQ * 4 / KW, "16-row tiles of the workgroup");                                              \
+    attn_body<HDP, NQ, KW>(a, items, table, Q, qs, scale, O, os, part, arrived);                                   \
   }
 PBX_KV_KERNELS(32)
 PBX_KV_KERNELS(64)
@@ -532,3 +706,17 @@ PBX_KV_KERNELS(96)
 PBX_KV_KERNELS(128)
 PBX_KV_KERNELS(192)
 PBX_KV_KERNELS(256)
+PBX_KV_ATTN(32, 1, 1, 4, 4)
+PBX_KV_ATTN(32, 2, 2, 4, 4)
+PBX_KV_ATTN(32, 4, 2, 2, 4)
+PBX_KV_ATTN(64, 1, 1, 4, 4)
+PBX_KV_ATTN(64, 2, 2, 4, 3)
+PBX_KV_ATTN(64, 4, 2, 2, 3)
+PBX_KV_ATTN(96, 1, 1, 4, 3)
+PBX_KV_ATTN(96, 2, 1, 2, 3)
+PBX_KV_ATTN(128, 1, 1, 4, 3)
+PBX_KV_ATTN(128, 2, 1, 2, 3)
+PBX_KV_ATTN(192, 1, 1, 4, 2)
+PBX_KV_ATTN(192, 2, 1, 2, 2)
+PBX_KV_ATTN(256, 1, 1, 4, 2)
+PBX_KV_ATTN(256, 2, 1, 2, 2)

@@ -44,13 +44,15 @@ struct pbx_kv_batch {
   bool set = false;
   bool stale = false;     // positions of it were dropped
   bool captured = false;  // a graph may hold its calls
-  // the plan on the device: blocks, attention items, joins, row positions, page ids
+  // the plan on the device: blocks, attention items, row positions, page ids
   int32_t *dev = nullptr, *host = nullptr;
   size_t dev_cap = 0, host_cap = 0;
-  size_t at_attn = 0, at_joins = 0, at_pos = 0, at_table = 0;
+  size_t at_attn = 0, at_pos = 0, at_table = 0;
   hipEvent_t copied = nullptr;
   float *part = nullptr;  // partial results of split rows
   size_t part_cap = 0;
+  unsigned *arrived = nullptr;  // [split rows][KV head] parts done so far (zero between launches)
+  size_t arrived_cap = 0;
 };
 
 static bool kv_ok(const pbx_kv *kv) { return kv && kv->magic == PBX_KV_MAGIC; }
@@ -63,6 +65,9 @@ static int kv_padded(int hd) {
   return 0;
 }
 
+// 16-row query tiles of the widest attention kernel for a head size.
+static int kv_max_tiles(int hdp) { return hdp <= 64 ? 4 : 2; }
+
 static int kv_launch(pbx_ctx *c, const std::string &name, int64_t grid, int block, void **args) {
   hipFunction_t f = pbx_kernel_by_name(c, name);
   if (!f) return pbx_fail(c, PBX_ELOAD, "kv: kernel %s not found", name.c_str());
@@ -74,6 +79,7 @@ static void batch_release(pbx_kv_batch *b) {
   if (b->dev) hipFree(b->dev);
   if (b->host) hipHostFree(b->host);
   if (b->part) hipFree(b->part);
+  if (b->arrived) hipFree(b->arrived);
   if (b->copied) hipEventDestroy(b->copied);
   b->magic = 0;
   delete b;
@@ -284,8 +290,7 @@ static int batch_upload(pbx_kv_batch *b) {
   const kv_batch_plan &p = b->plan;
   const size_t n_blocks = p.blocks.size() * sizeof(kv_block_item) / 4;
   b->at_attn = n_blocks;
-  b->at_joins = b->at_attn + p.attn.size() * sizeof(kv_attn_item) / 4;
-  b->at_pos = b->at_joins + p.joins.size() * sizeof(kv_join_item) / 4;
+  b->at_pos = b->at_attn + p.attn.size() * sizeof(kv_attn_item) / 4;
   b->at_table = b->at_pos + p.row_pos.size();
   const size_t n = b->at_table + p.table.size();
   if (!n) return PBX_OK;
@@ -297,12 +302,20 @@ static int batch_upload(pbx_kv_batch *b) {
     return rc;
   memcpy(b->host, p.blocks.data(), n_blocks * 4);
   memcpy(b->host + b->at_attn, p.attn.data(), p.attn.size() * sizeof(kv_attn_item));
-  memcpy(b->host + b->at_joins, p.joins.data(), p.joins.size() * sizeof(kv_join_item));
   memcpy(b->host + b->at_pos, p.row_pos.data(), p.row_pos.size() * 4);
   memcpy(b->host + b->at_table, p.table.data(), p.table.size() * 4);
   // per slot and KV head: 16 rows of hdp sums, then their maxima and weights
   const size_t part = (size_t)p.n_slots * kv->cfg.n_kv_heads * 16 * (kv->hdp + 2) * 4;
-  if (part && (rc = pbx_ensure_dev(c, (void **)&b->part, &b->part_cap, part))) return rc;
+  const size_t joins = (size_t)p.n_joins * kv->cfg.n_kv_heads * 4, joins_had = b->arrived_cap;
+  if (part && ((rc = pbx_ensure_dev(c, (void **)&b->part, &b->part_cap, part)) ||
+               (rc = pbx_ensure_dev(c, (void **)&b->arrived, &b->arrived_cap, joins))))
+    return rc;
+  if (b->arrived_cap != joins_had && hipMemsetAsync(b->arrived, 0, b->arrived_cap, c->stream) != hipSuccess) {
+    hipFree(b->arrived);
+    b->arrived = nullptr;
+    b->arrived_cap = 0;
+    return pbx_fail(c, PBX_EHIP, "pbx_kv_batch_set: clearing the counts failed");
+  }
   if (hipMemcpyAsync(b->dev, b->host, n * 4, hipMemcpyHostToDevice, c->stream) != hipSuccess ||
       hipEventRecord(b->copied, c->stream) != hipSuccess)
     return pbx_fail(c, PBX_EHIP, "pbx_kv_batch_set: copy failed");
@@ -331,7 +344,8 @@ extern "C" int pbx_kv_batch_set(pbx_kv_batch *b, int n, const int32_t *seqs, con
     b->set = false;
     try {
       std::swap(b->plan, plan);
-      kv_plan_work(kv->pages, kv->cfg.n_heads / kv->cfg.n_kv_heads, kv->cfg.n_kv_heads, 4 * c->cu_count, &b->plan);
+      kv_plan_work(kv->pages, kv->cfg.n_heads / kv->cfg.n_kv_heads, kv->cfg.n_kv_heads, kv_max_tiles(kv->hdp),
+                   2 * c->cu_count, &b->plan);
       rc = batch_upload(b);
     } catch (const std::bad_alloc &) {
       rc = pbx_fail(c, PBX_ENOMEM, "pbx_kv_batch_set: out of host memory");
@@ -429,15 +443,17 @@ extern "C" int pbx_kv_attention_dev(pbx_kv_batch *b, int layer, const float *dQ,
       (rc = rows_check(c, who, "dOut", dOut, &out_stride, g.n_heads, g.head_dim)))
     return rc;
   if (scale == 0.f) scale = (float)(1.0 / sqrt((double)g.head_dim));
-  const int32_t *items = b->dev + b->at_attn, *joins = b->dev + b->at_joins, *table = b->dev + b->at_table;
-  void *args[] = {&a, &items, &table, &dQ, &q_stride, &scale, &dOut, &out_stride, &b->part};
-  if ((rc = kv_launch(c, "pbx_kv_attn_" + std::to_string(kv->hdp), (int64_t)b->plan.attn.size() * g.n_kv_heads,
-                      256, args)) ||
-      b->plan.joins.empty())
-    return rc;
-  void *jargs[] = {&a, &joins, &b->part, &dOut, &out_stride};
-  return kv_launch(c, "pbx_kv_join_" + std::to_string(kv->hdp), (int64_t)b->plan.joins.size() * g.n_kv_heads, 256,
-                   jargs);
+  const int32_t *items = b->dev + b->at_attn, *table = b->dev + b->at_table;
+  for (int k = 0; k < 4; ++k) {
+    const int n = b->plan.n_attn[k];
+    if (!n) continue;
+    void *args[] = {&a, &items, &table, &dQ, &q_stride, &scale, &dOut, &out_stride, &b->part, &b->arrived};
+    if ((rc = kv_launch(c, "pbx_kv_attn_" + std::to_string(kv->hdp) + "_" + std::to_string(1 << k),
+                        (int64_t)n * g.n_kv_heads, 256, args)))
+      return rc;
+    items += n * (sizeof(kv_attn_item) / 4);
+  }
+  return PBX_OK;
 }
 
 extern "C" int pbx_kv_read_dev(pbx_kv_batch *b, int layer, float *dK, int64_t k_stride, float *dV,

@@ -61,20 +61,18 @@ struct kv_block_item {
   int32_t row0;         // first packed row
   int32_t pad[2];
 };
-// Query rows 16 tile .. of a sequence ((row, head of the KV group) pairs, the
-// head fastest) over its blocks blk0..blk1 - 1.
+// Query rows 16 u tile .. of a sequence ((row, head of the KV group) pairs, the
+// head fastest) over its blocks blk0..blk1 - 1: u 16-row tiles, 1, 2, 4 or 8.
 struct kv_attn_item {
   int32_t start, count, row0;
   int32_t tile;
   int32_t blk0, blk1;
-  int32_t tab;   // the sequence's page ids, from here on in the page table
-  int32_t slot;  // partial result to write, or -1: the only item of its rows
-};
-// The partial results of one tile: slots slot .. slot + n - 1.
-struct kv_join_item {
-  int32_t count, row0, tile;
-  int32_t slot, n;
-  int32_t pad[3];
+  int32_t tab;       // the sequence's page ids, from here on in the page table
+  int32_t part, parts;  // this item's place among those of its rows
+  int32_t slot;      // the first part's partial result, in units of 16 rows (parts > 1)
+  int32_t join;      // which rows these are among those that are split (parts > 1)
+  int32_t pad;
+  int32_t pages[4];  // the pages from block blk0 on (as far as blk1 needs them)
 };
 
 struct kv_batch_plan {
@@ -83,11 +81,11 @@ struct kv_batch_plan {
   std::vector<int32_t> seqs, starts, counts;
   // work lists, in the order they lie in device memory
   std::vector<kv_block_item> blocks;
-  std::vector<kv_attn_item> attn;
-  std::vector<kv_join_item> joins;
+  std::vector<kv_attn_item> attn;  // those of u 1, then 2, 4, 8
   std::vector<int32_t> row_pos;  // position of every packed row
   std::vector<int32_t> table;    // page ids, sequence by sequence
-  int n_slots = 0;
+  int n_attn[4] = {0, 0, 0, 0};
+  int n_slots = 0, n_joins = 0;
 };
 
 // Checks a batch and, if it holds, takes its pages and fills the plan; refused
@@ -157,52 +155,77 @@ inline int kv_plan_rows(kv_pages *kv, int n, const int32_t *seqs, const int32_t 
   return PBX_OK;
 }
 
+#define KV_MAX_PARTS 64
+
 // The work lists of a planned batch: `groups` = n_heads / n_kv_heads query
 // heads a KV head, `kv_heads` KV heads (each item runs once per KV head),
-// `want` workgroups that fill the GPU.
-inline void kv_plan_work(const kv_pages &kv, int groups, int kv_heads, int want, kv_batch_plan *p) {
+// `max_u` 16-row tiles of the widest kernel for this head size, `want`
+// workgroups that fill the GPU.
+inline void kv_plan_work(const kv_pages &kv, int groups, int kv_heads, int max_u, int want, kv_batch_plan *p) {
   const int n = (int)p->seqs.size();
   p->blocks.clear();
   p->attn.clear();
-  p->joins.clear();
   p->row_pos.clear();
   p->table.clear();
-  p->n_slots = 0;
+  p->n_slots = p->n_joins = 0;
   p->last = true;
-  int64_t total = 0;  // blocks that the tiles visit
-  auto tiles_of = [&](int i) { return (int)(((int64_t)p->counts[i] * groups + 15) / 16); };
+  // a few rows (tokens, a verify) take the narrowest kernel that holds them
+  auto log_u = [&](int i) {
+    const int64_t rows = (int64_t)p->counts[i] * groups;
+    int k = 0;
+    while (2 << k <= max_u && rows > 16 << k) ++k;
+    return k;
+  };
+  auto tiles_of = [&](int i) {
+    const int t = 16 << log_u(i);
+    return (int)(((int64_t)p->counts[i] * groups + t - 1) / t);
+  };
   auto blocks_of = [&](int i, int tile) {  // visible to the tile's last row
-    const int64_t last = std::min<int64_t>((int64_t)p->counts[i] * groups, 16 * ((int64_t)tile + 1)) - 1;
+    const int64_t rows = (int64_t)p->counts[i] * groups;
+    const int64_t last = std::min<int64_t>(rows, (16 << log_u(i)) * ((int64_t)tile + 1)) - 1;
     return (int)((p->starts[i] + last / groups) / PBX_KV_BLOCK + 1);
   };
+  int64_t total = 0;  // blocks that the tiles visit
   for (int i = 0; i < n; ++i)
     for (int t = 0; t < tiles_of(i); ++t) total += blocks_of(i, t);
-  // an item: at least 8 blocks (two a wave), and about `want` workgroups in all
-  const int64_t chunk = std::max<int64_t>(8, (total * kv_heads + want - 1) / want);
+  // an item: at least 16 blocks (four a wave), and about `want` workgroups in all
+  const int64_t chunk = std::max<int64_t>(16, (total * kv_heads + want - 1) / want);
+  const int per_page = kv.page_tokens / PBX_KV_BLOCK;
+  std::vector<kv_attn_item> by_u[4];
   int row0 = 0;
   for (int i = 0; i < n; ++i) {
     const kv_seq &s = kv.seqs[p->seqs[i]];
-    const int start = p->starts[i], count = p->counts[i], tab = (int)p->table.size();
+    const int start = p->starts[i], count = p->counts[i], tab = (int)p->table.size(), lu = log_u(i);
     if (!count) continue;
     if (start + count != s.len) p->last = false;
     const int used = kv.pages_of(start + count);
     p->table.insert(p->table.end(), s.pages.begin(), s.pages.begin() + used);
-    const int per_page = kv.page_tokens / PBX_KV_BLOCK;
     for (int b = start / PBX_KV_BLOCK; b * PBX_KV_BLOCK < start + count; ++b)
       p->blocks.push_back({s.pages[b / per_page], b % per_page, b * PBX_KV_BLOCK, start, count, row0, {0, 0}});
     for (int t = 0; t < count; ++t) p->row_pos.push_back(start + t);
     for (int t = 0; t < tiles_of(i); ++t) {
       const int nb = blocks_of(i, t);
-      const int parts = (int)((nb + chunk - 1) / chunk);
-      for (int k = 0; k < parts; ++k)
-        p->attn.push_back({start, count, row0, t, (int)((int64_t)nb * k / parts),
-                           (int)((int64_t)nb * (k + 1) / parts), tab, parts > 1 ? p->n_slots + k : -1});
+      const int parts = (int)std::min<int64_t>(KV_MAX_PARTS, (nb + chunk - 1) / chunk);
+      for (int k = 0; k < parts; ++k) {
+        kv_attn_item x = {start, count, row0, t, (int)((int64_t)nb * k / parts), (int)((int64_t)nb * (k + 1) / parts),
+                          tab, k, parts, p->n_slots, p->n_joins, 0, {0, 0, 0, 0}};
+        for (int j = 0; j < 4; ++j) x.pages[j] = s.pages[std::min(x.blk0 / per_page + j, (x.blk1 - 1) / per_page)];
+        by_u[lu].push_back(x);
+      }
       if (parts > 1) {
-        p->joins.push_back({count, row0, t, p->n_slots, parts, {0, 0, 0}});
-        p->n_slots += parts;
+        p->n_slots += parts << lu;
+        ++p->n_joins;
       }
     }
     row0 += count;
+  }
+  for (int c = 0; c < 4; ++c) {
+    // the items with the most blocks first, so that none of them is the last to start
+    std::stable_sort(by_u[c].begin(), by_u[c].end(), [](const kv_attn_item &x, const kv_attn_item &y) {
+      return x.blk1 - x.blk0 > y.blk1 - y.blk0;
+    });
+    p->attn.insert(p->attn.end(), by_u[c].begin(), by_u[c].end());
+    p->n_attn[c] = (int)by_u[c].size();
   }
 }
 

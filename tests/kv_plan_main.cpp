@@ -30,12 +30,21 @@ static void check_pages(const kv_pages &kv, int n_pages) {
   CHECK((int)all.size() == n_pages && *all.begin() == 0 && *all.rbegin() == n_pages - 1);
 }
 
-static void check_work(const kv_pages &kv, const kv_batch_plan &p, int groups) {
+static void check_work(const kv_pages &kv, const kv_batch_plan &p, int groups, int max_u) {
   const int per_page = kv.page_tokens / PBX_KV_BLOCK;
   CHECK((int)p.row_pos.size() == p.n_rows);
-  size_t bi = 0, ai = 0, ji = 0;
+  CHECK(p.n_attn[0] + p.n_attn[1] + p.n_attn[2] + p.n_attn[3] == (int)p.attn.size());
+  // the items of a tile, by (first row, tile)
+  std::map<std::pair<int, int>, std::vector<std::pair<kv_attn_item, int>>> items;
+  int at = 0;
+  for (int c = 0; c < 4; ++c)
+    for (int k = 0; k < p.n_attn[c]; ++k, ++at) {
+      CHECK(!k || p.attn[at - 1].blk1 - p.attn[at - 1].blk0 >= p.attn[at].blk1 - p.attn[at].blk0);
+      items[{p.attn[at].row0, p.attn[at].tile}].push_back({p.attn[at], 1 << c});
+    }
+  size_t bi = 0, used_items = 0;
   int row0 = 0, tab = 0;
-  std::set<int> slots;
+  std::set<int> slots, joins;
   for (size_t i = 0; i < p.seqs.size(); ++i) {
     const kv_seq &s = kv.seqs[p.seqs[i]];
     const int start = p.starts[i], count = p.counts[i], end = start + count;
@@ -53,33 +62,36 @@ static void check_work(const kv_pages &kv, const kv_batch_plan &p, int groups) {
     // every row in a tile, and every position that it sees in one of the tile's items
     int tiles = 0, row = 0;
     while (row < count * groups) {
-      const int last = std::min(count * groups, row + 16) - 1;
+      CHECK(items.count({row0, tiles}));
+      auto list = items[{row0, tiles}];
+      std::sort(list.begin(), list.end(), [](auto &x, auto &y) { return x.first.part < y.first.part; });
+      const int u16 = list[0].second, parts = (int)list.size();
+      CHECK(u16 <= max_u && parts <= KV_MAX_PARTS);
+      const int last = std::min(count * groups, row + 16 * u16) - 1;
       const int seen = start + last / groups + 1;  // positions
-      int blk = 0, parts = 0;
-      const size_t first = ai;
-      while (ai < p.attn.size() && p.attn[ai].row0 == row0 && p.attn[ai].tile == tiles) {
-        const kv_attn_item &x = p.attn[ai++];
+      int blk = 0;
+      for (int k = 0; k < parts; ++k) {
+        const kv_attn_item &x = list[k].first;
+        CHECK(list[k].second == u16 && x.part == k && x.parts == parts);
         CHECK(x.start == start && x.count == count && x.tab == tab);
         CHECK(x.blk0 == blk && x.blk1 > x.blk0 && (x.blk1 - 1) / per_page < used);
+        for (int b = x.blk0; b < std::min(x.blk1, x.blk0 + 4); ++b)
+          CHECK(x.pages[b / per_page - x.blk0 / per_page] == s.pages[b / per_page]);
         blk = x.blk1;
-        ++parts;
-        if (x.slot >= 0) CHECK(x.slot < p.n_slots && slots.insert(x.slot).second);
+        CHECK(x.slot == list[0].first.slot && x.join == list[0].first.join);
+        for (int u = 0; parts > 1 && u < u16; ++u)
+          CHECK(x.slot + k * u16 + u < p.n_slots && slots.insert(x.slot + k * u16 + u).second);
       }
       CHECK(blk == (seen + PBX_KV_BLOCK - 1) / PBX_KV_BLOCK);
-      if (parts > 1) {
-        const kv_join_item &j = p.joins[ji++];
-        CHECK(j.row0 == row0 && j.tile == tiles && j.count == count && j.n == parts);
-        for (int k = 0; k < parts; ++k) CHECK(p.attn[first + k].slot == j.slot + k);
-      } else {
-        CHECK(p.attn[first].slot == -1);
-      }
-      row += 16;
+      if (parts > 1) CHECK(list[0].first.join < p.n_joins && joins.insert(list[0].first.join).second);
+      used_items += parts;
+      row += 16 * u16;
       ++tiles;
     }
     row0 += count;
     tab += used;
   }
-  CHECK(bi == p.blocks.size() && ai == p.attn.size() && ji == p.joins.size());
+  CHECK(bi == p.blocks.size() && used_items == p.attn.size() && (int)joins.size() == p.n_joins);
   CHECK((int)slots.size() == p.n_slots && row0 == p.n_rows && tab == (int)p.table.size());
 }
 
@@ -131,8 +143,9 @@ int main() {
       } else {
         for (size_t i = 0; i < seqs.size(); ++i)
           CHECK(kv.seqs[seqs[i]].len == std::max(before[seqs[i]].len, starts[i] + counts[i]));
-        kv_plan_work(kv, groups, heads, pick(1, 2000), &p);
-        check_work(kv, p, groups);
+        const int max_u = 1 << pick(0, 3);
+        kv_plan_work(kv, groups, heads, max_u, pick(1, 2000), &p);
+        check_work(kv, p, groups, max_u);
         bool last = true;
         for (size_t i = 0; i < seqs.size(); ++i) {
           last = last && (!counts[i] || starts[i] + counts[i] == kv.seqs[seqs[i]].len);

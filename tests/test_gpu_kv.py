@@ -207,6 +207,19 @@ def test_a_bad_value_stays_in_its_block(ctx, bad):
     p.free()
 
 
+@pytest.mark.parametrize("rows", [6, 12, 60])
+def test_a_bad_block_does_not_reach_rows_before_it(ctx, rows):
+    """Rows that share a tile with rows that see a NaN block, and do not see it themselves, stay as they are."""
+    p = Pair(ctx, 4, 2, 64, style="none", seed=19)
+    p.append([0], [28])
+    data = p.rows(rows)
+    data[1][4:, 0], data[2][5:, 1] = np.nan, np.inf  # block 1: keys of head 0, values of head 1
+    b, q = p.append([0], [rows], data)
+    got = p.attend(b, [0], [28], [rows], q)
+    assert np.isfinite(got[:4]).all() and np.isnan(got[5:]).all()
+    p.free()
+
+
 def test_a_bad_query_is_its_own_row(ctx):
     p = Pair(ctx, 4, 2, 64, style="none", seed=8)
     b, q = p.append([0], [40])
