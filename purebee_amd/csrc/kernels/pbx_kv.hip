@@ -279,36 +279,28 @@ __device__ __forceinline__ half8 halves(unsigned w0, unsigned w1) {
 // Score of a masked key and the running maximum before any visible one: finite,
 // so that differences of maxima need no special case.
 constexpr float NONE = -1e38f;
-// Probabilities are held times 2^12 (their sum too): an fp16 pair then keeps
-// 22 bits of them down to 2^-15 of the row's largest, and some down to 2^-36.
-constexpr float LIFT = 12.f;
+// Probabilities are held times 2^6 (their sum too): an fp16 pair then keeps 22
+// bits of them down to 2^-9 of the row's largest, and some down to 2^-30 (more
+// would cost the exponentials' arguments bits: 12 left 1.3 times the error).
+// A row's maximum follows its scores only when they pass it by 2^SLACK (its
+// probabilities then reach 2^12, below fp16's largest): a new maximum rescales
+// all sums, and in some row of a tile nearly every block brings one.
+constexpr float LIFT = 6.f, SLACK = 6.f;
 
-// A block's codes as a wave loads them, and its scales.
-template <int HDP>
-struct Keys {
-  uintx4 pair[2][HDP / 64 ? HDP / 64 : 1];  // [16-key tile][64 dims]
-  uintx2 rest[2];                           // the last 32 dims of an odd HDP / 32
-};
-template <int HDP>
-struct Values {
-  uintx4 w[HDP / 32];
-};
-
-template <int HDP>
-__device__ __forceinline__ void load_keys(Keys<HDP> &k, const uint8_t *kb, int c, int g) {
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-#pragma unroll
-    for (int p = 0; p < HDP / 64; ++p)
-      k.pair[t][p] = *reinterpret_cast<const uintx4 *>(kb + p * (BLK * 64) + (16 * t + c) * 64 + 16 * g);
-    if constexpr (HDP / 32 % 2)
-      k.rest[t] = *reinterpret_cast<const uintx2 *>(kb + HDP / 64 * (BLK * 64) + (16 * t + c) * 32 + 8 * g);
-  }
+// Codes reach LDS by DMA (global_load_lds: lane i's 16 bytes land at the
+// instruction's LDS base + 16 i), without registers in between; waits are
+// counted by hand, so every wave issues the same number of them for a block.
+__device__ __forceinline__ unsigned lds_address(const void *p) {
+  return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void *)p;
 }
-template <int HDP>
-__device__ __forceinline__ void load_values(Values<HDP> &v, const uint8_t *vb, int c, int g) {
-#pragma unroll
-  for (int i = 0; i < HDP / 32; ++i) v.w[i] = *reinterpret_cast<const uintx4 *>(vb + i * 1024 + c * 64 + 16 * g);
+__device__ __forceinline__ void dma16(const uint8_t *base, unsigned offset, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               ::"v"(offset), "s"(base), "s"(lds) : "memory");
+}
+// Waits until at most N of the wave's vector memory operations are under way.
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
 // A constant that the compiler cannot see through.
@@ -355,19 +347,24 @@ __device__ __forceinline__ float2 get2(const float *p) {
 // of two near the row's largest) and probabilities enter as fp16 pairs, two
 // products each, summed in f32.  The block's key scale joins the row's factor,
 // its value scale weighs the block's products as they are added up.
-// A block's keys are fetched while the one before goes through its softmax, its
-// values while the next scores are computed; no LDS until the waves' states are
-// put together.  Where a tile's blocks are split over several workgroups, the
-// one that finishes last puts their states together, in the order of the keys.
-template <int HDP, int NQ, int KW>
+// Every wave keeps a ring of RING blocks' codes in LDS, fetched RING - 1 blocks
+// ahead (RING 1: a block's keys while the one before goes through its softmax,
+// its values while the next scores are computed).  Where a tile's blocks are
+// split over several workgroups, the one that finishes last puts their states
+// together, in the order of the keys.
+template <int HDP, int NQ, int KW, int RING>
 __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items, const int *table, const float *Q,
                                           int64_t qs, float scale, float *O, int64_t os, float *part,
                                           unsigned *arrived) {
   constexpr int HC = HDP / 32, PAIRS = HDP / 64, DT = HDP / 16;
   constexpr int U = NQ * 4 / KW;        // 16-row tiles of the workgroup
   constexpr int UNIT = 16 * (HDP + 2);  // floats of 16 rows' partial state
-  constexpr int MERGED = KW > 1 ? 4 : 1;
-  __shared__ __attribute__((aligned(16))) float mrg[MERGED][NQ * DT][256];
+  constexpr int HALF = BLK * HDP, NI = HALF / 1024;  // bytes of a block's keys (or values), DMA instructions for them
+  constexpr int MERGE = KW > 1 ? 4 * NQ * DT * 1024 : 0, LDS = 4 * RING * 2 * HALF;
+  // the waves' rings, and the merge of their states after them
+  __shared__ __attribute__((aligned(16))) uint8_t lds[LDS > MERGE ? LDS : MERGE];
+  static_assert(LDS >= 256 * 8 * 4, "room for the join's shares");
+  float(*mrg)[NQ * DT][256] = reinterpret_cast<float(*)[NQ * DT][256]>(lds);
   __shared__ float mrg_m[4][NQ][16], mrg_l[4][NQ][16];
   __shared__ unsigned order;
   const AttnItem &it = items[blockIdx.x / a.kv_heads];
@@ -376,15 +373,17 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int blk0 = it.blk0, blk1 = it.blk1, start = it.start, count = it.count, tile = it.tile;
   const int sub_mask = (1 << a.page_shift) - 1;
-  auto codes_at = [&](int page, int b) {
-    return a.codes + block_index(a, page, head, b & sub_mask) * (2 * BLK * HDP);
-  };
-  auto scales_at = [&](int page, int b) {
-    return *reinterpret_cast<const float2 *>(a.scales + 2 * block_index(a, page, head, b & sub_mask));
-  };
+  const int tab = it.tab, parts = it.parts, row0 = it.row0;
+  const int part_at = it.slot + it.part * U, slot0 = it.slot, join = it.join;
+  auto block_at = [&](int page, int b) { return block_index(a, page, head, b & sub_mask); };
   // wave (qw, kw): query tiles qw NQ .., blocks b0, b0 + KW, ..: page ids one a lane, 64 at a time; the
   // first one's comes with the item
   const int qw = wave / KW, kw = wave % KW;
+  // query row r of the workgroup: token first_tok + k and head of the group; the
+  // quotient of numbers this small is exact in f32
+  const int first_tok = tile * 16 * U / a.groups, skip = tile * 16 * U % a.groups;
+  const float per_group = 1.f / (float)a.groups;
+  auto token_of = [&](int r) { return (int)(((float)(skip + r) + 0.5f) * per_group); };
   const int rows = min(16 * U, count * a.groups - tile * 16 * U);  // that are there
   // (with all keys in one wave, those that its rows see)
   const int seen = KW > 1 ? blk1
@@ -392,36 +391,64 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
   const int first_pos = start + (tile * 16 * U + 16 * NQ * qw) / a.groups;  // of the wave's rows
   const int b0 = blk0 + kw;
   const int n = 16 * NQ * qw < rows ? (seen - b0 + KW - 1) / KW : 0;  // <= 0: none
-  auto pages_from = [&](int i) {
-    return table[it.tab + (min(b0 + KW * (i + lane), blk1 - 1) >> a.page_shift)];
-  };
   // the larger of two raw products is their median with infinity: fmaxf puts a
   // canonicalising move before each (of numbers; a NaN travels with the sums)
   const float inf = opaque(INFINITY), minus_one = opaque(-1.f);
-  Keys<HDP> kr;
-  Values<HDP> vr;
-  float2 sc = make_float2(0.f, 0.f);
-  int pages = 0;
+  uint8_t *ring = lds + wave * (RING * 2 * HALF);
+  const unsigned ring_at = __builtin_amdgcn_readfirstlane((int)lds_address(ring));
+  // lane (c, g) fetches what it reads: 64 dims' 16 g .. of key c of each tile,
+  // or 16 bytes g of value dim c; the last 32 dims' keys as they lie
+  const unsigned mine16 = c * 64 + 16 * g;
+  auto fetch_keys = [&](const uint8_t *p, int slot) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      dma16(p, i * 1024 + (i < 2 * PAIRS ? mine16 : 16u * lane), ring_at + slot * (2 * HALF) + i * 1024);
+  };
+  auto fetch_values = [&](const uint8_t *p, int slot) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) dma16(p, HALF + i * 1024 + mine16, ring_at + slot * (2 * HALF) + HALF + i * 1024);
+  };
+  // 64 blocks' places and scales from `base` on, one a lane; the first block's page comes
+  // with the item, so its codes are on their way before the page table is read
+  constexpr int AHEAD = RING > 1 ? RING - 1 : 1;
+  int base = 0, slot = 0;
+  int64_t place = 0;
+  float2 scales = make_float2(0.f, 0.f);
+  auto look_up = [&](int i) {
+    const int b = min(b0 + KW * (i + lane), blk1 - 1);
+    place = block_at(table[tab + (b >> a.page_shift)], b);
+    scales = *reinterpret_cast<const float2 *>(a.scales + 2 * place);
+  };
+  auto codes_of = [&](int i) {
+    const unsigned lo = __builtin_amdgcn_readlane((unsigned)place, i - base);
+    const unsigned hi = __builtin_amdgcn_readlane((unsigned)(place >> 32), i - base);
+    return a.codes + (int64_t)((uint64_t)hi << 32 | lo) * (2 * HALF);
+  };
   if (n > 0) {
     const int j = (b0 >> a.page_shift) - (blk0 >> a.page_shift);
     const int page = j == 0 ? it.pages[0] : j == 1 ? it.pages[1] : j == 2 ? it.pages[2] : it.pages[3];
-    const uint8_t *p = codes_at(page, b0);
-    load_keys<HDP>(kr, p, c, g);
-    load_values<HDP>(vr, p + BLK * HDP, c, g);
-    sc = scales_at(page, b0);
-    pages = pages_from(0);
+    const uint8_t *p = a.codes + block_at(page, b0) * (2 * HALF);
+    fetch_keys(p, 0);
+    fetch_values(p, 0);
+    look_up(0);
+#pragma unroll
+    for (int i = 1; i < RING - 1; ++i)
+      if (i < n) {
+        fetch_keys(codes_of(i), i);
+        fetch_values(codes_of(i), i);
+      }
   }
   half8 qh[NQ][HC], ql[NQ][HC];
   float factor[NQ];  // of the products: the row's power of two, scale, log2(e)
   int pos[NQ];
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
-    const int r = (tile * U + qw * NQ + q) * 16 + c, tok = r / a.groups;
-    const bool live = tok < count;
+    const int r = 16 * (qw * NQ + q) + c, k = token_of(r), tok = first_tok + k;
+    const bool live = r < rows;
     pos[q] = live ? start + tok : -1;
     // (rows past the end load the last one's: no load waits behind a branch)
-    const float *src = Q + ((int64_t)it.row0 + min(tok, count - 1)) * qs +
-                       (int64_t)(head * a.groups + r % a.groups) * a.head_dim;
+    const float *src = Q + ((int64_t)row0 + min(tok, count - 1)) * qs +
+                       (int64_t)(head * a.groups + skip + r - k * a.groups) * a.head_dim;
     float x[HC][8];
     unsigned peak = 0;
 #pragma unroll
@@ -451,49 +478,82 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
   }
   const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
   floatx4 acc[NQ][DT];
-  float m[NQ], l[NQ];
+  float m[NQ];
+  floatx4 l[NQ];  // a column's sum in every row: products with ones
+  half8 ones;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ones[e] = (_Float16)1.f;
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     m[q] = NONE;
-    l[q] = 0.f;
+    l[q] = zero;
 #pragma unroll
     for (int i = 0; i < DT; ++i) acc[q][i] = zero;
   }
   for (int i = 0; i < n; ++i) {
-    const int b = b0 + KW * i;
-    const bool more = i + 1 < n;
-    if (((i + 1) & 63) == 0 && more) pages = pages_from(i + 1);
-    const int page = __builtin_amdgcn_readlane(pages, (i + 1) & 63);
-    const uint8_t *next = codes_at(more ? page : 0, more ? b + KW : 0);
+    const int b = b0 + KW * i, ahead = i + AHEAD;
+    if (ahead - base > 63) {
+      look_up(i);
+      base = i;
+    }
+    const float sk = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scales.x), i - base));
+    const float svb = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(scales.y), i - base));
+    const uint8_t *next = codes_of(min(ahead, n - 1));
+    const uint8_t *codes = ring + (RING > 1 ? slot * (2 * HALF) : 0);
+    // the block is there when at most what was fetched after it is under way
+    if (RING > 1 ? RING > 2 && ahead - 1 < n : i > 0)
+      wait_vm<RING == 1 ? NI : (RING - 2) * 2 * NI>();
+    else
+      wait_vm<0>();
+    if constexpr (RING > 1) {
+      // into the slot of the block before, which has been read
+      if (ahead < n) {
+        const int to = slot ? slot - 1 : RING - 1;
+        fetch_keys(next, to);
+        fetch_values(next, to);
+      }
+      slot = slot + 1 < RING ? slot + 1 : 0;
+    }
     floatx4 s[NQ][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
       for (int q = 0; q < NQ; ++q) s[q][t] = zero;
 #pragma unroll
-      for (int p = 0; p < HC; ++p) {
-        half8 k;
-        if (p < 2 * PAIRS)
-          k = halves(kr.pair[t][p / 2][2 * (p & 1)], kr.pair[t][p / 2][2 * (p & 1) + 1]);
-        else
-          k = halves(kr.rest[t][0], kr.rest[t][1]);
+      for (int p = 0; p < HC; p += 2) {
+        uintx4 w;
+        if (p < 2 * PAIRS) {
+          w = *reinterpret_cast<const uintx4 *>(codes + (p + t) * 1024 + 16 * lane);
+        } else {
+          const uintx2 x = *reinterpret_cast<const uintx2 *>(codes + 2 * PAIRS * 1024 + (16 * t + c) * 32 + 8 * g);
+          w[0] = x[0];
+          w[1] = x[1];
+        }
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) s[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[q][p], s[q][t], 0, 0, 0);
+        for (int j = 0; j < (p < 2 * PAIRS ? 2 : 1); ++j) {
+          const half8 k = halves(w[2 * j], w[2 * j + 1]);
 #pragma unroll
-        for (int q = 0; q < NQ; ++q) s[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[q][p], s[q][t], 0, 0, 0);
+          for (int q = 0; q < NQ; ++q)
+            s[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[q][p + j], s[q][t], 0, 0, 0);
+#pragma unroll
+          for (int q = 0; q < NQ; ++q)
+            s[q][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[q][p + j], s[q][t], 0, 0, 0);
+        }
       }
     }
-    if (more) load_keys<HDP>(kr, next, c, g);
+    if constexpr (RING == 1) {
+      if (ahead < n) fetch_keys(next, 0);
+    }
     half8 ph[NQ], pl[NQ];
-    float al[NQ], sv[NQ];
+    float mn[NQ], sv[NQ];
     bool moved = false;
     const bool whole = b * BLK + BLK - 1 <= first_pos;  // every live row sees the block
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
       // never 0, so that masked scores stay -inf (a block of zeros has scale 0)
-      float f = factor[q] * sc.x;
+      float f = factor[q] * sk;
       f = f < 1e-30f ? 1e-30f : f;
-      sv[q] = sc.y;
+      sv[q] = svb;
       if (!whole) {
         // a row that sees nothing of the block takes nothing of its scales either
         const bool none = b * BLK > pos[q];
@@ -507,60 +567,72 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
 #pragma unroll
       for (int e = 1; e < 8; ++e) mx = __builtin_amdgcn_fmed3f(mx, s[q][e >> 2][e & 3], inf);
       mx = pair_max<32>(pair_max<16>(mx));
-      const float mn = fmaxf(m[q], mx * f);
-      al[q] = __builtin_amdgcn_exp2f(m[q] - mn);
-      moved = moved || mn != m[q];
-      const float base = mn - LIFT;
-      float p[8], sum = 0.f;
+      mx *= f;
+      const bool up = mx > m[q] + SLACK;
+      mn[q] = up ? mx : m[q];
+      moved = moved || up;
+      const float base = mn[q] - LIFT;
+      float p[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(fmaf(s[q][e >> 2][e & 3], f, -base));
-        sum += p[e];
-      }
+      for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[q][e >> 2][e & 3], f, -base));
       split8(p, minus_one, ph[q], pl[q]);
-      l[q] = fmaf(l[q], al[q], sum);  // of this lane's keys: the column's sum is taken at the end
-      m[q] = mn;
     }
     if (__any(moved)) {
 #pragma unroll
-      for (int q = 0; q < NQ; ++q)
+      for (int q = 0; q < NQ; ++q) {
+        const float al = __builtin_amdgcn_exp2f(m[q] - mn[q]);
+        m[q] = mn[q];
+        l[q] *= al;
 #pragma unroll
-        for (int d = 0; d < DT; ++d) acc[q][d] *= al[q];
+        for (int d = 0; d < DT; ++d) acc[q][d] *= al;
+      }
     }
 #pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      const half8 v = halves(vr.w[d / 2][2 * (d & 1)], vr.w[d / 2][2 * (d & 1) + 1]);
-      floatx4 o[NQ];
+    for (int q = 0; q < NQ; ++q) l[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[q], l[q], 0, 0, 0);
 #pragma unroll
-      for (int q = 0; q < NQ; ++q) o[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[q], zero, 0, 0, 0);
-#pragma unroll
-      for (int q = 0; q < NQ; ++q) o[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[q], o[q], 0, 0, 0);
-#pragma unroll
-      for (int q = 0; q < NQ; ++q)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[q][d][e] = fmaf(o[q][e], sv[q], acc[q][d][e]);
+    for (int q = 0; q < NQ; ++q) l[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[q], l[q], 0, 0, 0);
+    if constexpr (RING == 1) {
+      if (ahead < n)
+        wait_vm<NI>();
+      else
+        wait_vm<0>();
     }
-    if (more) {
-      load_values<HDP>(vr, next + BLK * HDP, c, g);
-      sc = scales_at(page, b + KW);
+#pragma unroll
+    for (int h = 0; h < HC; ++h) {
+      const uintx4 w = *reinterpret_cast<const uintx4 *>(codes + HALF + h * 1024 + 16 * lane);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const half8 v = halves(w[2 * j], w[2 * j + 1]);
+        floatx4 o[NQ];
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) o[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[q], zero, 0, 0, 0);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) o[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[q], o[q], 0, 0, 0);
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[q][2 * h + j][e] = fmaf(o[q][e], sv[q], acc[q][2 * h + j][e]);
+      }
+    }
+    if constexpr (RING == 1) {
+      if (ahead < n) fetch_values(next, 0);
     }
   }
-#pragma unroll
-  for (int q = 0; q < NQ; ++q) l[q] = pair_sum<32>(pair_sum<16>(l[q]));
   if constexpr (KW > 1) {
     // the states of the waves with the same rows put together: one maximum, then
     // the sums, each wave a share of the 16 x 16 output tiles
 #pragma unroll
     for (int q = 0; q < NQ; ++q)
       if (g == 0) mrg_m[wave][q][c] = m[q];
-    __syncthreads();
+    __syncthreads();  // (and every wave is done with its ring)
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
       float M = mrg_m[qw * KW][q][c];
 #pragma unroll
       for (int w = 1; w < KW; ++w) M = fmaxf(M, mrg_m[qw * KW + w][q][c]);
       const float f = __builtin_amdgcn_exp2f(m[q] - M);
-      if (g == 0) mrg_l[wave][q][c] = l[q] * f;
+      if (g == 0) mrg_l[wave][q][c] = l[q][0] * f;
       m[q] = M;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
@@ -568,7 +640,11 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
     }
     __syncthreads();
   }
-  float *mine = part + ((int64_t)(it.slot + it.part * U) * a.kv_heads + head * U) * UNIT;
+  auto out_row = [&](int r) {
+    const int k = token_of(r);
+    return O + ((int64_t)row0 + first_tok + k) * os + (int64_t)(head * a.groups + skip + r - k * a.groups) * a.head_dim;
+  };
+  float *mine = part + ((int64_t)part_at * a.kv_heads + head * U) * UNIT;
 #pragma unroll
   for (int u = 0; u < NQ * DT; ++u) {
     if (u % KW != kw) continue;
@@ -585,60 +661,75 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
       }
     } else {
       o = acc[q][u % DT];
-      sum = l[q];
+      sum = l[q][0];
     }
     if (r >= rows) continue;
-    if (it.parts > 1) {
+    if (parts > 1) {
       float *p = mine + (qw * NQ + q) * UNIT;
       put2(p + c * HDP + d, o[0], o[1]);
       put2(p + c * HDP + d + 2, o[2], o[3]);
       if (u % DT == 0 && g == 0) put2(p + 16 * HDP + 2 * c, m[q], sum);
     } else if (d < a.head_dim) {
       const float inv = 1.f / sum;
-      const int t = tile * 16 * U + r;
-      *reinterpret_cast<float4 *>(O + ((int64_t)it.row0 + t / a.groups) * os +
-                                  (int64_t)(head * a.groups + t % a.groups) * a.head_dim + d) =
+      *reinterpret_cast<float4 *>(out_row(r) + d) =
           make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
     }
   }
-  if (it.parts == 1) return;
+  if (parts == 1) return;
   // this part's state is at the coherence point before its workgroup counts
   // itself in; the workgroup that completes the count reads the others' from there
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (threadIdx.x == 0)
-    order = __hip_atomic_fetch_add(&arrived[it.join * a.kv_heads + head], 1u, __ATOMIC_RELAXED,
+    order = __hip_atomic_fetch_add(&arrived[32 * (join * a.kv_heads + head)], 1u, __ATOMIC_RELAXED,
                                    __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
-  if (order != (unsigned)it.parts - 1) return;
+  if (order != (unsigned)parts - 1) return;
   if (threadIdx.x == 0)
-    __hip_atomic_store(&arrived[it.join * a.kv_heads + head], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(&arrived[32 * (join * a.kv_heads + head)], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   const int64_t step = (int64_t)a.kv_heads * U * UNIT;  // from part to part
-  const float *first = part + ((int64_t)it.slot * a.kv_heads + head * U) * UNIT;
-  // unit: four dims of a row; the parts in `ways` shares where there are few units
+  const float *first = part + ((int64_t)slot0 * a.kv_heads + head * U) * UNIT;
+  // unit: four dims of a row; the parts in `ways` shares where there are few
+  // units.  Eight parts' loads are under way at once: they come from the
+  // coherence point, one round trip after the other took 14 us for 64 parts
   const int units = rows * (HDP / 4);
-  const int ways = units >= 256 ? 1 : units >= 128 ? 2 : 4;  // at least 64 units
-  __shared__ __attribute__((aligned(16))) float shares[256][8];
+  int ways = 1;
+  while (ways < 16 && 2 * ways * units <= 256) ways *= 2;
+  float(*shares)[8] = reinterpret_cast<float(*)[8]>(lds);
   for (int u0 = 0; u0 < units; u0 += 256 / ways) {
     const int u = u0 + (int)threadIdx.x / ways, way = (int)threadIdx.x % ways;
-    const int r = u / (HDP / 4), d = 4 * (u % (HDP / 4));
+    const int r = min(u, units - 1) / (HDP / 4), d = 4 * (min(u, units - 1) % (HDP / 4));
     float M = NONE, sum = 0.f;
     floatx4 o = zero;
-    if (u < units) {
-      const float *p = first + (r >> 4) * UNIT;
-      const int rr = r & 15;
-#pragma unroll 4
-      for (int k = way; k < it.parts; k += ways) {
-        const float2 ml = get2(p + k * step + 16 * HDP + 2 * rr);
-        const float2 x = get2(p + k * step + rr * HDP + d), y = get2(p + k * step + rr * HDP + d + 2);
-        const float mn = fmaxf(M, ml.x);
-        const float f = __builtin_amdgcn_exp2f(M - mn), h = __builtin_amdgcn_exp2f(ml.x - mn);
-        M = mn;
-        sum = fmaf(ml.y, h, sum * f);
-        o[0] = fmaf(x.x, h, o[0] * f);
-        o[1] = fmaf(x.y, h, o[1] * f);
-        o[2] = fmaf(y.x, h, o[2] * f);
-        o[3] = fmaf(y.y, h, o[3] * f);
+    const float *p = first + (r >> 4) * UNIT;
+    const int rr = r & 15;
+    for (int k0 = way; k0 < parts; k0 += 8 * ways) {
+      float2 ml[8], x[8], y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float *at = p + (int64_t)min(k0 + j * ways, parts - 1) * step;
+        ml[j] = get2(at + 16 * HDP + 2 * rr);
+        x[j] = get2(at + rr * HDP + d);
+        y[j] = get2(at + rr * HDP + d + 2);
+      }
+      float mn = M;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (k0 + j * ways >= parts) ml[j] = make_float2(NONE, 0.f), x[j] = y[j] = make_float2(0.f, 0.f);
+        mn = fmaxf(mn, ml[j].x);
+      }
+      const float f = __builtin_amdgcn_exp2f(M - mn);
+      M = mn;
+      sum *= f;
+      o *= f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float h = __builtin_amdgcn_exp2f(ml[j].x - mn);
+        sum = fmaf(ml[j].y, h, sum);
+        o[0] = fmaf(x[j].x, h, o[0]);
+        o[1] = fmaf(x[j].y, h, o[1]);
+        o[2] = fmaf(y[j].x, h, o[2]);
+        o[3] = fmaf(y[j].y, h, o[3]);
       }
     }
     if (ways > 1) {  // (one pass: the units fit)
@@ -661,9 +752,7 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
     }
     if (u < units && d < a.head_dim) {
       const float inv = 1.f / sum;
-      const int t = tile * 16 * U + r;
-      *reinterpret_cast<float4 *>(O + ((int64_t)it.row0 + t / a.groups) * os +
-                                  (int64_t)(head * a.groups + t % a.groups) * a.head_dim + d) =
+      *reinterpret_cast<float4 *>(out_row(r) + d) =
           make_float4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
     }
   }
@@ -693,12 +782,12 @@ pbx_kv_rope_table(const double *freq, double *table, int half, int64_t n) {
       pbx_kv_read_##HDP(KvArgs a, const BlockItem *items, float *K, int64_t ks, float *V, int64_t vs) {            \
     read_body<HDP>(a, items, K, ks, V, vs);                                                                        \
   }
-#define PBX_KV_ATTN(HDP, U, NQ, KW, WAVES)                                                                         \
+#define PBX_KV_ATTN(HDP, U, NQ, KW, RING, WAVES)                                                                   \
   extern "C" __global__ void __launch_bounds__(256, WAVES)                                                         \
       pbx_kv_attn_##HDP##_##U(KvArgs a, const AttnItem *items, const int *table, const float *Q, int64_t qs,       \
                               float scale, float *O, int64_t os, float *part, unsigned *arrived) {                 \
     static_assert(U == NQ * 4 / KW, "16-row tiles of the workgroup");                                              \
-    attn_body<HDP, NQ, KW>(a, items, table, Q, qs, scale, O, os, part, arrived);                                   \
+    attn_body<HDP, NQ, KW, RING>(a, items, table, Q, qs, scale, O, os, part, arrived);                             \
   }
 PBX_KV_KERNELS(32)
 PBX_KV_KERNELS(64)
@@ -706,17 +795,17 @@ PBX_KV_KERNELS(96)
 PBX_KV_KERNELS(128)
 PBX_KV_KERNELS(192)
 PBX_KV_KERNELS(256)
-PBX_KV_ATTN(32, 1, 1, 4, 4)
-PBX_KV_ATTN(32, 2, 2, 4, 4)
-PBX_KV_ATTN(32, 4, 2, 2, 4)
-PBX_KV_ATTN(64, 1, 1, 4, 4)
-PBX_KV_ATTN(64, 2, 2, 4, 3)
-PBX_KV_ATTN(64, 4, 2, 2, 3)
-PBX_KV_ATTN(96, 1, 1, 4, 3)
-PBX_KV_ATTN(96, 2, 1, 2, 3)
-PBX_KV_ATTN(128, 1, 1, 4, 3)
-PBX_KV_ATTN(128, 2, 1, 2, 3)
-PBX_KV_ATTN(192, 1, 1, 4, 2)
-PBX_KV_ATTN(192, 2, 1, 2, 2)
-PBX_KV_ATTN(256, 1, 1, 4, 2)
-PBX_KV_ATTN(256, 2, 1, 2, 2)
+PBX_KV_ATTN(32, 1, 1, 4, 3, 4)
+PBX_KV_ATTN(32, 2, 2, 4, 3, 4)
+PBX_KV_ATTN(32, 4, 2, 2, 3, 4)
+PBX_KV_ATTN(64, 1, 1, 4, 3, 3)
+PBX_KV_ATTN(64, 2, 2, 4, 2, 3)
+PBX_KV_ATTN(64, 4, 2, 2, 1, 3)
+PBX_KV_ATTN(96, 1, 1, 4, 2, 3)
+PBX_KV_ATTN(96, 2, 2, 4, 2, 2)
+PBX_KV_ATTN(128, 1, 1, 4, 2, 2)
+PBX_KV_ATTN(128, 2, 2, 4, 2, 2)
+PBX_KV_ATTN(192, 1, 1, 4, 1, 2)
+PBX_KV_ATTN(192, 2, 1, 2, 1, 2)
+PBX_KV_ATTN(256, 1, 1, 4, 1, 2)
+PBX_KV_ATTN(256, 2, 1, 2, 1, 2)

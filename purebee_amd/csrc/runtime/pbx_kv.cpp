@@ -51,7 +51,9 @@ struct pbx_kv_batch {
   hipEvent_t copied = nullptr;
   float *part = nullptr;  // partial results of split rows
   size_t part_cap = 0;
-  unsigned *arrived = nullptr;  // [split rows][KV head] parts done so far (zero between launches)
+  // [split rows][KV head][32] parts done so far (zero between launches), each count in a
+  // cache line of its own: atomics on one line queue up
+  unsigned *arrived = nullptr;
   size_t arrived_cap = 0;
 };
 
@@ -306,7 +308,7 @@ static int batch_upload(pbx_kv_batch *b) {
   memcpy(b->host + b->at_table, p.table.data(), p.table.size() * 4);
   // per slot and KV head: 16 rows of hdp sums, then their maxima and weights
   const size_t part = (size_t)p.n_slots * kv->cfg.n_kv_heads * 16 * (kv->hdp + 2) * 4;
-  const size_t joins = (size_t)p.n_joins * kv->cfg.n_kv_heads * 4, joins_had = b->arrived_cap;
+  const size_t joins = (size_t)p.n_joins * kv->cfg.n_kv_heads * 128, joins_had = b->arrived_cap;
   if (part && ((rc = pbx_ensure_dev(c, (void **)&b->part, &b->part_cap, part)) ||
                (rc = pbx_ensure_dev(c, (void **)&b->arrived, &b->arrived_cap, joins))))
     return rc;
