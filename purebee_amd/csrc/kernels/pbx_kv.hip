@@ -58,13 +58,14 @@ __device__ __forceinline__ int value_byte(int key, int dim) {
   return (dim >> 5) * 1024 + (dim & 15) * 64 + (slot >> 3) * 16 + ((dim >> 4) & 1) * 8 + (slot & 7);
 }
 
-// x / s rounded half to even, as the true quotient: x * (1 / s) is a few ulp off
-// it, so only quotients next to a border need the division.
-__device__ __forceinline__ int code_of(double x, double s, double inv) {
+// x / s rounded half to even, as the true quotient.  In f32, x * (1 / s) of at
+// most 128 is off it by less than 2^-15, so only quotients nearer than 10^-4 to
+// a border (one in 5,000) need the division.
+__device__ __forceinline__ int code_of(double x, double s, float inv) {
   if (!(s > 0.0 && s < INFINITY)) return 0;
-  const double q = x * inv;
-  double r = rint(q);
-  if (fabs(fabs(q - r) - 0.5) < 1e-9) r = rint(x / s);
+  const float q = (float)x * inv;
+  float r = rintf(q);
+  if (fabsf(fabsf(q - r) - 0.5f) < 1e-4f) r = (float)rint(x / s);
   return (int)r;
 }
 
@@ -91,39 +92,37 @@ __device__ __forceinline__ void unit_dims(const KvRope &r, int u, int &a, int &b
     b = 4 * u + 2;
   }
 }
-// Turns unit u by position pos: x[0..1] at dims a, a + 1, x[2..3] at b, b + 1.
-__device__ __forceinline__ void turn(const KvRope &r, int u, int pos, double x[4]) {
-  if (4 * u >= r.dim) return;
+// cos and sin of unit u's two pairs at position pos.
+struct Angles {
+  double2 p, q;
+};
+__device__ __forceinline__ Angles angles_of(const KvRope &r, int u, int pos) {
+  if (4 * u >= r.dim) return {make_double2(1.0, 0.0), make_double2(1.0, 0.0)};
   const double2 *cs = reinterpret_cast<const double2 *>(r.table) + (size_t)pos * (r.dim / 2) + 2 * u;
-  const double2 p = cs[0], q = cs[1];
+  return {cs[0], cs[1]};
+}
+// Turns unit u: x[0..1] at dims a, a + 1, x[2..3] at b, b + 1.
+__device__ __forceinline__ void turn(const KvRope &r, int u, const Angles &cs, double x[4]) {
+  if (4 * u >= r.dim) return;
   const double x0 = x[0], x1 = x[1], x2 = x[2], x3 = x[3];
   if (r.style == 2) {
-    x[0] = x0 * p.x - x2 * p.y;
-    x[2] = x0 * p.y + x2 * p.x;
-    x[1] = x1 * q.x - x3 * q.y;
-    x[3] = x1 * q.y + x3 * q.x;
+    x[0] = x0 * cs.p.x - x2 * cs.p.y;
+    x[2] = x0 * cs.p.y + x2 * cs.p.x;
+    x[1] = x1 * cs.q.x - x3 * cs.q.y;
+    x[3] = x1 * cs.q.y + x3 * cs.q.x;
   } else {
-    x[0] = x0 * p.x - x1 * p.y;
-    x[1] = x0 * p.y + x1 * p.x;
-    x[2] = x2 * q.x - x3 * q.y;
-    x[3] = x2 * q.y + x3 * q.x;
+    x[0] = x0 * cs.p.x - x1 * cs.p.y;
+    x[1] = x0 * cs.p.y + x1 * cs.p.x;
+    x[2] = x2 * cs.q.x - x3 * cs.q.y;
+    x[3] = x2 * cs.q.y + x3 * cs.q.x;
   }
 }
 
-__device__ __forceinline__ uint64_t block_max_u64(uint64_t v, uint64_t *red) {
-  v = wave_max_u64(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = red[0];
-  for (int w = 1; w < 4; ++w) v = red[w] > v ? red[w] : v;
-  return v;
-}
-
-// Append: workgroup (block, KV head), then workgroups of 256 query units.  The
-// block's new rows are read once, turned and held in registers; the block's
-// codes are put together in LDS (with the earlier rows' codes, if there are any)
-// and stored whole.
+// Append: workgroup (block, KV head), then a workgroup for each row's queries.
+// The block's new rows are read once, keys turned, and held in registers (keys
+// by 4 dims, values by 4 positions, as their codes lie side by side); the
+// block's codes are put together in LDS (with the earlier rows' codes, if there
+// are any) and stored whole.
 template <int HDP>
 __device__ __forceinline__ void append_body(const KvArgs &a, const KvRope &r, const BlockItem *items,
                                             int n_blocks, const int *row_pos, int n_rows, const float *K,
@@ -131,24 +130,43 @@ __device__ __forceinline__ void append_body(const KvArgs &a, const KvRope &r, co
                                             float *Qout, int64_t qos) {
   constexpr int UNITS = BLK * HDP / 4 / 256;  // a thread's units of a block
   __shared__ __attribute__((aligned(16))) uint8_t img[2 * BLK * HDP];
-  __shared__ uint64_t red[4];
+  __shared__ uint64_t red_k[4];
+  __shared__ unsigned red_v[4];
   const int units = a.head_dim / 4, tid = threadIdx.x;
   const int64_t wg = blockIdx.x;
   if (wg >= (int64_t)n_blocks * a.kv_heads) {
-    const int64_t i = (wg - (int64_t)n_blocks * a.kv_heads) * 256 + tid;
-    const int heads = a.kv_heads * a.groups;
-    const int64_t row = i / (heads * units);
-    if (row >= n_rows) return;
-    const int h = (int)(i % (heads * units)) / units, u = (int)(i % units);
-    int da, db;
-    unit_dims(r, u, da, db);
-    const float *q = Q + row * qs + (int64_t)h * a.head_dim;
-    const float2 lo = *reinterpret_cast<const float2 *>(q + da), hi = *reinterpret_cast<const float2 *>(q + db);
-    double x[4] = {lo.x, lo.y, hi.x, hi.y};
-    turn(r, u, row_pos[row], x);
-    float *o = Qout + row * qos + (int64_t)h * a.head_dim;
-    *reinterpret_cast<float2 *>(o + da) = make_float2((float)x[0], (float)x[1]);
-    *reinterpret_cast<float2 *>(o + db) = make_float2((float)x[2], (float)x[3]);
+    const int64_t row = wg - (int64_t)n_blocks * a.kv_heads;
+    const int n = a.kv_heads * a.groups * units, pos = row_pos[row];
+    const float *q = Q + row * qs;
+    float *o = Qout + row * qos;
+    // four units at a time, all read before any is written (in place, too: a unit
+    // is read and written by one thread); with a power of two of units a head a
+    // thread meets the same angles in every head
+    const bool same = 256 % units == 0;
+    Angles cs = angles_of(r, tid % units, pos);
+    for (int i0 = tid; i0 < n; i0 += 4 * 256) {
+      float2 x[4][2];
+      int at[4][2];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = min(i0 + 256 * k, n - 1), u = i % units, h = 4 * (i - u);  // h: the head's first dim
+        unit_dims(r, u, at[k][0], at[k][1]);
+        at[k][0] += h;
+        at[k][1] += h;
+        x[k][0] = *reinterpret_cast<const float2 *>(q + at[k][0]);
+        x[k][1] = *reinterpret_cast<const float2 *>(q + at[k][1]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = i0 + 256 * k, u = i % units;
+        if (i >= n) break;
+        if (!same) cs = angles_of(r, u, pos);
+        double y[4] = {x[k][0].x, x[k][0].y, x[k][1].x, x[k][1].y};
+        turn(r, u, cs, y);
+        *reinterpret_cast<float2 *>(o + at[k][0]) = make_float2((float)y[0], (float)y[1]);
+        *reinterpret_cast<float2 *>(o + at[k][1]) = make_float2((float)y[2], (float)y[3]);
+      }
+    }
     return;
   }
   const BlockItem it = items[wg / a.kv_heads];
@@ -158,29 +176,40 @@ __device__ __forceinline__ void append_body(const KvArgs &a, const KvRope &r, co
   // rows lo .. hi - 1 of the block are new, those before lo were there
   const int lo = it.start > it.pos0 ? it.start - it.pos0 : 0;
   const int hi = min(BLK, it.start + it.count - it.pos0);
-  const int nu = (hi - lo) * units;  // units of the new rows
+  const int64_t row0 = (int64_t)it.row0 + it.pos0 - it.start;  // of the block's first position
+  K += row0 * ks + (int64_t)head * a.head_dim;
+  V += row0 * vs + (int64_t)head * a.head_dim;
+  const int nk_units = (hi - lo) * units;
+  const int v0 = lo / 4, nv_units = ((hi + 3) / 4 - v0) * a.head_dim;
   double xk[UNITS][4];
   float xv[UNITS][4];
-  uint64_t pk = 0, pv = 0;
+  uint64_t pk = 0;
+  unsigned pv = 0;
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
     const int j = tid + 256 * i;
-    if (j < nu) {
-      const int key = lo + j / units, u = j % units;
-      const int64_t row = (int64_t)it.row0 + it.pos0 + key - it.start;
-      int da, db;
-      unit_dims(r, u, da, db);
-      const float *k = K + row * ks + (int64_t)head * a.head_dim;
-      const float2 k0 = *reinterpret_cast<const float2 *>(k + da), k1 = *reinterpret_cast<const float2 *>(k + db);
-      const float4 v = *reinterpret_cast<const float4 *>(V + row * vs + (int64_t)head * a.head_dim + 4 * u);
-      xk[i][0] = k0.x; xk[i][1] = k0.y; xk[i][2] = k1.x; xk[i][3] = k1.y;
-      xv[i][0] = v.x; xv[i][1] = v.y; xv[i][2] = v.z; xv[i][3] = v.w;
-      turn(r, u, it.pos0 + key, xk[i]);
+    if (j < nv_units) {
+      const int key = 4 * (v0 + j / a.head_dim), d = j % a.head_dim;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint64_t mk = magnitude(xk[i][e]), mv = magnitude(xv[i][e]);
+        // (a quad's positions that are not new load one that is)
+        const float x = V[min(max(key + e, lo), hi - 1) * vs + d];
+        xv[i][e] = x;
+        pv = max(pv, __float_as_uint(x) & 0x7fffffffu);
+      }
+    }
+    if (j < nk_units) {
+      const int key = lo + j / units, u = j % units;
+      int da, db;
+      unit_dims(r, u, da, db);
+      const float2 k0 = *reinterpret_cast<const float2 *>(K + key * ks + da);
+      const float2 k1 = *reinterpret_cast<const float2 *>(K + key * ks + db);
+      xk[i][0] = k0.x; xk[i][1] = k0.y; xk[i][2] = k1.x; xk[i][3] = k1.y;
+      turn(r, u, angles_of(r, u, it.pos0 + key), xk[i]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint64_t mk = magnitude(xk[i][e]);
         pk = mk > pk ? mk : pk;
-        pv = mv > pv ? mv : pv;
       }
     }
   }
@@ -190,12 +219,24 @@ __device__ __forceinline__ void append_body(const KvArgs &a, const KvRope &r, co
     ov = a.scales[2 * bi + 1];
     for (int i = tid; i < 2 * BLK * HDP / 16; i += 256)
       reinterpret_cast<uintx4 *>(img)[i] = reinterpret_cast<const uintx4 *>(codes)[i];
-  } else {
+  } else if (hi < BLK || a.head_dim < HDP) {
     for (int i = tid; i < 2 * BLK * HDP / 4; i += 256) reinterpret_cast<unsigned *>(img)[i] = 0x80808080u;
   }
-  const float nk = larger(ok, scale_of(block_max_u64(pk, red))), nv = larger(ov, scale_of(block_max_u64(pv, red)));
-  const double ik = 1.0 / (double)nk, iv = 1.0 / (double)nv;
-  // (the reductions' barriers order the image's fill before this)
+  pk = wave_max_u64(pk);
+#pragma unroll
+  for (int off = 32; off >= 1; off /= 2) pv = max(pv, (unsigned)__shfl_xor((int)pv, off, 64));
+  if ((tid & 63) == 0) {
+    red_k[tid >> 6] = pk;
+    red_v[tid >> 6] = pv;
+  }
+  __syncthreads();  // (and the image is filled)
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    pk = red_k[w] > pk ? red_k[w] : pk;
+    pv = max(pv, red_v[w]);
+  }
+  const float nk = larger(ok, scale_of(pk)), nv = larger(ov, scale_of(magnitude((double)__uint_as_float(pv))));
+  const float ik = 1.f / nk, iv = 1.f / nv;
   if (lo > 0) {
     const bool gk = __float_as_uint(nk) != __float_as_uint(ok), gv = __float_as_uint(nv) != __float_as_uint(ov);
     if (gk || gv) {
@@ -205,20 +246,34 @@ __device__ __forceinline__ void append_body(const KvArgs &a, const KvRope &r, co
         if (gk) *pkb = (uint8_t)(code_of((double)((int)*pkb - 128) * (double)ok, nk, ik) + 128);
         if (gv) *pvb = (uint8_t)(code_of((double)((int)*pvb - 128) * (double)ov, nv, iv) + 128);
       }
+      __syncthreads();  // a quad of values below may hold earlier positions' codes
     }
   }
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
     const int j = tid + 256 * i;
-    if (j < nu) {
+    if (j < nk_units) {
       const int key = lo + j / units, u = j % units;
       int da, db;
       unit_dims(r, u, da, db);
+      unsigned w = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int dk = (e < 2 ? da : db) + (e & 1);
-        img[key_byte<HDP>(key, dk)] = (uint8_t)(code_of(xk[i][e], nk, ik) + 128);
-        img[BLK * HDP + value_byte(key, 4 * u + e)] = (uint8_t)(code_of(xv[i][e], nv, iv) + 128);
+      for (int e = 0; e < 4; ++e) w |= (unsigned)(code_of(xk[i][e], nk, ik) + 128) << (8 * e);
+      *reinterpret_cast<uint16_t *>(img + key_byte<HDP>(key, da)) = (uint16_t)w;
+      *reinterpret_cast<uint16_t *>(img + key_byte<HDP>(key, db)) = (uint16_t)(w >> 16);
+    }
+    if (j < nv_units) {
+      const int key = 4 * (v0 + j / a.head_dim), d = j % a.head_dim;
+      uint8_t *at = img + BLK * HDP + value_byte(key, d);
+      unsigned w = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w |= (unsigned)(code_of(xv[i][e], nv, iv) + 128) << (8 * e);
+      if (key >= lo && key + 4 <= hi) {
+        *reinterpret_cast<unsigned *>(at) = w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (key + e >= lo && key + e < hi) at[e] = (uint8_t)(w >> (8 * e));
       }
     }
   }

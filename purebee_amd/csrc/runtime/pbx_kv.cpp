@@ -422,12 +422,10 @@ extern "C" int pbx_kv_append_dev(pbx_kv_batch *b, int layer, const float *dQ, in
   KvRopeHost r{kv->rope, g.rope_style, g.rope_dim};
   const int32_t *items = b->dev, *pos = b->dev + b->at_pos;
   const int n_blocks = (int)b->plan.blocks.size(), n_rows = b->plan.n_rows;
-  // 256 threads turn 256 groups of 4 query dims
-  const int64_t qunits = dQ ? (int64_t)n_rows * g.n_heads * (g.head_dim / 4) : 0;
   void *args[] = {&a, &r, &items, (void *)&n_blocks, &pos, (void *)&n_rows, &dK, &k_stride, &dV, &v_stride,
                   &dQ, &q_stride, &dQout, &qout_stride};
   return kv_launch(c, "pbx_kv_append_" + std::to_string(kv->hdp),
-                   (int64_t)n_blocks * g.n_kv_heads + (qunits + 255) / 256, 256, args);
+                   (int64_t)n_blocks * g.n_kv_heads + (dQ ? n_rows : 0), 256, args);
 }
 
 extern "C" int pbx_kv_attention_dev(pbx_kv_batch *b, int layer, const float *dQ, int64_t q_stride, float scale,
