@@ -48,34 +48,54 @@ __device__ __forceinline__ float key_value(uint64_t k) {
   return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 
-__device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int mask) {
-  const unsigned lo = (unsigned)__shfl_xor((int)(unsigned)v, mask, 64);
-  const unsigned hi = (unsigned)__shfl_xor((int)(unsigned)(v >> 32), mask, 64);
-  return (uint64_t)hi << 32 | lo;
+// The value of the lane that differs in bit OFF, without a trip through LDS:
+// DPP moves inside a row of 16 lanes (lane ^ 4 as (lane ^ 7) ^ 3), lane swaps
+// across rows and halves.
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
 }
-// One step of a bitonic network: the lane whose partner bit is clear keeps the
-// larger value.
-__device__ __forceinline__ uint64_t exchange(uint64_t v, int mask, int lane, int bit) {
-  const uint64_t o = shfl_xor_u64(v, mask);
-  return ((lane & bit) == 0) == (o > v) ? o : v;
-}
-// A wave's 64 keys in descending order.
-__device__ __forceinline__ uint64_t sort_wave(uint64_t v, int lane) {
-#pragma unroll
-  for (int k = 2; k <= 64; k *= 2) {
-    v = exchange(v, k - 1, lane, k / 2);  // against the mirrored half
-#pragma unroll
-    for (int j = k / 4; j >= 1; j /= 2) v = exchange(v, j, lane, j);
+template <int OFF>
+__device__ __forceinline__ unsigned partner(unsigned v, bool upper) {
+  if constexpr (OFF == 1) return dpp<0xB1>(v);         // quad_perm 1 0 3 2
+  else if constexpr (OFF == 2) return dpp<0x4E>(v);    // quad_perm 2 3 0 1
+  else if constexpr (OFF == 4) return dpp<0x1B>(dpp<0x141>(v));  // row_half_mirror, quad_perm 3 2 1 0
+  else if constexpr (OFF == 8) return dpp<0x128>(v);   // row_ror 8
+  else if constexpr (OFF == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return upper ? r[0] : r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return upper ? r[0] : r[1];
   }
+}
+// One step of a bitonic network over bit OFF: the lanes with `first` keep the
+// larger key.
+template <int OFF>
+__device__ __forceinline__ uint64_t exchange(uint64_t v, int lane, bool first) {
+  const bool upper = lane & OFF;
+  const uint64_t o = (uint64_t)partner<OFF>((unsigned)(v >> 32), upper) << 32 | partner<OFF>((unsigned)v, upper);
+  return first == (o > v) ? o : v;
+}
+// From a bitonic sequence over 2 OFF lanes to a sorted one.
+template <int OFF>
+__device__ __forceinline__ uint64_t settle(uint64_t v, int lane, bool down) {
+  v = exchange<OFF>(v, lane, ((lane & OFF) == 0) == down);
+  if constexpr (OFF > 1) v = settle<OFF / 2>(v, lane, down);
   return v;
 }
-// The 64 largest of two descending lists, in descending order.
-__device__ __forceinline__ uint64_t merge_wave(uint64_t a, uint64_t b, int lane) {
-  const uint64_t o = shfl_xor_u64(b, 63);
-  uint64_t v = o > a ? o : a;
-#pragma unroll
-  for (int j = 32; j >= 1; j /= 2) v = exchange(v, j, lane, j);
-  return v;
+// A wave's 64 keys in descending (down) or ascending order.
+__device__ __forceinline__ uint64_t sort_wave(uint64_t v, int lane, bool down) {
+  v = settle<1>(v, lane, (lane & 2) == 0);
+  v = settle<2>(v, lane, (lane & 4) == 0);
+  v = settle<4>(v, lane, (lane & 8) == 0);
+  v = settle<8>(v, lane, (lane & 16) == 0);
+  v = settle<16>(v, lane, (lane & 32) == 0);
+  return settle<32>(v, lane, down);
+}
+// The 64 largest of a descending list and an ascending one, in descending order.
+__device__ __forceinline__ uint64_t merge_wave(uint64_t down, uint64_t up, int lane) {
+  return settle<32>(up > down ? up : down, lane, true);
 }
 
 // The 64 largest keys of W waves' descending lists, in wave 0.
@@ -85,7 +105,7 @@ __device__ __forceinline__ uint64_t merge_waves(uint64_t v, uint64_t (*buf)[64],
   for (int h = W / 2; h >= 1; h /= 2) {
     if (wave >= h && wave < 2 * h) buf[wave][lane] = v;
     __syncthreads();
-    if (wave < h) v = merge_wave(v, buf[wave + h][lane], lane);
+    if (wave < h) v = merge_wave(v, buf[wave + h][63 - lane], lane);
     __syncthreads();
   }
   return v;
@@ -133,16 +153,38 @@ __device__ __forceinline__ void answer(const Out &o, int64_t row, const float *x
   }
 }
 
-// The group of four elements that start at i (aligned to 16 bytes; i < 0 or
-// i + 3 >= vocab at a row's ends: absent ones as -inf).
-__device__ __forceinline__ float4 group_at(const float *x, int i, int vocab) {
-  if (i >= 0 && i + 3 < vocab) return *reinterpret_cast<const float4 *>(x + i);
+// Four elements join a thread's sums, and the group its first largest one.  The
+// maximum follows only when passed by SLACK (e^8 of a probability): among 64
+// lanes some would meet a new maximum in nearly every group.
+constexpr float SLACK = 8.f;
+struct Share {
+  Sums a;
+  float best;
+  int at;
+};
+__device__ __forceinline__ void take(Share &t, float4 v, int g) {
+  const float top4 = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+  if (top4 > t.best || t.at < 0 || (top4 == t.best && g < t.at)) {
+    t.best = top4;
+    t.at = g;
+  }
+  if (top4 > t.a.m + SLACK) t.a = moved(t.a, top4);
+  const float d[4] = {v.x - t.a.m, v.y - t.a.m, v.z - t.a.m, v.w - t.a.m};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float p = exp_of(d[e]);
+    t.a.s += p;
+    t.a.t = fmaf(p, bounded(d[e]), t.a.t);
+  }
+}
+
+// The elements i .. i + 3 of a row at its ends: absent ones as -inf.
+__device__ __forceinline__ float4 end_group(const float *x, int i, int vocab) {
   float v[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = i + e >= 0 && i + e < vocab ? x[i + e] : -INFINITY;
   return make_float4(v[0], v[1], v[2], v[3]);
 }
-
 }  // namespace
 
 // Workgroup (part, row): the row's 16-byte groups in `parts` pieces of at most
@@ -159,7 +201,7 @@ pbx_logprobs_part(const float *logits, int64_t stride, int vocab, int parts, int
   __shared__ int chosen[LP_TOP];
   __shared__ int count, n_chosen;
   __shared__ uint64_t limit;
-  __shared__ uint64_t list[LP_TOP * LP_SHARE * 4];
+  __shared__ uint64_t list[LP_TOP * LP_SHARE * 4 + 8];  // (and the cut groups)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x / parts;
   const int part = (int)(blockIdx.x % parts);
@@ -167,30 +209,31 @@ pbx_logprobs_part(const float *logits, int64_t stride, int vocab, int parts, int
   const int skew = (int)((uintptr_t)x / 4 & 3);  // elements of the first group before the row
   const int groups = (int)(((int64_t)vocab + skew + 3) / 4);
   const int g0 = (int)((int64_t)groups * part / parts), g1 = (int)((int64_t)groups * (part + 1) / parts);
-  Sums a = {LOWEST, 0.f, 0.f};
-  float best = -INFINITY;
-  int at = -1;
-  for (int g = g0 + tid; g < g1; g += LP_T) {
-    const float4 v = group_at(x, 4 * g - skew, vocab);
-    const float top4 = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
-    if (top4 > best || at < 0) {
-      best = top4;
-      at = g;
-    }
-    if (top4 > a.m) a = moved(a, top4);
-    const float d[4] = {v.x - a.m, v.y - a.m, v.z - a.m, v.w - a.m};
+  // whole groups, four of a thread under way at once, then a row's cut ones
+  const int full = (vocab + skew) / 4;
+  const int f0 = max(g0, skew ? 1 : 0), f1 = min(g1, full);
+  Share t = {{LOWEST, 0.f, 0.f}, -INFINITY, -1};
+  const float4 *x4 = reinterpret_cast<const float4 *>(x - skew);
+  int g = f0 + tid;
+  for (; g + 3 * LP_T < f1; g += 4 * LP_T) {
+    float4 v[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float p = exp_of(d[e]);
-      a.s += p;
-      a.t = fmaf(p, bounded(d[e]), a.t);
-    }
+    for (int k = 0; k < 4; ++k) v[k] = x4[g + k * LP_T];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) take(t, v[k], g + k * LP_T);
   }
+  for (; g < f1; g += LP_T) take(t, x4[g], g);
+  // (a row that lies within one group is its first)
+  const bool head = skew && g0 == 0, tail = full < groups && g1 == groups && !(skew && full == 0);
+  if (head && tid == 0) take(t, end_group(x, -skew, vocab), 0);
+  if (tail && tid == 64) take(t, end_group(x, 4 * full - skew, vocab), full);
+  Sums a = t.a;
+  const int at = t.at;
   a = join_waves<W>(a, sbuf, wave, lane);
   uint64_t key = 0;
   if (top) {
-    const uint64_t mine = at < 0 ? 0 : key_of(best, (unsigned)at);
-    key = merge_waves<W>(sort_wave(mine, lane), kbuf, wave, lane);
+    const uint64_t mine = at < 0 ? 0 : key_of(t.best, (unsigned)at);
+    key = merge_waves<W>(sort_wave(mine, lane, true), kbuf, wave, lane);
     if (tid == top - 1) limit = key;
     if (tid == 0) count = n_chosen = 0;
     __syncthreads();
@@ -198,23 +241,29 @@ pbx_logprobs_part(const float *logits, int64_t stride, int vocab, int parts, int
     __syncthreads();
     // a group's key is at most those of its largest elements, which have its value
     const float floor_value = limit ? key_value(limit) : -INFINITY;
-    const int share = (g1 - g0 + LP_T - 1) / LP_T, n = n_chosen * share;
-    for (int i = tid; i < n; i += LP_T) {
-      const int g = g0 + chosen[i / share] + i % share * LP_T;
-      if (g >= g1) continue;
-      const int i0 = 4 * g - skew;
-      const float4 v = group_at(x, i0, vocab);
+    auto look = [&](float4 v, int i0) {
       const float u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         if (i0 + e >= 0 && i0 + e < vocab && u[e] >= floor_value)
           list[atomicAdd(&count, 1)] = key_of(u[e], (unsigned)(i0 + e));
+    };
+    const int share = (max(f1 - f0, 0) + LP_T - 1) / LP_T, n = n_chosen * share;
+    for (int i = tid; i < n; i += LP_T) {
+      const int g = f0 + chosen[i / share] + i % share * LP_T;
+      if (g < f1) look(x4[g], 4 * g - skew);
     }
+    if (head && tid == 0) look(end_group(x, -skew, vocab), -skew);
+    if (tail && tid == 64) look(end_group(x, 4 * full - skew, vocab), 4 * full - skew);
     __syncthreads();
     key = 0;
-    for (int i = 64 * wave; i < count; i += LP_T)
-      key = merge_wave(key, sort_wave(i + lane < count ? list[i + lane] : 0, lane), lane);
-    key = merge_waves<W>(key, kbuf, wave, lane);
+    if (count <= 64) {  // nearly always
+      if (!wave) key = sort_wave(lane < count ? list[lane] : 0, lane, true);
+    } else {
+      for (int i = 64 * wave; i < count; i += LP_T)
+        key = merge_wave(key, sort_wave(i + lane < count ? list[i + lane] : 0, lane, false), lane);
+      key = merge_waves<W>(key, kbuf, wave, lane);
+    }
   }
   if (wave) return;
   if (parts == 1) {
@@ -247,7 +296,7 @@ pbx_logprobs_join(const float *logits, int64_t stride, int vocab, int parts, int
   if (top) {
     const int n = parts * top;
     for (int i = 64 * wave; i < n; i += 256)
-      key = merge_wave(key, sort_wave(i + lane < n ? keys[row * n + i + lane] : 0, lane), lane);
+      key = merge_wave(key, sort_wave(i + lane < n ? keys[row * n + i + lane] : 0, lane, false), lane);
     key = merge_waves<4>(key, kbuf, wave, lane);
   }
   if (!wave) answer(out, row, logits + row * stride, vocab, top, a, key, lane);
