@@ -15,8 +15,6 @@ namespace {
 // The maximum before any element: finite, so differences need no special case
 // (an element of -inf adds nothing; a row of nothing else keeps S == 0).
 constexpr float LOWEST = -3.402823466e38f;
-constexpr int LP_T = 512;      // threads of a part
-constexpr int LP_SHARE = 64;   // float4 groups a thread takes at most
 constexpr int LP_TOP = 32;
 
 struct Sums {
@@ -111,20 +109,28 @@ __device__ __forceinline__ uint64_t merge_waves(uint64_t v, uint64_t (*buf)[64],
   return v;
 }
 
+// The sums of all threads of W waves: one maximum first, then each moves once.
 template <int W>
-__device__ __forceinline__ Sums join_waves(Sums a, float (*buf)[3], int wave, int lane) {
+__device__ __forceinline__ Sums join_waves(Sums a, float (*buf)[4], int wave, int lane) {
+  float m = wave_max(a.m);
+  if (lane == 0) buf[wave][0] = m;
+  __syncthreads();
+  m = buf[0][0];
 #pragma unroll
-  for (int off = 32; off >= 1; off /= 2)
-    a = joined(a, {__shfl_xor(a.m, off, 64), __shfl_xor(a.s, off, 64), __shfl_xor(a.t, off, 64)});
+  for (int w = 1; w < W; ++w) m = fmaxf(m, buf[w][0]);
+  a = moved(a, m);
+  const float s = wave_sum(a.s), t = wave_sum(a.t);
   if (lane == 0) {
-    buf[wave][0] = a.m;
-    buf[wave][1] = a.s;
-    buf[wave][2] = a.t;
+    buf[wave][1] = s;
+    buf[wave][2] = t;
   }
   __syncthreads();
-  a = {buf[0][0], buf[0][1], buf[0][2]};
+  a = {m, 0.f, 0.f};
 #pragma unroll
-  for (int w = 1; w < W; ++w) a = joined(a, {buf[w][0], buf[w][1], buf[w][2]});
+  for (int w = 0; w < W; ++w) {
+    a.s += buf[w][1];
+    a.t += buf[w][2];
+  }
   return a;
 }
 
@@ -185,18 +191,16 @@ __device__ __forceinline__ float4 end_group(const float *x, int i, int vocab) {
   for (int e = 0; e < 4; ++e) v[e] = i + e >= 0 && i + e < vocab ? x[i + e] : -INFINITY;
   return make_float4(v[0], v[1], v[2], v[3]);
 }
-}  // namespace
-
 // Workgroup (part, row): the row's 16-byte groups in `parts` pieces of at most
 // LP_SHARE groups a thread.  A thread keeps its sums and its first largest
 // group; the `top` threads with the largest ones hold the piece's `top` largest
 // elements among them (those threads' maxima alone are `top` elements as large),
 // so only their groups, read again, are looked through.
-extern "C" __global__ void __launch_bounds__(LP_T)
-pbx_logprobs_part(const float *logits, int64_t stride, int vocab, int parts, int top, Out out, float *sums,
-                  uint64_t *keys) {
+template <int LP_T, int LP_SHARE>
+__device__ __forceinline__ void part_body(const float *logits, int64_t stride, int vocab, int parts, int top, Out out,
+                                          float *sums, uint64_t *keys) {
   constexpr int W = LP_T / 64;
-  __shared__ float sbuf[W][3];
+  __shared__ float sbuf[W][4];
   __shared__ uint64_t kbuf[W][64];
   __shared__ int chosen[LP_TOP];
   __shared__ int count, n_chosen;
@@ -278,11 +282,26 @@ pbx_logprobs_part(const float *logits, int64_t stride, int vocab, int parts, int
   if (lane < top) keys[blockIdx.x * (int64_t)top + lane] = key;
 }
 
+}  // namespace
+
+// Parts of up to 8 groups a thread (short ones, whose time is their latency) run
+// on four waves, with a merge less; longer ones on eight.
+extern "C" __global__ void __launch_bounds__(256)
+pbx_logprobs_part_256(const float *logits, int64_t stride, int vocab, int parts, int top, Out out, float *sums,
+                      uint64_t *keys) {
+  part_body<256, 8>(logits, stride, vocab, parts, top, out, sums, keys);
+}
+extern "C" __global__ void __launch_bounds__(512)
+pbx_logprobs_part_512(const float *logits, int64_t stride, int vocab, int parts, int top, Out out, float *sums,
+                      uint64_t *keys) {
+  part_body<512, 64>(logits, stride, vocab, parts, top, out, sums, keys);
+}
+
 // A row's parts put together: one workgroup of four waves a row.
 extern "C" __global__ void __launch_bounds__(256)
 pbx_logprobs_join(const float *logits, int64_t stride, int vocab, int parts, int top, Out out, const float *sums,
                   const uint64_t *keys) {
-  __shared__ float sbuf[4][3];
+  __shared__ float sbuf[4][4];
   __shared__ uint64_t kbuf[4][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x;

@@ -4,8 +4,10 @@
 
 #include <algorithm>
 
-// LP_T * LP_SHARE * 4 of pbx_logprobs.hip: elements of one workgroup at most
+// LP_T * LP_SHARE * 4 of pbx_logprobs.hip: elements of one workgroup at most,
+// in the kernels of 512 and of 256 threads
 #define LP_ELEMENTS (512 * 64 * 4)
+#define LP_ELEMENTS_256 (256 * 8 * 4)
 
 struct LogprobsOutHost {  // Out in pbx_logprobs.hip
   const int32_t *targets;
@@ -26,7 +28,7 @@ static int lp_check(pbx_ctx *c, const char *who, int64_t rows, int64_t vocab, in
 // Workgroups a row: as many as fill the GPU twice over, of at least 4096
 // logits, and no more logits than a workgroup can take.
 static int64_t lp_parts(const pbx_ctx *c, int64_t rows, int64_t vocab) {
-  const int64_t least = (vocab + 3 + LP_ELEMENTS - 1) / LP_ELEMENTS;
+  const int64_t least = (vocab + 3 + 8 + LP_ELEMENTS - 1) / LP_ELEMENTS;
   const int64_t fill = 2 * c->cu_count / std::max<int64_t>(rows, 1);
   return std::max(least, std::min<int64_t>({fill, (vocab + 4095) / 4096, 64}));
 }
@@ -63,14 +65,17 @@ extern "C" int pbx_logprobs_dev(pbx_ctx *c, const float *dLogits, int64_t stride
     return pbx_fail(c, PBX_EINVAL, "%s: needs %zu bytes of 16-byte aligned workspace, got %zu", who, need, work_bytes);
   if (rows * parts64 > 0x7fffffff) return pbx_fail(c, PBX_ENOTSUP, "%s: too many rows", who);
   if (hipSetDevice(c->device) != hipSuccess) return pbx_fail(c, PBX_EHIP, "%s: hipSetDevice failed", who);
-  hipFunction_t part = pbx_kernel_by_name(c, "pbx_logprobs_part"), join = pbx_kernel_by_name(c, "pbx_logprobs_join");
+  // (a part has at most a group more than its even share)
+  const bool small = (vocab + 3) / parts64 + 8 <= LP_ELEMENTS_256;
+  const char *name = small ? "pbx_logprobs_part_256" : "pbx_logprobs_part_512";
+  hipFunction_t part = pbx_kernel_by_name(c, name), join = pbx_kernel_by_name(c, "pbx_logprobs_join");
   if (!part || !join) return pbx_fail(c, PBX_ELOAD, "%s: kernels not found", who);
   LogprobsOutHost out{dTargets, dLogp, dEntropy, dTopIds, dTopLogp};
   int v = (int)vocab, parts = (int)parts64;
   void *keys = work;
   float *sums = need ? (float *)((char *)work + 8 * (size_t)rows * parts * top) : nullptr;
   void *args[] = {(void *)&dLogits, &stride, &v, &parts, &top, &out, &sums, &keys};
-  rc = pbx_launch_fn(c, part, "pbx_logprobs_part", dim3((unsigned)(rows * parts)), dim3(512), args, c->stream);
+  rc = pbx_launch_fn(c, part, name, dim3((unsigned)(rows * parts)), dim3(small ? 256 : 512), args, c->stream);
   if (rc || parts == 1) return rc;
   return pbx_launch_fn(c, join, "pbx_logprobs_join", dim3((unsigned)rows), dim3(256), args, c->stream);
 }

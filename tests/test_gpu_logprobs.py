@@ -130,6 +130,20 @@ def test_equal_logits_go_to_the_lower_index(ctx):
     check(ctx, np.zeros((600, 9000), np.float32), np.arange(600), 32)
 
 
+@pytest.mark.parametrize("vocab", [8181, 8184, 8192, 8200, 131061, 131064, 131072, 131080])
+def test_equal_logits_at_a_workgroups_share(ctx, vocab):
+    """Rows of equal logits around the most that a workgroup takes: every element of the chosen threads is a candidate."""
+    for rows in (600, 2):
+        if rows * vocab > 1 << 25:
+            rows = 257  # one workgroup a row as far as it can take one
+        x = np.zeros((rows, vocab), np.float32)
+        logp, ent, ids, tops = run(ctx, x, np.arange(rows), 32)
+        assert np.array_equal(ids, np.tile(np.arange(32), (rows, 1)))
+        # log of a sum of ones: f32 sums of up to 2^17 are exact, the logarithm and the entropy are an ulp off
+        for got, want in ((logp, -np.log(vocab)), (tops, -np.log(vocab)), (ent, np.log(vocab))):
+            assert np.abs(got - want).max() <= 2.0 ** -22 * np.log(vocab)
+
+
 def test_sorted_rows(ctx):
     """Rising and falling rows: every thread's best lies at its end, or at its start."""
     x = np.linspace(-20, 20, 128256, dtype=np.float32)
