@@ -526,6 +526,26 @@ int pbx_logprobs_dev(pbx_ctx *ctx, const float *dLogits, int64_t stride, int64_t
                      float *dEntropy, int32_t *dTopIds, float *dTopLogp, void *work,
                      size_t work_bytes);
 
+/* pbx_model_forward_batch that answers with log probabilities instead of n
+ * rows of logits: row t's target is targets[t] (usually tokens[t + 1]; outside
+ * the vocabulary: NaN).  Host arrays [n_tokens] or [n_tokens][top], as above;
+ * any of the four outputs may be NULL (logp is needed with targets). */
+int pbx_model_logprobs(pbx_model *m, const int32_t *tokens, int n_tokens, int start_pos,
+                       const int32_t *targets, int top, float *logp, float *entropy,
+                       int32_t *top_ids, float *top_logp);
+/* One forward over the rows of a batch of sequences in a paged 8-bit cache (of
+ * the model's context and with its layers, heads and head_dim; the model's own
+ * cache is not touched): tokens[pbx_kv_batch_rows], packed as the batch's rows,
+ * which must be the last of their sequences.  The cache's rotation counts:
+ * PBX_ROPE_PAIRS with the model's rope_theta is the model's own.  Answers for
+ * every row (all_rows), or for the last row of each sequence that has one, in
+ * the batch's order: logits [rows][vocab], next_tokens (argmax), and the four
+ * of pbx_model_logprobs with targets [rows]; each may be NULL.  Blocks until
+ * they are there.  A forward that fails leaves its rows of the cache undefined. */
+int pbx_model_forward_kv(pbx_model *m, pbx_kv_batch *b, const int32_t *tokens, int all_rows,
+                         float *logits, int32_t *next_tokens, const int32_t *targets, int top,
+                         float *logp, float *entropy, int32_t *top_ids, float *top_logp);
+
 #ifdef __cplusplus
 }
 #endif

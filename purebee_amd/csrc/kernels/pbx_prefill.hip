@@ -70,6 +70,19 @@ pbx_rmsnorm_rows(const float *x, const float *w, float *out, int dim, float eps)
   for (int i = threadIdx.x; i < dim; i += blockDim.x) o[i] = xr[i] * inv * w[i];
 }
 
+// The same of the rows that `rows` lists, packed.
+extern "C" __global__ void __launch_bounds__(256)
+pbx_rmsnorm_rows_at(const float *x, const float *w, float *out, int dim, float eps, const int *rows) {
+  __shared__ float red[4];
+  const float *xr = x + (size_t)rows[blockIdx.x] * dim;
+  float ss = 0.f;
+  for (int i = threadIdx.x; i < dim; i += blockDim.x) ss = fmaf(xr[i], xr[i], ss);
+  ss = block_reduce256(ss, false, red);
+  const float inv = 1.0f / sqrtf(ss / (float)dim + eps);
+  float *o = out + (size_t)blockIdx.x * dim;
+  for (int i = threadIdx.x; i < dim; i += blockDim.x) o[i] = xr[i] * inv * w[i];
+}
+
 // RoPE of q and k in place for each row t (position start + t) and append of
 // k, v to the cache (llama.js:159-191, 243-255).  qkv rows: [dim | kv | kv].
 // With part, the rows are first the sum of the KS split-K partials

@@ -208,5 +208,14 @@ int pbx_model_generate_layers(pbx_model *m, int32_t token, int start_pos, int n_
                               int max_layers, int32_t *out_tokens);
 const pbx_model_config *pbx_model_cfg(const pbx_model *m);
 pbx_ctx *pbx_model_ctx(const pbx_model *m);
+// What a forward needs of a batch of the paged KV cache; 0 if b is not a live,
+// set one (pbx_last_error says which).
+struct pbx_kv_batch_view {
+  pbx_ctx *ctx;
+  const pbx_kv_config *cfg;
+  int rows, seqs;            // rows, and sequences that have any
+  const int32_t *last_rows;  // [seqs] on the device: the last row of each
+};
+int pbx_kv_batch_look(const pbx_kv_batch *b, pbx_kv_batch_view *out);
 
 #endif

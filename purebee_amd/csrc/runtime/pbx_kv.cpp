@@ -44,10 +44,10 @@ struct pbx_kv_batch {
   bool set = false;
   bool stale = false;     // positions of it were dropped
   bool captured = false;  // a graph may hold its calls
-  // the plan on the device: blocks, attention items, row positions, page ids
+  // the plan on the device: blocks, attention items, row positions, last rows, page ids
   int32_t *dev = nullptr, *host = nullptr;
   size_t dev_cap = 0, host_cap = 0;
-  size_t at_attn = 0, at_pos = 0, at_table = 0;
+  size_t at_attn = 0, at_pos = 0, at_last = 0, at_table = 0;
   hipEvent_t copied = nullptr;
   float *part = nullptr;  // partial results of split rows
   size_t part_cap = 0;
@@ -293,7 +293,8 @@ static int batch_upload(pbx_kv_batch *b) {
   const size_t n_blocks = p.blocks.size() * sizeof(kv_block_item) / 4;
   b->at_attn = n_blocks;
   b->at_pos = b->at_attn + p.attn.size() * sizeof(kv_attn_item) / 4;
-  b->at_table = b->at_pos + p.row_pos.size();
+  b->at_last = b->at_pos + p.row_pos.size();
+  b->at_table = b->at_last + p.last_rows.size();
   const size_t n = b->at_table + p.table.size();
   if (!n) return PBX_OK;
   if (hipEventSynchronize(b->copied) != hipSuccess)
@@ -305,6 +306,7 @@ static int batch_upload(pbx_kv_batch *b) {
   memcpy(b->host, p.blocks.data(), n_blocks * 4);
   memcpy(b->host + b->at_attn, p.attn.data(), p.attn.size() * sizeof(kv_attn_item));
   memcpy(b->host + b->at_pos, p.row_pos.data(), p.row_pos.size() * 4);
+  memcpy(b->host + b->at_last, p.last_rows.data(), p.last_rows.size() * 4);
   memcpy(b->host + b->at_table, p.table.data(), p.table.size() * 4);
   // per slot and KV head: 16 rows of hdp sums, then their maxima and weights
   const size_t part = (size_t)p.n_slots * kv->cfg.n_kv_heads * 16 * (kv->hdp + 2) * 4;
@@ -379,6 +381,13 @@ static int batch_begin(pbx_kv_batch *b, const char *who, int layer, KvArgsHost *
   *a = {kv->codes + layer * kv->layer_codes, kv->scales + layer * kv->layer_scales, g.n_kv_heads,
         g.n_heads / g.n_kv_heads, g.head_dim, kv->page_shift};
   if (capturing(c)) b->captured = true;
+  return PBX_OK;
+}
+
+int pbx_kv_batch_look(const pbx_kv_batch *b, pbx_kv_batch_view *out) {
+  if (!batch_ok(b)) return pbx_fail(nullptr, PBX_EINVAL, "not a live batch");
+  if (!b->set) return pbx_fail(b->kv->c, PBX_EINVAL, "the batch is not set");
+  *out = {b->kv->c, &b->kv->cfg, b->plan.n_rows, (int)b->plan.last_rows.size(), b->dev + b->at_last};
   return PBX_OK;
 }
 

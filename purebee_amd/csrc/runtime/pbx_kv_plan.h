@@ -83,6 +83,7 @@ struct kv_batch_plan {
   std::vector<kv_block_item> blocks;
   std::vector<kv_attn_item> attn;  // those of u 1, then 2, 4, 8
   std::vector<int32_t> row_pos;  // position of every packed row
+  std::vector<int32_t> last_rows;  // the last row of each sequence that has any
   std::vector<int32_t> table;    // page ids, sequence by sequence
   int n_attn[4] = {0, 0, 0, 0};
   int n_slots = 0, n_joins = 0;
@@ -166,6 +167,7 @@ inline void kv_plan_work(const kv_pages &kv, int groups, int kv_heads, int max_u
   p->blocks.clear();
   p->attn.clear();
   p->row_pos.clear();
+  p->last_rows.clear();
   p->table.clear();
   p->n_slots = p->n_joins = 0;
   p->last = true;
@@ -218,6 +220,7 @@ inline void kv_plan_work(const kv_pages &kv, int groups, int kv_heads, int max_u
       }
     }
     row0 += count;
+    p->last_rows.push_back(row0 - 1);
   }
   for (int c = 0; c < 4; ++c) {
     // the items with the most blocks first, so that none of them is the last to start

@@ -288,6 +288,9 @@ struct pbx_model {
   int32_t *h_tok = nullptr, *h_next = nullptr;
   int32_t *d_tok = nullptr, *d_next = nullptr;
   hipEvent_t tok_ev = nullptr;
+  // log probabilities: the answers, the targets, the kernels' workspace
+  void *blp = nullptr;
+  size_t blp_cap = 0;
   // [logits_cap][64]: per row, the running maximum key and the count of
   // pbx_argmax_rows (zero between launches)
   uint64_t *bkeys = nullptr;
@@ -1260,7 +1263,7 @@ static void model_release(pbx_model *m) {
     if (p) hipFree(p);
   for (void *p : {(void *)m->bx, (void *)m->bxn, (void *)m->bqkv, (void *)m->battn,
                   (void *)m->bgu, (void *)m->bh, (void *)m->btmp, (void *)m->blogits,
-                  (void *)m->bnext, (void *)m->bkeys, (void *)m->mr_cell,
+                  (void *)m->bnext, (void *)m->bkeys, (void *)m->mr_cell, m->blp,
                   m->g16, m->g16lo,
                   (void *)m->ginv, (void *)m->gpart})
     if (p) hipFree(p);
@@ -1534,7 +1537,7 @@ static int grow(pbx_model *m, void **p, size_t bytes) {
 #define MR_MAX 5
 #define MR_XS 15  // K slices of the split rows GEMV at most (4-bit counts)
 
-static int ensure_batch(pbx_model *m, int rows, bool all_logits) {
+static int ensure_batch(pbx_model *m, int rows, int logit_rows) {
   const pbx_model_config &g = m->cfg;
   int rc = PBX_OK;
   if (!m->mr_cell) {
@@ -1574,18 +1577,18 @@ static int ensure_batch(pbx_model *m, int rows, bool all_logits) {
     }
     m->batch_cap = rows;
   }
-  if (all_logits && rows > m->logits_cap) {
-    if ((rc = grow(m, (void **)&m->blogits, (size_t)rows * g.vocab_size * 4)) ||
-        (rc = grow(m, (void **)&m->bkeys, (size_t)rows * 64 * 8))) {
+  if (logit_rows > m->logits_cap) {
+    if ((rc = grow(m, (void **)&m->blogits, (size_t)logit_rows * g.vocab_size * 4)) ||
+        (rc = grow(m, (void **)&m->bkeys, (size_t)logit_rows * 64 * 8))) {
       m->logits_cap = 0;
       return rc;
     }
     // pbx_argmax_rows' cells start at zero (and each launch leaves them so)
-    if (hipMemsetAsync(m->bkeys, 0, (size_t)rows * 64 * 8, m->c->stream) != hipSuccess) {
+    if (hipMemsetAsync(m->bkeys, 0, (size_t)logit_rows * 64 * 8, m->c->stream) != hipSuccess) {
       m->logits_cap = 0;
       return pbx_fail(m->c, PBX_EHIP, "model: clearing the argmax cells failed");
     }
-    m->logits_cap = rows;
+    m->logits_cap = logit_rows;
   }
   return PBX_OK;
 }
@@ -1842,10 +1845,20 @@ static int fused_residual_norm(pbx_model *m, const pbx_gemm_plan *p, int M, int 
   return launch_k(m, "pbx_gemm_prep_rms", dim3(Mpad), dim3(256), args);
 }
 
+// Rotation, append and attention of layer l's q|k|v rows in a paged cache.
+static int kv_attention(pbx_model *m, pbx_kv_batch *kv, int l) {
+  const int64_t rl = m->qkv_rows;
+  const float *k = m->bqkv + m->cfg.dim, *v = k + m->kvdim;
+  const int rc = pbx_kv_append_dev(kv, l, m->bqkv, rl, k, rl, v, rl, m->bqkv, rl);
+  return rc ? rc : pbx_kv_attention_dev(kv, l, m->bqkv, rl, 0.f, m->battn, m->cfg.dim);
+}
+
 // Runs the first nl layers of the stack over n rows (the KV cache of later
 // layers is not written, as llama-streaming.js:765-792 with maxLayers);
-// leaves the residual stream in m->bx.
-static int batch_layers(pbx_model *m, const int32_t *tokens, int n, int start, int nl) {
+// leaves the residual stream in m->bx.  With kv, the rows are those of a batch
+// of sequences in a paged cache (start does not count).
+static int batch_layers(pbx_model *m, const int32_t *tokens, int n, int start, int nl,
+                        pbx_kv_batch *kv = nullptr) {
   pbx_ctx *c = m->c;
   const pbx_model_config &g = m->cfg;
   int rc;
@@ -1888,31 +1901,37 @@ static int batch_layers(pbx_model *m, const int32_t *tokens, int n, int start, i
       Layer &L = m->layers[l];
       float *kc = m->kcache + l * layer_kv, *vc = m->vcache + l * layer_kv;
       if ((rc = fused_gemm(m, L.wqkv, P.qkv, m->bqkv, false))) return rc;
-      {
-        float *qkv = m->bqkv, *rope = m->rope;
-        const float *part = P.qkv.KS > 1 ? m->gpart : nullptr;
-        int st = start, nh = g.n_heads, nkv = g.n_kv_heads, hd = g.head_dim, ks = P.qkv.KS;
-        void *args[] = {&qkv, &kc, &vc, &rope, &st, &nh, &nkv, &hd, (void *)&part, &ks};
-        if ((rc = launch_k(m, "pbx_rope_append_rows", dim3(n), dim3(256), args))) return rc;
-      }
-      {
-        float *qkv = m->bqkv, *out = m->battn;
-        int st = start, nh = g.n_heads, nkv = g.n_kv_heads, hd = g.head_dim, rows = n;
-        float scale = (float)(1.0 / sqrt((double)g.head_dim));
-        if (g.head_dim <= 64 && n >= 16) {
-          void *args[] = {&qkv, &kc, &vc, &out, &st, &rows, &nh, &nkv, &hd, &scale};
-          const bool mf = g.head_dim % 16 == 0;
-          rc = launch_k(m, mf ? prefill_attention_mfma() : "pbx_attention_tiled",
-                        dim3(g.n_heads, (n + 63) / 64), dim3(mf ? prefill_attention_threads() : 256),
-                        args);
-        } else {
-          void *args[] = {&qkv, &kc, &vc, &out, &st, &nh, &nkv, &hd, &scale};
-          if (g.head_dim <= 64)
-            rc = launch_k(m, "pbx_attention_head_rows", dim3(g.n_heads, n), dim3(512), args);
-          else
-            rc = launch_k(m, "pbx_attention_rows", dim3(g.n_heads, n), dim3(256), args);
+      if (kv) {
+        if ((P.qkv.KS > 1 && (rc = fused_reduce(m, P.qkv, (int)L.wqkv->N, m->bqkv, false))) ||
+            (rc = kv_attention(m, kv, l)))
+          return rc;
+      } else {
+        {
+          float *qkv = m->bqkv, *rope = m->rope;
+          const float *part = P.qkv.KS > 1 ? m->gpart : nullptr;
+          int st = start, nh = g.n_heads, nkv = g.n_kv_heads, hd = g.head_dim, ks = P.qkv.KS;
+          void *args[] = {&qkv, &kc, &vc, &rope, &st, &nh, &nkv, &hd, (void *)&part, &ks};
+          if ((rc = launch_k(m, "pbx_rope_append_rows", dim3(n), dim3(256), args))) return rc;
         }
-        if (rc) return rc;
+        {
+          float *qkv = m->bqkv, *out = m->battn;
+          int st = start, nh = g.n_heads, nkv = g.n_kv_heads, hd = g.head_dim, rows = n;
+          float scale = (float)(1.0 / sqrt((double)g.head_dim));
+          if (g.head_dim <= 64 && n >= 16) {
+            void *args[] = {&qkv, &kc, &vc, &out, &st, &rows, &nh, &nkv, &hd, &scale};
+            const bool mf = g.head_dim % 16 == 0;
+            rc = launch_k(m, mf ? prefill_attention_mfma() : "pbx_attention_tiled",
+                          dim3(g.n_heads, (n + 63) / 64), dim3(mf ? prefill_attention_threads() : 256),
+                          args);
+          } else {
+            void *args[] = {&qkv, &kc, &vc, &out, &st, &nh, &nkv, &hd, &scale};
+            if (g.head_dim <= 64)
+              rc = launch_k(m, "pbx_attention_head_rows", dim3(g.n_heads, n), dim3(512), args);
+            else
+              rc = launch_k(m, "pbx_attention_rows", dim3(g.n_heads, n), dim3(256), args);
+          }
+          if (rc) return rc;
+        }
       }
       {
         float *x = m->battn;
@@ -1953,7 +1972,8 @@ static int batch_layers(pbx_model *m, const int32_t *tokens, int n, int start, i
     // and the cache append (no pbx_rope_append_rows)
     const bool mr = rows_int && n <= MR_MAX && (int)L.wqkv->B == 64 && g.head_dim <= 64 &&
                     g.head_dim % 2 == 0 && g.dim % 16 == 0 && m->kvdim % 16 == 0;
-    if (mr) {
+    const bool mr_rope = mr && !kv;  // that kernel appends to the model's own cache
+    if (mr_rope) {
       const MrShape qs = mr_shape("qkv", 1, 8);
       if ((rc = launch_mr(m, qs.name("qkvr").c_str(), L.wqkv, m->bx, L.attn_norm, m->bqkv, n,
                           qs.rw, qs.ks, l, start)))
@@ -1966,37 +1986,41 @@ static int batch_layers(pbx_model *m, const int32_t *tokens, int n, int start, i
       if ((rc = rmsnorm_rows(m, m->bx, L.attn_norm, m->bxn, n))) return rc;
       if ((rc = linear_rows(m, L.wqkv, m->bxn, n, m->bqkv, false))) return rc;
     }
-    if (!mr) {
-      float *qkv = m->bqkv, *rope = m->rope;
-      int st = start, nh = g.n_heads, nkv = g.n_kv_heads, hd = g.head_dim;
-      const float *part = nullptr;
-      int ks = 1;
-      void *args[] = {&qkv, &kc, &vc, &rope, &st, &nh, &nkv, &hd, (void *)&part, &ks};
-      if ((rc = launch_k(m, "pbx_rope_append_rows", dim3(n), dim3(256), args))) return rc;
-    }
-    {
-      float *qkv = m->bqkv, *out = m->battn;
-      int st = start, nh = g.n_heads, nkv = g.n_kv_heads, hd = g.head_dim, rows = n;
-      float scale = (float)(1.0 / sqrt((double)g.head_dim));
-      // 64-row query tiles sharing K/V tiles in LDS pay off from 16 rows; a
-      // few rows (speculative verify) spread better one workgroup per row.
-      if (g.head_dim <= 64 && n >= 16) {
-        // MFMA kernel for head dims that are a multiple of 16, else fp32 FMAs
-        void *args[] = {&qkv, &kc, &vc, &out, &st, &rows, &nh, &nkv, &hd, &scale};
-        const bool mf = g.head_dim % 16 == 0;
-        rc = launch_k(m, mf ? prefill_attention_mfma() : "pbx_attention_tiled",
-                      dim3(g.n_heads, (n + 63) / 64), dim3(mf ? prefill_attention_threads() : 256),
-                      args);
-      } else {
-        void *args[] = {&qkv, &kc, &vc, &out, &st, &nh, &nkv, &hd, &scale};
-        // head_dim <= 64: the decode kernel's flash layout per (head, row);
-        // the generic one-workgroup-per-(head, row) kernel otherwise
-        if (g.head_dim <= 64)
-          rc = launch_k(m, "pbx_attention_head_rows", dim3(g.n_heads, n), dim3(512), args);
-        else
-          rc = launch_k(m, "pbx_attention_rows", dim3(g.n_heads, n), dim3(256), args);
+    if (kv) {
+      if ((rc = kv_attention(m, kv, l))) return rc;
+    } else {
+      if (!mr_rope) {
+        float *qkv = m->bqkv, *rope = m->rope;
+        int st = start, nh = g.n_heads, nkv = g.n_kv_heads, hd = g.head_dim;
+        const float *part = nullptr;
+        int ks = 1;
+        void *args[] = {&qkv, &kc, &vc, &rope, &st, &nh, &nkv, &hd, (void *)&part, &ks};
+        if ((rc = launch_k(m, "pbx_rope_append_rows", dim3(n), dim3(256), args))) return rc;
       }
-      if (rc) return rc;
+      {
+        float *qkv = m->bqkv, *out = m->battn;
+        int st = start, nh = g.n_heads, nkv = g.n_kv_heads, hd = g.head_dim, rows = n;
+        float scale = (float)(1.0 / sqrt((double)g.head_dim));
+        // 64-row query tiles sharing K/V tiles in LDS pay off from 16 rows; a
+        // few rows (speculative verify) spread better one workgroup per row.
+        if (g.head_dim <= 64 && n >= 16) {
+          // MFMA kernel for head dims that are a multiple of 16, else fp32 FMAs
+          void *args[] = {&qkv, &kc, &vc, &out, &st, &rows, &nh, &nkv, &hd, &scale};
+          const bool mf = g.head_dim % 16 == 0;
+          rc = launch_k(m, mf ? prefill_attention_mfma() : "pbx_attention_tiled",
+                        dim3(g.n_heads, (n + 63) / 64), dim3(mf ? prefill_attention_threads() : 256),
+                        args);
+        } else {
+          void *args[] = {&qkv, &kc, &vc, &out, &st, &nh, &nkv, &hd, &scale};
+          // head_dim <= 64: the decode kernel's flash layout per (head, row);
+          // the generic one-workgroup-per-(head, row) kernel otherwise
+          if (g.head_dim <= 64)
+            rc = launch_k(m, "pbx_attention_head_rows", dim3(g.n_heads, n), dim3(512), args);
+          else
+            rc = launch_k(m, "pbx_attention_rows", dim3(g.n_heads, n), dim3(256), args);
+        }
+        if (rc) return rc;
+      }
     }
     if (mr && (int)L.wd->B == 256) {
       // 8 or 16 waves a workgroup (K slices across waves): the dots of a wave
@@ -2043,7 +2067,7 @@ static int batch_layers(pbx_model *m, const int32_t *tokens, int n, int start, i
 // and argmax on the last row, which leave the device state at
 // (start + n, next token) as n sequential steps would.
 static int prefill_batched(pbx_model *m, const int32_t *tokens, int n, int start, int nl) {
-  int rc = ensure_batch(m, n, false);
+  int rc = ensure_batch(m, n, 0);
   if (rc) return rc;
   if (!m->ops_ready && (rc = build_ops(m))) return rc;
   if ((rc = batch_layers(m, tokens, n, start, nl))) return rc;
@@ -2113,66 +2137,192 @@ extern "C" int pbx_model_forward_layers(pbx_model *m, const int32_t *tokens, int
   return PBX_OK;
 }
 
-extern "C" int pbx_model_forward_batch(pbx_model *m, const int32_t *tokens, int n_tokens,
-                                       int start_pos, float *logits, int32_t *next_tokens) {
-  if (!model_ok(m))
-    return pbx_fail(nullptr, PBX_EINVAL, "pbx_model_forward_batch: not a live model");
-  pbx_ctx *c = m->c;
-  const pbx_model_config &g = m->cfg;
-  if (!tokens || n_tokens <= 0)
-    return pbx_fail(c, PBX_EINVAL, "pbx_model_forward_batch: need at least one token");
-  if (n_tokens > 65535)
-    return pbx_fail(c, PBX_ENOTSUP, "pbx_model_forward_batch: %d rows exceed 65535", n_tokens);
-  if (start_pos < 0 || (int64_t)start_pos + n_tokens > g.max_seq)
-    return pbx_fail(c, PBX_EINVAL,
-                    "pbx_model_forward_batch: positions [%d, %lld) exceed max_seq %d", start_pos,
-                    (long long)start_pos + n_tokens, g.max_seq);
-  for (int t = 0; t < n_tokens; ++t)
-    if (tokens[t] < 0 || tokens[t] >= g.vocab_size)
-      return pbx_fail(c, PBX_EINVAL, "pbx_model_forward_batch: token %d out of range [0, %d)",
-                      tokens[t], g.vocab_size);
-  int rc = check_complete(m);
-  if (rc) return rc;
-  if (hipSetDevice(c->device) != hipSuccess)
-    return pbx_fail(c, PBX_EHIP, "pbx_model_forward_batch: hipSetDevice failed");
-  const int n = n_tokens;
-  if ((rc = ensure_batch(m, n, true))) return rc;
-  if ((rc = batch_layers(m, tokens, n, start_pos, g.n_layers))) return rc;
+// The LM head over the n rows of the residual stream that `at` lists on the
+// device (null: the first n), into m->blogits.
+static int head_rows(pbx_model *m, int n, const int32_t *at) {
+  int rc;
   const pbx_weight *head = m->output ? m->output : m->embd;
-  if (n <= ROWS_MAX && rows_int_ok(m)) {
+  if (!at && n <= ROWS_MAX && rows_int_ok(m)) {
     // RMSNorm + LM head over the rows: a Q4_0 head at K = 2048 on the rows
     // kernel, 8 tiles a workgroup (5 rows: 46 us against 64 on the skinny
     // MFMA kernel, which takes the other heads)
     const bool mr_head = head->type == PBX_TYPE_Q4_0 && head->B == 64 && n <= MR_MAX;
-    if (mr_head) {
-      const MrShape hs = mr_shape("lm_head", 8, 1);
-      if ((rc = launch_mr(m, hs.name("store").c_str(), head, m->bx, m->out_norm, m->blogits, n,
-                          hs.rw, hs.ks)))
-        return rc;
-    } else if ((rc = launch_skinny(m, "pbx_sk_q4_store", head, m->bx, m->out_norm, m->blogits, n)))
-      return rc;
+    if (!mr_head) return launch_skinny(m, "pbx_sk_q4_store", head, m->bx, m->out_norm, m->blogits, n);
+    const MrShape hs = mr_shape("lm_head", 8, 1);
+    return launch_mr(m, hs.name("store").c_str(), head, m->bx, m->out_norm, m->blogits, n, hs.rw,
+                     hs.ks);
+  }
+  if (at) {
+    const float *x = m->bx, *w = m->out_norm;
+    int dim = m->cfg.dim;
+    float eps = m->cfg.rms_eps;
+    void *args[] = {(void *)&x, (void *)&w, &m->bxn, &dim, &eps, (void *)&at};
+    rc = launch_k(m, "pbx_rmsnorm_rows_at", dim3(n), dim3(256), args);
   } else {
-    if ((rc = rmsnorm_rows(m, m->bx, m->out_norm, m->bxn, n))) return rc;
-    if ((rc = linear_rows(m, head, m->bxn, n, m->blogits, false))) return rc;
+    rc = rmsnorm_rows(m, m->bx, m->out_norm, m->bxn, n);
   }
-  {
-    // P workgroups per row, ~2048 columns each, meeting in the row's cells
-    const float *lg = m->blogits;
-    int vocab = g.vocab_size;
-    int P = std::min(64, (g.vocab_size + 2047) / 2048);
-    int chunk = (g.vocab_size + P - 1) / P;
-    unsigned long long *cells = (unsigned long long *)m->bkeys;
-    int stride = 64;
-    int *out = next_tokens ? m->d_next : m->bnext;  // straight into host memory
-    void *a1[] = {(void *)&lg, &vocab, &chunk, &cells, &stride, &P, &out};
-    if ((rc = launch_k(m, "pbx_argmax_rows", dim3(P, n), dim3(256), a1))) return rc;
-  }
+  return rc ? rc : linear_rows(m, head, m->bxn, n, m->blogits, false);
+}
+
+// The argmax of each of n rows of m->blogits into out.
+static int argmax_rows(pbx_model *m, int n, int *out) {
+  // P workgroups per row, ~2048 columns each, meeting in the row's cells
+  const float *lg = m->blogits;
+  int vocab = m->cfg.vocab_size;
+  int P = std::min(64, (vocab + 2047) / 2048);
+  int chunk = (vocab + P - 1) / P;
+  unsigned long long *cells = (unsigned long long *)m->bkeys;
+  int stride = 64;
+  void *a1[] = {(void *)&lg, &vocab, &chunk, &cells, &stride, &P, &out};
+  return launch_k(m, "pbx_argmax_rows", dim3(P, n), dim3(256), a1);
+}
+
+// What a caller wants to know of the rows' distributions (host arrays).
+struct LogprobsWanted {
+  const int32_t *targets;
+  int top;
+  float *logp, *entropy;
+  int32_t *top_ids;
+  float *top_logp;
+  bool any() const { return logp || entropy || top_ids || top_logp; }
+};
+
+static int check_logprobs(pbx_model *m, const char *who, const LogprobsWanted &w) {
+  if (!w.targets != !w.logp)
+    return pbx_fail(m->c, PBX_EINVAL, "%s: targets and logp come together", who);
+  if (w.top < 0 || w.top > PBX_LOGPROBS_TOP_MAX || w.top > m->cfg.vocab_size)
+    return pbx_fail(m->c, PBX_EINVAL, "%s: top %d outside [0, min(%d, vocab)]", who, w.top, PBX_LOGPROBS_TOP_MAX);
+  return PBX_OK;
+}
+
+// Enqueues the log probabilities of n rows of m->blogits; the answers lie in
+// m->blp: log probabilities, entropies, top ids, top log probabilities.
+static int logprobs_rows(pbx_model *m, int n, const LogprobsWanted &w) {
+  pbx_ctx *c = m->c;
+  const size_t V = m->cfg.vocab_size, T = w.top, N = n;
+  size_t ws = 0;
+  int rc = pbx_logprobs_workspace(c, n, (int64_t)V, w.top, &ws);
+  if (rc) return rc;
+  const size_t out = (N * (2 + 2 * T) + 3) / 4 * 4, tgt = (N + 3) / 4 * 4;  // in 4-byte words
+  if ((rc = pbx_ensure_dev(c, &m->blp, &m->blp_cap, (out + tgt) * 4 + ws))) return rc;
+  float *lp = (float *)m->blp, *ent = lp + N, *tl = ent + N + N * T;
+  int32_t *ids = (int32_t *)(ent + N), *dt = (int32_t *)(lp + out);
+  if (w.targets && hipMemcpyAsync(dt, w.targets, N * 4, hipMemcpyHostToDevice, c->stream) != hipSuccess)
+    return pbx_fail(c, PBX_EHIP, "model: target copy failed");
+  return pbx_logprobs_dev(c, m->blogits, 0, n, (int64_t)V, w.targets ? dt : nullptr, w.top, w.logp ? lp : nullptr,
+                          ent, T ? ids : nullptr, T ? tl : nullptr, lp + out + tgt, ws);
+}
+
+// Copies the answers out (after logprobs_rows, before the synchronisation).
+static int logprobs_fetch(pbx_model *m, int n, const LogprobsWanted &w) {
+  const size_t N = n, T = w.top;
+  const float *lp = (const float *)m->blp, *ent = lp + N;
+  const struct {
+    void *to;
+    const void *from;
+    size_t bytes;
+  } parts[] = {{w.logp, lp, N * 4}, {w.entropy, ent, N * 4}, {w.top_ids, ent + N, N * T * 4},
+               {w.top_logp, ent + N + N * T, N * T * 4}};
+  for (const auto &p : parts)
+    if (p.to && p.bytes &&
+        hipMemcpyAsync(p.to, p.from, p.bytes, hipMemcpyDeviceToHost, m->c->stream) != hipSuccess)
+      return pbx_fail(m->c, PBX_EHIP, "model: log probability copy failed");
+  return PBX_OK;
+}
+
+// The shared checks and body of the forwards that answer for every row of a
+// batch at start_pos.
+static int forward_rows(pbx_model *m, const char *who, const int32_t *tokens, int n_tokens,
+                        int start_pos, float *logits, int32_t *next_tokens, const LogprobsWanted &w) {
+  pbx_ctx *c = m->c;
+  const pbx_model_config &g = m->cfg;
+  if (!tokens || n_tokens <= 0)
+    return pbx_fail(c, PBX_EINVAL, "%s: need at least one token", who);
+  if (n_tokens > 65535)
+    return pbx_fail(c, PBX_ENOTSUP, "%s: %d rows exceed 65535", who, n_tokens);
+  if (start_pos < 0 || (int64_t)start_pos + n_tokens > g.max_seq)
+    return pbx_fail(c, PBX_EINVAL, "%s: positions [%d, %lld) exceed max_seq %d", who, start_pos,
+                    (long long)start_pos + n_tokens, g.max_seq);
+  for (int t = 0; t < n_tokens; ++t)
+    if (tokens[t] < 0 || tokens[t] >= g.vocab_size)
+      return pbx_fail(c, PBX_EINVAL, "%s: token %d out of range [0, %d)", who, tokens[t],
+                      g.vocab_size);
+  int rc = check_complete(m);
+  if (rc) return rc;
+  if (hipSetDevice(c->device) != hipSuccess)
+    return pbx_fail(c, PBX_EHIP, "%s: hipSetDevice failed", who);
+  const int n = n_tokens;
+  if ((rc = ensure_batch(m, n, n))) return rc;
+  if ((rc = batch_layers(m, tokens, n, start_pos, g.n_layers))) return rc;
+  if ((rc = head_rows(m, n, nullptr))) return rc;
+  // the argmax straight into host memory when it is wanted there
+  if ((next_tokens || !w.any()) && (rc = argmax_rows(m, n, next_tokens ? m->d_next : m->bnext)))
+    return rc;
+  if (w.any() && ((rc = logprobs_rows(m, n, w)) || (rc = logprobs_fetch(m, n, w)))) return rc;
   if (logits && hipMemcpyAsync(logits, m->blogits, (size_t)n * g.vocab_size * 4,
                                hipMemcpyDeviceToHost, c->stream) != hipSuccess)
-    return pbx_fail(c, PBX_EHIP, "pbx_model_forward_batch: logits copy failed");
+    return pbx_fail(c, PBX_EHIP, "%s: logits copy failed", who);
   if (hipStreamSynchronize(c->stream) != hipSuccess)
-    return pbx_fail(c, PBX_EHIP, "pbx_model_forward_batch: forward failed on the device");
+    return pbx_fail(c, PBX_EHIP, "%s: forward failed on the device", who);
   if (next_tokens) memcpy(next_tokens, m->h_next, (size_t)n * 4);
+  return PBX_OK;
+}
+
+extern "C" int pbx_model_forward_batch(pbx_model *m, const int32_t *tokens, int n_tokens,
+                                       int start_pos, float *logits, int32_t *next_tokens) {
+  if (!model_ok(m))
+    return pbx_fail(nullptr, PBX_EINVAL, "pbx_model_forward_batch: not a live model");
+  return forward_rows(m, "pbx_model_forward_batch", tokens, n_tokens, start_pos, logits, next_tokens, {});
+}
+
+extern "C" int pbx_model_logprobs(pbx_model *m, const int32_t *tokens, int n_tokens, int start_pos,
+                                  const int32_t *targets, int top, float *logp, float *entropy,
+                                  int32_t *top_ids, float *top_logp) {
+  const char *who = "pbx_model_logprobs";
+  if (!model_ok(m)) return pbx_fail(nullptr, PBX_EINVAL, "%s: not a live model", who);
+  const LogprobsWanted w{targets, top, logp, entropy, top_ids, top_logp};
+  const int rc = check_logprobs(m, who, w);
+  return rc ? rc : forward_rows(m, who, tokens, n_tokens, start_pos, nullptr, nullptr, w);
+}
+
+extern "C" int pbx_model_forward_kv(pbx_model *m, pbx_kv_batch *b, const int32_t *tokens, int all_rows,
+                                    float *logits, int32_t *next_tokens, const int32_t *targets, int top,
+                                    float *logp, float *entropy, int32_t *top_ids, float *top_logp) {
+  const char *who = "pbx_model_forward_kv";
+  if (!model_ok(m)) return pbx_fail(nullptr, PBX_EINVAL, "%s: not a live model", who);
+  pbx_ctx *c = m->c;
+  const pbx_model_config &g = m->cfg;
+  pbx_kv_batch_view v;
+  int rc = pbx_kv_batch_look(b, &v);
+  if (rc) return pbx_fail(c, rc, "%s: not a live batch that is set", who);
+  const LogprobsWanted w{targets, top, logp, entropy, top_ids, top_logp};
+  if ((rc = check_logprobs(m, who, w))) return rc;
+  if (v.ctx != c) return pbx_fail(c, PBX_EINVAL, "%s: model and cache of different contexts", who);
+  if (v.cfg->n_layers != g.n_layers || v.cfg->n_heads != g.n_heads || v.cfg->n_kv_heads != g.n_kv_heads ||
+      v.cfg->head_dim != g.head_dim)
+    return pbx_fail(c, PBX_EINVAL, "%s: the cache is of another shape than the model", who);
+  const int n = v.rows, rows = all_rows ? n : v.seqs;
+  if (n > 65535) return pbx_fail(c, PBX_ENOTSUP, "%s: %d rows exceed 65535", who, n);
+  if (!n) return PBX_OK;
+  if (!tokens) return pbx_fail(c, PBX_EINVAL, "%s: tokens is NULL", who);
+  for (int t = 0; t < n; ++t)
+    if (tokens[t] < 0 || tokens[t] >= g.vocab_size)
+      return pbx_fail(c, PBX_EINVAL, "%s: token %d out of range [0, %d)", who, tokens[t], g.vocab_size);
+  if ((rc = check_complete(m))) return rc;
+  if (hipSetDevice(c->device) != hipSuccess)
+    return pbx_fail(c, PBX_EHIP, "%s: hipSetDevice failed", who);
+  const bool heads = logits || next_tokens || w.any();
+  if ((rc = ensure_batch(m, n, heads ? rows : 0)) || (rc = batch_layers(m, tokens, n, 0, g.n_layers, b)))
+    return rc;
+  if (heads && (rc = head_rows(m, rows, rows == n ? nullptr : v.last_rows))) return rc;
+  if (next_tokens && (rc = argmax_rows(m, rows, m->d_next))) return rc;
+  if (w.any() && ((rc = logprobs_rows(m, rows, w)) || (rc = logprobs_fetch(m, rows, w)))) return rc;
+  if (logits && hipMemcpyAsync(logits, m->blogits, (size_t)rows * g.vocab_size * 4, hipMemcpyDeviceToHost,
+                               c->stream) != hipSuccess)
+    return pbx_fail(c, PBX_EHIP, "%s: logits copy failed", who);
+  if (hipStreamSynchronize(c->stream) != hipSuccess)
+    return pbx_fail(c, PBX_EHIP, "%s: forward failed on the device", who);
+  if (next_tokens) memcpy(next_tokens, m->h_next, (size_t)rows * 4);
   return PBX_OK;
 }
 

@@ -134,6 +134,15 @@ class HipLlamaRuntime {
     return addon.modelForward(this._model, Int32Array.from(tokenIds), startPos).logits;
   }
 
+  /**
+   * Log probabilities instead of logits, of every position of one batched pass:
+   * {logp [n] (of targets; null without), entropy [n], topIds, topLogp [n*top]}.
+   */
+  logprobs(tokenIds, startPos, { targets = null, top = 0 } = {}) {
+    return addon.modelLogprobs(this._model, Int32Array.from(tokenIds), startPos,
+                               targets && Int32Array.from(targets), top);
+  }
+
   /** Every position's logits in one batched pass: {logits [n*vocab], next [n]}. */
   forwardAll(tokenIds, startPos) {
     return addon.modelForwardBatch(this._model, Int32Array.from(tokenIds), startPos);

@@ -626,6 +626,44 @@ napi_value Speculative(napi_env env, napi_callback_info info) {
   return o;
 }
 
+// modelLogprobs(model, tokens, startPos, targets = null, top = 0)
+//   -> {logp: Float32Array | null, entropy: Float32Array, topIds: Int32Array,
+//       topLogp: Float32Array}
+napi_value ModelLogprobs(napi_env env, napi_callback_info info) {
+  if (!need_ctx(env)) return nullptr;
+  napi_value argv[5];
+  get_args(env, info, 5, argv);
+  ModelRef *r = get_model(env, argv[0]);
+  std::vector<int32_t> tokens, targets;
+  int64_t start = 0, top = 0;
+  const bool with = !is_nullish(env, argv[3]);
+  if (!r || !get_tokens(env, argv[1], &tokens) || !get_i64(env, argv[2], &start) ||
+      (with && (!get_tokens(env, argv[3], &targets) || targets.size() != tokens.size())) ||
+      (!is_nullish(env, argv[4]) && !get_i64(env, argv[4], &top)) || top < 0 ||
+      top > PBX_LOGPROBS_TOP_MAX)
+    return throw_msg(env, "modelLogprobs(model, tokens, startPos, targets, top): bad arguments");
+  const size_t n = tokens.size();
+  float *lp = nullptr, *ent, *tl;
+  int32_t *ids;
+  napi_value vlp, vent = new_f32(env, n, &ent), vids = new_i32(env, n * top, &ids),
+                  vtl = new_f32(env, n * top, &tl);
+  if (with)
+    vlp = new_f32(env, n, &lp);
+  else
+    napi_get_null(env, &vlp);
+  if (!vlp || !vent || !vids || !vtl) return throw_msg(env, "modelLogprobs: out of memory");
+  int rc = pbx_model_logprobs(r->m, tokens.data(), (int)n, (int)start, with ? targets.data() : nullptr,
+                              (int)top, lp, ent, ids, tl);
+  if (rc) return throw_pbx(env, rc, "modelLogprobs");
+  napi_value o;
+  napi_create_object(env, &o);
+  napi_set_named_property(env, o, "logp", vlp);
+  napi_set_named_property(env, o, "entropy", vent);
+  napi_set_named_property(env, o, "topIds", vids);
+  napi_set_named_property(env, o, "topLogp", vtl);
+  return o;
+}
+
 // selfSpeculative(model, prompt, maxTokens, draftLayers = 4, draftCount = 4, eosIds = [2],
 //                 batched = true)
 //   -> {tokens: Int32Array, rounds, drafted, accepted, prefillMs, decodeMs}
@@ -688,6 +726,7 @@ napi_value ModuleInit(napi_env env, napi_value exports) {
              {"modelSetTensor", ModelSetTensor},
              {"modelForward", ModelForward},
              {"modelForwardBatch", ModelForwardBatch},
+             {"modelLogprobs", ModelLogprobs},
              {"modelGenerate", ModelGenerate},
              {"modelRollback", ModelRollback},
              {"modelReset", ModelReset},

@@ -48,7 +48,7 @@ EXPORTS = (
     "pbx_kv_create", "pbx_kv_free", "pbx_kv_info", "pbx_kv_length", "pbx_kv_truncate",
     "pbx_kv_batch_create", "pbx_kv_batch_free", "pbx_kv_batch_set", "pbx_kv_batch_rows",
     "pbx_kv_append_dev", "pbx_kv_attention_dev", "pbx_kv_read_dev",
-    "pbx_logprobs_workspace", "pbx_logprobs_dev",
+    "pbx_logprobs_workspace", "pbx_logprobs_dev", "pbx_model_logprobs", "pbx_model_forward_kv",
 )
 
 # Position rotations of a KvCache (PBX_ROPE_*).
@@ -221,6 +221,10 @@ def load_library():
                                                   ctypes.POINTER(ctypes.c_size_t)]),
         "pbx_logprobs_dev": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i64, _vp, ctypes.c_int, _vp, _vp,
                                             _vp, _vp, _vp, ctypes.c_size_t]),
+        "pbx_model_logprobs": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int,
+                                              _vp, _vp, _vp, _vp]),
+        "pbx_model_forward_kv": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, _vp, _vp, _vp,
+                                                ctypes.c_int, _vp, _vp, _vp, _vp]),
         "pbx_speculative_generate": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, ctypes.c_int,
                                                     ctypes.c_int, _vp, ctypes.c_int, ctypes.c_int,
                                                     _vp, ctypes.POINTER(ctypes.c_int),
@@ -473,6 +477,21 @@ def _i32(a):
     return np.ascontiguousarray(list(a), np.int32)
 
 
+def _logprobs_arrays(rows, targets, top):
+    """(address of the targets, the answers' arrays, their addresses)."""
+    out = {"entropy": np.empty(rows, np.float32), "top_ids": np.empty((rows, top), np.int32),
+           "top_logp": np.empty((rows, top), np.float32)}
+    t = None
+    if targets is not None:
+        out["targets"] = t = np.ascontiguousarray(targets, np.int32)
+        if t.ndim != 1 or t.size != rows:
+            raise ValueError(f"{t.size} targets for {rows} rows")
+        out["logp"] = np.empty(rows, np.float32)
+    ptrs = [out["logp"].ctypes.data if t is not None else None, out["entropy"].ctypes.data,
+            out["top_ids"].ctypes.data, out["top_logp"].ctypes.data]
+    return None if t is None else t.ctypes.data, out, ptrs
+
+
 class KvCache:
     """A paged 8-bit KV cache that many sequences share (pbx_kv_*): n_pages pages
     of page_tokens positions, sequence ids 0..max_seqs - 1."""
@@ -554,6 +573,7 @@ class KvBatch:
             raise ValueError("seqs, counts and starts of different length")
         self.ctx._call("pbx_kv_batch_set", self._ptr, len(s), s.ctypes.data,
                        None if a is None else a.ctypes.data, c.ctypes.data)
+        self.sequences = int((c > 0).sum())  # that have rows
         return self
 
     @property
@@ -715,6 +735,30 @@ class Model:
         self._mcall("pbx_model_forward_batch", toks.ctypes.data, len(toks), start_pos,
                     None if logits is None else logits.ctypes.data, nxt.ctypes.data)
         return logits, nxt
+
+    def logprobs(self, tokens, start_pos, targets=None, top=0):
+        """One batched forward that answers with {"logp" [n] (of targets), "entropy"
+        [n], "top_ids" and "top_logp" [n, top]} instead of n rows of logits."""
+        toks = np.ascontiguousarray(tokens, np.int32)
+        t, out, ptrs = _logprobs_arrays(len(toks), targets, top)
+        self._mcall("pbx_model_logprobs", toks.ctypes.data, len(toks), start_pos, t, top, *ptrs)
+        return out
+
+    def forward_kv(self, batch, tokens, all_rows=False, want_logits=True, targets=None, top=None):
+        """One forward over a KvBatch's rows: (logits [rows, vocab] or None, argmax
+        [rows]) of every row (all_rows) or of each sequence's last; with targets or
+        top also the dictionary that logprobs gives."""
+        toks = np.ascontiguousarray(tokens, np.int32)
+        if len(toks) != batch.rows:
+            raise ValueError(f"{len(toks)} tokens for {batch.rows} rows")
+        rows = len(toks) if all_rows else batch.sequences
+        logits = np.empty((rows, self.vocab), np.float32) if want_logits else None
+        nxt = np.empty(rows, np.int32)
+        ask = targets is not None or top is not None
+        t, out, ptrs = _logprobs_arrays(rows, targets, top or 0) if ask else (None, None, [None] * 4)
+        self._mcall("pbx_model_forward_kv", batch._ptr, toks.ctypes.data, 1 if all_rows else 0,
+                    None if logits is None else logits.ctypes.data, nxt.ctypes.data, t, top or 0, *ptrs)
+        return (logits, nxt, out) if ask else (logits, nxt)
 
     def generate(self, token, start_pos, n_steps, want_logits=False):
         out = np.empty(n_steps, np.int32)

@@ -42,7 +42,7 @@ static void check_work(const kv_pages &kv, const kv_batch_plan &p, int groups, i
       CHECK(!k || p.attn[at - 1].blk1 - p.attn[at - 1].blk0 >= p.attn[at].blk1 - p.attn[at].blk0);
       items[{p.attn[at].row0, p.attn[at].tile}].push_back({p.attn[at], 1 << c});
     }
-  size_t bi = 0, used_items = 0;
+  size_t bi = 0, used_items = 0, last = 0;
   int row0 = 0, tab = 0;
   std::set<int> slots, joins;
   for (size_t i = 0; i < p.seqs.size(); ++i) {
@@ -67,8 +67,8 @@ static void check_work(const kv_pages &kv, const kv_batch_plan &p, int groups, i
       std::sort(list.begin(), list.end(), [](auto &x, auto &y) { return x.first.part < y.first.part; });
       const int u16 = list[0].second, parts = (int)list.size();
       CHECK(u16 <= max_u && parts <= KV_MAX_PARTS);
-      const int last = std::min(count * groups, row + 16 * u16) - 1;
-      const int seen = start + last / groups + 1;  // positions
+      const int bottom = std::min(count * groups, row + 16 * u16) - 1;
+      const int seen = start + bottom / groups + 1;  // positions
       int blk = 0;
       for (int k = 0; k < parts; ++k) {
         const kv_attn_item &x = list[k].first;
@@ -90,7 +90,10 @@ static void check_work(const kv_pages &kv, const kv_batch_plan &p, int groups, i
     }
     row0 += count;
     tab += used;
+    CHECK(last < p.last_rows.size() && p.last_rows[last] == row0 - 1);
+    ++last;
   }
+  CHECK(last == p.last_rows.size());
   CHECK(bi == p.blocks.size() && used_items == p.attn.size() && (int)joins.size() == p.n_joins);
   CHECK((int)slots.size() == p.n_slots && row0 == p.n_rows && tab == (int)p.table.size());
 }
