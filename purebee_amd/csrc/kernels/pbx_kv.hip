@@ -123,15 +123,19 @@ __device__ __forceinline__ void turn(const KvRope &r, int u, const Angles &cs, d
 // by 4 dims, values by 4 positions, as their codes lie side by side); the
 // block's codes are put together in LDS (with the earlier rows' codes, if there
 // are any) and stored whole.
+// Threads of a workgroup: two units each (a wide head's block on 256 threads took
+// three times as long where there are few).
+constexpr int append_threads(int hdp) { return hdp <= 64 ? 256 : 4 * hdp; }
+
 template <int HDP>
 __device__ __forceinline__ void append_body(const KvArgs &a, const KvRope &r, const BlockItem *items,
                                             int n_blocks, const int *row_pos, int n_rows, const float *K,
                                             int64_t ks, const float *V, int64_t vs, const float *Q, int64_t qs,
                                             float *Qout, int64_t qos) {
-  constexpr int UNITS = BLK * HDP / 4 / 256;  // a thread's units of a block
+  constexpr int T = append_threads(HDP), UNITS = BLK * HDP / 4 / T;  // a thread's units of a block
   __shared__ __attribute__((aligned(16))) uint8_t img[2 * BLK * HDP];
-  __shared__ uint64_t red_k[4];
-  __shared__ unsigned red_v[4];
+  __shared__ uint64_t red_k[T / 64];
+  __shared__ unsigned red_v[T / 64];
   const int units = a.head_dim / 4, tid = threadIdx.x;
   const int64_t wg = blockIdx.x;
   if (wg >= (int64_t)n_blocks * a.kv_heads) {
@@ -142,14 +146,14 @@ __device__ __forceinline__ void append_body(const KvArgs &a, const KvRope &r, co
     // four units at a time, all read before any is written (in place, too: a unit
     // is read and written by one thread); with a power of two of units a head a
     // thread meets the same angles in every head
-    const bool same = 256 % units == 0;
+    const bool same = T % units == 0;
     Angles cs = angles_of(r, tid % units, pos);
-    for (int i0 = tid; i0 < n; i0 += 4 * 256) {
+    for (int i0 = tid; i0 < n; i0 += 4 * T) {
       float2 x[4][2];
       int at[4][2];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int i = min(i0 + 256 * k, n - 1), u = i % units, h = 4 * (i - u);  // h: the head's first dim
+        const int i = min(i0 + T * k, n - 1), u = i % units, h = 4 * (i - u);  // h: the head's first dim
         unit_dims(r, u, at[k][0], at[k][1]);
         at[k][0] += h;
         at[k][1] += h;
@@ -158,7 +162,7 @@ __device__ __forceinline__ void append_body(const KvArgs &a, const KvRope &r, co
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const int i = i0 + 256 * k, u = i % units;
+        const int i = i0 + T * k, u = i % units;
         if (i >= n) break;
         if (!same) cs = angles_of(r, u, pos);
         double y[4] = {x[k][0].x, x[k][0].y, x[k][1].x, x[k][1].y};
@@ -187,7 +191,7 @@ __device__ __forceinline__ void append_body(const KvArgs &a, const KvRope &r, co
   unsigned pv = 0;
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
-    const int j = tid + 256 * i;
+    const int j = tid + T * i;
     if (j < nv_units) {
       const int key = 4 * (v0 + j / a.head_dim), d = j % a.head_dim;
 #pragma unroll
@@ -217,10 +221,10 @@ __device__ __forceinline__ void append_body(const KvArgs &a, const KvRope &r, co
   if (lo > 0) {
     ok = a.scales[2 * bi];
     ov = a.scales[2 * bi + 1];
-    for (int i = tid; i < 2 * BLK * HDP / 16; i += 256)
+    for (int i = tid; i < 2 * BLK * HDP / 16; i += T)
       reinterpret_cast<uintx4 *>(img)[i] = reinterpret_cast<const uintx4 *>(codes)[i];
   } else if (hi < BLK || a.head_dim < HDP) {
-    for (int i = tid; i < 2 * BLK * HDP / 4; i += 256) reinterpret_cast<unsigned *>(img)[i] = 0x80808080u;
+    for (int i = tid; i < 2 * BLK * HDP / 4; i += T) reinterpret_cast<unsigned *>(img)[i] = 0x80808080u;
   }
   pk = wave_max_u64(pk);
 #pragma unroll
@@ -231,7 +235,7 @@ __device__ __forceinline__ void append_body(const KvArgs &a, const KvRope &r, co
   }
   __syncthreads();  // (and the image is filled)
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < T / 64; ++w) {
     pk = red_k[w] > pk ? red_k[w] : pk;
     pv = max(pv, red_v[w]);
   }
@@ -240,7 +244,7 @@ __device__ __forceinline__ void append_body(const KvArgs &a, const KvRope &r, co
   if (lo > 0) {
     const bool gk = __float_as_uint(nk) != __float_as_uint(ok), gv = __float_as_uint(nv) != __float_as_uint(ov);
     if (gk || gv) {
-      for (int i = tid; i < lo * HDP; i += 256) {
+      for (int i = tid; i < lo * HDP; i += T) {
         const int key = i / HDP, dim = i % HDP;
         uint8_t *pkb = img + key_byte<HDP>(key, dim), *pvb = img + BLK * HDP + value_byte(key, dim);
         if (gk) *pkb = (uint8_t)(code_of((double)((int)*pkb - 128) * (double)ok, nk, ik) + 128);
@@ -251,7 +255,7 @@ __device__ __forceinline__ void append_body(const KvArgs &a, const KvRope &r, co
   }
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
-    const int j = tid + 256 * i;
+    const int j = tid + T * i;
     if (j < nk_units) {
       const int key = lo + j / units, u = j % units;
       int da, db;
@@ -278,7 +282,7 @@ __device__ __forceinline__ void append_body(const KvArgs &a, const KvRope &r, co
     }
   }
   __syncthreads();
-  for (int i = tid; i < 2 * BLK * HDP / 16; i += 256)
+  for (int i = tid; i < 2 * BLK * HDP / 16; i += T)
     reinterpret_cast<uintx4 *>(codes)[i] = reinterpret_cast<const uintx4 *>(img)[i];
   if (tid == 0) *reinterpret_cast<float2 *>(a.scales + 2 * bi) = make_float2(nk, nv);
 }
@@ -827,7 +831,7 @@ pbx_kv_rope_table(const double *freq, double *table, int half, int64_t n) {
 }
 
 #define PBX_KV_KERNELS(HDP)                                                                                        \
-  extern "C" __global__ void __launch_bounds__(256)                                                                \
+  extern "C" __global__ void __launch_bounds__(append_threads(HDP))                                                                \
       pbx_kv_append_##HDP(KvArgs a, KvRope r, const BlockItem *items, int n_blocks, const int *row_pos,            \
                           int n_rows, const float *K, int64_t ks, const float *V, int64_t vs, const float *Q,      \
                           int64_t qs, float *Qout, int64_t qos) {                                                  \

@@ -434,7 +434,8 @@ extern "C" int pbx_kv_append_dev(pbx_kv_batch *b, int layer, const float *dQ, in
   void *args[] = {&a, &r, &items, (void *)&n_blocks, &pos, (void *)&n_rows, &dK, &k_stride, &dV, &v_stride,
                   &dQ, &q_stride, &dQout, &qout_stride};
   return kv_launch(c, "pbx_kv_append_" + std::to_string(kv->hdp),
-                   (int64_t)n_blocks * g.n_kv_heads + (dQ ? n_rows : 0), 256, args);
+                   (int64_t)n_blocks * g.n_kv_heads + (dQ ? n_rows : 0),
+                   kv->hdp <= 64 ? 256 : 4 * kv->hdp /* append_threads of pbx_kv.hip */, args);
 }
 
 extern "C" int pbx_kv_attention_dev(pbx_kv_batch *b, int layer, const float *dQ, int64_t q_stride, float scale,
