@@ -287,30 +287,37 @@ __device__ __forceinline__ void append_body(const KvArgs &a, const KvRope &r, co
   if (tid == 0) *reinterpret_cast<float2 *>(a.scales + 2 * bi) = make_float2(nk, nv);
 }
 
-// Reading back: workgroup (block, KV head).
+// Reading back: workgroup (block, KV head); the codes by way of LDS, where single
+// bytes are cheap.
 template <int HDP>
 __device__ __forceinline__ void read_body(const KvArgs &a, const BlockItem *items, float *K, int64_t ks, float *V,
                                           int64_t vs) {
+  constexpr int T = append_threads(HDP);
+  __shared__ __attribute__((aligned(16))) uint8_t img[2 * BLK * HDP];
   const BlockItem it = items[blockIdx.x / a.kv_heads];
   const int head = (int)(blockIdx.x % a.kv_heads);
   const int64_t bi = block_index(a, it.page, head, it.sub);
   const uint8_t *codes = a.codes + bi * (2 * BLK * HDP);
   const float sk = a.scales[2 * bi], sv = a.scales[2 * bi + 1];
+  for (int i = threadIdx.x; i < 2 * BLK * HDP / 16; i += T)
+    reinterpret_cast<uintx4 *>(img)[i] = reinterpret_cast<const uintx4 *>(codes)[i];
+  __syncthreads();
   const int lo = it.start > it.pos0 ? it.start - it.pos0 : 0;
   const int hi = min(BLK, it.start + it.count - it.pos0);
   const int units = a.head_dim / 4;
-  for (int j = threadIdx.x; j < (hi - lo) * units; j += 256) {
+  for (int j = threadIdx.x; j < (hi - lo) * units; j += T) {
     const int key = lo + j / units, d = 4 * (j % units);
     const int64_t row = (int64_t)it.row0 + it.pos0 + key - it.start;
     if (K) {
-      const uint8_t *p = codes + key_byte<HDP>(key, d);
+      const unsigned w = *reinterpret_cast<const unsigned *>(img + key_byte<HDP>(key, d));
       *reinterpret_cast<float4 *>(K + row * ks + (int64_t)head * a.head_dim + d) =
-          make_float4((p[0] - 128) * sk, (p[1] - 128) * sk, (p[2] - 128) * sk, (p[3] - 128) * sk);
+          make_float4(((int)(w & 255) - 128) * sk, ((int)(w >> 8 & 255) - 128) * sk,
+                      ((int)(w >> 16 & 255) - 128) * sk, ((int)(w >> 24) - 128) * sk);
     }
     if (V) {
       float v[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (codes[BLK * HDP + value_byte(key, d + e)] - 128) * sv;
+      for (int e = 0; e < 4; ++e) v[e] = (img[BLK * HDP + value_byte(key, d + e)] - 128) * sv;
       *reinterpret_cast<float4 *>(V + row * vs + (int64_t)head * a.head_dim + d) =
           make_float4(v[0], v[1], v[2], v[3]);
     }
@@ -831,13 +838,13 @@ pbx_kv_rope_table(const double *freq, double *table, int half, int64_t n) {
 }
 
 #define PBX_KV_KERNELS(HDP)                                                                                        \
-  extern "C" __global__ void __launch_bounds__(append_threads(HDP))                                                                \
+  extern "C" __global__ void __launch_bounds__(append_threads(HDP))                                                \
       pbx_kv_append_##HDP(KvArgs a, KvRope r, const BlockItem *items, int n_blocks, const int *row_pos,            \
                           int n_rows, const float *K, int64_t ks, const float *V, int64_t vs, const float *Q,      \
                           int64_t qs, float *Qout, int64_t qos) {                                                  \
     append_body<HDP>(a, r, items, n_blocks, row_pos, n_rows, K, ks, V, vs, Q, qs, Qout, qos);                      \
   }                                                                                                                \
-  extern "C" __global__ void __launch_bounds__(256)                                                                \
+  extern "C" __global__ void __launch_bounds__(append_threads(HDP))                                                \
       pbx_kv_read_##HDP(KvArgs a, const BlockItem *items, float *K, int64_t ks, float *V, int64_t vs) {            \
     read_body<HDP>(a, items, K, ks, V, vs);                                                                        \
   }

@@ -67,6 +67,9 @@ static int kv_padded(int hd) {
   return 0;
 }
 
+// Threads of the append and read workgroups (append_threads of pbx_kv.hip).
+static int kv_threads(int hdp) { return hdp <= 64 ? 256 : 4 * hdp; }
+
 // 16-row query tiles of the widest attention kernel for a head size.
 static int kv_max_tiles(int hdp) { return hdp <= 64 ? 4 : 2; }
 
@@ -435,7 +438,7 @@ extern "C" int pbx_kv_append_dev(pbx_kv_batch *b, int layer, const float *dQ, in
                   &dQ, &q_stride, &dQout, &qout_stride};
   return kv_launch(c, "pbx_kv_append_" + std::to_string(kv->hdp),
                    (int64_t)n_blocks * g.n_kv_heads + (dQ ? n_rows : 0),
-                   kv->hdp <= 64 ? 256 : 4 * kv->hdp /* append_threads of pbx_kv.hip */, args);
+                   kv_threads(kv->hdp), args);
 }
 
 extern "C" int pbx_kv_attention_dev(pbx_kv_batch *b, int layer, const float *dQ, int64_t q_stride, float scale,
@@ -481,6 +484,6 @@ extern "C" int pbx_kv_read_dev(pbx_kv_batch *b, int layer, float *dK, int64_t k_
     return rc;
   const int32_t *items = b->dev;
   void *args[] = {&a, &items, &dK, &k_stride, &dV, &v_stride};
-  return kv_launch(c, "pbx_kv_read_" + std::to_string(kv->hdp), (int64_t)b->plan.blocks.size() * g.n_kv_heads, 256,
-                   args);
+  return kv_launch(c, "pbx_kv_read_" + std::to_string(kv->hdp), (int64_t)b->plan.blocks.size() * g.n_kv_heads,
+                   kv_threads(kv->hdp), args);
 }
