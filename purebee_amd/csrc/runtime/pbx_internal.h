@@ -12,6 +12,10 @@
 
 // Kernels of pbx_kernels.hsaco, looked up by name at pbx_init.
 #define PBX_KERNEL_LIST(X)                                   \
+  X(PBX_K_LOGPROBS_PART_256, "pbx_logprobs_part_256")        \
+  X(PBX_K_LOGPROBS_PART_512, "pbx_logprobs_part_512")        \
+  X(PBX_K_LOGPROBS_JOIN, "pbx_logprobs_join")                \
+  X(PBX_K_KV_ROPE_TABLE, "pbx_kv_rope_table")                \
   X(PBX_K_REPACK_Q4_0, "pbx_repack_q4_0")                    \
   X(PBX_K_REPACK_Q8_0, "pbx_repack_q8_0")                    \
   X(PBX_K_REPACK_Q4_1, "pbx_repack_q4_1")                    \

@@ -34,6 +34,8 @@ struct pbx_kv {
   float *scales = nullptr;   // [layer][page][kv head][block][key, value]
   double *rope = nullptr;    // [max_seq][rope_dim / 2][cos, sin]
   size_t layer_codes = 0, layer_scales = 0, bytes = 0;
+  // the kernels for this head size; attention by log2 of the query tiles
+  hipFunction_t append = nullptr, read = nullptr, attn[4] = {};
   std::vector<pbx_kv_batch *> batches;
 };
 
@@ -73,11 +75,9 @@ static int kv_threads(int hdp) { return hdp <= 64 ? 256 : 4 * hdp; }
 // 16-row query tiles of the widest attention kernel for a head size.
 static int kv_max_tiles(int hdp) { return hdp <= 64 ? 4 : 2; }
 
-static int kv_launch(pbx_ctx *c, const std::string &name, int64_t grid, int block, void **args) {
-  hipFunction_t f = pbx_kernel_by_name(c, name);
-  if (!f) return pbx_fail(c, PBX_ELOAD, "kv: kernel %s not found", name.c_str());
+static int kv_launch(pbx_ctx *c, hipFunction_t f, const char *name, int64_t grid, int block, void **args) {
   if (grid > 0x7fffffff) return pbx_fail(c, PBX_ENOTSUP, "kv: %lld workgroups", (long long)grid);
-  return pbx_launch_fn(c, f, name.c_str(), dim3((unsigned)grid), dim3(block), args, c->stream);
+  return pbx_launch_fn(c, f, name, dim3((unsigned)grid), dim3(block), args, c->stream);
 }
 
 static void batch_release(pbx_kv_batch *b) {
@@ -157,6 +157,15 @@ static int kv_make(pbx_ctx *c, const pbx_kv_config &g, pbx_kv *kv) {
   kv->cfg.rope_factors = nullptr;  // the caller's array need not outlive the call
   if (hipSetDevice(c->device) != hipSuccess)
     return pbx_fail(c, PBX_EHIP, "pbx_kv_create: hipSetDevice failed");
+  const std::string hdp = std::to_string(kv->hdp);
+  kv->append = pbx_kernel_by_name(c, "pbx_kv_append_" + hdp);
+  kv->read = pbx_kernel_by_name(c, "pbx_kv_read_" + hdp);
+  bool found = kv->append && kv->read;
+  for (int k = 0; 1 << k <= kv_max_tiles(kv->hdp); ++k) {
+    kv->attn[k] = pbx_kernel_by_name(c, "pbx_kv_attn_" + hdp + "_" + std::to_string(1 << k));
+    found = found && kv->attn[k];
+  }
+  if (!found) return pbx_fail(c, PBX_ELOAD, "pbx_kv_create: kernels for head_dim %d not found", g.head_dim);
   double *dfreq = nullptr;
   if (hipMalloc((void **)&kv->codes, codes) != hipSuccess ||
       hipMalloc((void **)&kv->scales, scales) != hipSuccess ||
@@ -175,7 +184,7 @@ static int kv_make(pbx_ctx *c, const pbx_kv_config &g, pbx_kv *kv) {
       rc = pbx_fail(c, PBX_EHIP, "pbx_kv_create: frequency copy failed");
     const int64_t n = (int64_t)g.max_seq * half;
     void *args[] = {&dfreq, &kv->rope, (void *)&half, (void *)&n};
-    if (!rc) rc = kv_launch(c, "pbx_kv_rope_table", (n + 255) / 256, 256, args);
+    if (!rc) rc = kv_launch(c, c->fn[PBX_K_KV_ROPE_TABLE], "pbx_kv_rope_table", (n + 255) / 256, 256, args);
   }
   if (hipStreamSynchronize(c->stream) != hipSuccess && !rc)
     rc = pbx_fail(c, PBX_EHIP, "pbx_kv_create: initialisation failed");
@@ -436,8 +445,7 @@ extern "C" int pbx_kv_append_dev(pbx_kv_batch *b, int layer, const float *dQ, in
   const int n_blocks = (int)b->plan.blocks.size(), n_rows = b->plan.n_rows;
   void *args[] = {&a, &r, &items, (void *)&n_blocks, &pos, (void *)&n_rows, &dK, &k_stride, &dV, &v_stride,
                   &dQ, &q_stride, &dQout, &qout_stride};
-  return kv_launch(c, "pbx_kv_append_" + std::to_string(kv->hdp),
-                   (int64_t)n_blocks * g.n_kv_heads + (dQ ? n_rows : 0),
+  return kv_launch(c, kv->append, "pbx_kv_append", (int64_t)n_blocks * g.n_kv_heads + (dQ ? n_rows : 0),
                    kv_threads(kv->hdp), args);
 }
 
@@ -461,9 +469,7 @@ extern "C" int pbx_kv_attention_dev(pbx_kv_batch *b, int layer, const float *dQ,
     const int n = b->plan.n_attn[k];
     if (!n) continue;
     void *args[] = {&a, &items, &table, &dQ, &q_stride, &scale, &dOut, &out_stride, &b->part, &b->arrived};
-    if ((rc = kv_launch(c, "pbx_kv_attn_" + std::to_string(kv->hdp) + "_" + std::to_string(1 << k),
-                        (int64_t)n * g.n_kv_heads, 256, args)))
-      return rc;
+    if ((rc = kv_launch(c, kv->attn[k], "pbx_kv_attn", (int64_t)n * g.n_kv_heads, 256, args))) return rc;
     items += n * (sizeof(kv_attn_item) / 4);
   }
   return PBX_OK;
@@ -484,6 +490,6 @@ extern "C" int pbx_kv_read_dev(pbx_kv_batch *b, int layer, float *dK, int64_t k_
     return rc;
   const int32_t *items = b->dev;
   void *args[] = {&a, &items, &dK, &k_stride, &dV, &v_stride};
-  return kv_launch(c, "pbx_kv_read_" + std::to_string(kv->hdp), (int64_t)b->plan.blocks.size() * g.n_kv_heads,
+  return kv_launch(c, kv->read, "pbx_kv_read", (int64_t)b->plan.blocks.size() * g.n_kv_heads,
                    kv_threads(kv->hdp), args);
 }

@@ -67,15 +67,13 @@ extern "C" int pbx_logprobs_dev(pbx_ctx *c, const float *dLogits, int64_t stride
   if (hipSetDevice(c->device) != hipSuccess) return pbx_fail(c, PBX_EHIP, "%s: hipSetDevice failed", who);
   // (a part has at most a group more than its even share)
   const bool small = (vocab + 3) / parts64 + 8 <= LP_ELEMENTS_256;
-  const char *name = small ? "pbx_logprobs_part_256" : "pbx_logprobs_part_512";
-  hipFunction_t part = pbx_kernel_by_name(c, name), join = pbx_kernel_by_name(c, "pbx_logprobs_join");
-  if (!part || !join) return pbx_fail(c, PBX_ELOAD, "%s: kernels not found", who);
   LogprobsOutHost out{dTargets, dLogp, dEntropy, dTopIds, dTopLogp};
   int v = (int)vocab, parts = (int)parts64;
   void *keys = work;
   float *sums = need ? (float *)((char *)work + 8 * (size_t)rows * parts * top) : nullptr;
   void *args[] = {(void *)&dLogits, &stride, &v, &parts, &top, &out, &sums, &keys};
-  rc = pbx_launch_fn(c, part, name, dim3((unsigned)(rows * parts)), dim3(small ? 256 : 512), args, c->stream);
+  rc = pbx_launch(c, small ? PBX_K_LOGPROBS_PART_256 : PBX_K_LOGPROBS_PART_512, dim3((unsigned)(rows * parts)),
+                  dim3(small ? 256 : 512), args);
   if (rc || parts == 1) return rc;
-  return pbx_launch_fn(c, join, "pbx_logprobs_join", dim3((unsigned)rows), dim3(256), args, c->stream);
+  return pbx_launch(c, PBX_K_LOGPROBS_JOIN, dim3((unsigned)rows), dim3(256), args);
 }

@@ -358,11 +358,14 @@ class Context:
         self._p = p.value
         self.L = L
 
+    def _raise(self, rc):
+        msg = self.L.pbx_last_error(self._p)
+        raise PbxError(rc, msg.decode() if msg else "")
+
     def _call(self, name, *args):
         rc = getattr(self.L, name)(*args)
         if rc != 0:
-            msg = self.L.pbx_last_error(self._p)
-            raise PbxError(rc, msg.decode() if msg else "")
+            self._raise(rc)
 
     def close(self):
         if self._p:
@@ -560,11 +563,14 @@ class KvBatch:
         p = _vp()
         self.ctx._call("pbx_kv_batch_create", cache._ptr, ctypes.byref(p))
         self._b = p.value
+        L = self.ctx.L  # a step makes these calls for every layer: no look-ups on the way
+        self._append, self._attention, self._read = (L.pbx_kv_append_dev, L.pbx_kv_attention_dev,
+                                                     L.pbx_kv_read_dev)
 
     @property
     def _ptr(self):
         # a freed cache has freed its batches
-        return self._b if self.cache._ptr else None
+        return self._b if self.cache._kv and self.ctx._p else None
 
     def set(self, seqs, counts, starts=None):
         s, c = _i32(seqs), _i32(counts)
@@ -584,16 +590,21 @@ class KvBatch:
 
     def append_dev(self, layer, dQ, dK, dV, dQout, q_stride=0, k_stride=0, v_stride=0, qout_stride=0):
         """Rotate queries (into dQout) and keys, append keys and values."""
-        self.ctx._call("pbx_kv_append_dev", self._ptr, layer, dQ, q_stride, dK, k_stride, dV, v_stride,
-                       dQout, qout_stride)
+        rc = self._append(self._ptr, layer, dQ, q_stride, dK, k_stride, dV, v_stride, dQout, qout_stride)
+        if rc:
+            self.ctx._raise(rc)
 
     def attention_dev(self, layer, dQ, dOut, scale=0.0, q_stride=0, out_stride=0):
         """Causal attention of the batch's rotated query rows over the cache."""
-        self.ctx._call("pbx_kv_attention_dev", self._ptr, layer, dQ, q_stride, scale, dOut, out_stride)
+        rc = self._attention(self._ptr, layer, dQ, q_stride, scale, dOut, out_stride)
+        if rc:
+            self.ctx._raise(rc)
 
     def read_dev(self, layer, dK, dV, k_stride=0, v_stride=0):
         """The batch's rows of the cache as the f32 values they stand for."""
-        self.ctx._call("pbx_kv_read_dev", self._ptr, layer, dK, k_stride, dV, v_stride)
+        rc = self._read(self._ptr, layer, dK, k_stride, dV, v_stride)
+        if rc:
+            self.ctx._raise(rc)
 
     def free(self):
         if self._ptr:
