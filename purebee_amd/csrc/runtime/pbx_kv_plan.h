@@ -213,8 +213,12 @@ inline void kv_plan_work(const kv_pages &kv, int groups, int kv_heads, int max_u
   int64_t total = 0;  // blocks that the tiles visit
   for (int i = 0; i < n; ++i)
     for (int t = 0; t < tiles_of(i); ++t) total += blocks_of(i, t);
-  // an item: at least 16 blocks (four a wave), and about `want` workgroups in all
-  const int64_t chunk = std::max<int64_t>(least, (total * kv_heads + want - 1) / want);
+  // an item: at least 16 blocks (four a wave), and about `want` workgroups in all;
+  // wide tiles that fill the GPU as they are, longest first, are split only where
+  // one is far longer than that: their partial results cost more than the
+  // better balance brings (a 1,000-token prompt 32 -> 23 us)
+  const int64_t even = std::max<int64_t>(least, (total * kv_heads + want - 1) / want);
+  const int64_t wide = workgroups() < want / 2 ? even : 4 * even;
   const int per_page = kv.page_tokens / PBX_KV_BLOCK;
   std::vector<kv_attn_item> by_u[4];
   int row0 = 0;
@@ -230,6 +234,7 @@ inline void kv_plan_work(const kv_pages &kv, int groups, int kv_heads, int max_u
     for (int t = 0; t < count; ++t) p->row_pos.push_back(start + t);
     for (int t = 0; t < tiles_of(i); ++t) {
       const int nb = blocks_of(i, t);
+      const int64_t chunk = lu ? wide : even;
       const int parts = (int)std::min<int64_t>(KV_MAX_PARTS, (nb + chunk - 1) / chunk);
       for (int k = 0; k < parts; ++k) {
         kv_attn_item x = {start, count, row0, t, (int)((int64_t)nb * k / parts), (int)((int64_t)nb * (k + 1) / parts),
