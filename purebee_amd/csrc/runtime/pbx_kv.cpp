@@ -144,6 +144,9 @@ static int kv_make(pbx_ctx *c, const pbx_kv_config &g, pbx_kv *kv) {
   const int per_page = g.page_tokens / PBX_KV_BLOCK;
   while ((1 << kv->page_shift) < per_page) ++kv->page_shift;
   kv->pages.init(g.page_tokens, g.n_pages, g.max_seqs, g.max_seq);
+  // (sizes that overflow would pass for small ones)
+  if ((double)g.n_layers * g.n_pages * g.n_kv_heads * g.page_tokens * kv->hdp > 0x1p46)
+    return pbx_fail(c, PBX_ENOMEM, "pbx_kv_create: a pool of more than 2^47 bytes");
   const size_t blocks = (size_t)g.n_pages * g.n_kv_heads * per_page;
   kv->layer_codes = blocks * 2 * PBX_KV_BLOCK * kv->hdp;
   kv->layer_scales = blocks * 2;

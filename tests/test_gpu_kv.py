@@ -493,3 +493,10 @@ def test_refusals(ctx):
             h.read_dev(0, x.ptr, None)
     x.free()
     assert BLOCK == pb.native.KV_BLOCK
+
+
+def test_a_pool_whose_size_overflows_is_refused(ctx):
+    """2^25 layers x 2^26 pages x 2 heads x 16 KiB are 2^66 bytes: nothing, in 64 bits."""
+    with pytest.raises(pb.PbxError) as e:
+        pb.KvCache(ctx, 1 << 25, 2, 2, 256, 1 << 26, 1, 100, page_tokens=32)
+    assert e.value.code == -3
