@@ -473,8 +473,10 @@ int pbx_kv_truncate(pbx_kv *kv, int seq, int n_tokens);
  * enqueue on the context's stream; of one batch they use the same workspace, so
  * work captured from one batch into graphs is replayed on one stream at a time.
  * A batch whose calls were captured keeps its rows (set refuses, PBX_EINVAL):
- * a replay runs over the same positions, which the sequences must still hold,
- * and the batch lives as long as the graph.
+ * a replay runs over the same positions, which the sequences must still hold
+ * (and, if it appends, end with), and the batch lives as long as the graph.
+ * Inside a capture no cache or batch is made, set or freed (PBX_EINVAL).
+ * Positions that a batch took hold nothing defined until they are appended.
  */
 int pbx_kv_batch_create(pbx_kv *kv, pbx_kv_batch **out);
 int pbx_kv_batch_free(pbx_kv_batch *b);
@@ -494,9 +496,10 @@ int pbx_kv_append_dev(pbx_kv_batch *b, int layer, const float *dQ, int64_t q_str
 /* Attention of the batch's (rotated) query rows over layer `layer` of their
  * sequences: head h of a row at position p sees KV head h / (n_heads /
  * n_kv_heads) at positions 0..p.  scale: of the products (0: 1 /
- * sqrt(head_dim)).  Rows as above; dOut [n_rows][n_heads][head_dim].  Values
- * are used as they stand in the cache, everything else in 22 bits or more; the
- * result of a row does not depend on the other rows' values. */
+ * sqrt(head_dim)).  Rows as above; dOut [n_rows][n_heads][head_dim], which may
+ * be dQ itself.  Values are used as they stand in the cache, everything else in
+ * 22 bits or more; the result of a row does not depend on the other rows'
+ * values. */
 int pbx_kv_attention_dev(pbx_kv_batch *b, int layer, const float *dQ, int64_t q_stride,
                          float scale, float *dOut, int64_t out_stride);
 /* The batch's rows of the cache as the values they stand for, f32 [n_rows]

@@ -275,9 +275,10 @@ __device__ __forceinline__ void part_body(const float *logits, int64_t stride, i
     return;
   }
   if (lane == 0) {
-    sums[3 * blockIdx.x] = a.m;
-    sums[3 * blockIdx.x + 1] = a.s;
-    sums[3 * blockIdx.x + 2] = a.t;
+    float *s = sums + 3 * (int64_t)blockIdx.x;
+    s[0] = a.m;
+    s[1] = a.s;
+    s[2] = a.t;
   }
   if (lane < top) keys[blockIdx.x * (int64_t)top + lane] = key;
 }

@@ -80,6 +80,16 @@ static int kv_launch(pbx_ctx *c, hipFunction_t f, const char *name, int64_t grid
   return pbx_launch_fn(c, f, name, dim3((unsigned)grid), dim3(block), args, c->stream);
 }
 
+static bool capturing(pbx_ctx *c) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  return hipStreamIsCapturing(c->stream, &st) != hipSuccess || st != hipStreamCaptureStatusNone;
+}
+
+// Creating and freeing wait for the stream, which would end a capture.
+static int not_capturing(pbx_ctx *c, const char *who) {
+  return capturing(c) ? pbx_fail(c, PBX_EINVAL, "%s: the context's stream is being captured", who) : PBX_OK;
+}
+
 static void batch_release(pbx_kv_batch *b) {
   if (b->dev) hipFree(b->dev);
   if (b->host) hipHostFree(b->host);
@@ -200,7 +210,7 @@ extern "C" int pbx_kv_create(pbx_ctx *c, const pbx_kv_config *cfg, pbx_kv **out)
   if (!cfg || !out) return pbx_fail(c, PBX_EINVAL, "pbx_kv_create: NULL argument");
   *out = nullptr;
   int rc = kv_check(c, *cfg);
-  if (rc) return rc;
+  if (rc || (rc = not_capturing(c, "pbx_kv_create"))) return rc;
   pbx_kv *kv = nullptr;
   try {
     kv = new pbx_kv();
@@ -223,6 +233,7 @@ extern "C" int pbx_kv_free(pbx_kv *kv) {
   if (!kv) return PBX_OK;
   if (!kv_ok(kv)) return pbx_fail(nullptr, PBX_EINVAL, "pbx_kv_free: not a live cache");
   pbx_ctx *c = kv->c;
+  if (const int rc = not_capturing(c, "pbx_kv_free")) return rc;
   hipSetDevice(c->device);
   hipStreamSynchronize(c->stream);
   auto *list = (std::vector<pbx_kv *> *)c->kvs;
@@ -260,6 +271,7 @@ extern "C" int pbx_kv_batch_create(pbx_kv *kv, pbx_kv_batch **out) {
   if (!kv_ok(kv)) return pbx_fail(nullptr, PBX_EINVAL, "pbx_kv_batch_create: not a live cache");
   if (!out) return pbx_fail(kv->c, PBX_EINVAL, "pbx_kv_batch_create: NULL argument");
   *out = nullptr;
+  if (const int rc = not_capturing(kv->c, "pbx_kv_batch_create")) return rc;
   try {
     kv->batches.reserve(kv->batches.size() + 1);
     pbx_kv_batch *b = new pbx_kv_batch();
@@ -281,6 +293,7 @@ extern "C" int pbx_kv_batch_free(pbx_kv_batch *b) {
   if (!b) return PBX_OK;
   if (!batch_ok(b)) return pbx_fail(nullptr, PBX_EINVAL, "pbx_kv_batch_free: not a live batch");
   pbx_kv *kv = b->kv;
+  if (const int rc = not_capturing(kv->c, "pbx_kv_batch_free")) return rc;
   hipSetDevice(kv->c->device);
   hipStreamSynchronize(kv->c->stream);
   kv->batches.erase(std::remove(kv->batches.begin(), kv->batches.end(), b), kv->batches.end());
@@ -293,11 +306,6 @@ extern "C" int pbx_kv_batch_rows(const pbx_kv_batch *b, int *n_rows) {
   if (!n_rows) return pbx_fail(b->kv->c, PBX_EINVAL, "pbx_kv_batch_rows: NULL argument");
   *n_rows = b->set ? b->plan.n_rows : 0;
   return PBX_OK;
-}
-
-static bool capturing(pbx_ctx *c) {
-  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-  return hipStreamIsCapturing(c->stream, &st) != hipSuccess || st != hipStreamCaptureStatusNone;
 }
 
 // Copies the plan's lists to the device, one after the other.
@@ -466,6 +474,8 @@ extern "C" int pbx_kv_attention_dev(pbx_kv_batch *b, int layer, const float *dQ,
   if ((rc = rows_check(c, who, "dQ", dQ, &q_stride, g.n_heads, g.head_dim)) ||
       (rc = rows_check(c, who, "dOut", dOut, &out_stride, g.n_heads, g.head_dim)))
     return rc;
+  if (dQ == dOut && q_stride != out_stride)
+    return pbx_fail(c, PBX_EINVAL, "%s: attention in place needs one stride", who);
   if (scale == 0.f) scale = (float)(1.0 / sqrt((double)g.head_dim));
   const int32_t *items = b->dev + b->at_attn, *table = b->dev + b->at_table;
   for (int k = 0; k < 4; ++k) {

@@ -500,3 +500,151 @@ def test_a_pool_whose_size_overflows_is_refused(ctx):
     with pytest.raises(pb.PbxError) as e:
         pb.KvCache(ctx, 1 << 25, 2, 2, 256, 1 << 26, 1, 100, page_tokens=32)
     assert e.value.code == -3
+
+
+def test_nothing_is_made_or_freed_inside_a_capture(ctx):
+    """Both would wait for the stream and spoil the capture, which goes on."""
+    hip = _hip()
+    p = Pair(ctx, 4, 2, 64, seed=18)
+    b, q = p.append([0], [50])
+    dq, do = Rows(ctx, 50, 256, q), Rows(ctx, 50, 256)
+    b.attention_dev(0, dq.ptr, do.ptr)
+    ctx.sync()
+    eager = do.get()
+    stream, graph, gexec = ctypes.c_void_p(ctx.stream()), ctypes.c_void_p(), ctypes.c_void_p()
+    assert hip.hipStreamBeginCapture(stream, 0) == 0
+    b.attention_dev(0, dq.ptr, do.ptr)
+    for call in (b.free, p.cache.free, lambda: Pair(ctx, 4, 2, 64), lambda: p.cache.batch([0], [1])):
+        with pytest.raises(pb.PbxError, match="captured"):
+            call()
+    assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(ctypes.byref(gexec), graph, None, None, 0) == 0
+    for _ in range(3):
+        do.buf.upload(do.host)
+        assert hip.hipGraphLaunch(gexec, stream) == 0
+        ctx.sync()
+        assert np.array_equal(do.get(), eager)
+    hip.hipGraphExecDestroy(gexec)
+    hip.hipGraphDestroy(graph)
+    for x in (dq, do):
+        x.free()
+    p.free()
+    assert p.cache._kv is None
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 32), (9, 3, 64), (8, 2, 96), (4, 2, 128), (4, 1, 192), (8, 1, 256)])
+def test_rows_of_long_contexts(ctx, heads, kv_heads, dim):
+    """Tiles of every width whose blocks are split over workgroups and joined, in place as well; the last tile is ragged."""
+    print(f"[case] rows of long contexts {heads}/{kv_heads}/{dim}", flush=True)
+    p = Pair(ctx, heads, kv_heads, dim, seqs=3, n_pages=150, seed=dim)
+    p.append([0, 1, 2], [2600, 1, 700])
+    b, q = p.append([0, 1, 2], [45, 2, 9])
+    got = p.attend(b, [0, 1, 2], [2600, 1, 700], [45, 2, 9], q, pad=4)
+    d = Rows(ctx, 56, heads * dim, q, heads * dim + 8)
+    for _ in range(2):
+        d.buf.upload(d.host)
+        b.attention_dev(0, d.ptr, d.ptr, 0.0, d.stride, d.stride)
+        ctx.sync()
+        assert np.array_equal(d.get().reshape(got.shape), got)
+    with pytest.raises(pb.PbxError, match="one stride"):
+        b.attention_dev(0, d.ptr, d.ptr, 0.0, d.stride, d.stride + 4)
+    d.free()
+    p.free()
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(32, 8), (71, 1), (6, 6)])
+def test_many_sequences(ctx, heads, kv_heads):
+    """Hundreds of short sequences in a batch, one row or two each, and groups of many heads."""
+    print(f"[case] 600 sequences {heads}/{kv_heads}", flush=True)
+    n = 600
+    p = Pair(ctx, heads, kv_heads, 32, seqs=n, n_pages=2 * n, seed=heads)
+    lengths = [i % 37 for i in range(n)]
+    seqs = [7 * i % n for i in range(n)]  # 7 and 600 have no common divisor
+    p.append(seqs, [lengths[s] for s in seqs])
+    counts = [1 + i % 2 for i in range(n)]
+    b, q = p.append(seqs, counts)
+    p.attend(b, seqs, [lengths[s] for s in seqs], counts, q)
+    p.check_values()
+    p.free()
+
+
+def test_tokens_and_prompts_in_one_batch(ctx):
+    """Single tokens over enough context for a launch of their own, beside prompts of wide tiles."""
+    p = Pair(ctx, 32, 8, 32, seqs=42, n_pages=42 * 34, seed=19)
+    past = [1050] * 40 + [0, 30]
+    p.append(list(range(42)), past)
+    seqs, counts = [41] + list(range(40)) + [40], [150] + [1] * 40 + [700]
+    b, q = p.append(seqs, counts)
+    p.attend(b, seqs, [past[s] for s in seqs], counts, q)
+    p.free()
+
+
+def test_the_same_rows_appended_again(ctx):
+    """An append made twice (a replay, a retry) leaves what one leaves, in blocks that others began as well."""
+    p = Pair(ctx, 4, 2, 64, seed=20)
+    p.append([0, 1], [40, 31])
+    q, k, v = p.rows(37, 3.0)
+    b, got = p.append([1, 0], [30, 7], (q, k, v))
+    dq, dk, dv = Rows(ctx, 37, 256, q), Rows(ctx, 37, 128, k), Rows(ctx, 37, 128, v)
+    for _ in range(2):
+        dq.buf.upload(dq.host)
+        b.append_dev(0, dq.ptr, dk.ptr, dv.ptr, dq.ptr)
+        ctx.sync()
+        assert np.array_equal(dq.get().reshape(got.shape), got)
+        p.check_values()
+    for x in (dq, dk, dv):
+        x.free()
+    p.free()
+
+
+def test_two_batches_in_two_graphs(ctx):
+    """Split contexts of two batches, captured apart, replayed in turn and with eager calls between: nothing is shared."""
+    hip = _hip()
+    p = Pair(ctx, 8, 2, 64, seqs=3, n_pages=200, seed=21)
+    p.append([0, 1, 2], [2000, 1500, 900])
+    stream = ctypes.c_void_p(ctx.stream())
+    made = []
+    for seqs, counts in (([0], [1]), ([1, 2], [2, 20])):
+        b, q = p.append(seqs, counts)
+        n = sum(counts)
+        dq, do = Rows(ctx, n, 512, q), Rows(ctx, n, 512)
+        b.attention_dev(0, dq.ptr, do.ptr)
+        ctx.sync()
+        graph, gexec = ctypes.c_void_p(), ctypes.c_void_p()
+        want = do.get()
+        assert hip.hipStreamBeginCapture(stream, 0) == 0
+        b.attention_dev(0, dq.ptr, do.ptr)
+        assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+        assert hip.hipGraphInstantiate(ctypes.byref(gexec), graph, None, None, 0) == 0
+        made.append((b, dq, do, want, graph, gexec))
+    for rep in range(3):
+        for b, dq, do, want, graph, gexec in made:
+            do.buf.upload(do.host)
+            assert hip.hipGraphLaunch(gexec, stream) == 0
+        ctx.sync()
+        for b, dq, do, want, graph, gexec in made:
+            assert np.array_equal(do.get(), want), rep
+        b, dq, do, want = made[rep % 2][:4]
+        do.buf.upload(do.host)
+        b.attention_dev(0, dq.ptr, do.ptr)
+        ctx.sync()
+        assert np.array_equal(do.get(), want), rep
+    for b, dq, do, want, graph, gexec in made:
+        hip.hipGraphExecDestroy(gexec)
+        hip.hipGraphDestroy(graph)
+        dq.free()
+        do.free()
+    p.free()
+
+
+def test_a_context_closes_over_its_caches():
+    """Caches and batches end with their context, and say so afterwards."""
+    c = pb.Context(0)
+    cache = pb.KvCache(c, 1, 4, 2, 64, 4, 2, 100)
+    b = cache.batch([0], [3])
+    c.close()
+    for call in (lambda: b.attention_dev(0, 16, 16), lambda: cache.length(0), lambda: cache.batch([1], [1])):
+        with pytest.raises(pb.PbxError):
+            call()
+    b.free()
+    cache.free()

@@ -1,5 +1,7 @@
 """Log probabilities, entropy and top tokens of rows of logits against 64-bit
 numpy."""
+import ctypes
+
 import numpy as np
 import pytest
 
@@ -226,3 +228,60 @@ def test_refusals(ctx):
         with pytest.raises(pb.PbxError):
             ctx.logprobs_dev(**a)
     b.free()
+
+
+def test_captured_calls_replay(ctx):
+    """Both launches of a split row captured: every replay equals the eager call, with other calls of the same
+    workspace and synchronisations between."""
+    hip = ctypes.CDLL("libamdhip64.so")
+    vp = ctypes.c_void_p
+    hip.hipStreamBeginCapture.argtypes = [vp, ctypes.c_int]
+    hip.hipStreamEndCapture.argtypes = [vp, ctypes.POINTER(vp)]
+    hip.hipGraphInstantiate.argtypes = [ctypes.POINTER(vp), vp, vp, ctypes.c_char_p, ctypes.c_size_t]
+    hip.hipGraphLaunch.argtypes = [vp, vp]
+    hip.hipGraphExecDestroy.argtypes = [vp]
+    hip.hipGraphDestroy.argtypes = [vp]
+    rng = np.random.default_rng(7)
+    x = (3 * rng.standard_normal((2, 3, 50257))).astype(np.float32)
+    dx = [ctx.alloc(x[i].nbytes).upload(x[i]) for i in range(2)]
+    dt = ctx.alloc(12).upload(np.array([1, 50256, 9], np.int32))
+    size = ctx.logprobs_workspace(3, 50257, 7)
+    assert size > 0
+    work, blank = ctx.alloc(size), np.full(48, 77, np.float32)
+    outs = [ctx.alloc(blank.nbytes) for _ in range(4)]
+
+    def call(i):
+        ctx.logprobs_dev(dx[i].ptr, 3, 50257, dt.ptr, 7, *(o.ptr for o in outs), work.ptr, size)
+
+    def answers():
+        ctx.sync()
+        return [o.download(np.uint32, 48) for o in outs]
+
+    def clear():
+        for o in outs:
+            o.upload(blank)
+
+    clear()
+    call(0)
+    eager = answers()
+    clear()
+    call(1)
+    other = answers()
+    stream, graph, gexec = vp(ctx.stream()), vp(), vp()
+    assert hip.hipStreamBeginCapture(stream, 0) == 0
+    call(0)
+    assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(ctypes.byref(gexec), graph, None, None, 0) == 0
+    for rep in range(3):
+        clear()
+        assert hip.hipGraphLaunch(gexec, stream) == 0
+        for got, want in zip(answers(), eager):
+            assert np.array_equal(got, want), rep
+        clear()
+        call(1)
+        for got, want in zip(answers(), other):
+            assert np.array_equal(got, want), rep
+    hip.hipGraphExecDestroy(gexec)
+    hip.hipGraphDestroy(graph)
+    for b in (*dx, dt, work, *outs):
+        b.free()
