@@ -185,15 +185,16 @@ inline void kv_plan_work(const kv_pages &kv, int groups, int kv_heads, int max_u
     const int64_t last = std::min<int64_t>(rows, (16 << width[i]) * ((int64_t)tile + 1)) - 1;
     return (int)((p->starts[i] + last / groups) / PBX_KV_BLOCK + 1);
   };
-  // Where the tiles are few, narrower ones: half as many rows a workgroup make
-  // twice as many workgroups (one sequence of 36 rows on 6,000 positions, 9 / 3
-  // heads of 64: 22.8 -> 10.7 us; 14 of up to 5 rows, 32 / 8 heads: 42 -> 27).
+  // Where the tiles are few (one and a half a CU: `want` is two), narrower ones:
+  // half as many rows a workgroup make twice as many workgroups (one sequence of
+  // 36 rows on 6,000 positions, 9 / 3 heads of 64: 22.8 -> 10.7 us; 17 of 6 to 34
+  // rows, 32 / 8 heads of 64: 7.9 -> 6.0, and at two a CU as many got slower).
   auto workgroups = [&]() {
     int64_t g = 0;
     for (int i = 0; i < n; ++i) g += tiles_of(i);
     return g * kv_heads;
   };
-  for (int w = 3; w > 0 && workgroups() < want / 2; --w)
+  for (int w = 3; w > 0 && workgroups() < 3 * want / 4; --w)
     for (int i = 0; i < n; ++i) width[i] = std::min(width[i], w - 1);
   // Each width is a launch of its own, one after the other.  One whose blocks do
   // not fill the GPU (16 a workgroup) is little but latency and joins the next
