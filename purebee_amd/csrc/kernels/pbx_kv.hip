@@ -122,7 +122,10 @@ __device__ __forceinline__ void turn(const KvRope &r, int u, const Angles &cs, d
 // The block's new rows are read once, keys turned, and held in registers (keys
 // by 4 dims, values by 4 positions, as their codes lie side by side); the
 // block's codes are put together in LDS (with the earlier rows' codes, if there
-// are any) and stored whole.
+// are any) and stored whole.  Bound by bytes where there are many rows (6,124 of
+// six prompts, 32 / 8 heads of 128: 62 us, 4.2 TB/s of queries in and out, keys,
+// values and codes), else by one chain of loads, maximum, LDS and store (one row:
+// 5 us, 64 of 64 sequences: 5.5; 32 / 8 heads of 64).
 // Threads of a workgroup: two units each (a wide head's block on 256 threads took
 // three times as long where there are few).
 constexpr int append_threads(int hdp) { return hdp <= 64 ? 256 : 4 * hdp; }
@@ -288,7 +291,7 @@ __device__ __forceinline__ void append_body(const KvArgs &a, const KvRope &r, co
 }
 
 // Reading back: workgroup (block, KV head); the codes by way of LDS, where single
-// bytes are cheap.
+// bytes are cheap.  Bound by bytes (the rows above: 14 us, 4.4 TB/s).
 template <int HDP>
 __device__ __forceinline__ void read_body(const KvArgs &a, const BlockItem *items, float *K, int64_t ks, float *V,
                                           int64_t vs) {
@@ -418,6 +421,16 @@ __device__ __forceinline__ float2 get2(const float *p) {
 // its values while the next scores are computed).  Where a tile's blocks are
 // split over several workgroups, the one that finishes last puts their states
 // together, in the order of the keys.
+// Single tokens are bound by the codes' bytes: 64 sequences of 64 to 8,000
+// positions, 32 / 8 heads of 64, 59 us (4.96 TB/s); one of 131,001 positions 35 us
+// (3.9 TB/s; with 96 or 128 parts for 64 it took 38 and 43); one of 129 4.9 us, a
+// launch's.  Prompts are bound by issue: a vector instruction does not run beside a
+// 16x16x32 product (a loop of 8 products and 32 fmas a wave, four waves a SIMD:
+// 358 ns, the products alone 226, the fmas 142), and 32 rows times 32 keys of 64
+// dims are 36 products (576 cycles) and about 265 vector instructions, so what
+// counts is fewer of either: 2,000 rows, 32 / 8 heads of 64, 50 us (656 TFLOP/s
+// of products); 1,183 rows on pasts of up to 2,000, 32 / 8 heads of 128, 93 us
+// (780 TFLOP/s).
 template <int HDP, int NQ, int KW, int RING>
 __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items, const int *table, const float *Q,
                                           int64_t qs, float scale, float *O, int64_t os, float *part,
