@@ -141,16 +141,18 @@ struct Out {
   float *top_logp;
 };
 
-// The answers for row `row` of x from its sums and (lane i) i-th largest key.
-__device__ __forceinline__ void answer(const Out &o, int64_t row, const float *x, int vocab, int top, Sums a,
-                                       uint64_t key, int lane) {
+// The target's logit in row `row` at x, NaN where there is none.  It is asked for
+// early, in two steps: one load waits for the other.
+__device__ __forceinline__ int target_of(const Out &o, int64_t row) { return o.logp ? o.targets[row] : -1; }
+__device__ __forceinline__ float logit_of(const float *x, int target, int vocab) {
+  return target >= 0 && target < vocab ? x[target] : __uint_as_float(0x7fc00000u);
+}
+// The answers for row `row` from its target's logit xt, its sums and (lane i) i-th largest key.
+__device__ __forceinline__ void answer(const Out &o, int64_t row, float xt, int top, Sums a, uint64_t key, int lane) {
   const bool none = !(a.s > 0.f && a.s < INFINITY);  // no distribution
   const float ls = logf(a.s), nan = __uint_as_float(0x7fc00000u);
   if (lane == 0) {
-    if (o.logp) {
-      const int t = o.targets[row];
-      o.logp[row] = none || t < 0 || t >= vocab ? nan : x[t] - a.m - ls;
-    }
+    if (o.logp) o.logp[row] = none ? nan : xt - a.m - ls;
     if (o.entropy) o.entropy[row] = none ? nan : ls - a.t / a.s;
   }
   if (lane < top) {
@@ -191,22 +193,59 @@ __device__ __forceinline__ float4 end_group(const float *x, int i, int vocab) {
   for (int e = 0; e < 4; ++e) v[e] = i + e >= 0 && i + e < vocab ? x[i + e] : -INFINITY;
   return make_float4(v[0], v[1], v[2], v[3]);
 }
+// Parts' results cross workgroups, of one launch as well: stores and loads at the
+// device's coherence point.
+template <typename T>
+__device__ __forceinline__ void put(T *p, T v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename T>
+__device__ __forceinline__ T get(const T *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Row `row`'s parts put together by W waves.
+template <int W>
+__device__ __forceinline__ void join_parts(int parts, int top, const Out &out, const float *sums,
+                                           const uint64_t *keys, int64_t row, float xt, float (*sbuf)[4],
+                                           uint64_t (*kbuf)[64]) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  Sums a = {LOWEST, 0.f, 0.f};
+  for (int i = tid; i < parts; i += 64 * W) {
+    const float *s = sums + 3 * (row * parts + i);
+    a = joined(a, {get(s), get(s + 1), get(s + 2)});
+  }
+  uint64_t key = 0;
+  const int n = parts * top;
+  for (int i = tid - lane; i < n; i += 64 * W)
+    key = merge_wave(key, sort_wave(i + lane < n ? get(keys + row * n + i + lane) : 0, lane, false), lane);
+  a = join_waves<W>(a, sbuf, wave, lane);
+  if (top) key = merge_waves<W>(key, kbuf, wave, lane);
+  if (!wave) answer(out, row, xt, top, a, key, lane);
+}
+
+// Parts done so far of a row, each count in a cache line of its own; zero between
+// launches.  Every context loads its own; its eager launches follow one another.
+constexpr int LP_MERGED_ROWS = 512;
+__device__ unsigned lp_arrived[32 * LP_MERGED_ROWS];
+
 // Workgroup (part, row): the row's 16-byte groups in `parts` pieces of at most
 // LP_SHARE groups a thread.  A thread keeps its sums and its first largest
 // group; the `top` threads with the largest ones hold the piece's `top` largest
 // elements among them (those threads' maxima alone are `top` elements as large),
 // so only their groups, read again, are looked through.  Many rows are bound by
-// bytes (512 x 128256, 20 tokens: 57 us, 4.6 TB/s); few by one chain of loads,
-// sorts and merges, and the second launch (1 x 128256, 8 tokens: 7.3 us, and 3.9
-// for the parts put together; 37 x 32003, 5 tokens: 8.5 and 4.4).
+// bytes (512 x 128256, 20 tokens: 56 us, 4.7 TB/s); few by one chain of loads,
+// sorts and merges, and the same again where parts are joined (1 x 128256, 8
+// tokens: 10.2 us; 37 x 32003, 5 tokens, not split: 9.8).  The last workgroup of a
+// row joins its parts: 6 % less than in a launch of its own.
 template <int LP_T, int LP_SHARE>
 __device__ __forceinline__ void part_body(const float *logits, int64_t stride, int vocab, int parts, int top, Out out,
-                                          float *sums, uint64_t *keys) {
+                                          float *sums, uint64_t *keys, int merged) {
   constexpr int W = LP_T / 64;
   __shared__ float sbuf[W][4];
   __shared__ uint64_t kbuf[W][64];
   __shared__ int chosen[LP_TOP];
-  __shared__ int count, n_chosen;
+  __shared__ int count, n_chosen, last;
   __shared__ uint64_t limit;
   __shared__ uint64_t list[LP_TOP * LP_SHARE * 4 + 8];  // (and the cut groups)
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -219,6 +258,7 @@ __device__ __forceinline__ void part_body(const float *logits, int64_t stride, i
   // whole groups, four of a thread under way at once, then a row's cut ones
   const int full = (vocab + skew) / 4;
   const int f0 = max(g0, skew ? 1 : 0), f1 = min(g1, full);
+  const int target = target_of(out, row);
   Share t = {{LOWEST, 0.f, 0.f}, -INFINITY, -1};
   const float4 *x4 = reinterpret_cast<const float4 *>(x - skew);
   int g = f0 + tid;
@@ -234,6 +274,7 @@ __device__ __forceinline__ void part_body(const float *logits, int64_t stride, i
   const bool head = skew && g0 == 0, tail = full < groups && g1 == groups && !(skew && full == 0);
   if (head && tid == 0) take(t, end_group(x, -skew, vocab), 0);
   if (tail && tid == 64) take(t, end_group(x, 4 * full - skew, vocab), full);
+  const float xt = logit_of(x, target, vocab);
   Sums a = t.a;
   const int at = t.at;
   a = join_waves<W>(a, sbuf, wave, lane);
@@ -272,18 +313,26 @@ __device__ __forceinline__ void part_body(const float *logits, int64_t stride, i
       key = merge_waves<W>(key, kbuf, wave, lane);
     }
   }
-  if (wave) return;
   if (parts == 1) {
-    answer(out, row, x, vocab, top, a, key, lane);
+    if (!wave) answer(out, row, xt, top, a, key, lane);
     return;
   }
-  if (lane == 0) {
+  if (!wave) {
     float *s = sums + 3 * (int64_t)blockIdx.x;
-    s[0] = a.m;
-    s[1] = a.s;
-    s[2] = a.t;
+    if (lane < 3) put(s + lane, lane == 0 ? a.m : lane == 1 ? a.s : a.t);
+    if (lane < top) put(keys + blockIdx.x * (int64_t)top + lane, key);
   }
-  if (lane < top) keys[blockIdx.x * (int64_t)top + lane] = key;
+  if (!merged) return;
+  // the part lies at the coherence point before it is counted; the workgroup
+  // that completes the row's count reads the others' from there
+  if (tid == 0) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    last = __hip_atomic_fetch_add(&lp_arrived[32 * row], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+           (unsigned)parts - 1;
+    if (last) __hip_atomic_store(&lp_arrived[32 * row], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (last) join_parts<W>(parts, top, out, sums, keys, row, xt, sbuf, kbuf);
 }
 
 }  // namespace
@@ -292,35 +341,22 @@ __device__ __forceinline__ void part_body(const float *logits, int64_t stride, i
 // on four waves, with a merge less; longer ones on eight.
 extern "C" __global__ void __launch_bounds__(256)
 pbx_logprobs_part_256(const float *logits, int64_t stride, int vocab, int parts, int top, Out out, float *sums,
-                      uint64_t *keys) {
-  part_body<256, 8>(logits, stride, vocab, parts, top, out, sums, keys);
+                      uint64_t *keys, int merged) {
+  part_body<256, 8>(logits, stride, vocab, parts, top, out, sums, keys, merged);
 }
 extern "C" __global__ void __launch_bounds__(512)
 pbx_logprobs_part_512(const float *logits, int64_t stride, int vocab, int parts, int top, Out out, float *sums,
-                      uint64_t *keys) {
-  part_body<512, 64>(logits, stride, vocab, parts, top, out, sums, keys);
+                      uint64_t *keys, int merged) {
+  part_body<512, 64>(logits, stride, vocab, parts, top, out, sums, keys, merged);
 }
 
-// A row's parts put together: one workgroup of four waves a row.
+// A row's parts put together in a launch of their own: one workgroup of four waves a row.
 extern "C" __global__ void __launch_bounds__(256)
 pbx_logprobs_join(const float *logits, int64_t stride, int vocab, int parts, int top, Out out, const float *sums,
                   const uint64_t *keys) {
   __shared__ float sbuf[4][4];
   __shared__ uint64_t kbuf[4][64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t row = blockIdx.x;
-  Sums a = {LOWEST, 0.f, 0.f};
-  for (int i = tid; i < parts; i += 256) {
-    const float *s = sums + 3 * (row * parts + i);
-    a = joined(a, {s[0], s[1], s[2]});
-  }
-  a = join_waves<4>(a, sbuf, wave, lane);
-  uint64_t key = 0;
-  if (top) {
-    const int n = parts * top;
-    for (int i = 64 * wave; i < n; i += 256)
-      key = merge_wave(key, sort_wave(i + lane < n ? keys[row * n + i + lane] : 0, lane, false), lane);
-    key = merge_waves<4>(key, kbuf, wave, lane);
-  }
-  if (!wave) answer(out, row, logits + row * stride, vocab, top, a, key, lane);
+  const float xt = logit_of(logits + row * stride, target_of(out, row), vocab);
+  join_parts<4>(parts, top, out, sums, keys, row, xt, sbuf, kbuf);
 }

@@ -285,3 +285,23 @@ def test_captured_calls_replay(ctx):
     hip.hipGraphDestroy(graph)
     for b in (*dx, dt, work, *outs):
         b.free()
+
+
+def test_rows_around_where_they_are_split(ctx):
+    """Vocabularies in one workgroup and in several, many rows over several workgroups each (joined in the same
+    launch, or past 512 rows in a second one)."""
+    rng = np.random.default_rng(8)
+    for rows, vocab, top in ((3, 35999, 9), (3, 36000, 32), (3, 36001, 32), (200, 36003, 3), (2, 131075, 32)):
+        print(f"[case] logprobs {rows} x {vocab}", flush=True)
+        x = (3 * rng.standard_normal((rows, vocab))).astype(np.float32)
+        check(ctx, x, rng.integers(0, vocab, rows), top)
+    x = np.tile((3 * rng.standard_normal((3, 131073))).astype(np.float32), (171, 1))  # 513 rows, two parts each
+    assert ctx.logprobs_workspace(513, 131073, 2) > 0
+    t = np.tile([5, 131072, 70000], 171)
+    logp, ent, ids, tops = run(ctx, x, t, 2)
+    rl, re, ri, rt, t1, t2 = reference(x[:3], t[:3], 2)
+    for r in range(0, 513, 3):
+        near(logp[r:r + 3], rl, t1)
+        near(ent[r:r + 3], re, t2)
+        assert np.array_equal(ids[r:r + 3], ri)
+        near(tops[r:r + 3], rt, t1[:, None] + np.zeros(rt.shape), 2.0 ** -22)
