@@ -60,12 +60,14 @@ __device__ __forceinline__ int value_byte(int key, int dim) {
 
 // x / s rounded half to even, as the true quotient.  In f32, x * (1 / s) of at
 // most 128 is off it by less than 2^-15, so only quotients nearer than 10^-4 to
-// a border (one in 5,000) need the division.
+// a border (one in 5,000) need the division.  A turned pair may be past f32's
+// range though both its keys are in it: q is then infinite, its distance from r a
+// NaN, and the comparison, which holds for no NaN, leaves the division to it too.
 __device__ __forceinline__ int code_of(double x, double s, float inv) {
   if (!(s > 0.0 && s < INFINITY)) return 0;
   const float q = (float)x * inv;
   float r = rintf(q);
-  if (fabsf(fabsf(q - r) - 0.5f) < 1e-4f) r = (float)rint(x / s);
+  if (!(fabsf(fabsf(q - r) - 0.5f) >= 1e-4f)) r = (float)rint(x / s);
   return (int)r;
 }
 
