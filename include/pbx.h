@@ -497,9 +497,11 @@ int pbx_kv_append_dev(pbx_kv_batch *b, int layer, const float *dQ, int64_t q_str
  * sequences: head h of a row at position p sees KV head h / (n_heads /
  * n_kv_heads) at positions 0..p.  scale: of the products (0: 1 /
  * sqrt(head_dim)).  Rows as above; dOut [n_rows][n_heads][head_dim], which may
- * be dQ itself.  Values are used as they stand in the cache, everything else in
- * 22 bits or more; the result of a row does not depend on the other rows'
- * values. */
+ * be dQ itself.  Values are used as they stand in the cache and sums are held in
+ * f32.  Queries enter with 22 bits (2^-25 of their row's largest at least), a
+ * probability with 22 bits, or 2^-30 of the largest in its block of
+ * PBX_KV_BLOCK positions where that is more.  The result of a row does not
+ * depend on the other rows' values. */
 int pbx_kv_attention_dev(pbx_kv_batch *b, int layer, const float *dQ, int64_t q_stride,
                          float scale, float *dOut, int64_t out_stride);
 /* The batch's rows of the cache as the values they stand for, f32 [n_rows]

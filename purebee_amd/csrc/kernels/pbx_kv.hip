@@ -350,13 +350,17 @@ __device__ __forceinline__ half8 halves(unsigned w0, unsigned w1) {
 // Score of a masked key and the running maximum before any visible one: finite,
 // so that differences of maxima need no special case.
 constexpr float NONE = -1e38f;
-// Probabilities are held times 2^6 (their sum too): an fp16 pair then keeps 22
-// bits of them down to 2^-9 of the row's largest, and some down to 2^-30 (more
-// would cost the exponentials' arguments bits: 12 left 1.3 times the error).
-// A row's maximum follows its scores only when they pass it by 2^SLACK (its
-// probabilities then reach 2^12, below fp16's largest): a new maximum rescales
-// all sums, and in some row of a tile nearly every block brings one.
-constexpr float LIFT = 6.f, SLACK = 6.f;
+// A row's probabilities in a block are taken against the block's own largest
+// score, rounded up to a whole number of powers of two, and times 2^LIFT: an fp16
+// pair then keeps 22 bits of them down to 2^-9 of the block's largest and resolves
+// 2^-30 of it below (more would cost the exponentials' arguments bits).  The block
+// joins the row's sums in f32 with its weight, a power of two, so keys far below
+// the row's largest keep their bits and add up, however many they are.
+// A row's maximum follows the blocks' only when they pass it by 2^SLACK: a new
+// maximum rescales all sums, and in some row of a tile nearly every block brings one.
+// (All of a row against one maximum was 0 to 2 % faster on prompts and lost what lay
+// below 2^-31 of it: a quarter of a tail of 4,000 keys behind one strong one.)
+constexpr float LIFT = 6.f, SLACK = 12.f;
 
 // Codes reach LDS by DMA (global_load_lds: lane i's 16 bytes land at the
 // instruction's LDS base + 16 i), without registers in between; waits are
@@ -559,15 +563,14 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
   }
   const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
   floatx4 acc[NQ][DT];
-  float m[NQ];
-  floatx4 l[NQ];  // a column's sum in every row: products with ones
+  float m[NQ], l[NQ];
   half8 ones;
 #pragma unroll
   for (int e = 0; e < 8; ++e) ones[e] = (_Float16)1.f;
 #pragma unroll
   for (int q = 0; q < NQ; ++q) {
     m[q] = NONE;
-    l[q] = zero;
+    l[q] = 0.f;
 #pragma unroll
     for (int i = 0; i < DT; ++i) acc[q][i] = zero;
   }
@@ -626,7 +629,7 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
       if (ahead < n) fetch_keys(next, 0);
     }
     half8 ph[NQ], pl[NQ];
-    float mn[NQ], sv[NQ];
+    float mn[NQ], sv[NQ], wt[NQ];
     bool moved = false;
     const bool whole = b * BLK + BLK - 1 <= first_pos;  // every live row sees the block
 #pragma unroll
@@ -648,11 +651,14 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
 #pragma unroll
       for (int e = 1; e < 8; ++e) mx = __builtin_amdgcn_fmed3f(mx, s[q][e >> 2][e & 3], inf);
       mx = pair_max<32>(pair_max<16>(mx));
-      mx *= f;
+      // (a row that sees nothing of the block has -inf here)
+      mx = __builtin_amdgcn_fmed3f(__builtin_ceilf(mx * f), NONE, inf);
       const bool up = mx > m[q] + SLACK;
       mn[q] = up ? mx : m[q];
       moved = moved || up;
-      const float base = mn[q] - LIFT;
+      const float base = mx - LIFT;  // whole numbers: exact, as the weight is
+      wt[q] = __builtin_amdgcn_exp2f(base - mn[q]);
+      sv[q] *= wt[q];
       float p[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(fmaf(s[q][e >> 2][e & 3], f, -base));
@@ -668,10 +674,13 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
         for (int d = 0; d < DT; ++d) acc[q][d] *= al;
       }
     }
+    floatx4 bl[NQ];  // a column's sum in every row: products with ones
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) l[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[q], l[q], 0, 0, 0);
+    for (int q = 0; q < NQ; ++q) bl[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[q], zero, 0, 0, 0);
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) l[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[q], l[q], 0, 0, 0);
+    for (int q = 0; q < NQ; ++q) bl[q] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pl[q], bl[q], 0, 0, 0);
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) l[q] = fmaf(bl[q][0], wt[q], l[q]);
     if constexpr (RING == 1) {
       if (ahead < n)
         wait_vm<NI>();
@@ -713,7 +722,7 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
 #pragma unroll
       for (int w = 1; w < KW; ++w) M = fmaxf(M, mrg_m[qw * KW + w][q][c]);
       const float f = __builtin_amdgcn_exp2f(m[q] - M);
-      if (g == 0) mrg_l[wave][q][c] = l[q][0] * f;
+      if (g == 0) mrg_l[wave][q][c] = l[q] * f;
       m[q] = M;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
@@ -742,7 +751,7 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
       }
     } else {
       o = acc[q][u % DT];
-      sum = l[q][0];
+      sum = l[q];
     }
     if (r >= rows) continue;
     if (parts > 1) {

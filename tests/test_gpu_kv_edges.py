@@ -2,6 +2,7 @@
 import numpy as np
 import pytest
 
+from tests.kv_ref import Rows, within
 from tests.test_gpu_kv import Pair
 
 pytestmark = pytest.mark.gpu
@@ -31,3 +32,78 @@ def test_keys_that_leave_f32_when_turned(ctx, style, held):
     assert past.min() < 110 and past.max() == 127   # past f32's largest, not only at the largest code
     p.check_values([0])
     p.free()
+
+
+def one_key_and_a_tail(ctx, heads, kv_heads, dim, past, rows, at, strength, others=0):
+    """`rows` query rows after `past` positions whose keys and values are alike but for one, at `at`, whose score is
+    `strength` (natural) above the others' and whose value is 0: the answer is the others' alone.  `others` sequences hold
+    the same and are in the batch.
+
+    The bound is RefCache.attention's for roundings relative to each probability, and one for what a probability far below
+    its block's largest loses: a pair of fp16 resolves 2^-25, a block's largest is held above 2^5, so 2^-30 of it each
+    (2^-36 and less of the sums that other blocks bring), counted for the sum as well."""
+    n, seqs = past + rows, 1 + others
+    p = Pair(ctx, heads, kv_heads, dim, seqs=seqs, n_pages=seqs * -(-n // 64), page=64, max_seq=8192, style="none",
+             seed=int(strength) * 100 + n)
+    k = np.zeros((n, kv_heads, dim), np.float32)
+    k[..., 1] = 0.25
+    k[at, :, 0] = 2 * strength
+    v = (1 + 0.1 * p.rng.standard_normal(k.shape)).astype(np.float32)
+    v[at] = 0
+    q = np.zeros((n, heads, dim), np.float32)
+    q[..., 0] = np.sqrt(dim) / 2 * (1 + 0.02 * p.rng.random((n, heads)))
+    q[..., 1] = p.rng.standard_normal((n, heads))
+    part = lambda a, e: tuple(x[a:e] for x in (q, k, v))  # noqa: E731
+    p.append([0], [past], part(0, past))
+    _, qr = p.append([0], [rows], part(past, n))
+    dk, dv = Rows(ctx, n, kv_heads * dim, k), Rows(ctx, n, kv_heads * dim, v)
+    for s in range(1, seqs):
+        for a, m in ((0, past), (past, rows)):
+            p.cache.batch([s], [m]).append_dev(0, None, dk.ptr + 4 * a * dk.width, dv.ptr + 4 * a * dv.width, None)
+    b = p.cache.batch(range(seqs), [rows] * seqs, [past] * seqs)
+    want, tol = p.ref.attention([0], [past], [rows], qr)
+    kk, vv = p.ref.k[0].values().astype(np.float64), p.ref.v[0].values().astype(np.float64)
+    for t in range(rows):
+        e = past + t + 1
+        for h in range(heads):
+            g = h // (heads // kv_heads)
+            x = kk[:e, g] @ qr[t, h].astype(np.float64) / np.sqrt(dim)
+            pr = np.exp(x - x.max())
+            pr /= pr.sum()
+            top = np.repeat(np.maximum.reduceat(pr, np.arange(0, e, 32)), 32)[:e] * 2.0 ** -30
+            tol[t, h] += top @ np.abs(vv[:e, g]) + top.sum() * np.abs(want[t, h])
+    w = heads * dim
+    dq, do = Rows(ctx, seqs * rows, w, np.tile(qr, (seqs, 1, 1))), Rows(ctx, seqs * rows, w)
+    b.attention_dev(0, dq.ptr, do.ptr)
+    ctx.sync()
+    for got in do.get().reshape(seqs, *want.shape):
+        within(got, want, tol)
+    for x in (dq, do, dk, dv):
+        x.free()
+    p.free()
+
+
+@pytest.mark.parametrize("strength", [6, 9, 13, 18, 23, 40])
+@pytest.mark.parametrize("past,at", [(300, 0), (300, 37), (300, 298), (6000, 0), (6000, 3000), (6000, 5998)])
+@pytest.mark.parametrize("rows", [1, 24])
+def test_one_key_before_a_long_tail(ctx, strength, past, at, rows):
+    """Keys far below a row's largest add up: none is lost to the one that outweighs them, in whole and in split contexts."""
+    print(f"[case] one key {strength} above {past}, at {at}, {rows} rows", flush=True)
+    one_key_and_a_tail(ctx, 8, 2, 64, past, rows, at, strength)
+
+
+@pytest.mark.parametrize("dim", [32, 96, 128, 192, 256])
+@pytest.mark.parametrize("past", [200, 3000])
+@pytest.mark.parametrize("rows", [1, 9])
+def test_one_key_before_a_tail_by_head_size(ctx, dim, past, rows):
+    print(f"[case] one key, heads of {dim}, {past}, {rows} rows", flush=True)
+    one_key_and_a_tail(ctx, 4, 2, dim, past, rows, 70, 16)
+
+
+@pytest.mark.parametrize("strength", [13, 16, 18, 20, 21, 23])
+@pytest.mark.parametrize("heads,kv_heads,dim,past,rows", [(16, 8, 64, 4000, 1), (8, 8, 64, 2500, 40), (8, 8, 128, 4000, 1),
+                                                          (8, 8, 256, 4000, 1)])
+def test_one_key_before_tails_that_are_not_split(ctx, strength, heads, kv_heads, dim, past, rows):
+    """As many sequences as fill the GPU: a wave goes through a quarter or half of a context by itself."""
+    print(f"[case] one key {strength} above {past}, heads of {dim}, {rows} rows, 64 sequences", flush=True)
+    one_key_and_a_tail(ctx, heads, kv_heads, dim, past, rows, 0, strength, others=63)
