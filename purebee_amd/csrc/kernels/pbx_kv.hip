@@ -365,6 +365,8 @@ constexpr float LIFT = 6.f, SLACK = 12.f;
 // Codes reach LDS by DMA (global_load_lds: lane i's 16 bytes land at the
 // instruction's LDS base + 16 i), without registers in between; waits are
 // counted by hand, so every wave issues the same number of them for a block.
+// M0 is the compiler's own (no asm may name it as clobbered): it writes it right
+// before each use, and nothing else in these kernels uses it.
 __device__ __forceinline__ unsigned lds_address(const void *p) {
   return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) void *)p;
 }
@@ -377,6 +379,9 @@ template <int N>
 __device__ __forceinline__ void wait_vm() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
+
+// The wave's LDS reads so far have their values: what they read may be fetched over.
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // A constant that the compiler cannot see through.
 __device__ __forceinline__ float opaque(float x) {
@@ -592,6 +597,7 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
     if constexpr (RING > 1) {
       // into the slot of the block before, which has been read
       if (ahead < n) {
+        wait_lds();
         const int to = slot ? slot - 1 : RING - 1;
         fetch_keys(next, to);
         fetch_values(next, to);
@@ -626,6 +632,7 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
       }
     }
     if constexpr (RING == 1) {
+      wait_lds();
       if (ahead < n) fetch_keys(next, 0);
     }
     half8 ph[NQ], pl[NQ];
@@ -706,6 +713,7 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
       }
     }
     if constexpr (RING == 1) {
+      wait_lds();
       if (ahead < n) fetch_values(next, 0);
     }
   }
