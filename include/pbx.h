@@ -474,7 +474,9 @@ int pbx_kv_truncate(pbx_kv *kv, int seq, int n_tokens);
  * work captured from one batch into graphs is replayed on one stream at a time.
  * A batch whose calls were captured keeps its rows (set refuses, PBX_EINVAL):
  * a replay runs over the same positions, which the sequences must still hold
- * (and, if it appends, end with), and the batch lives as long as the graph.
+ * (and, if it appends, end with), and the batch lives as long as the graph (a
+ * batch whose capture was thrown away is freed, and another one set).  A call
+ * that is refused, or has no rows, holds nothing.
  * Inside a capture no cache or batch is made, set or freed (PBX_EINVAL).
  * Positions that a batch took hold nothing defined until they are appended.
  */

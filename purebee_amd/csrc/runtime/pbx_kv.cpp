@@ -390,6 +390,14 @@ extern "C" int pbx_kv_batch_set(pbx_kv_batch *b, int n, const int32_t *seqs, con
   return PBX_OK;
 }
 
+// A launch of a batch's call; one that goes into a graph holds the batch's rows from then on.
+static int batch_launch(pbx_kv_batch *b, hipFunction_t f, const char *name, int64_t grid, int block, void **args) {
+  pbx_ctx *c = b->kv->c;
+  const int rc = kv_launch(c, f, name, grid, block, args);
+  if (!rc && capturing(c)) b->captured = true;
+  return rc;
+}
+
 // What the three calls check alike; fills the kernels' view of the layer.
 static int batch_begin(pbx_kv_batch *b, const char *who, int layer, KvArgsHost *a) {
   if (!batch_ok(b)) return pbx_fail(nullptr, PBX_EINVAL, "%s: not a live batch", who);
@@ -403,7 +411,6 @@ static int batch_begin(pbx_kv_batch *b, const char *who, int layer, KvArgsHost *
   if (hipSetDevice(c->device) != hipSuccess) return pbx_fail(c, PBX_EHIP, "%s: hipSetDevice failed", who);
   *a = {kv->codes + layer * kv->layer_codes, kv->scales + layer * kv->layer_scales, g.n_kv_heads,
         g.n_heads / g.n_kv_heads, g.head_dim, kv->page_shift};
-  if (capturing(c)) b->captured = true;
   return PBX_OK;
 }
 
@@ -456,8 +463,8 @@ extern "C" int pbx_kv_append_dev(pbx_kv_batch *b, int layer, const float *dQ, in
   const int n_blocks = (int)b->plan.blocks.size(), n_rows = b->plan.n_rows;
   void *args[] = {&a, &r, &items, (void *)&n_blocks, &pos, (void *)&n_rows, &dK, &k_stride, &dV, &v_stride,
                   &dQ, &q_stride, &dQout, &qout_stride};
-  return kv_launch(c, kv->append, "pbx_kv_append", (int64_t)n_blocks * g.n_kv_heads + (dQ ? n_rows : 0),
-                   kv_threads(kv->hdp), args);
+  return batch_launch(b, kv->append, "pbx_kv_append", (int64_t)n_blocks * g.n_kv_heads + (dQ ? n_rows : 0),
+                      kv_threads(kv->hdp), args);
 }
 
 extern "C" int pbx_kv_attention_dev(pbx_kv_batch *b, int layer, const float *dQ, int64_t q_stride, float scale,
@@ -482,7 +489,7 @@ extern "C" int pbx_kv_attention_dev(pbx_kv_batch *b, int layer, const float *dQ,
     const int n = b->plan.n_attn[k];
     if (!n) continue;
     void *args[] = {&a, &items, &table, &dQ, &q_stride, &scale, &dOut, &out_stride, &b->part, &b->arrived};
-    if ((rc = kv_launch(c, kv->attn[k], "pbx_kv_attn", (int64_t)n * g.n_kv_heads, 256, args))) return rc;
+    if ((rc = batch_launch(b, kv->attn[k], "pbx_kv_attn", (int64_t)n * g.n_kv_heads, 256, args))) return rc;
     items += n * (sizeof(kv_attn_item) / 4);
   }
   return PBX_OK;
@@ -503,6 +510,6 @@ extern "C" int pbx_kv_read_dev(pbx_kv_batch *b, int layer, float *dK, int64_t k_
     return rc;
   const int32_t *items = b->dev;
   void *args[] = {&a, &items, &dK, &k_stride, &dV, &v_stride};
-  return kv_launch(c, kv->read, "pbx_kv_read", (int64_t)b->plan.blocks.size() * g.n_kv_heads,
-                   kv_threads(kv->hdp), args);
+  return batch_launch(b, kv->read, "pbx_kv_read", (int64_t)b->plan.blocks.size() * g.n_kv_heads,
+                      kv_threads(kv->hdp), args);
 }

@@ -1,9 +1,12 @@
-"""The paged KV cache at the ends of its numbers, against tests/kv_ref.py."""
+"""The paged KV cache at the ends of its numbers, against tests/kv_ref.py, and around captures."""
+import ctypes
+
 import numpy as np
 import pytest
 
+import purebee_amd as pb
 from tests.kv_ref import Rows, within
-from tests.test_gpu_kv import Pair
+from tests.test_gpu_kv import Pair, _hip
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +110,40 @@ def test_one_key_before_tails_that_are_not_split(ctx, strength, heads, kv_heads,
     """As many sequences as fill the GPU: a wave goes through a quarter or half of a context by itself."""
     print(f"[case] one key {strength} above {past}, heads of {dim}, {rows} rows, 64 sequences", flush=True)
     one_key_and_a_tail(ctx, heads, kv_heads, dim, past, rows, 0, strength, others=63)
+
+
+def test_calls_that_a_capture_does_not_hold_leave_the_batch_free(ctx):
+    """Refused calls, and those of a batch without rows, put nothing into a graph: the batch can be set again after them."""
+    hip = _hip()
+    p = Pair(ctx, 4, 2, 64, seed=41)
+    b, q = p.append([0], [50])
+    none = p.cache.batch([0], [0])
+    x = Rows(ctx, 50, 256, q)
+    stream, graph = ctypes.c_void_p(ctx.stream()), ctypes.c_void_p()
+    assert hip.hipStreamBeginCapture(stream, 0) == 0
+    for call in (lambda: b.attention_dev(0, None, x.ptr), lambda: b.attention_dev(0, x.ptr, x.ptr, float("nan")),
+                 lambda: b.attention_dev(1, x.ptr, x.ptr), lambda: b.append_dev(0, x.ptr, None, x.ptr, x.ptr),
+                 lambda: b.append_dev(0, x.ptr, x.ptr, x.ptr, x.ptr, q_stride=252), lambda: b.read_dev(0, x.ptr + 4, None)):
+        with pytest.raises(pb.PbxError):
+            call()
+    b.read_dev(0, None, None)           # nothing is asked for
+    none.append_dev(0, None, None, None, None)
+    none.attention_dev(0, None, None)
+    none.read_dev(0, x.ptr, x.ptr)
+    assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+    hip.hipGraphDestroy(graph)
+    none.set([0], [0])
+    b.set([0], [50], [0])
+    p.attend(b, [0], [0], [50], q)
+    # a call that a graph does hold keeps the batch's rows, thrown away or not; another batch takes its place
+    assert hip.hipStreamBeginCapture(stream, 0) == 0
+    b.attention_dev(0, x.ptr, x.ptr)
+    assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+    hip.hipGraphDestroy(graph)
+    with pytest.raises(pb.PbxError, match="captured"):
+        b.set([0], [50], [0])
+    b.free()
+    b = p.cache.batch([0], [50], [0])
+    p.attend(b, [0], [0], [50], q)
+    x.free()
+    p.free()
