@@ -536,7 +536,9 @@ int pbx_logprobs_dev(pbx_ctx *ctx, const float *dLogits, int64_t stride, int64_t
 /* pbx_model_forward_batch that answers with log probabilities instead of n
  * rows of logits: row t's target is targets[t] (usually tokens[t + 1]; outside
  * the vocabulary: NaN).  Host arrays [n_tokens] or [n_tokens][top], as above;
- * any of the four outputs may be NULL (logp is needed with targets). */
+ * any of the four outputs may be NULL (logp is needed with targets).  Waits for
+ * its answers, so it is refused while the context's stream is captured, as
+ * pbx_model_forward_kv is. */
 int pbx_model_logprobs(pbx_model *m, const int32_t *tokens, int n_tokens, int start_pos,
                        const int32_t *targets, int top, float *logp, float *entropy,
                        int32_t *top_ids, float *top_logp);
@@ -547,8 +549,8 @@ int pbx_model_logprobs(pbx_model *m, const int32_t *tokens, int n_tokens, int st
  * PBX_ROPE_PAIRS with the model's rope_theta is the model's own.  Answers for
  * every row (all_rows), or for the last row of each sequence that has one, in
  * the batch's order: logits [rows][vocab], next_tokens (argmax), and the four
- * of pbx_model_logprobs with targets [rows]; each may be NULL.  Blocks until
- * they are there.  A forward that fails leaves its rows of the cache undefined. */
+ * of pbx_model_logprobs with targets [rows]; each may be NULL.  At most
+ * 65,535 rows.  Blocks until the answers are there.  A forward that fails leaves its rows of the cache undefined. */
 int pbx_model_forward_kv(pbx_model *m, pbx_kv_batch *b, const int32_t *tokens, int all_rows,
                          float *logits, int32_t *next_tokens, const int32_t *targets, int top,
                          float *logp, float *entropy, int32_t *top_ids, float *top_logp);

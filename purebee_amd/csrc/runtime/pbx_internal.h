@@ -205,6 +205,10 @@ int pbx_gemm_launch(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M,
 size_t pbx_type_row_bytes(int type, int64_t K);
 void pbx_model_release_all(pbx_ctx *c);
 void pbx_kv_release_all(pbx_ctx *c);
+// Whether the context's stream is being captured; and PBX_EINVAL if so, for calls
+// that wait for the stream.
+bool pbx_capturing(pbx_ctx *c);
+int pbx_not_capturing(pbx_ctx *c, const char *who);
 int pbx_model_clear_range(pbx_model *m, int from, int to);
 // pbx_model_generate with every step stopping after the first max_layers
 // layers (0: all); the self-speculative draft.

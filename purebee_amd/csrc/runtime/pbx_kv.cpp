@@ -80,14 +80,14 @@ static int kv_launch(pbx_ctx *c, hipFunction_t f, const char *name, int64_t grid
   return pbx_launch_fn(c, f, name, dim3((unsigned)grid), dim3(block), args, c->stream);
 }
 
-static bool capturing(pbx_ctx *c) {
+bool pbx_capturing(pbx_ctx *c) {
   hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
   return hipStreamIsCapturing(c->stream, &st) != hipSuccess || st != hipStreamCaptureStatusNone;
 }
 
 // Creating and freeing wait for the stream, which would end a capture.
-static int not_capturing(pbx_ctx *c, const char *who) {
-  return capturing(c) ? pbx_fail(c, PBX_EINVAL, "%s: the context's stream is being captured", who) : PBX_OK;
+int pbx_not_capturing(pbx_ctx *c, const char *who) {
+  return pbx_capturing(c) ? pbx_fail(c, PBX_EINVAL, "%s: the context's stream is being captured", who) : PBX_OK;
 }
 
 static void batch_release(pbx_kv_batch *b) {
@@ -210,7 +210,7 @@ extern "C" int pbx_kv_create(pbx_ctx *c, const pbx_kv_config *cfg, pbx_kv **out)
   if (!cfg || !out) return pbx_fail(c, PBX_EINVAL, "pbx_kv_create: NULL argument");
   *out = nullptr;
   int rc = kv_check(c, *cfg);
-  if (rc || (rc = not_capturing(c, "pbx_kv_create"))) return rc;
+  if (rc || (rc = pbx_not_capturing(c, "pbx_kv_create"))) return rc;
   pbx_kv *kv = nullptr;
   try {
     kv = new pbx_kv();
@@ -233,7 +233,7 @@ extern "C" int pbx_kv_free(pbx_kv *kv) {
   if (!kv) return PBX_OK;
   if (!kv_ok(kv)) return pbx_fail(nullptr, PBX_EINVAL, "pbx_kv_free: not a live cache");
   pbx_ctx *c = kv->c;
-  if (const int rc = not_capturing(c, "pbx_kv_free")) return rc;
+  if (const int rc = pbx_not_capturing(c, "pbx_kv_free")) return rc;
   hipSetDevice(c->device);
   hipStreamSynchronize(c->stream);
   auto *list = (std::vector<pbx_kv *> *)c->kvs;
@@ -271,7 +271,7 @@ extern "C" int pbx_kv_batch_create(pbx_kv *kv, pbx_kv_batch **out) {
   if (!kv_ok(kv)) return pbx_fail(nullptr, PBX_EINVAL, "pbx_kv_batch_create: not a live cache");
   if (!out) return pbx_fail(kv->c, PBX_EINVAL, "pbx_kv_batch_create: NULL argument");
   *out = nullptr;
-  if (const int rc = not_capturing(kv->c, "pbx_kv_batch_create")) return rc;
+  if (const int rc = pbx_not_capturing(kv->c, "pbx_kv_batch_create")) return rc;
   try {
     kv->batches.reserve(kv->batches.size() + 1);
     pbx_kv_batch *b = new pbx_kv_batch();
@@ -293,7 +293,7 @@ extern "C" int pbx_kv_batch_free(pbx_kv_batch *b) {
   if (!b) return PBX_OK;
   if (!batch_ok(b)) return pbx_fail(nullptr, PBX_EINVAL, "pbx_kv_batch_free: not a live batch");
   pbx_kv *kv = b->kv;
-  if (const int rc = not_capturing(kv->c, "pbx_kv_batch_free")) return rc;
+  if (const int rc = pbx_not_capturing(kv->c, "pbx_kv_batch_free")) return rc;
   hipSetDevice(kv->c->device);
   hipStreamSynchronize(kv->c->stream);
   kv->batches.erase(std::remove(kv->batches.begin(), kv->batches.end(), b), kv->batches.end());
@@ -358,7 +358,7 @@ extern "C" int pbx_kv_batch_set(pbx_kv_batch *b, int n, const int32_t *seqs, con
     return pbx_fail(c, PBX_EINVAL, "pbx_kv_batch_set: bad arguments");
   if (hipSetDevice(c->device) != hipSuccess)
     return pbx_fail(c, PBX_EHIP, "pbx_kv_batch_set: hipSetDevice failed");
-  if (b->captured || capturing(c))
+  if (b->captured || pbx_capturing(c))
     return pbx_fail(c, PBX_EINVAL, "pbx_kv_batch_set: the batch's calls are captured in a graph, or its stream "
                     "is being captured");
   try {
@@ -394,7 +394,7 @@ extern "C" int pbx_kv_batch_set(pbx_kv_batch *b, int n, const int32_t *seqs, con
 static int batch_launch(pbx_kv_batch *b, hipFunction_t f, const char *name, int64_t grid, int block, void **args) {
   pbx_ctx *c = b->kv->c;
   const int rc = kv_launch(c, f, name, grid, block, args);
-  if (!rc && capturing(c)) b->captured = true;
+  if (!rc && pbx_capturing(c)) b->captured = true;
   return rc;
 }
 

@@ -2281,7 +2281,8 @@ extern "C" int pbx_model_logprobs(pbx_model *m, const int32_t *tokens, int n_tok
   const char *who = "pbx_model_logprobs";
   if (!model_ok(m)) return pbx_fail(nullptr, PBX_EINVAL, "%s: not a live model", who);
   const LogprobsWanted w{targets, top, logp, entropy, top_ids, top_logp};
-  const int rc = check_logprobs(m, who, w);
+  int rc = check_logprobs(m, who, w);
+  if (!rc) rc = pbx_not_capturing(m->c, who);
   return rc ? rc : forward_rows(m, who, tokens, n_tokens, start_pos, nullptr, nullptr, w);
 }
 
@@ -2296,7 +2297,7 @@ extern "C" int pbx_model_forward_kv(pbx_model *m, pbx_kv_batch *b, const int32_t
   int rc = pbx_kv_batch_look(b, &v);
   if (rc) return pbx_fail(c, rc, "%s: not a live batch that is set", who);
   const LogprobsWanted w{targets, top, logp, entropy, top_ids, top_logp};
-  if ((rc = check_logprobs(m, who, w))) return rc;
+  if ((rc = check_logprobs(m, who, w)) || (rc = pbx_not_capturing(c, who))) return rc;
   if (v.ctx != c) return pbx_fail(c, PBX_EINVAL, "%s: model and cache of different contexts", who);
   if (v.cfg->n_layers != g.n_layers || v.cfg->n_heads != g.n_heads || v.cfg->n_kv_heads != g.n_kv_heads ||
       v.cfg->head_dim != g.head_dim)

@@ -7,6 +7,7 @@ import pytest
 import purebee_amd as pb
 from tests.kv_ref import Rows, within
 from tests.test_gpu_kv import Pair, _hip
+from tests.test_gpu_model_kv import CONFIGS, Server
 
 pytestmark = pytest.mark.gpu
 
@@ -147,3 +148,38 @@ def test_calls_that_a_capture_does_not_hold_leave_the_batch_free(ctx):
     p.attend(b, [0], [0], [50], q)
     x.free()
     p.free()
+
+
+def test_forwards_wait_and_are_refused_in_a_capture(ctx):
+    """forward_kv and logprobs wait for their answers: inside a capture they are refused before they begin, the capture goes
+    on, and the batch stays free."""
+    hip = _hip()
+    s = Server(ctx, CONFIGS["f32"])
+    tokens = np.arange(1, 41, dtype=np.int32)
+    b = s.cache.batch([0], [40])
+    want = s.model.forward_kv(b, tokens)[0]
+    lp = s.model.logprobs(tokens, 0, tokens)
+    k = Rows(ctx, 40, 64)
+    stream, graph, gexec = ctypes.c_void_p(ctx.stream()), ctypes.c_void_p(), ctypes.c_void_p()
+    other = s.cache.batch([0], [40], [0])
+    other.read_dev(0, k.ptr, None)
+    ctx.sync()
+    held = k.get()
+    assert hip.hipStreamBeginCapture(stream, 0) == 0
+    other.read_dev(0, k.ptr, None)
+    for call in (lambda: s.model.forward_kv(b, tokens), lambda: s.model.logprobs(tokens, 0, tokens)):
+        with pytest.raises(pb.PbxError, match="captured"):
+            call()
+    assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(ctypes.byref(gexec), graph, None, None, 0) == 0
+    for _ in range(3):
+        k.buf.upload(k.host)
+        assert hip.hipGraphLaunch(gexec, stream) == 0
+        ctx.sync()
+        assert np.array_equal(k.get(), held)
+        assert np.array_equal(s.model.forward_kv(b.set([0], [40], [0]), tokens)[0], want)
+        assert np.array_equal(s.model.logprobs(tokens, 0, tokens)["logp"], lp["logp"])
+    hip.hipGraphExecDestroy(gexec)
+    hip.hipGraphDestroy(graph)
+    k.free()
+    s.free()
