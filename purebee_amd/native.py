@@ -497,12 +497,18 @@ def _logprobs_arrays(rows, targets, top):
 
 class KvCache:
     """A paged 8-bit KV cache that many sequences share (pbx_kv_*): n_pages pages
-    of page_tokens positions, sequence ids 0..max_seqs - 1."""
+    of page_tokens positions, sequence ids 0..max_seqs - 1.
+
+    The cache's rotation is the one that counts, in Model.forward_kv too.
+    rope_theta left out is 10000, which a model of another theta refuses; one that
+    is given is taken as meant."""
 
     def __init__(self, ctx, n_layers, n_heads, n_kv_heads, head_dim, n_pages, max_seqs, max_seq,
-                 page_tokens=64, rope="pairs", rope_dim=0, rope_theta=10000.0, rope_scale=1.0,
+                 page_tokens=64, rope="pairs", rope_dim=0, rope_theta=None, rope_scale=1.0,
                  rope_factors=None):
         self.ctx = ctx
+        self._theta_given = rope_theta is not None
+        rope_theta = rope_theta if self._theta_given else 10000.0
         self._kv = None
         f = None if rope_factors is None else np.ascontiguousarray(rope_factors, np.float32)
         style = ROPE[rope]
@@ -762,6 +768,9 @@ class Model:
         toks = np.ascontiguousarray(tokens, np.int32)
         if len(toks) != batch.rows:
             raise ValueError(f"{len(toks)} tokens for {batch.rows} rows")
+        kv = batch.cache
+        if not kv._theta_given and kv.cfg.rope_style and kv.cfg.rope_theta != self.cfg.rope_theta:
+            raise ValueError(f"the cache was made without rope_theta, which is {self.cfg.rope_theta} in this model")
         rows = len(toks) if all_rows else batch.sequences
         logits = np.empty((rows, self.vocab), np.float32) if want_logits else None
         nxt = np.empty(rows, np.int32)

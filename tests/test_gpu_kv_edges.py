@@ -183,3 +183,28 @@ def test_forwards_wait_and_are_refused_in_a_capture(ctx):
     hip.hipGraphDestroy(graph)
     k.free()
     s.free()
+
+
+def test_a_cache_whose_theta_was_left_out(ctx):
+    """A model of another theta than the default refuses it (its tokens would be wrong without an error); a rotation that
+    was given is taken as meant."""
+    s = Server(ctx, dict(CONFIGS["f32"], rope_theta=500000.0))
+    tokens = [1, 2, 3]
+    want = s.model.forward_kv(s.cache.batch([0], [3]), tokens)[0]
+    shape = (ctx, 2, 4, 2, 32, 8, 2, 64)
+    left_out = pb.KvCache(*shape)
+    with pytest.raises(ValueError, match="500000"):
+        s.model.forward_kv(left_out.batch([0], [3]), tokens)
+    for kw, same in ((dict(rope_theta=500000.0), True), (dict(rope_theta=10000.0), False), (dict(rope="none"), False),
+                     (dict(rope_theta=500000.0, rope_scale=2.0), False), (dict(rope="halves", rope_theta=500000.0), False)):
+        c = pb.KvCache(*shape, **kw)
+        assert np.array_equal(s.model.forward_kv(c.batch([0], [3]), tokens)[0], want) == same, kw
+        c.free()
+    left_out.free()
+    s.free()
+    s = Server(ctx, CONFIGS["f32"])     # the default is this model's
+    want = s.model.forward_kv(s.cache.batch([0], [3]), tokens)[0]
+    left_out = pb.KvCache(*shape)
+    assert np.array_equal(s.model.forward_kv(left_out.batch([0], [3]), tokens)[0], want)
+    left_out.free()
+    s.free()
