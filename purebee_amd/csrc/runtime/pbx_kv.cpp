@@ -363,8 +363,6 @@ extern "C" int pbx_kv_batch_set(pbx_kv_batch *b, int n, const int32_t *seqs, con
                     "is being captured");
   try {
     std::string why;
-    std::vector<int> before;
-    for (const kv_seq &s : kv->pages.seqs) before.push_back(s.len);
     kv_batch_plan plan;
     int rc = kv_plan_rows(&kv->pages, n, seqs, starts, counts, &plan, &why);
     if (rc) return pbx_fail(c, rc, "pbx_kv_batch_set: %s", why.c_str());
@@ -378,8 +376,7 @@ extern "C" int pbx_kv_batch_set(pbx_kv_batch *b, int n, const int32_t *seqs, con
       rc = pbx_fail(c, PBX_ENOMEM, "pbx_kv_batch_set: out of host memory");
     }
     if (rc) {  // the sequences stay as they were
-      for (size_t s = 0; s < before.size(); ++s)
-        if (kv->pages.seqs[s].len > before[s]) kv->pages.truncate((int)s, before[s], &why);
+      kv_plan_undo(&kv->pages, b->plan);
       return rc;
     }
   } catch (const std::bad_alloc &) {

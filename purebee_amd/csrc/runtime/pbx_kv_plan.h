@@ -16,11 +16,13 @@
 
 struct kv_seq {
   int len = 0;
+  uint64_t met = 0;  // the last batch that named it (kv_pages::batches)
   std::vector<int32_t> pages;
 };
 
 struct kv_pages {
   int page_tokens = 0, max_seq = 0;
+  uint64_t batches = 0;  // planned so far, refused ones too
   std::vector<int32_t> free_list;  // handed out from the back
   std::vector<kv_seq> seqs;
 
@@ -79,6 +81,7 @@ struct kv_batch_plan {
   int n_rows = 0;
   bool last = true;  // the rows are the last of their sequences
   std::vector<int32_t> seqs, starts, counts;
+  std::vector<int32_t> had;  // the sequences' lengths before
   // work lists, in the order they lie in device memory
   std::vector<kv_block_item> blocks;
   std::vector<kv_attn_item> attn;  // those of u 1, then 2, 4, 8
@@ -90,18 +93,19 @@ struct kv_batch_plan {
 };
 
 // Checks a batch and, if it holds, takes its pages and fills the plan; refused
-// batches change nothing.
+// batches change nothing.  Costs what the batch is, however many sequences the
+// cache could hold.
 inline int kv_plan_rows(kv_pages *kv, int n, const int32_t *seqs, const int32_t *starts,
                         const int32_t *counts, kv_batch_plan *p, std::string *why) {
   char buf[200];
-  std::vector<char> seen(kv->seqs.size(), 0);
+  ++kv->batches;
   int64_t rows = 0, need = 0;
   for (int i = 0; i < n; ++i) {
     const int s = seqs[i];
     buf[0] = 0;
     if (s < 0 || s >= (int)kv->seqs.size()) {
       snprintf(buf, sizeof buf, "sequence %d outside [0, %d)", s, (int)kv->seqs.size());
-    } else if (seen[s]) {
+    } else if (kv->seqs[s].met == kv->batches) {
       snprintf(buf, sizeof buf, "sequence %d twice in one batch", s);
     } else if (counts[i] < 0) {
       snprintf(buf, sizeof buf, "sequence %d: %d rows", s, counts[i]);
@@ -119,7 +123,7 @@ inline int kv_plan_rows(kv_pages *kv, int n, const int32_t *seqs, const int32_t 
       *why = buf;
       return PBX_EINVAL;
     }
-    seen[s] = 1;
+    kv->seqs[s].met = kv->batches;
     rows += counts[i];
   }
   if (rows > (1 << 26)) {
@@ -138,6 +142,7 @@ inline int kv_plan_rows(kv_pages *kv, int n, const int32_t *seqs, const int32_t 
     q.seqs.push_back(seqs[i]);
     q.starts.push_back(starts ? starts[i] : s.len);
     q.counts.push_back(counts[i]);
+    q.had.push_back(s.len);
     s.pages.reserve(kv->pages_of(q.starts[i] + counts[i]));
   }
   q.n_rows = (int)rows;
@@ -154,6 +159,13 @@ inline int kv_plan_rows(kv_pages *kv, int n, const int32_t *seqs, const int32_t 
   }
   std::swap(*p, q);
   return PBX_OK;
+}
+
+// Takes a planned batch back (before another one is planned): the lengths and
+// pages are as they were.
+inline void kv_plan_undo(kv_pages *kv, const kv_batch_plan &p) {
+  std::string why;
+  for (size_t i = p.seqs.size(); i-- > 0;) kv->truncate(p.seqs[i], p.had[i], &why);
 }
 
 #define KV_MAX_PARTS 64
