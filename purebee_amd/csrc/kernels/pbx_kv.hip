@@ -134,7 +134,7 @@ constexpr int append_threads(int hdp) { return hdp <= 64 ? 256 : 4 * hdp; }
 
 template <int HDP>
 __device__ __forceinline__ void append_body(const KvArgs &a, const KvRope &r, const BlockItem *items,
-                                            int n_blocks, const int *row_pos, int n_rows, const float *K,
+                                            int n_blocks, const int *row_pos, const float *K,
                                             int64_t ks, const float *V, int64_t vs, const float *Q, int64_t qs,
                                             float *Qout, int64_t qos) {
   constexpr int T = append_threads(HDP), UNITS = BLK * HDP / 4 / T;  // a thread's units of a block
@@ -450,10 +450,12 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
   constexpr int U = NQ * 4 / KW;        // 16-row tiles of the workgroup
   constexpr int UNIT = 16 * (HDP + 2);  // floats of 16 rows' partial state
   constexpr int HALF = BLK * HDP, NI = HALF / 1024;  // bytes of a block's keys (or values), DMA instructions for them
-  constexpr int MERGE = KW > 1 ? 4 * NQ * DT * 1024 : 0, LDS = 4 * RING * 2 * HALF;
+  constexpr int MERGE = 4 * NQ * DT * 1024, LDS = 4 * RING * 2 * HALF;
   // the waves' rings, and the merge of their states after them
   __shared__ __attribute__((aligned(16))) uint8_t lds[LDS > MERGE ? LDS : MERGE];
   static_assert(LDS >= 256 * 8 * 4, "room for the join's shares");
+  // (in place, too: the merge's barriers stand between the waves' query reads and the stores)
+  static_assert(KW > 1, "waves with the same rows, whose states are merged");
   float(*mrg)[NQ * DT][256] = reinterpret_cast<float(*)[NQ * DT][256]>(lds);
   __shared__ float mrg_m[4][NQ][16], mrg_l[4][NQ][16];
   __shared__ unsigned order;
@@ -475,12 +477,9 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
   const float per_group = 1.f / (float)a.groups;
   auto token_of = [&](int r) { return (int)(((float)(skip + r) + 0.5f) * per_group); };
   const int rows = min(16 * U, count * a.groups - tile * 16 * U);  // that are there
-  // (with all keys in one wave, those that its rows see)
-  const int seen = KW > 1 ? blk1
-                          : min(blk1, (start + (tile * 16 * U + min(rows, 16 * NQ * (qw + 1)) - 1) / a.groups) / BLK + 1);
   const int first_pos = start + (tile * 16 * U + 16 * NQ * qw) / a.groups;  // of the wave's rows
   const int b0 = blk0 + kw;
-  const int n = 16 * NQ * qw < rows ? (seen - b0 + KW - 1) / KW : 0;  // <= 0: none
+  const int n = 16 * NQ * qw < rows ? (blk1 - b0 + KW - 1) / KW : 0;  // <= 0: none
   // the larger of two raw products is their median with infinity: fmaxf puts a
   // canonicalising move before each (of numbers; a NaN travels with the sums)
   const float inf = opaque(INFINITY), minus_one = opaque(-1.f);
@@ -717,27 +716,25 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
       if (ahead < n) fetch_values(next, 0);
     }
   }
-  if constexpr (KW > 1) {
-    // the states of the waves with the same rows put together: one maximum, then
-    // the sums, each wave a share of the 16 x 16 output tiles
+  // the states of the waves with the same rows put together: one maximum, then
+  // the sums, each wave a share of the 16 x 16 output tiles
 #pragma unroll
-    for (int q = 0; q < NQ; ++q)
-      if (g == 0) mrg_m[wave][q][c] = m[q];
-    __syncthreads();  // (and every wave is done with its ring)
+  for (int q = 0; q < NQ; ++q)
+    if (g == 0) mrg_m[wave][q][c] = m[q];
+  __syncthreads();  // (and every wave is done with its ring)
 #pragma unroll
-    for (int q = 0; q < NQ; ++q) {
-      float M = mrg_m[qw * KW][q][c];
+  for (int q = 0; q < NQ; ++q) {
+    float M = mrg_m[qw * KW][q][c];
 #pragma unroll
-      for (int w = 1; w < KW; ++w) M = fmaxf(M, mrg_m[qw * KW + w][q][c]);
-      const float f = __builtin_amdgcn_exp2f(m[q] - M);
-      if (g == 0) mrg_l[wave][q][c] = l[q] * f;
-      m[q] = M;
+    for (int w = 1; w < KW; ++w) M = fmaxf(M, mrg_m[qw * KW + w][q][c]);
+    const float f = __builtin_amdgcn_exp2f(m[q] - M);
+    if (g == 0) mrg_l[wave][q][c] = l[q] * f;
+    m[q] = M;
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
-        *reinterpret_cast<floatx4 *>(&mrg[wave][q * DT + d][4 * lane]) = acc[q][d] * f;
-    }
-    __syncthreads();
+    for (int d = 0; d < DT; ++d)
+      *reinterpret_cast<floatx4 *>(&mrg[wave][q * DT + d][4 * lane]) = acc[q][d] * f;
   }
+  __syncthreads();
   auto out_row = [&](int r) {
     const int k = token_of(r);
     return O + ((int64_t)row0 + first_tok + k) * os + (int64_t)(head * a.groups + skip + r - k * a.groups) * a.head_dim;
@@ -747,19 +744,12 @@ __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items
   for (int u = 0; u < NQ * DT; ++u) {
     if (u % KW != kw) continue;
     const int q = u / DT, d = 16 * (u % DT) + 4 * g, r = 16 * (qw * NQ + q) + c;
-    floatx4 o;
-    float sum;
-    if constexpr (KW > 1) {
-      o = zero;
-      sum = 0.f;
+    floatx4 o = zero;
+    float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < KW; ++w) {
-        o += *reinterpret_cast<const floatx4 *>(&mrg[qw * KW + w][u][4 * lane]);
-        sum += mrg_l[qw * KW + w][q][c];
-      }
-    } else {
-      o = acc[q][u % DT];
-      sum = l[q];
+    for (int w = 0; w < KW; ++w) {
+      o += *reinterpret_cast<const floatx4 *>(&mrg[qw * KW + w][u][4 * lane]);
+      sum += mrg_l[qw * KW + w][q][c];
     }
     if (r >= rows) continue;
     if (parts > 1) {
@@ -872,9 +862,9 @@ pbx_kv_rope_table(const double *freq, double *table, int half, int64_t n) {
 #define PBX_KV_KERNELS(HDP)                                                                                        \
   extern "C" __global__ void __launch_bounds__(append_threads(HDP))                                                \
       pbx_kv_append_##HDP(KvArgs a, KvRope r, const BlockItem *items, int n_blocks, const int *row_pos,            \
-                          int n_rows, const float *K, int64_t ks, const float *V, int64_t vs, const float *Q,      \
-                          int64_t qs, float *Qout, int64_t qos) {                                                  \
-    append_body<HDP>(a, r, items, n_blocks, row_pos, n_rows, K, ks, V, vs, Q, qs, Qout, qos);                      \
+                          const float *K, int64_t ks, const float *V, int64_t vs, const float *Q, int64_t qs,      \
+                          float *Qout, int64_t qos) {                                                              \
+    append_body<HDP>(a, r, items, n_blocks, row_pos, K, ks, V, vs, Q, qs, Qout, qos);                              \
   }                                                                                                                \
   extern "C" __global__ void __launch_bounds__(append_threads(HDP))                                                \
       pbx_kv_read_##HDP(KvArgs a, const BlockItem *items, float *K, int64_t ks, float *V, int64_t vs) {            \

@@ -34,8 +34,8 @@ struct pbx_kv {
   float *scales = nullptr;   // [layer][page][kv head][block][key, value]
   double *rope = nullptr;    // [max_seq][rope_dim / 2][cos, sin]
   size_t layer_codes = 0, layer_scales = 0, bytes = 0;
-  // the kernels for this head size; attention by log2 of the query tiles
-  hipFunction_t append = nullptr, read = nullptr, attn[4] = {};
+  // the kernels for this head size; attention by log2 of the query tiles (4 at most)
+  hipFunction_t append = nullptr, read = nullptr, attn[3] = {};
   std::vector<pbx_kv_batch *> batches;
 };
 
@@ -457,10 +457,10 @@ extern "C" int pbx_kv_append_dev(pbx_kv_batch *b, int layer, const float *dQ, in
   }
   KvRopeHost r{kv->rope, g.rope_style, g.rope_dim};
   const int32_t *items = b->dev, *pos = b->dev + b->at_pos;
-  const int n_blocks = (int)b->plan.blocks.size(), n_rows = b->plan.n_rows;
-  void *args[] = {&a, &r, &items, (void *)&n_blocks, &pos, (void *)&n_rows, &dK, &k_stride, &dV, &v_stride,
-                  &dQ, &q_stride, &dQout, &qout_stride};
-  return batch_launch(b, kv->append, "pbx_kv_append", (int64_t)n_blocks * g.n_kv_heads + (dQ ? n_rows : 0),
+  const int n_blocks = (int)b->plan.blocks.size();
+  void *args[] = {&a, &r, &items, (void *)&n_blocks, &pos, &dK, &k_stride, &dV, &v_stride, &dQ, &q_stride,
+                  &dQout, &qout_stride};
+  return batch_launch(b, kv->append, "pbx_kv_append", (int64_t)n_blocks * g.n_kv_heads + (dQ ? b->plan.n_rows : 0),
                       kv_threads(kv->hdp), args);
 }
 
@@ -482,7 +482,7 @@ extern "C" int pbx_kv_attention_dev(pbx_kv_batch *b, int layer, const float *dQ,
     return pbx_fail(c, PBX_EINVAL, "%s: attention in place needs one stride", who);
   if (scale == 0.f) scale = (float)(1.0 / sqrt((double)g.head_dim));
   const int32_t *items = b->dev + b->at_attn, *table = b->dev + b->at_table;
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < 3; ++k) {
     const int n = b->plan.n_attn[k];
     if (!n) continue;
     void *args[] = {&a, &items, &table, &dQ, &q_stride, &scale, &dOut, &out_stride, &b->part, &b->arrived};

@@ -64,7 +64,7 @@ struct kv_block_item {
   int32_t pad[2];
 };
 // Query rows 16 u tile .. of a sequence ((row, head of the KV group) pairs, the
-// head fastest) over its blocks blk0..blk1 - 1: u 16-row tiles, 1, 2, 4 or 8.
+// head fastest) over its blocks blk0..blk1 - 1: u 16-row tiles, 1, 2, 4 or 8 (the kernels have 4 at most).
 struct kv_attn_item {
   int32_t start, count, row0;
   int32_t tile;
