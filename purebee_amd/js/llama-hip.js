@@ -137,10 +137,11 @@ class HipLlamaRuntime {
   /**
    * Log probabilities instead of logits, of every position of one batched pass:
    * {logp [n] (of targets; null without), entropy [n], topIds, topLogp [n*top]}.
+   * Ids that int32 does not hold are in no vocabulary.
    */
   logprobs(tokenIds, startPos, { targets = null, top = 0 } = {}) {
-    return addon.modelLogprobs(this._model, Int32Array.from(tokenIds), startPos,
-                               targets && Int32Array.from(targets), top);
+    const ids = (a) => Int32Array.from(a, (t) => (t === (t | 0) ? t : -1));
+    return addon.modelLogprobs(this._model, ids(tokenIds), startPos, targets && ids(targets), top);
   }
 
   /** Every position's logits in one batched pass: {logits [n*vocab], next [n]}. */

@@ -640,7 +640,7 @@ napi_value ModelLogprobs(napi_env env, napi_callback_info info) {
   if (!r || !get_tokens(env, argv[1], &tokens) || !get_i64(env, argv[2], &start) ||
       (with && (!get_tokens(env, argv[3], &targets) || targets.size() != tokens.size())) ||
       (!is_nullish(env, argv[4]) && !get_i64(env, argv[4], &top)) || top < 0 ||
-      top > PBX_LOGPROBS_TOP_MAX)
+      top > PBX_LOGPROBS_TOP_MAX || start != (int64_t)(int)start)
     return throw_msg(env, "modelLogprobs(model, tokens, startPos, targets, top): bad arguments");
   const size_t n = tokens.size();
   float *lp = nullptr, *ent, *tl;

@@ -480,13 +480,29 @@ def _i32(a):
     return np.ascontiguousarray(list(a), np.int32)
 
 
+def _int32(v):
+    """v, where a C int holds it (ctypes would wrap it)."""
+    if not -2**31 <= v < 2**31:
+        raise OverflowError(f"{v} is past 32 bits")
+    return v
+
+
+def _token_ids(a):
+    """int32 token ids; what int32 does not hold (and would wrap into the
+    vocabulary) as -1, which is in none."""
+    a = np.asarray(a)
+    if a.dtype != np.int32:
+        a = np.where((a < -2**31) | (a >= 2**31), -1, a).astype(np.int32)
+    return np.ascontiguousarray(a)
+
+
 def _logprobs_arrays(rows, targets, top):
     """(address of the targets, the answers' arrays, their addresses)."""
     out = {"entropy": np.empty(rows, np.float32), "top_ids": np.empty((rows, top), np.int32),
            "top_logp": np.empty((rows, top), np.float32)}
     t = None
     if targets is not None:
-        out["targets"] = t = np.ascontiguousarray(targets, np.int32)
+        out["targets"] = t = _token_ids(targets)
         if t.ndim != 1 or t.size != rows:
             raise ValueError(f"{t.size} targets for {rows} rows")
         out["logp"] = np.empty(rows, np.float32)
@@ -544,12 +560,12 @@ class KvCache:
 
     def length(self, seq):
         n = ctypes.c_int()
-        self.ctx._call("pbx_kv_length", self._ptr, seq, ctypes.byref(n))
+        self.ctx._call("pbx_kv_length", self._ptr, _int32(seq), ctypes.byref(n))
         return n.value
 
     def truncate(self, seq, n_tokens=0):
         """Drop the positions from n_tokens on, and the pages they leave empty."""
-        self.ctx._call("pbx_kv_truncate", self._ptr, seq, n_tokens)
+        self.ctx._call("pbx_kv_truncate", self._ptr, _int32(seq), _int32(n_tokens))
 
     def free(self):
         """Frees the cache and its batches."""
@@ -756,16 +772,16 @@ class Model:
     def logprobs(self, tokens, start_pos, targets=None, top=0):
         """One batched forward that answers with {"logp" [n] (of targets), "entropy"
         [n], "top_ids" and "top_logp" [n, top]} instead of n rows of logits."""
-        toks = np.ascontiguousarray(tokens, np.int32)
+        toks = _token_ids(tokens)
         t, out, ptrs = _logprobs_arrays(len(toks), targets, top)
-        self._mcall("pbx_model_logprobs", toks.ctypes.data, len(toks), start_pos, t, top, *ptrs)
+        self._mcall("pbx_model_logprobs", toks.ctypes.data, len(toks), _int32(start_pos), t, top, *ptrs)
         return out
 
     def forward_kv(self, batch, tokens, all_rows=False, want_logits=True, targets=None, top=None):
         """One forward over a KvBatch's rows: (logits [rows, vocab] or None, argmax
         [rows]) of every row (all_rows) or of each sequence's last; with targets or
         top also the dictionary that logprobs gives."""
-        toks = np.ascontiguousarray(tokens, np.int32)
+        toks = _token_ids(tokens)
         if len(toks) != batch.rows:
             raise ValueError(f"{len(toks)} tokens for {batch.rows} rows")
         kv = batch.cache

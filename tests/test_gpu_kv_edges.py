@@ -1,11 +1,15 @@
 """The paged KV cache at the ends of its numbers, against tests/kv_ref.py, and around captures."""
 import ctypes
+import json
+import os
 
 import numpy as np
 import pytest
 
 import purebee_amd as pb
+from purebee_amd import synth
 from tests.kv_ref import Rows, within
+from tests.test_gpu_js import JS, run_node
 from tests.test_gpu_kv import Pair, _hip
 from tests.test_gpu_model_kv import CONFIGS, Server
 
@@ -208,3 +212,56 @@ def test_a_cache_whose_theta_was_left_out(ctx):
     assert np.array_equal(s.model.forward_kv(left_out.batch([0], [3]), tokens)[0], want)
     left_out.free()
     s.free()
+
+
+def test_ids_that_int32_does_not_hold(ctx):
+    """64-bit ids a multiple of 2^32 away from tokens are not those tokens: no distribution's probability, or refused."""
+    s = Server(ctx, CONFIGS["f32"])
+    tokens, far = np.arange(5), np.arange(5, dtype=np.int64) + 2 ** 32
+    for targets in (far, -far, np.uint64(far), list(far)):
+        assert np.isnan(s.model.logprobs(tokens, 0, targets)["logp"]).all()
+        lp = s.model.forward_kv(s.cache.batch([0], [5], [0]), tokens, all_rows=True, targets=targets)[2]
+        assert np.isnan(lp["logp"]).all()
+    for bad in (far, -far):
+        with pytest.raises(pb.PbxError, match="out of range"):
+            s.model.logprobs(bad, 0)
+        with pytest.raises(pb.PbxError, match="out of range"):
+            s.model.forward_kv(s.cache.batch([0], [5], [0]), bad)
+    want = s.model.logprobs(np.int32(tokens), 0, np.int32(tokens))["logp"]
+    for call in (lambda: s.model.logprobs(tokens, 2 ** 32), lambda: s.cache.truncate(2 ** 32), lambda: s.cache.length(2 ** 32),
+                 lambda: s.cache.truncate(0, 2 ** 32)):
+        with pytest.raises(OverflowError):
+            call()
+    assert s.cache.length(0) == 5
+    for kind in (np.int64, np.uint8, list):
+        assert np.array_equal(s.model.logprobs(kind(tokens), 0, kind(tokens))["logp"], want)
+    s.free()
+
+
+def test_ids_and_positions_that_int32_does_not_hold_from_node(ctx, tmp_path):
+    cfg = CONFIGS["f32"]
+    names, files = dict(synth.GGUF_NAMES), []
+
+    def keep(spec, data):
+        tid, layer, N, K, t = spec
+        fn = f"t{len(files)}.bin"
+        np.ascontiguousarray(data).tofile(tmp_path / fn)
+        files.append([names[tid] if layer < 0 else f"blk.{layer}.{names[tid]}", fn])
+
+    synth.build(ctx, cfg, 77, keep).free()
+    out = run_node(tmp_path, f"""
+const {{ HipLlamaRuntime }} = require({os.path.join(JS, 'llama-hip.js')!r});
+const c = meta.cfg, far = 2 ** 32;
+const rt = new HipLlamaRuntime({{ dim: c.dim, hiddenDim: c.hidden_dim, nLayers: c.n_layers, nHeads: c.n_heads,
+  nKvHeads: c.n_kv_heads, vocabSize: c.vocab_size, seqLen: c.max_seq, ropeTheta: c.rope_theta,
+  weightType: 'f32', embedType: 'f32' }});
+for (const [nm, fn] of meta.files) rt.loadTensor(nm, rd(fn, Float32Array));
+const a = rt.logprobs([1, 2, 3], 0, {{ targets: [2, far + 3, 4] }});
+let refused = 0;
+for (const [t, at] of [[[1, far + 2, 3], 0], [[1, 2, 3], far], [[1, 2, 3], -far]]) {{
+  try {{ rt.logprobs(t, at); }} catch (e) {{ refused++; }}
+}}
+console.log(JSON.stringify({{ logp: [...a.logp].map(Number.isNaN), refused }}));
+rt.free();
+""", {"cfg": cfg, "files": files})
+    assert json.loads(out.strip().splitlines()[-1]) == {"logp": [False, True, False], "refused": 3}
