@@ -549,7 +549,7 @@ class KvCache:
         b = KvBatch(self)
         try:
             return b.set(seqs, counts, starts)
-        except PbxError:
+        except Exception:
             b.free()
             raise
 
@@ -582,6 +582,7 @@ class KvBatch:
     def __init__(self, cache):
         self.cache, self.ctx = cache, cache.ctx
         self._b = None
+        self.sequences = 0
         p = _vp()
         self.ctx._call("pbx_kv_batch_create", cache._ptr, ctypes.byref(p))
         self._b = p.value

@@ -265,3 +265,21 @@ console.log(JSON.stringify({{ logp: [...a.logp].map(Number.isNaN), refused }}));
 rt.free();
 """, {"cfg": cfg, "files": files})
     assert json.loads(out.strip().splitlines()[-1]) == {"logp": [False, True, False], "refused": 3}
+
+
+def test_a_batch_that_was_never_set(ctx):
+    """It is refused by the library, and one whose arguments do not match is not left behind."""
+    s = Server(ctx, CONFIGS["f32"])
+    with pytest.raises(pb.PbxError):
+        s.model.forward_kv(pb.KvBatch(s.cache), [])
+    made = []
+    free = pb.KvBatch.free
+    pb.KvBatch.free = lambda b: (made.append(b), free(b))
+    try:
+        for args in (([0], [1, 2]), ([0], [2 ** 40])):
+            with pytest.raises((ValueError, OverflowError)):
+                s.cache.batch(*args)
+    finally:
+        pb.KvBatch.free = free
+    assert len(made) == 2 and not any(b._b for b in made)
+    s.free()
