@@ -469,9 +469,10 @@ int pbx_kv_truncate(pbx_kv *kv, int seq, int n_tokens);
  * pool (PBX_ENOMEM, and nothing changed, when it has too few); starts[i] is at
  * most its length, and starts == NULL means each sequence's end.  counts[i] may
  * be 0.  The set-up is made once and used by every layer's calls below; it waits
- * for no GPU work but the previous set-up of the same batch.  The three calls
- * enqueue on the context's stream; of one batch they use the same workspace, so
- * work captured from one batch into graphs is replayed on one stream at a time.
+ * for no GPU work but the previous set-up of the same batch (and the context's
+ * stream, where a batch larger than any before needs more memory).  The three
+ * calls enqueue on the context's stream; of one batch they use the same workspace,
+ * so its calls and replays of graphs that captured them run on one stream at a time.
  * A batch whose calls were captured keeps its rows (set refuses, PBX_EINVAL):
  * a replay runs over the same positions, which the sequences must still hold
  * (and, if it appends, end with), and the batch lives as long as the graph (a

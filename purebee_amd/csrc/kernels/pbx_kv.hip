@@ -125,9 +125,11 @@ __device__ __forceinline__ void turn(const KvRope &r, int u, const Angles &cs, d
 // by 4 dims, values by 4 positions, as their codes lie side by side); the
 // block's codes are put together in LDS (with the earlier rows' codes, if there
 // are any) and stored whole.  Bound by bytes where there are many rows (6,124 of
-// six prompts, 32 / 8 heads of 128: 62 us, 4.2 TB/s of queries in and out, keys,
-// values and codes), else by one chain of loads, maximum, LDS and store (one row:
-// 5 us, 64 of 64 sequences: 5.5; 32 / 8 heads of 64).
+// six prompts, 32 / 8 heads of 128: 60 us, 4.4 TB/s of queries in and out, keys,
+// values and codes), else by one chain of loads, maximum, LDS and store: 32 / 8
+// heads of 64, one row 4.7 us and 64 of 64 sequences 5.6 where no scale rises (the
+// same rows again), 5.4 and 7.4 at new positions, of which most blocks round some
+// earlier codes again, 6.5 and 7.9 where every row raises its block's scale.
 // Threads of a workgroup: two units each (a wide head's block on 256 threads took
 // three times as long where there are few).
 constexpr int append_threads(int hdp) { return hdp <= 64 ? 256 : 4 * hdp; }
@@ -427,21 +429,27 @@ __device__ __forceinline__ float2 get2(const float *p) {
 // of two near the row's largest) and probabilities enter as fp16 pairs, two
 // products each, summed in f32.  The block's key scale joins the row's factor,
 // its value scale weighs the block's products as they are added up.
-// Every wave keeps a ring of RING blocks' codes in LDS, fetched RING - 1 blocks
-// ahead (RING 1: a block's keys while the one before goes through its softmax,
-// its values while the next scores are computed).  Where a tile's blocks are
-// split over several workgroups, the one that finishes last puts their states
-// together, in the order of the keys.
+// Every wave keeps a ring of RING blocks' codes in LDS; a block is asked for
+// RING - 1 blocks ahead (RING 1: its keys after the scores of the one before, its
+// values after that one's).  The counted waits allow for what was asked for later,
+// but the compiler adds one: `scales` may have just been loaded in a branch of the
+// loop, and it waits for all vector memory before each block's use of them.  So
+// whatever is under way as a block begins is waited for, the block fetched ahead
+// (RING 3) or its own values (RING 1) too.
+// Where a tile's blocks are split over several workgroups, the one that finishes
+// last puts their states together, in the order of the keys.
 // Single tokens are bound by the codes' bytes: 64 sequences of 64 to 8,000
-// positions, 32 / 8 heads of 64, 59 us (4.96 TB/s); one of 131,001 positions 35 us
+// positions, 32 / 8 heads of 64, 58 us (4.97 TB/s); one of 131,001 positions 35 us
 // (3.9 TB/s; with 96 or 128 parts for 64 it took 38 and 43); one of 129 4.9 us, a
 // launch's.  Prompts are bound by issue: a vector instruction does not run beside a
 // 16x16x32 product (a loop of 8 products and 32 fmas a wave, four waves a SIMD:
 // 358 ns, the products alone 226, the fmas 142), and 32 rows times 32 keys of 64
-// dims are 36 products (576 cycles) and about 265 vector instructions, so what
-// counts is fewer of either: 2,000 rows, 32 / 8 heads of 64, 50 us (656 TFLOP/s
-// of products); 1,183 rows on pasts of up to 2,000, 32 / 8 heads of 128, 93 us
-// (780 TFLOP/s).
+// dims are 36 products (576 cycles) and about 275 vector instructions, so what
+// counts is fewer of either: 2,000 rows, 32 / 8 heads of 64, 52 us (635 TFLOP/s
+// of products); 1,183 rows on pasts of up to 2,000, 32 / 8 heads of 128, 96 us
+// (760 TFLOP/s); 2,000 rows, 16 / 8 heads of 192, 76 us (650), 8 / 1 of 256, 60 us
+// (540).  Clocks rise over the first 600 launches or so (the first 60 of these
+// prompts take 60 and 114 us); the figures are those after.
 template <int HDP, int NQ, int KW, int RING>
 __device__ __forceinline__ void attn_body(const KvArgs &a, const AttnItem *items, const int *table, const float *Q,
                                           int64_t qs, float scale, float *O, int64_t os, float *part,
