@@ -503,8 +503,8 @@ int pbx_kv_append_dev(pbx_kv_batch *b, int layer, const float *dQ, int64_t q_str
  * be dQ itself.  Values are used as they stand in the cache and sums are held in
  * f32.  Queries enter with 22 bits (2^-25 of their row's largest at least), a
  * probability with 22 bits, or 2^-30 of the largest in its block of
- * PBX_KV_BLOCK positions where that is more.  The result of a row does not
- * depend on the other rows' values. */
+ * PBX_KV_BLOCK positions where that is more.  Scores (scale q . K) are to stay
+ * below 10^8.  The result of a row does not depend on the other rows' values. */
 int pbx_kv_attention_dev(pbx_kv_batch *b, int layer, const float *dQ, int64_t q_stride,
                          float scale, float *dOut, int64_t out_stride);
 /* The batch's rows of the cache as the values they stand for, f32 [n_rows]

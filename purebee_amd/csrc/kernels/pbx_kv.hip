@@ -360,8 +360,11 @@ constexpr float NONE = -1e38f;
 // the row's largest keep their bits and add up, however many they are.
 // A row's maximum follows the blocks' only when they pass it by 2^SLACK: a new
 // maximum rescales all sums, and in some row of a tile nearly every block brings one.
-// (All of a row against one maximum was 0 to 2 % faster on prompts and lost what lay
-// below 2^-31 of it: a quarter of a tail of 4,000 keys behind one strong one.)
+// (All of a row against one maximum took 2 to 4 % less on prompts of heads up to 128,
+// as much elsewhere, and lost what lay below 2^-31 of it: a quarter of a tail of 4,000
+// keys behind one strong one.)
+// Scores past 2^28 (in powers of two) are so coarse in f32 that an exponent's rounding
+// would leave fp16's range.
 constexpr float LIFT = 6.f, SLACK = 12.f;
 
 // Codes reach LDS by DMA (global_load_lds: lane i's 16 bytes land at the
