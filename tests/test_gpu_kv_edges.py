@@ -283,3 +283,34 @@ def test_a_batch_that_was_never_set(ctx):
         pb.KvBatch.free = free
     assert len(made) == 2 and not any(b._b for b in made)
     s.free()
+
+
+@pytest.mark.parametrize("size", [1e3, 1e6, 3e7, 9.5e7])
+@pytest.mark.parametrize("past,rows", [(70, 2), (1500, 1), (40, 40)])
+def test_scores_of_any_size(ctx, size, past, rows):
+    """Scores up to 10^8, of either sign, with the largest far ahead of the next: the answer is its value."""
+    print(f"[case] scores of {size} after {past}, {rows} rows", flush=True)
+    n = past + rows
+    for sign in (1, -1):
+        p = Pair(ctx, 4, 2, 64, seqs=1, n_pages=60, style="none", seed=61 + past)
+        q, k, v = p.rows(n)
+        # one dim counts: whole codes 1 to 127 (of either sign) times a power of two, the best key alone at its end
+        code = p.rng.integers(30, 100, (n, 2)) if sign > 0 else -p.rng.integers(30, 100, (n, 2))
+        best = past // 2
+        code[best] = 127 if sign > 0 else -10
+        k[:], q[:] = 0, 0
+        k[..., 0], k[..., 1] = code / 128, 127 / 128      # (every block's scale is 1 / 128)
+        q[..., 0] = size
+        part = lambda a, e: tuple(x[a:e] for x in (q, k, v))  # noqa: E731
+        p.append([0], [past], part(0, past))
+        b, qr = p.append([0], [rows], part(past, n))
+        dq, do = Rows(ctx, rows, 256, qr), Rows(ctx, rows, 256)
+        b.attention_dev(0, dq.ptr, do.ptr, 128 / 127)
+        ctx.sync()
+        want = np.broadcast_to(np.repeat(p.ref.v[0].values()[best], 2, axis=0), (rows, 4, 64))
+        # the others lie 20 codes and more below, size / 127 each: nothing of them is left; a rounding of 1 / sum and one more
+        tol = 2.0 ** -22 * np.abs(want) + 2 * n * np.abs(v).max() * np.exp(-20 * size / 127)
+        within(do.get().reshape(want.shape), want, tol)
+        for x in (dq, do):
+            x.free()
+        p.free()
