@@ -463,6 +463,30 @@ int pbx_kv_info(const pbx_kv *kv, int *free_pages, size_t *device_bytes);
 int pbx_kv_length(const pbx_kv *kv, int seq, int *n_tokens);
 int pbx_kv_truncate(pbx_kv *kv, int seq, int n_tokens);
 
+/* Branches: sequence dsts[i] (none twice) comes to hold the first lens[i] positions
+ * (lens == NULL: all) that srcs[i] held before the call, for all i at once, so beams
+ * may take each other's places; what dsts[i] held is let go of, as by truncation, and
+ * dsts[i] == srcs[i] only shortens.  Nothing is copied: the sequences share pages, which
+ * free_pages counts once.  A batch that lengthens a sequence inside a shared page gives
+ * it a copy of the page first (pbx_kv_batch_set, from the pool; the last one to hold a
+ * page keeps it), and other batches over that sequence have to be set again.  Rows in
+ * pages that have come to be shared since their batch was set cannot be appended
+ * (PBX_EINVAL), nor can pages be shared to which a captured batch appends.  Waits for
+ * no GPU work. */
+int pbx_kv_fork(pbx_kv *kv, int n, const int32_t *dsts, const int32_t *srcs, const int32_t *lens);
+/* Sequence seqs[i] (none twice) keeps counts[i] of its positions and drops the others;
+ * `positions` lists them, rising, one sequence after the other.  The k-th that is kept
+ * becomes position k: its key is turned from its old to its new position (with no
+ * rotation it stays) and its block is coded anew, as if rows of the values that the old
+ * codes stand for were appended together.  Blocks whose rows all stay where they are
+ * stay as they are.  A block that gets a row from a block that reads as NaN reads as NaN.
+ * Pages from the first row that moves on are written into free pages of the pool, at
+ * least one (PBX_ENOMEM, and nothing changed; the fewer there are, the more launches),
+ * and given back; sequences that share them keep theirs.  Batches over moved positions
+ * are refused from then on.  Enqueues on the context's stream, and waits for no GPU work
+ * but the lists of the compaction before. */
+int pbx_kv_compact(pbx_kv *kv, int n, const int32_t *seqs, const int32_t *counts, const int32_t *positions);
+
 /* A batch: counts[i] rows of sequence seqs[i] (none twice) at the positions
  * starts[i].., packed in this order (all rows of a sequence side by side).
  * pbx_kv_batch_set lengthens a sequence to hold its rows, with pages from the
@@ -478,7 +502,8 @@ int pbx_kv_truncate(pbx_kv *kv, int seq, int n_tokens);
  * (and, if it appends, end with), and the batch lives as long as the graph (a
  * batch whose capture was thrown away is freed, and another one set).  A call
  * that is refused, or has no rows, holds nothing.
- * Inside a capture no cache or batch is made, set or freed (PBX_EINVAL).
+ * Inside a capture no cache or batch is made, set or freed, and no sequence forked or
+ * compacted (PBX_EINVAL).
  * Positions that a batch took hold nothing defined until they are appended.
  */
 int pbx_kv_batch_create(pbx_kv *kv, pbx_kv_batch **out);

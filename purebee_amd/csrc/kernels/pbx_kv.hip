@@ -331,6 +331,149 @@ __device__ __forceinline__ void read_body(const KvArgs &a, const BlockItem *item
   }
 }
 
+// kv_pack_item and kv_page_copy of pbx_kv_plan.h
+struct PackItem {
+  int page, sub, pos0, rows, at, tab, raw, pad;
+};
+struct PageCopy {
+  int from, to, blocks, pad;
+};
+struct KvPack {
+  uint8_t *codes;  // of layer 0
+  float *scales;
+  int64_t layer_codes, layer_scales;
+  const void *items;
+  const int *positions, *table;
+  int n_items, kv_heads, head_dim, page_shift;  // (copying: head_dim is a block's bytes)
+};
+
+__device__ __forceinline__ int64_t block_index(const KvPack &a, int page, int head, int sub) {
+  return (((int64_t)page * a.kv_heads + head) << a.page_shift) + sub;
+}
+
+// Compaction: workgroup (layer, block of new rows, KV head).  A block's rows come from
+// up to 32 old blocks; each code stands for code * s (exact in 64 bits), keys turn back
+// by the distance that they move down, and the block is coded as a new one is.  Rows'
+// codes are fetched one by one: keys as pairs of dims, values byte by byte, as they lie
+// 64 bytes apart for consecutive dims.
+template <int HDP>
+__device__ __forceinline__ void pack_body(const KvPack &a, const KvRope &r) {
+  constexpr int T = append_threads(HDP), UNITS = BLK * HDP / 4 / T, BYTES = 2 * BLK * HDP;
+  __shared__ __attribute__((aligned(16))) uint8_t img[BYTES];
+  __shared__ uint64_t red_k[T / 64], red_v[T / 64];
+  __shared__ int64_t src[BLK];  // the rows' old blocks
+  __shared__ int key_of[BLK], down[BLK];
+  __shared__ float sk[BLK], sv[BLK];
+  const int units = a.head_dim / 4, tid = threadIdx.x;
+  const int per_layer = a.n_items * a.kv_heads;
+  const int layer = blockIdx.x / per_layer, in_layer = blockIdx.x % per_layer;
+  const PackItem it = reinterpret_cast<const PackItem *>(a.items)[in_layer / a.kv_heads];
+  const int head = in_layer % a.kv_heads;
+  uint8_t *codes = a.codes + layer * a.layer_codes;
+  float *scales = a.scales + layer * a.layer_scales;
+  const int64_t bi = block_index(a, it.page, head, it.sub);
+  const int block_mask = (1 << a.page_shift) - 1;
+  if (it.raw) {
+    const int blk = it.pos0 / BLK;
+    const int64_t from = block_index(a, a.table[it.tab + (blk >> a.page_shift)], head, blk & block_mask);
+    for (int i = tid; i < BYTES / 16; i += T)
+      reinterpret_cast<uintx4 *>(codes + bi * BYTES)[i] = reinterpret_cast<const uintx4 *>(codes + from * BYTES)[i];
+    if (tid == 0) *reinterpret_cast<float2 *>(scales + 2 * bi) = *reinterpret_cast<const float2 *>(scales + 2 * from);
+    return;
+  }
+  if (tid < it.rows) {
+    const int pos = a.positions[it.at + tid], blk = pos / BLK;
+    const int64_t from = block_index(a, a.table[it.tab + (blk >> a.page_shift)], head, blk & block_mask);
+    src[tid] = from;
+    key_of[tid] = pos % BLK;
+    down[tid] = pos - (it.pos0 + tid);
+    sk[tid] = scales[2 * from];
+    sv[tid] = scales[2 * from + 1];
+  }
+  if (it.rows < BLK || a.head_dim < HDP)
+    for (int i = tid; i < BYTES / 4; i += T) reinterpret_cast<unsigned *>(img)[i] = 0x80808080u;
+  __syncthreads();
+  const int nk_units = it.rows * units, nv_units = (it.rows + 3) / 4 * a.head_dim;
+  double xk[UNITS][4], xv[UNITS][4];
+  uint64_t pk = 0, pv = 0;
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    const int j = tid + T * i;
+    if (j < nv_units) {
+      const int row = j / a.head_dim * 4, d = j % a.head_dim;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int w = min(row + e, it.rows - 1);
+        const int code = codes[src[w] * BYTES + BLK * HDP + value_byte(key_of[w], d)];
+        xv[i][e] = (double)(code - 128) * (double)sv[w];
+        const uint64_t m = magnitude(xv[i][e]);
+        pv = m > pv ? m : pv;
+      }
+    }
+    if (j < nk_units) {
+      const int w = j / units, u = j % units;
+      int da, db;
+      unit_dims(r, u, da, db);
+      const uint8_t *from = codes + src[w] * BYTES;
+      const unsigned c0 = *reinterpret_cast<const uint16_t *>(from + key_byte<HDP>(key_of[w], da));
+      const unsigned c1 = *reinterpret_cast<const uint16_t *>(from + key_byte<HDP>(key_of[w], db));
+      const double s = sk[w];
+      xk[i][0] = (double)((int)(c0 & 255) - 128) * s;
+      xk[i][1] = (double)((int)(c0 >> 8) - 128) * s;
+      xk[i][2] = (double)((int)(c1 & 255) - 128) * s;
+      xk[i][3] = (double)((int)(c1 >> 8) - 128) * s;
+      Angles cs = angles_of(r, u, down[w]);
+      cs.p.y = -cs.p.y;
+      cs.q.y = -cs.q.y;
+      turn(r, u, cs, xk[i]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint64_t m = magnitude(xk[i][e]);
+        pk = m > pk ? m : pk;
+      }
+    }
+  }
+  pk = wave_max_u64(pk);
+  pv = wave_max_u64(pv);
+  if ((tid & 63) == 0) {
+    red_k[tid >> 6] = pk;
+    red_v[tid >> 6] = pv;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < T / 64; ++w) {
+    pk = red_k[w] > pk ? red_k[w] : pk;
+    pv = red_v[w] > pv ? red_v[w] : pv;
+  }
+  const float nk = scale_of(pk), nv = scale_of(pv);
+  const float ik = 1.f / nk, iv = 1.f / nv;
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    const int j = tid + T * i;
+    if (j < nk_units) {
+      const int w = j / units, u = j % units;
+      int da, db;
+      unit_dims(r, u, da, db);
+      unsigned c = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c |= (unsigned)(code_of(xk[i][e], nk, ik) + 128) << (8 * e);
+      *reinterpret_cast<uint16_t *>(img + key_byte<HDP>(w, da)) = (uint16_t)c;
+      *reinterpret_cast<uint16_t *>(img + key_byte<HDP>(w, db)) = (uint16_t)(c >> 16);
+    }
+    if (j < nv_units) {
+      const int row = j / a.head_dim * 4, d = j % a.head_dim;
+      uint8_t *at = img + BLK * HDP + value_byte(row, d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (row + e < it.rows) at[e] = (uint8_t)(code_of(xv[i][e], nv, iv) + 128);
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < BYTES / 16; i += T)
+    reinterpret_cast<uintx4 *>(codes + bi * BYTES)[i] = reinterpret_cast<const uintx4 *>(img)[i];
+  if (tid == 0) *reinterpret_cast<float2 *>(scales + 2 * bi) = make_float2(nk, nv);
+}
+
 // 8 codes + 128 as halves: byte b under the exponent byte 0x64 is the half
 // 1024 + b.
 __device__ __forceinline__ half8 halves(unsigned w0, unsigned w1) {
@@ -870,6 +1013,23 @@ pbx_kv_rope_table(const double *freq, double *table, int half, int64_t n) {
   table[2 * i + 1] = s;
 }
 
+// Pages that sequences shared: the filled blocks of one page and KV head (which lie side
+// by side) and their scales, a workgroup (layer, page, head).
+extern "C" __global__ void __launch_bounds__(256) pbx_kv_copy(KvPack a) {
+  const int per_layer = a.n_items * a.kv_heads;
+  const int layer = blockIdx.x / per_layer, in_layer = blockIdx.x % per_layer;
+  const PageCopy it = reinterpret_cast<const PageCopy *>(a.items)[in_layer / a.kv_heads];
+  const int head = in_layer % a.kv_heads;
+  const int64_t from = block_index(a, it.from, head, 0), to = block_index(a, it.to, head, 0);
+  uint8_t *codes = a.codes + layer * a.layer_codes;
+  float *scales = a.scales + layer * a.layer_scales;
+  const uintx4 *x = reinterpret_cast<const uintx4 *>(codes + from * a.head_dim);
+  uintx4 *y = reinterpret_cast<uintx4 *>(codes + to * a.head_dim);
+  const int n = it.blocks * (a.head_dim / 16);
+  for (int i = threadIdx.x; i < n; i += 256) y[i] = x[i];
+  if ((int)threadIdx.x < 2 * it.blocks) scales[2 * to + threadIdx.x] = scales[2 * from + threadIdx.x];
+}
+
 #define PBX_KV_KERNELS(HDP)                                                                                        \
   extern "C" __global__ void __launch_bounds__(append_threads(HDP))                                                \
       pbx_kv_append_##HDP(KvArgs a, KvRope r, const BlockItem *items, int n_blocks, const int *row_pos,            \
@@ -880,6 +1040,9 @@ pbx_kv_rope_table(const double *freq, double *table, int half, int64_t n) {
   extern "C" __global__ void __launch_bounds__(append_threads(HDP))                                                \
       pbx_kv_read_##HDP(KvArgs a, const BlockItem *items, float *K, int64_t ks, float *V, int64_t vs) {            \
     read_body<HDP>(a, items, K, ks, V, vs);                                                                        \
+  }                                                                                                                \
+  extern "C" __global__ void __launch_bounds__(append_threads(HDP)) pbx_kv_pack_##HDP(KvPack a, KvRope r) {        \
+    pack_body<HDP>(a, r);                                                                                          \
   }
 #define PBX_KV_ATTN(HDP, U, NQ, KW, RING, WAVES)                                                                   \
   extern "C" __global__ void __launch_bounds__(256, WAVES)                                                         \

@@ -35,8 +35,12 @@ struct pbx_kv {
   double *rope = nullptr;    // [max_seq][rope_dim / 2][cos, sin]
   size_t layer_codes = 0, layer_scales = 0, bytes = 0;
   // the kernels for this head size; attention by log2 of the query tiles (4 at most)
-  hipFunction_t append = nullptr, read = nullptr, attn[3] = {};
+  hipFunction_t append = nullptr, read = nullptr, pack = nullptr, attn[3] = {};
   std::vector<pbx_kv_batch *> batches;
+  // the lists of a compaction on the device, and when the host's copy of them is read
+  int32_t *lists = nullptr, *host_lists = nullptr;
+  size_t lists_cap = 0, host_lists_cap = 0;
+  hipEvent_t copied = nullptr;
 };
 
 struct pbx_kv_batch {
@@ -44,12 +48,14 @@ struct pbx_kv_batch {
   pbx_kv *kv = nullptr;
   kv_batch_plan plan;
   bool set = false;
-  bool stale = false;     // positions of it were dropped
+  bool stale = false;     // positions of it were dropped or moved
   bool captured = false;  // a graph may hold its calls
+  bool appends = false;   // appends among them
+  uint64_t alone = 0;     // forks after which its rows' pages were seen to be its sequences' alone, and one
   // the plan on the device: blocks, attention items, row positions, last rows, page ids
   int32_t *dev = nullptr, *host = nullptr;
   size_t dev_cap = 0, host_cap = 0;
-  size_t at_attn = 0, at_pos = 0, at_last = 0, at_table = 0;
+  size_t at_attn = 0, at_pos = 0, at_last = 0, at_table = 0, at_copies = 0;
   hipEvent_t copied = nullptr;
   float *part = nullptr;  // partial results of split rows
   size_t part_cap = 0;
@@ -102,8 +108,10 @@ static void batch_release(pbx_kv_batch *b) {
 
 static void kv_release(pbx_kv *kv) {
   for (pbx_kv_batch *b : kv->batches) batch_release(b);
-  for (void *p : {(void *)kv->codes, (void *)kv->scales, (void *)kv->rope})
+  for (void *p : {(void *)kv->codes, (void *)kv->scales, (void *)kv->rope, (void *)kv->lists})
     if (p) hipFree(p);
+  if (kv->host_lists) hipHostFree(kv->host_lists);
+  if (kv->copied) hipEventDestroy(kv->copied);
   kv->magic = 0;
   delete kv;
 }
@@ -173,12 +181,15 @@ static int kv_make(pbx_ctx *c, const pbx_kv_config &g, pbx_kv *kv) {
   const std::string hdp = std::to_string(kv->hdp);
   kv->append = pbx_kernel_by_name(c, "pbx_kv_append_" + hdp);
   kv->read = pbx_kernel_by_name(c, "pbx_kv_read_" + hdp);
-  bool found = kv->append && kv->read;
+  kv->pack = pbx_kernel_by_name(c, "pbx_kv_pack_" + hdp);
+  bool found = kv->append && kv->read && kv->pack;
   for (int k = 0; 1 << k <= kv_max_tiles(kv->hdp); ++k) {
     kv->attn[k] = pbx_kernel_by_name(c, "pbx_kv_attn_" + hdp + "_" + std::to_string(1 << k));
     found = found && kv->attn[k];
   }
   if (!found) return pbx_fail(c, PBX_ELOAD, "pbx_kv_create: kernels for head_dim %d not found", g.head_dim);
+  if (hipEventCreateWithFlags(&kv->copied, hipEventDisableTiming) != hipSuccess)
+    return pbx_fail(c, PBX_EHIP, "pbx_kv_create: event creation failed");
   double *dfreq = nullptr;
   if (hipMalloc((void **)&kv->codes, codes) != hipSuccess ||
       hipMalloc((void **)&kv->scales, scales) != hipSuccess ||
@@ -267,6 +278,103 @@ extern "C" int pbx_kv_truncate(pbx_kv *kv, int seq, int n) {
   return PBX_OK;
 }
 
+extern "C" int pbx_kv_fork(pbx_kv *kv, int n, const int32_t *dsts, const int32_t *srcs, const int32_t *lens) {
+  const char *who = "pbx_kv_fork";
+  if (!kv_ok(kv)) return pbx_fail(nullptr, PBX_EINVAL, "%s: not a live cache", who);
+  pbx_ctx *c = kv->c;
+  if (n < 0 || (n && (!dsts || !srcs))) return pbx_fail(c, PBX_EINVAL, "%s: bad arguments", who);
+  if (const int rc = pbx_not_capturing(c, who)) return rc;
+  kv_pages &pages = kv->pages;
+  const int known = (int)pages.seqs.size();
+  // replays of a captured append write its rows' pages, whoever holds them by then
+  for (const pbx_kv_batch *b : kv->batches) {
+    if (!b->appends || b->stale) continue;
+    for (int i = 0; i < n; ++i) {
+      const int s = srcs[i];
+      if (s < 0 || s >= known || s == dsts[i]) continue;
+      const int len = lens ? lens[i] : pages.seqs[s].len;
+      for (size_t k = 0; k < b->plan.seqs.size(); ++k)
+        if (b->plan.seqs[k] == s && b->plan.counts[k] && b->plan.starts[k] / pages.page_tokens < pages.pages_of(len))
+          return pbx_fail(c, PBX_EINVAL, "%s: a captured graph appends to pages of sequence %d", who, s);
+    }
+  }
+  try {
+    std::string why;
+    const int rc = pages.fork(n, dsts, srcs, lens, &why);
+    if (rc) return pbx_fail(c, rc, "%s: %s", who, why.c_str());
+    for (pbx_kv_batch *b : kv->batches)
+      if (kv_plan_moved(pages, b->plan)) b->stale = true;
+  } catch (const std::bad_alloc &) {
+    return pbx_fail(c, PBX_ENOMEM, "%s: out of host memory", who);
+  }
+  return PBX_OK;
+}
+
+struct KvPackHost {  // KvPack in pbx_kv.hip
+  uint8_t *codes;
+  float *scales;
+  int64_t layer_codes, layer_scales;  // from one layer to the next
+  const int32_t *items, *positions, *table;
+  int n_items, kv_heads, head_dim, page_shift;
+};
+
+extern "C" int pbx_kv_compact(pbx_kv *kv, int n, const int32_t *seqs, const int32_t *counts,
+                              const int32_t *positions) {
+  const char *who = "pbx_kv_compact";
+  if (!kv_ok(kv)) return pbx_fail(nullptr, PBX_EINVAL, "%s: not a live cache", who);
+  pbx_ctx *c = kv->c;
+  if (n < 0 || (n && (!seqs || !counts))) return pbx_fail(c, PBX_EINVAL, "%s: bad arguments", who);
+  for (int i = 0; i < n; ++i)
+    if (counts[i] > 0 && !positions) return pbx_fail(c, PBX_EINVAL, "%s: positions is NULL", who);
+  if (int rc = pbx_not_capturing(c, who)) return rc;
+  if (hipSetDevice(c->device) != hipSuccess) return pbx_fail(c, PBX_EHIP, "%s: hipSetDevice failed", who);
+  const pbx_kv_config &g = kv->cfg;
+  try {
+    std::string why;
+    kv_pack_plan p;
+    int rc = kv_plan_pack(&kv->pages, n, seqs, counts, positions, &p, &why);
+    if (rc) return pbx_fail(c, rc, "%s: %s", who, why.c_str());
+    const size_t n_items = p.items.size() * sizeof(kv_pack_item) / 4;
+    const size_t at_table = n_items + p.positions.size(), words = at_table + p.table.size();
+    if (words) {
+      if (hipEventSynchronize(kv->copied) != hipSuccess)
+        rc = pbx_fail(c, PBX_EHIP, "%s: waiting for the last lists failed", who);
+      if (!rc) rc = pbx_ensure_pinned(c, (void **)&kv->host_lists, &kv->host_lists_cap, words * 4);
+      if (!rc) rc = pbx_ensure_dev(c, (void **)&kv->lists, &kv->lists_cap, words * 4);
+      if (!rc) {
+        memcpy(kv->host_lists, p.items.data(), n_items * 4);
+        memcpy(kv->host_lists + n_items, p.positions.data(), p.positions.size() * 4);
+        memcpy(kv->host_lists + at_table, p.table.data(), p.table.size() * 4);
+        if (hipMemcpyAsync(kv->lists, kv->host_lists, words * 4, hipMemcpyHostToDevice, c->stream) != hipSuccess ||
+            hipEventRecord(kv->copied, c->stream) != hipSuccess)
+          rc = pbx_fail(c, PBX_EHIP, "%s: copy failed", who);
+      }
+      KvRopeHost r{kv->rope, g.rope_style, g.rope_dim};
+      const int32_t *items = kv->lists;
+      for (size_t k = 0; k < p.launches.size() && !rc; ++k) {
+        KvPackHost a{kv->codes, kv->scales, (int64_t)kv->layer_codes, (int64_t)kv->layer_scales, items,
+                     kv->lists + n_items, kv->lists + at_table, p.launches[k], g.n_kv_heads, g.head_dim,
+                     kv->page_shift};
+        void *args[] = {&a, &r};
+        rc = kv_launch(c, kv->pack, "pbx_kv_pack", (int64_t)p.launches[k] * g.n_kv_heads * g.n_layers,
+                       kv_threads(kv->hdp), args);
+        // (the first launch writes pages that were free: the sequences are whole until the second)
+        if (rc && k) return rc;
+        items += (size_t)p.launches[k] * sizeof(kv_pack_item) / 4;
+      }
+    }
+    if (rc) {
+      kv_pack_undo(&kv->pages, &p);
+      return rc;
+    }
+    for (pbx_kv_batch *b : kv->batches)
+      if (kv_plan_moved(kv->pages, b->plan)) b->stale = true;
+  } catch (const std::bad_alloc &) {
+    return pbx_fail(c, PBX_ENOMEM, "%s: out of host memory", who);
+  }
+  return PBX_OK;
+}
+
 extern "C" int pbx_kv_batch_create(pbx_kv *kv, pbx_kv_batch **out) {
   if (!kv_ok(kv)) return pbx_fail(nullptr, PBX_EINVAL, "pbx_kv_batch_create: not a live cache");
   if (!out) return pbx_fail(kv->c, PBX_EINVAL, "pbx_kv_batch_create: NULL argument");
@@ -318,7 +426,8 @@ static int batch_upload(pbx_kv_batch *b) {
   b->at_pos = b->at_attn + p.attn.size() * sizeof(kv_attn_item) / 4;
   b->at_last = b->at_pos + p.row_pos.size();
   b->at_table = b->at_last + p.last_rows.size();
-  const size_t n = b->at_table + p.table.size();
+  b->at_copies = b->at_table + p.table.size();
+  const size_t n = b->at_copies + p.copies.size() * sizeof(kv_page_copy) / 4;
   if (!n) return PBX_OK;
   if (hipEventSynchronize(b->copied) != hipSuccess)
     return pbx_fail(c, PBX_EHIP, "pbx_kv_batch_set: waiting for the last set-up failed");
@@ -331,6 +440,8 @@ static int batch_upload(pbx_kv_batch *b) {
   memcpy(b->host + b->at_pos, p.row_pos.data(), p.row_pos.size() * 4);
   memcpy(b->host + b->at_last, p.last_rows.data(), p.last_rows.size() * 4);
   memcpy(b->host + b->at_table, p.table.data(), p.table.size() * 4);
+  if (!p.copies.empty())
+    memcpy(b->host + b->at_copies, p.copies.data(), p.copies.size() * sizeof(kv_page_copy));
   // per slot and KV head: 16 rows of hdp sums, then their maxima and weights
   const size_t part = (size_t)p.n_slots * kv->cfg.n_kv_heads * 16 * (kv->hdp + 2) * 4;
   const size_t joins = (size_t)p.n_joins * kv->cfg.n_kv_heads * 128, joins_had = b->arrived_cap;
@@ -346,6 +457,32 @@ static int batch_upload(pbx_kv_batch *b) {
   if (hipMemcpyAsync(b->dev, b->host, n * 4, hipMemcpyHostToDevice, c->stream) != hipSuccess ||
       hipEventRecord(b->copied, c->stream) != hipSuccess)
     return pbx_fail(c, PBX_EHIP, "pbx_kv_batch_set: copy failed");
+  return PBX_OK;
+}
+
+// Pages that the batch's sequences shared, copied for them.  Other batches that run
+// over those sequences know the old pages: they have to be set again, and a graph
+// that holds one cannot be, so then the batch is refused.
+static int batch_own_pages(pbx_kv_batch *b) {
+  pbx_kv *kv = b->kv;
+  pbx_ctx *c = kv->c;
+  const kv_batch_plan &p = b->plan;
+  if (p.copies.empty()) return PBX_OK;
+  auto knows = [&](const pbx_kv_batch *o) { return o != b && !o->stale && kv_plan_moved(kv->pages, o->plan); };
+  for (const pbx_kv_batch *o : kv->batches)
+    if (o->captured && knows(o))
+      return pbx_fail(c, PBX_EINVAL, "pbx_kv_batch_set: a captured graph runs over pages that a sequence shares and "
+                      "would leave");
+  const int32_t *copies = b->dev + b->at_copies;
+  const pbx_kv_config &g = kv->cfg;
+  KvPackHost a{kv->codes, kv->scales, (int64_t)kv->layer_codes, (int64_t)kv->layer_scales, copies, nullptr, nullptr,
+               (int)p.copies.size(), g.n_kv_heads, 2 * PBX_KV_BLOCK * kv->hdp, kv->page_shift};
+  void *args[] = {&a};
+  const int rc = kv_launch(c, c->fn[PBX_K_KV_COPY], "pbx_kv_copy", (int64_t)p.copies.size() * g.n_kv_heads * g.n_layers,
+                           256, args);
+  if (rc) return rc;
+  for (pbx_kv_batch *o : kv->batches)
+    if (knows(o)) o->stale = true;
   return PBX_OK;
 }
 
@@ -372,6 +509,7 @@ extern "C" int pbx_kv_batch_set(pbx_kv_batch *b, int n, const int32_t *seqs, con
       kv_plan_work(kv->pages, kv->cfg.n_heads / kv->cfg.n_kv_heads, kv->cfg.n_kv_heads, kv_max_tiles(kv->hdp),
                    2 * c->cu_count, &b->plan);
       rc = batch_upload(b);
+      if (!rc) rc = batch_own_pages(b);
     } catch (const std::bad_alloc &) {
       rc = pbx_fail(c, PBX_ENOMEM, "pbx_kv_batch_set: out of host memory");
     }
@@ -384,6 +522,7 @@ extern "C" int pbx_kv_batch_set(pbx_kv_batch *b, int n, const int32_t *seqs, con
   }
   b->set = true;
   b->stale = false;
+  b->alone = 0;
   return PBX_OK;
 }
 
@@ -391,7 +530,10 @@ extern "C" int pbx_kv_batch_set(pbx_kv_batch *b, int n, const int32_t *seqs, con
 static int batch_launch(pbx_kv_batch *b, hipFunction_t f, const char *name, int64_t grid, int block, void **args) {
   pbx_ctx *c = b->kv->c;
   const int rc = kv_launch(c, f, name, grid, block, args);
-  if (!rc && pbx_capturing(c)) b->captured = true;
+  if (!rc && pbx_capturing(c)) {
+    b->captured = true;
+    b->appends = b->appends || f == b->kv->append;
+  }
   return rc;
 }
 
@@ -402,7 +544,7 @@ static int batch_begin(pbx_kv_batch *b, const char *who, int layer, KvArgsHost *
   pbx_ctx *c = kv->c;
   const pbx_kv_config &g = kv->cfg;
   if (!b->set) return pbx_fail(c, PBX_EINVAL, "%s: the batch is not set", who);
-  if (b->stale) return pbx_fail(c, PBX_EINVAL, "%s: positions of the batch were dropped", who);
+  if (b->stale) return pbx_fail(c, PBX_EINVAL, "%s: positions of the batch were dropped or moved", who);
   if (layer < 0 || layer >= g.n_layers)
     return pbx_fail(c, PBX_EINVAL, "%s: layer %d outside [0, %d)", who, layer, g.n_layers);
   if (hipSetDevice(c->device) != hipSuccess) return pbx_fail(c, PBX_EHIP, "%s: hipSetDevice failed", who);
@@ -445,6 +587,19 @@ extern "C" int pbx_kv_append_dev(pbx_kv_batch *b, int layer, const float *dQ, in
     if (b->plan.counts[i] && kv->pages.seqs[b->plan.seqs[i]].len != b->plan.starts[i] + b->plan.counts[i])
       return pbx_fail(c, PBX_EINVAL, "%s: sequence %d grew past the batch's rows", who, b->plan.seqs[i]);
   if (!b->plan.n_rows) return PBX_OK;
+  // a batch that lengthened its sequences got pages of their own for its rows; since then, or
+  // where it runs over rows that were there, others may share them
+  const kv_pages &pages = kv->pages;
+  if (b->alone != pages.forks + 1) {
+    for (size_t i = 0; i < b->plan.seqs.size(); ++i) {
+      const int s = b->plan.seqs[i], end = b->plan.starts[i] + b->plan.counts[i];
+      for (int j = b->plan.starts[i] / pages.page_tokens; b->plan.counts[i] && j < pages.pages_of(end); ++j)
+        if (pages.refs[pages.seqs[s].pages[j]] > 1)
+          return pbx_fail(c, PBX_EINVAL, "%s: sequence %d shares pages of the batch's rows: truncate it to %d and set "
+                          "the batch again", who, s, b->plan.starts[i]);
+    }
+    b->alone = pages.forks + 1;
+  }
   if ((rc = rows_check(c, who, "dK", dK, &k_stride, g.n_kv_heads, g.head_dim)) ||
       (rc = rows_check(c, who, "dV", dV, &v_stride, g.n_kv_heads, g.head_dim)))
     return rc;

@@ -16,14 +16,18 @@
 
 struct kv_seq {
   int len = 0;
-  uint64_t met = 0;  // the last batch that named it (kv_pages::batches)
+  uint64_t met = 0;    // the last call that named it (kv_pages::batches)
+  uint64_t moved = 0;  // the last call that dropped its positions, or moved them or their
+  int moved_at = 0;    // pages, from position moved_at on
   std::vector<int32_t> pages;
 };
 
 struct kv_pages {
   int page_tokens = 0, max_seq = 0;
-  uint64_t batches = 0;  // planned so far, refused ones too
+  uint64_t batches = 0;  // planned so far, refused ones too (and forks and compactions)
+  uint64_t forks = 0;    // forks so far: pages that a sequence had alone may be shared since
   std::vector<int32_t> free_list;  // handed out from the back
+  std::vector<int32_t> refs;       // sequences that hold a page
   std::vector<kv_seq> seqs;
 
   void init(int page_tokens_, int n_pages, int max_seqs, int max_seq_) {
@@ -31,7 +35,27 @@ struct kv_pages {
     max_seq = max_seq_;
     free_list.resize(n_pages);
     for (int i = 0; i < n_pages; ++i) free_list[i] = n_pages - 1 - i;
+    refs.assign(n_pages, 0);
     seqs.assign(max_seqs, kv_seq());
+  }
+  // A page for one sequence (the caller has seen that there is one), and one that a
+  // sequence lets go of; untake and ungive take the last such call back.  None of
+  // them allocates: the free list never holds more than it did at first.
+  int32_t take() {
+    const int32_t p = free_list.back();
+    free_list.pop_back();
+    refs[p] = 1;
+    return p;
+  }
+  void give(int32_t p) {
+    if (!--refs[p]) free_list.push_back(p);
+  }
+  void untake(int32_t p) {
+    refs[p] = 0;
+    free_list.push_back(p);
+  }
+  void ungive(int32_t p) {
+    if (!refs[p]++) free_list.pop_back();
   }
   int pages_of(int tokens) const { return (int)(((int64_t)tokens + page_tokens - 1) / page_tokens); }
 
@@ -45,13 +69,51 @@ struct kv_pages {
       kv_seq &s = seqs[seq];
       s.len = n;
       while ((int)s.pages.size() > pages_of(n)) {
-        free_list.push_back(s.pages.back());
+        give(s.pages.back());
         s.pages.pop_back();
       }
       return PBX_OK;
     }
     *why = buf;
     return PBX_EINVAL;
+  }
+
+  // Sequence dsts[i] comes to hold the first lens[i] positions (lens == NULL: all)
+  // that srcs[i] held before the call, in the same pages.
+  int fork(int n, const int32_t *dsts, const int32_t *srcs, const int32_t *lens, std::string *why) {
+    char buf[160];
+    ++batches;
+    std::vector<std::vector<int32_t>> held(n);
+    std::vector<int> len(n);
+    for (int i = 0; i < n; ++i) {
+      const int d = dsts[i], s = srcs[i], known = (int)seqs.size();
+      buf[0] = 0;
+      if (d < 0 || d >= known || s < 0 || s >= known)
+        snprintf(buf, sizeof buf, "sequence %d outside [0, %d)", d < 0 || d >= known ? d : s, known);
+      else if (seqs[d].met == batches)
+        snprintf(buf, sizeof buf, "sequence %d twice among those that are made", d);
+      else if (lens && (lens[i] < 0 || lens[i] > seqs[s].len))
+        snprintf(buf, sizeof buf, "sequence %d holds %d positions, not %d", s, seqs[s].len, lens[i]);
+      if (buf[0]) {
+        *why = buf;
+        return PBX_EINVAL;
+      }
+      seqs[d].met = batches;
+      len[i] = lens ? lens[i] : seqs[s].len;
+      held[i].assign(seqs[s].pages.begin(), seqs[s].pages.begin() + pages_of(len[i]));
+    }
+    ++forks;
+    for (auto &h : held)
+      for (int32_t p : h) ++refs[p];
+    for (int i = 0; i < n; ++i) {
+      kv_seq &d = seqs[dsts[i]];
+      for (int32_t p : d.pages) give(p);
+      d.pages.swap(held[i]);
+      d.len = len[i];
+      d.moved = batches;
+      d.moved_at = dsts[i] == srcs[i] ? len[i] : 0;
+    }
+    return PBX_OK;
   }
 };
 
@@ -77,11 +139,22 @@ struct kv_attn_item {
   int32_t pages[4];  // the pages from block blk0 on (as far as blk1 needs them)
 };
 
+// A page of a sequence that grows in it while others hold it too: the sequence gets
+// a copy of its filled blocks, in every layer.
+struct kv_page_copy {
+  int32_t from, to, blocks, pad;
+};
+struct kv_own_page {  // where such a copy took its place
+  int32_t seq, index;
+};
+
 struct kv_batch_plan {
   int n_rows = 0;
   bool last = true;  // the rows are the last of their sequences
   std::vector<int32_t> seqs, starts, counts;
   std::vector<int32_t> had;  // the sequences' lengths before
+  std::vector<kv_page_copy> copies;
+  std::vector<kv_own_page> owned;  // [copies]
   // work lists, in the order they lie in device memory
   std::vector<kv_block_item> blocks;
   std::vector<kv_attn_item> attn;  // those of u 1, then 2, 4, 8
@@ -100,6 +173,18 @@ inline int kv_plan_rows(kv_pages *kv, int n, const int32_t *seqs, const int32_t 
   char buf[200];
   ++kv->batches;
   int64_t rows = 0, need = 0;
+  // Pages that the batch's sequences will have left to others, taken off their
+  // counts while the batch is looked over: the last holder needs no copy.
+  struct Left {
+    kv_pages *kv;
+    std::vector<int32_t> pages;
+    ~Left() {
+      for (int32_t p : pages) ++kv->refs[p];
+    }
+  };
+  kv_batch_plan q;
+  {
+  Left left{kv, {}};
   for (int i = 0; i < n; ++i) {
     const int s = seqs[i];
     buf[0] = 0;
@@ -118,6 +203,14 @@ inline int kv_plan_rows(kv_pages *kv, int n, const int32_t *seqs, const int32_t 
                  (long long)at + counts[i], kv->max_seq);
       else
         need += std::max(0, kv->pages_of(at + counts[i]) - (int)kv->seqs[s].pages.size());
+      const std::vector<int32_t> &held = kv->seqs[s].pages;
+      for (int j = at / kv->page_tokens; !buf[0] && at + counts[i] > len && j < (int)held.size(); ++j)
+        if (kv->refs[held[j]] > 1) {
+          left.pages.push_back(held[j]);
+          --kv->refs[held[j]];
+          q.owned.push_back({s, j});
+          ++need;
+        }
     }
     if (buf[0]) {
       *why = buf;
@@ -136,7 +229,7 @@ inline int kv_plan_rows(kv_pages *kv, int n, const int32_t *seqs, const int32_t 
     *why = buf;
     return PBX_ENOMEM;
   }
-  kv_batch_plan q;
+  }
   for (int i = 0; i < n; ++i) {
     kv_seq &s = kv->seqs[seqs[i]];
     q.seqs.push_back(seqs[i]);
@@ -147,14 +240,22 @@ inline int kv_plan_rows(kv_pages *kv, int n, const int32_t *seqs, const int32_t 
   }
   q.n_rows = (int)rows;
   q.row_pos.reserve(rows);
+  q.copies.reserve(q.owned.size());
   // nothing below allocates on behalf of a sequence: the pages change hands whole
+  for (const kv_own_page &o : q.owned) {
+    kv_seq &s = kv->seqs[o.seq];
+    const int32_t from = s.pages[o.index], to = kv->take();
+    const int filled = std::min(kv->page_tokens, s.len - o.index * kv->page_tokens);
+    q.copies.push_back({from, to, (filled + PBX_KV_BLOCK - 1) / PBX_KV_BLOCK, 0});
+    kv->give(from);
+    s.pages[o.index] = to;
+    if (s.moved != kv->batches) s.moved_at = o.index * kv->page_tokens;
+    s.moved = kv->batches;
+  }
   for (int i = 0; i < n; ++i) {
     kv_seq &s = kv->seqs[seqs[i]];
     const int end = q.starts[i] + counts[i];
-    while ((int)s.pages.size() < kv->pages_of(end)) {
-      s.pages.push_back(kv->free_list.back());
-      kv->free_list.pop_back();
-    }
+    while ((int)s.pages.size() < kv->pages_of(end)) s.pages.push_back(kv->take());
     s.len = std::max(s.len, end);
   }
   std::swap(*p, q);
@@ -166,6 +267,166 @@ inline int kv_plan_rows(kv_pages *kv, int n, const int32_t *seqs, const int32_t 
 inline void kv_plan_undo(kv_pages *kv, const kv_batch_plan &p) {
   std::string why;
   for (size_t i = p.seqs.size(); i-- > 0;) kv->truncate(p.seqs[i], p.had[i], &why);
+  for (size_t i = p.copies.size(); i-- > 0;) {
+    kv->seqs[p.owned[i].seq].pages[p.owned[i].index] = p.copies[i].from;
+    kv->ungive(p.copies[i].from);
+    kv->untake(p.copies[i].to);
+  }
+}
+
+// One block that a compaction fills: rows of the sequence's old positions, coded
+// anew, or (raw) the old block as it is.
+struct kv_pack_item {
+  int32_t page, sub;   // where it goes
+  int32_t pos0, rows;  // its first (new) position, and its rows
+  int32_t at;          // the old positions of its rows, from here on in the list
+  int32_t tab;         // the sequence's old pages, from here on in the list
+  int32_t raw, pad;
+};
+struct kv_pack_plan {
+  std::vector<kv_pack_item> items;
+  std::vector<int32_t> launches;  // items of each launch: later ones fill pages that earlier ones emptied
+  std::vector<int32_t> positions, table;
+  std::vector<int32_t> seqs;
+  std::vector<int32_t> log;  // pages taken (p) and given back (-1 - p), in order
+  std::vector<kv_seq> was;
+};
+
+inline void kv_pack_undo(kv_pages *kv, kv_pack_plan *p) {
+  for (size_t i = p->log.size(); i-- > 0;) {
+    const int32_t x = p->log[i];
+    if (x >= 0)
+      kv->untake(x);
+    else
+      kv->ungive(-1 - x);
+  }
+  for (size_t i = 0; i < p->was.size(); ++i) {
+    kv->seqs[p->seqs[i]].len = p->was[i].len;
+    kv->seqs[p->seqs[i]].pages.swap(p->was[i].pages);
+  }
+  p->log.clear();
+  p->was.clear();
+}
+
+// Sequence seqs[i] keeps counts[i] of its positions (rising; `positions` holds them
+// one sequence after the other), which move together to 0 .. counts[i] - 1.  Pages
+// whose rows all stay are kept; the rest goes to fresh pages, so that no block is
+// read after it was written over.  Positions only move down: once a page of new rows
+// is filled, as many old pages have been read for good, so a pool with few free pages
+// takes several launches (each fills pages that are free before it).
+inline int kv_plan_pack(kv_pages *kv, int n, const int32_t *seqs, const int32_t *counts, const int32_t *positions,
+                        kv_pack_plan *p, std::string *why) {
+  char buf[200];
+  ++kv->batches;
+  int64_t at = 0, all = 0, rows = 0;
+  for (int i = 0; i < n; ++i) {
+    const int s = seqs[i], known = (int)kv->seqs.size(), len = s < 0 || s >= known ? 0 : kv->seqs[s].len;
+    buf[0] = 0;
+    if (s < 0 || s >= known)
+      snprintf(buf, sizeof buf, "sequence %d outside [0, %d)", s, known);
+    else if (kv->seqs[s].met == kv->batches)
+      snprintf(buf, sizeof buf, "sequence %d twice", s);
+    else if (counts[i] < 0 || counts[i] > len)
+      snprintf(buf, sizeof buf, "sequence %d holds %d positions, %d are to stay", s, len, counts[i]);
+    for (int j = 0; !buf[0] && j < counts[i]; ++j)
+      if (positions[at + j] < (j ? positions[at + j - 1] + 1 : 0) || positions[at + j] >= len)
+        snprintf(buf, sizeof buf, "sequence %d: positions have to rise within [0, %d) (%d at place %d)", s, len,
+                 positions[at + j], j);
+    if (buf[0]) {
+      *why = buf;
+      return PBX_EINVAL;
+    }
+    kv->seqs[s].met = kv->batches;
+    at += counts[i];
+    all += (int64_t)kv->seqs[s].pages.size();
+    rows += counts[i];
+  }
+  if (rows > (1 << 26) || all > (1 << 26)) {
+    *why = "more than 2^26 positions in one call";
+    return PBX_ENOTSUP;
+  }
+  const int T = kv->page_tokens, per_page = T / PBX_KV_BLOCK;
+  // everything that may throw comes first (the log and the lists cannot grow past these)
+  p->seqs.assign(seqs, seqs + n);
+  p->was.resize(n);
+  p->log.reserve(2 * all + 2);
+  p->launches.reserve(all + 1);
+  p->items.reserve(all * per_page);
+  p->positions.reserve(rows);
+  p->table.reserve(all);
+  std::vector<std::vector<int32_t>> made(n);
+  std::vector<int> first(n), read(n);  // first page that is replaced, and old pages that are given back
+  std::vector<int> from(n);            // positions from which rows or pages move
+  at = 0;
+  for (int i = 0; i < n; ++i) {
+    int same = 0;
+    while (same < counts[i] && positions[at + same] == same) ++same;
+    first[i] = same == counts[i] ? kv->pages_of(same) : same / T;
+    read[i] = first[i];
+    from[i] = same == counts[i] ? same : first[i] * T;
+    made[i].reserve(kv->pages_of(counts[i]));
+    at += counts[i];
+  }
+  for (int i = 0; i < n; ++i) {
+    kv_seq &s = kv->seqs[seqs[i]];
+    p->was[i].len = s.len;
+    p->was[i].pages = s.pages;
+  }
+  size_t launched = 0;
+  auto give = [&](int i, int upto) {
+    for (; read[i] < upto; ++read[i]) {
+      kv->give(p->was[i].pages[read[i]]);
+      p->log.push_back(-1 - p->was[i].pages[read[i]]);
+    }
+  };
+  at = 0;
+  int done = 0;  // sequences whose old pages were given back
+  std::vector<int> need(n, 0);  // old pages that the pages planned so far have read for good
+  for (int i = 0; i < n; ++i) {
+    const std::vector<int32_t> &old = p->was[i].pages;
+    const int tab = (int)p->table.size(), list = (int)p->positions.size(), base = first[i] * T;
+    made[i].assign(old.begin(), old.begin() + first[i]);
+    if (first[i] < kv->pages_of(counts[i])) {
+      p->table.insert(p->table.end(), old.begin(), old.end());
+      p->positions.insert(p->positions.end(), positions + at + base, positions + at + counts[i]);
+    }
+    need[i] = first[i];
+    for (int j = first[i]; j < kv->pages_of(counts[i]); ++j) {
+      if (kv->free_list.empty()) {
+        if (p->items.size() > launched) p->launches.push_back((int32_t)(p->items.size() - launched));
+        launched = p->items.size();
+        for (; done < i; ++done) give(done, (int)p->was[done].pages.size());
+        give(i, need[i]);
+        if (kv->free_list.empty()) {
+          kv_pack_undo(kv, p);
+          snprintf(buf, sizeof buf, "no free page to move positions of sequence %d to", seqs[i]);
+          *why = buf;
+          return PBX_ENOMEM;
+        }
+      }
+      const int32_t page = kv->take();
+      p->log.push_back(page);
+      made[i].push_back(page);
+      for (int b = 0; b < per_page && j * T + b * PBX_KV_BLOCK < counts[i]; ++b) {
+        const int pos0 = j * T + b * PBX_KV_BLOCK, m = std::min(PBX_KV_BLOCK, counts[i] - pos0);
+        p->items.push_back({page, b, pos0, m, list + pos0 - base, tab,
+                            positions[at + pos0 + m - 1] == pos0 + m - 1, 0});
+      }
+      const int next = (j + 1) * T;
+      need[i] = next < counts[i] ? positions[at + next] / T : (int)old.size();
+    }
+    at += counts[i];
+  }
+  if (p->items.size() > launched) p->launches.push_back((int32_t)(p->items.size() - launched));
+  for (int i = 0; i < n; ++i) give(i, (int)p->was[i].pages.size());
+  for (int i = 0; i < n; ++i) {
+    kv_seq &s = kv->seqs[seqs[i]];
+    s.len = counts[i];
+    s.pages.swap(made[i]);
+    s.moved = kv->batches;
+    s.moved_at = from[i];
+  }
+  return PBX_OK;
 }
 
 #define KV_MAX_PARTS 64
@@ -277,6 +538,16 @@ inline void kv_plan_work(const kv_pages &kv, int groups, int kv_heads, int max_u
 inline bool kv_plan_reaches(const kv_batch_plan &p, int seq, int n) {
   for (size_t i = 0; i < p.seqs.size(); ++i)
     if (p.seqs[i] == seq) return p.counts[i] && p.starts[i] + p.counts[i] > n;
+  return false;
+}
+
+// Whether the batch runs over positions that the last call (a fork, a compaction, a
+// batch that took pages of its own) dropped or moved.
+inline bool kv_plan_moved(const kv_pages &kv, const kv_batch_plan &p) {
+  for (size_t i = 0; i < p.seqs.size(); ++i) {
+    const kv_seq &s = kv.seqs[p.seqs[i]];
+    if (p.counts[i] && s.moved == kv.batches && p.starts[i] + p.counts[i] > s.moved_at) return true;
+  }
   return false;
 }
 

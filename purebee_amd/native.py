@@ -46,6 +46,7 @@ EXPORTS = (
     "pbx_gguf_find_tensor", "pbx_gguf_get_int", "pbx_gguf_get_float", "pbx_gguf_get_string",
     "pbx_gguf_get_array", "pbx_gguf_model_config", "pbx_model_load_gguf",
     "pbx_kv_create", "pbx_kv_free", "pbx_kv_info", "pbx_kv_length", "pbx_kv_truncate",
+    "pbx_kv_fork", "pbx_kv_compact",
     "pbx_kv_batch_create", "pbx_kv_batch_free", "pbx_kv_batch_set", "pbx_kv_batch_rows",
     "pbx_kv_append_dev", "pbx_kv_attention_dev", "pbx_kv_read_dev",
     "pbx_logprobs_workspace", "pbx_logprobs_dev", "pbx_model_logprobs", "pbx_model_forward_kv",
@@ -208,6 +209,8 @@ def load_library():
                                        ctypes.POINTER(ctypes.c_size_t)]),
         "pbx_kv_length": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.POINTER(ctypes.c_int)]),
         "pbx_kv_truncate": (ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_int]),
+        "pbx_kv_fork": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _vp]),
+        "pbx_kv_compact": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _vp]),
         "pbx_kv_batch_create": (ctypes.c_int, [_vp, ctypes.POINTER(_vp)]),
         "pbx_kv_batch_free": (ctypes.c_int, [_vp]),
         "pbx_kv_batch_set": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _vp]),
@@ -477,6 +480,9 @@ class Context:
 
 
 def _i32(a):
+    """1-D int32 of a's whole numbers; OverflowError for one past 32 bits."""
+    if isinstance(a, np.ndarray) and a.dtype == np.int32 and a.ndim == 1:
+        return np.ascontiguousarray(a)
     return np.ascontiguousarray(list(a), np.int32)
 
 
@@ -566,6 +572,28 @@ class KvCache:
     def truncate(self, seq, n_tokens=0):
         """Drop the positions from n_tokens on, and the pages they leave empty."""
         self.ctx._call("pbx_kv_truncate", self._ptr, _int32(seq), _int32(n_tokens))
+
+    def fork(self, dsts, srcs, lengths=None):
+        """Sequence dsts[i] comes to hold the first lengths[i] positions (None: all) that
+        srcs[i] held before the call, in the same pages; a page is copied when a batch
+        lengthens a sequence in it."""
+        d, s = _i32(dsts), _i32(srcs)
+        n = None if lengths is None else _i32(lengths)
+        if len(s) != len(d) or (n is not None and len(n) != len(d)):
+            raise ValueError("dsts, srcs and lengths of different length")
+        self.ctx._call("pbx_kv_fork", self._ptr, len(d), d.ctypes.data, s.ctypes.data,
+                       None if n is None else n.ctypes.data)
+
+    def compact(self, seqs, kept):
+        """Sequence seqs[i] keeps the positions kept[i] (rising) and drops the others; the
+        k-th kept one becomes position k, its key turned to it."""
+        s = _i32(seqs)
+        kept = [_i32(k) for k in kept]
+        if len(kept) != len(s):
+            raise ValueError("seqs and kept of different length")
+        counts = np.array([len(k) for k in kept], np.int32)
+        at = np.concatenate(kept) if kept else np.empty(0, np.int32)
+        self.ctx._call("pbx_kv_compact", self._ptr, len(s), s.ctypes.data, counts.ctypes.data, at.ctypes.data)
 
     def free(self):
         """Frees the cache and its batches."""
