@@ -559,6 +559,32 @@ int pbx_logprobs_dev(pbx_ctx *ctx, const float *dLogits, int64_t stride, int64_t
                      float *dEntropy, int32_t *dTopIds, float *dTopLogp, void *work,
                      size_t work_bytes);
 
+/* The same of rows whose logits are X . W^T, without keeping those: a piece of the
+ * vocabulary at a time.  W: a head of any type but Q8_REF, [vocab, K]; dX [rows][K], at
+ * most 65,535 rows, 16-byte aligned.
+ *   dLogp[r]     log softmax at dTargets[r] (NaN for a target outside the vocabulary);
+ *                NULL, like dTargets, to leave it out
+ *   dEntropy[r]  -sum p log p, in nats; or NULL
+ *   dLse[r]      log of the sum of all e^logit, which the gradient needs; or NULL
+ * A row without a distribution (see above) answers with NaN.  Logits are those of
+ * pbx_linear.  Only enqueues on the context's stream.  work: device memory of the size
+ * that pbx_linear_logprobs_workspace gives (grad 1: for the gradient), 256-byte aligned,
+ * any content, for this call alone until it has run.  No reference counterpart. */
+int pbx_linear_logprobs_workspace(pbx_ctx *ctx, const pbx_weight *W, int64_t rows, int grad, size_t *bytes);
+int pbx_linear_logprobs_dev(pbx_ctx *ctx, const pbx_weight *W, const float *dX, int64_t rows,
+                            const int32_t *dTargets, float *dLogp, float *dEntropy, float *dLse,
+                            void *work, size_t work_bytes);
+/* The rows' gradient: dGradX[r] = dGradLogp[r] * d logp[r] / d x[r]
+ *   = dGradLogp[r] * (W[dTargets[r]] - sum_v e^(logit_v - dLse[r]) W[v]),
+ * 0 where a row's target is outside the vocabulary (padding), [rows][K], 16-byte aligned,
+ * not dX itself.  dLse as pbx_linear_logprobs_dev gave it for these rows.  Logits are
+ * computed again; probabilities and weights enter the second product with 22 bits
+ * (weights 2^-26 of the head's largest at least), sums are held in f32 and come out the
+ * same in every call.  The weights stay as they are: they have no gradient. */
+int pbx_linear_logprobs_grad_dev(pbx_ctx *ctx, const pbx_weight *W, const float *dX, int64_t rows,
+                                 const int32_t *dTargets, const float *dLse, const float *dGradLogp,
+                                 float *dGradX, void *work, size_t work_bytes);
+
 /* pbx_model_forward_batch that answers with log probabilities instead of n
  * rows of logits: row t's target is targets[t] (usually tokens[t + 1]; outside
  * the vocabulary: NaN).  Host arrays [n_tokens] or [n_tokens][top], as above;

@@ -1,0 +1,490 @@
+// pbx_head.hip -- log probabilities of rows straight from a head's weights, a piece of
+// the vocabulary at a time, and the rows' gradient.
+//
+// With logits l_v = x . W_v, m = max l, S = sum e^(l - m), T = sum e^(l - m) (l - m):
+//   lse = m + log S,  log p_t = l_t - lse,  entropy = log S - T / S,
+// where (m, S, T) of parts of the vocabulary join as
+//   S = S1 e^(m1 - m) + S2 e^(m2 - m),  T = sum (Ti + (mi - m) Si) e^(mi - m);
+// and d log p_t / dx = W_t - sum_v p_v W_v = sum_v G_v W_v with G = (v == t) - e^(l - lse).
+
+#include "pbx_gemv_impl.h"
+
+using namespace pbx;
+
+namespace {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2t __attribute__((ext_vector_type(2)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+// The maximum before any element: finite, so differences need no special case
+// (an element of -inf adds nothing; a row of nothing else keeps S == 0).
+constexpr float LOWEST = -3.402823466e38f;
+
+struct Sums {
+  float m, s, t;
+};
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504f); }
+// e^d is 0 from -104 on; the bound keeps products with 0 finite
+__device__ __forceinline__ float bounded(float d) { return fmaxf(d, -200.f); }
+__device__ __forceinline__ Sums moved(Sums a, float m) {  // to the larger maximum m
+  const float d = bounded(a.m - m), f = exp_of(d);
+  return {m, a.s * f, fmaf(d, a.s, a.t) * f};
+}
+
+// The sums of all 256 threads: one maximum first, then each moves once.
+__device__ __forceinline__ Sums join_threads(Sums a, float (*buf)[4]) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  float m = wave_max(a.m);
+  if (lane == 0) buf[wave][0] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(buf[0][0], buf[1][0]), fmaxf(buf[2][0], buf[3][0]));
+  a = moved(a, m);
+  const float s = wave_sum(a.s), t = wave_sum(a.t);
+  if (lane == 0) {
+    buf[wave][1] = s;
+    buf[wave][2] = t;
+  }
+  __syncthreads();
+  return {m, buf[0][1] + buf[1][1] + buf[2][1] + buf[3][1], buf[0][2] + buf[1][2] + buf[2][2] + buf[3][2]};
+}
+
+}  // namespace
+
+#define HEAD_SHARE 8192  // logits of a workgroup of pbx_head_stats
+
+// Sums of a piece's logits Z [M][stride] (n of a row count; it starts at vocabulary
+// entry v0): workgroup (part of 8192, row) -> parts[row][part0 + part], and the targets'
+// logits.
+extern "C" __global__ void __launch_bounds__(256)
+pbx_head_stats(const float *Z, int64_t stride, int n, int v0, const int *targets, float4 *parts, int n_parts,
+               int part0, float *hit) {
+  __shared__ float buf[4][4];
+  const int64_t row = blockIdx.y;
+  const float *z = Z + row * stride;
+  const int at = blockIdx.x * HEAD_SHARE;
+  float4 x[HEAD_SHARE / 1024];
+  Sums a{LOWEST, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < HEAD_SHARE / 1024; ++i) {
+    const int v = at + 4 * (int)threadIdx.x + 1024 * i;
+    x[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    if (v < n) {
+      x[i] = *reinterpret_cast<const float4 *>(z + v);
+      if (v + 1 >= n) x[i].y = -INFINITY;
+      if (v + 2 >= n) x[i].z = -INFINITY;
+      if (v + 3 >= n) x[i].w = -INFINITY;
+    }
+    a.m = fmaxf(fmaxf(fmaxf(a.m, x[i].x), fmaxf(x[i].y, x[i].z)), x[i].w);
+  }
+#pragma unroll
+  for (int i = 0; i < HEAD_SHARE / 1024; ++i) {
+    const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float d = bounded(v[e] - a.m), f = exp_of(d);
+      // (the bound hides a NaN: a NaN logit has to reach the sum)
+      a.s += v[e] != v[e] ? v[e] : f;
+      a.t = fmaf(d, f, a.t);
+    }
+  }
+  a = join_threads(a, buf);
+  if (threadIdx.x == 0) {
+    parts[row * n_parts + part0 + blockIdx.x] = make_float4(a.m, a.s, a.t, 0.f);
+    if (blockIdx.x == 0 && hit) {
+      const int64_t t = (int64_t)targets[row] - v0;
+      if (t >= 0 && t < n) hit[row] = z[t];
+    }
+  }
+}
+
+// A row's parts joined: workgroup = row.
+extern "C" __global__ void __launch_bounds__(256)
+pbx_head_join(const float4 *parts, int n_parts, const int *targets, int vocab, const float *hit, float *logp,
+              float *entropy, float *lse) {
+  __shared__ float buf[4][4];
+  const int64_t row = blockIdx.x;
+  Sums a{LOWEST, 0.f, 0.f};
+  for (int i = threadIdx.x; i < n_parts; i += 256) {
+    const float4 p = parts[row * n_parts + i];
+    const float m = fmaxf(a.m, p.x);
+    const Sums u = moved(a, m), w = moved({p.x, p.y, p.z}, m);
+    a = {m, u.s + w.s, u.t + w.t};
+  }
+  a = join_threads(a, buf);
+  if (threadIdx.x) return;
+  const float none = __uint_as_float(0x7fc00000u);
+  const bool ok = a.s > 0.f && a.s < INFINITY && a.m < INFINITY;
+  const float log_s = logf(a.s), all = a.m + log_s;
+  if (lse) lse[row] = ok ? all : none;
+  if (entropy) entropy[row] = ok ? log_s - a.t / a.s : none;
+  if (logp) {
+    const int t = targets[row];
+    // x_t - m first: it is exact where the target is the likeliest
+    logp[row] = ok && t >= 0 && t < vocab ? hit[row] - a.m - log_s : none;
+  }
+}
+
+// ---- the gradient --------------------------------------------------------------------
+
+// The largest scale of a quantised head: a workgroup's largest magnitude of its share of
+// the plane's halves, as bits.
+extern "C" __global__ void __launch_bounds__(256)
+pbx_head_scale(const uint16_t *plane, int64_t n8, unsigned *peaks) {  // n8 groups of 8 halves
+  __shared__ unsigned red[4];
+  unsigned m = 0;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n8; i += (int64_t)gridDim.x * 256) {
+    const uint4 v = reinterpret_cast<const uint4 *>(plane)[i];
+    const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = max(m, max(w[e] & 0x7fffu, (w[e] >> 16) & 0x7fffu));
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off /= 2) m = max(m, (unsigned)__shfl_xor((int)m, off, 64));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) peaks[blockIdx.x] = max(max(red[0], red[1]), max(red[2], red[3]));
+}
+
+#define HEAD_PEAKS 256  // workgroups of pbx_head_scale
+
+namespace {
+
+// The power of two that weights enter the products with: the largest scale (or Q4_1
+// minimum) comes to just below 2^TARGET.
+__device__ __forceinline__ int head_shift(const unsigned *peaks, int target) {
+  unsigned m = 0;
+  for (int i = threadIdx.x & 63; i < HEAD_PEAKS; i += 64) m = max(m, peaks[i]);
+#pragma unroll
+  for (int off = 32; off >= 1; off /= 2) m = max(m, (unsigned)__shfl_xor((int)m, off, 64));
+  int e = 0;
+  if (m) frexpf(f16_bits_to_f32(m), &e);  // 2^(e - 1) <= it < 2^e
+  if (m >= 0x7c00u) e = 16;
+  return __builtin_amdgcn_readfirstlane(target - e);
+}
+template <int TYPE> struct HeadTarget { static constexpr int value = TYPE == PBX_Q8 ? -5 : TYPE == PBX_Q6K ? -10 : TYPE == PBX_Q41 ? -2 : -1; };
+
+}  // namespace
+
+// G of a piece as fp16 pairs times 2^15, [n / 32][Mpad][32]: workgroup (block of 32
+// vocabulary entries, 64 rows); zeros past the vocabulary, the rows, and in rows
+// without a target.
+extern "C" __global__ void __launch_bounds__(256)
+pbx_head_g(const float *Z, int64_t stride, int n, int v0, const float *lse, const int *targets, int vocab, int M,
+           int Mpad, _Float16 *hi, _Float16 *lo) {
+  const int row = blockIdx.y * 64 + threadIdx.x / 4, v = blockIdx.x * 32 + 8 * (threadIdx.x % 4);
+  if (row >= Mpad) return;
+  half8 H = {}, L = {};
+  const int t = row < M ? targets[row] : -1;
+  if (t >= 0 && t < vocab) {
+    const float *z = Z + (int64_t)row * stride;
+    const float s = lse[row];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (v + e >= n) continue;
+      const float d = z[v + e] - s;
+      const float g = (v0 + v + e == t ? -expm1f(d) : -expf(d)) * 32768.f;
+      H[e] = (_Float16)g;
+      L[e] = (_Float16)(g - (float)H[e]);
+    }
+  }
+  const int64_t at = ((int64_t)blockIdx.x * Mpad + row) * 32 + 8 * (threadIdx.x % 4);
+  *reinterpret_cast<half8 *>(hi + at) = H;
+  *reinterpret_cast<half8 *>(lo + at) = L;
+}
+
+// The same in f32 for an F32 head: [n][Mpad].
+extern "C" __global__ void __launch_bounds__(256)
+pbx_head_g32(const float *Z, int64_t stride, int n, int v0, const float *lse, const int *targets, int vocab, int M,
+             int Mpad, float *G) {
+  const int row = blockIdx.y * 64 + (threadIdx.x & 63), v = blockIdx.x * 32 + 8 * (threadIdx.x >> 6);
+  if (row >= Mpad) return;
+  const int t = row < M ? targets[row] : -1;
+  const bool on = t >= 0 && t < vocab;
+  const float s = on ? lse[row] : 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float g = 0.f;
+    if (on && v + e < n) {
+      const float d = Z[(int64_t)row * stride + v + e] - s;
+      g = v0 + v + e == t ? -expm1f(d) : -expf(d);
+    }
+    G[(int64_t)(v + e) * Mpad + row] = g;
+  }
+}
+
+struct BackArgs {
+  const uint8_t *qs;   // planes from the piece's first row on
+  const uint16_t *dsc, *msc;
+  const _Float16 *hi, *lo;  // G
+  const float *G32;
+  const unsigned *peaks;
+  float *part;         // [KS][M][K]
+  int M, Mpad, K, B;   // B: 32-wide blocks of a row
+  int blocks, rows;    // blocks of 32 entries of the piece, and weight rows that may be read
+  int KS, add;         // add: to the partial sums of the pieces before
+};
+
+namespace {
+
+// hi and lo of 4 columns of weights at 8 consecutive vocabulary entries: column i's
+// operand is H[i], L[i].  Products of a code and its scale are exact as the pair
+// (19 bits at most); Q4_1 and Q6_K values are rounded to f32 first.
+struct Operand {
+  half8 H[4], L[4];
+};
+__device__ __forceinline__ half2t as_half2(unsigned x) { return __builtin_bit_cast(half2t, x); }
+// Byte i of x and of y, as two halves u * 2^-24 (the bits of a half of exponent 0).
+__device__ __forceinline__ unsigned byte_pair(unsigned x, unsigned y, int i) {
+  return __builtin_amdgcn_perm(y, x, 0x0c000c00u | (unsigned)i | (unsigned)(4 + i) << 16);
+}
+__device__ __forceinline__ void put_pair(Operand &o, int i, int p, half2t y, half2t d) {
+  const half2t h = y * d;
+  const half2t l = __builtin_elementwise_fma(y, d, -h);
+  o.H[i][2 * p] = h[0];
+  o.H[i][2 * p + 1] = h[1];
+  o.L[i][2 * p] = l[0];
+  o.L[i][2 * p + 1] = l[1];
+}
+__device__ __forceinline__ void put_value(Operand &o, int i, int e, float w) {
+  o.H[i][e] = (_Float16)w;
+  o.L[i][e] = (_Float16)(w - (float)o.H[i][e]);
+}
+
+template <int TYPE> struct HeadRaw {  // of one row
+  unsigned w;
+};
+template <> struct HeadRaw<PBX_F16> { uint2 w; };
+template <> struct HeadRaw<PBX_Q6K> {
+  unsigned ql0, ql1, qh, d;
+  uint2 sc;
+};
+
+// Column of the wave's 128 that lane lr's tile i holds.
+template <int TYPE>
+__device__ __forceinline__ int column_of(int lr, int i) {
+  if constexpr (TYPE == PBX_Q4 || TYPE == PBX_Q41) return 32 * (lr >> 3) + 16 * (i >> 1) + 2 * (lr & 7) + (i & 1);
+  if constexpr (TYPE == PBX_Q6K) return 32 * i + lr;
+  return 4 * lr + i;
+}
+
+// TT: 32-row tiles.
+template <int TYPE, int TT>
+__device__ __forceinline__ void back_body(const BackArgs &a) {
+  const int lane = threadIdx.x, lr = lane & 31, h = lane >> 5;
+  const int k0 = blockIdx.x * 128, m0 = blockIdx.y * (32 * TT);
+  const int b0 = (int)((int64_t)a.blocks * blockIdx.z / a.KS), b1 = (int)((int64_t)a.blocks * (blockIdx.z + 1) / a.KS);
+  constexpr bool NIB = TYPE == PBX_Q4 || TYPE == PBX_Q41;
+  const floatx16 zero = {};
+  floatx16 acc[TT][4];
+#pragma unroll
+  for (int t = 0; t < TT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[t][i] = zero;
+  const int shift = TYPE == PBX_F16 ? 0 : head_shift(a.peaks, HeadTarget<TYPE>::value);
+  // codes enter as u 2^-9, so their scales take 2^9 more; by two factors, either of
+  // which a half holds
+  const int both = shift + 9, s1 = min(15, max(-14, both));
+  const _Float16 f1 = (_Float16)ldexpf(1.f, s1), f2 = (_Float16)ldexpf(1.f, both - s1);
+  const float fs = ldexpf(1.f, shift);
+  // past the row's end columns repeat the last ones (and are not stored)
+  const int kc = min(k0 + 4 * lr, a.K - 4), kb = min((k0 >> 5) + (lr >> 3), a.B - 1);
+  for (int b = b0; b < b1; ++b) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int v = 32 * b + 16 * half + 8 * h;
+      half8 Ah[TT], Al[TT];
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const int64_t at = ((int64_t)b * a.Mpad + m0 + 32 * t + lr) * 32 + 16 * half + 8 * h;
+        Ah[t] = *reinterpret_cast<const half8 *>(a.hi + at);
+        Al[t] = *reinterpret_cast<const half8 *>(a.lo + at);
+      }
+      Operand o;
+      if constexpr (TYPE == PBX_F16) {
+        uint2 w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          w[e] = *reinterpret_cast<const uint2 *>(a.qs + ((int64_t)min(v + e, a.rows - 1) * a.K + kc) * 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            const unsigned x = i < 2 ? w[2 * p].x : w[2 * p].y, y = i < 2 ? w[2 * p + 1].x : w[2 * p + 1].y;
+            const half2t z = as_half2(__builtin_amdgcn_perm(y, x, i & 1 ? 0x07060302u : 0x05040100u));
+            o.H[i][2 * p] = z[0];
+            o.H[i][2 * p + 1] = z[1];
+          }
+      } else if constexpr (TYPE == PBX_Q6K) {
+        // 4 tiles are the four 32-code groups of half a superblock
+        const int SB = a.B >> 3, sb = min(k0 >> 8, SB - 1), hf = (k0 >> 7) & 1;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int n = min(v + e, a.rows - 1);
+          const uint8_t *blk = a.qs + ((int64_t)n * SB + sb) * PBX_Q6K_BYTES;
+          const unsigned l0 = blk[64 * hf + lr], l1 = blk[64 * hf + 32 + lr], q = blk[128 + 32 * hf + lr];
+          const uint2 sc = *reinterpret_cast<const uint2 *>(blk + 192 + 8 * hf);
+          const float d = f16_bits_to_f32(a.dsc[dsc_index(n, sb, SB)]) * fs;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const unsigned s8 = ((i < 2 ? sc.x : sc.y) >> (16 * (i & 1) + 8 * (lr >> 4))) & 255u;
+            const int code = (int)(((i & 1 ? l1 : l0) >> (4 * (i >> 1)) & 15u) | ((q >> (2 * i) & 3u) << 4)) - 32;
+            put_value(o, i, e, d * (float)(int8_t)s8 * (float)code);
+          }
+        }
+      } else {
+        unsigned w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int64_t n = min(v + e, a.rows - 1);
+          if constexpr (NIB)
+            w[e] = *reinterpret_cast<const uint16_t *>(a.qs + (n * a.B + kb) * 16 + 2 * (lr & 7));
+          else
+            w[e] = *reinterpret_cast<const unsigned *>(a.qs + n * a.K + kc) ^ 0x80808080u;
+        }
+        // scales of rows v .. v + 7: two groups of four (their rows are padded to 64)
+        uint2 d[2], mn[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const int n = min(v + 4 * g, a.rows - 4);
+          d[g] = *reinterpret_cast<const uint2 *>(a.dsc + dsc_index(n, kb, a.B));
+          mn[g] = TYPE == PBX_Q41 ? *reinterpret_cast<const uint2 *>(a.msc + dsc_index(n, kb, a.B)) : make_uint2(0, 0);
+        }
+        if constexpr (TYPE == PBX_Q41) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const unsigned dw = e & 2 ? d[e >> 2].y : d[e >> 2].x, mw = e & 2 ? mn[e >> 2].y : mn[e >> 2].x;
+            const float df = f16_bits_to_f32(dw >> (16 * (e & 1))) * fs, mf = f16_bits_to_f32(mw >> (16 * (e & 1))) * fs;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              put_value(o, i, e, fmaf((float)(w[e] >> (8 * (i & 1) + 4 * (i >> 1)) & 15u), df, mf));
+          }
+        } else {
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            const half2t dp = as_half2(p & 1 ? d[p >> 1].y : d[p >> 1].x) * f1 * f2;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              half2t y;
+              if constexpr (TYPE == PBX_Q4) {
+                const unsigned x = byte_pair(w[2 * p], w[2 * p + 1], i & 1);
+                const half2t off = {(_Float16)-0.015625f, (_Float16)-0.015625f};  // -8 2^-9
+                const _Float16 up = i < 2 ? (_Float16)32768.f : (_Float16)2048.f;
+                y = __builtin_elementwise_fma(as_half2(x & (i < 2 ? 0x000F000Fu : 0x00F000F0u)), half2t{up, up}, off);
+              } else {
+                const half2t off = {(_Float16)-0.25f, (_Float16)-0.25f};  // -128 2^-9
+                const half2t up = {(_Float16)32768.f, (_Float16)32768.f};
+                y = __builtin_elementwise_fma(as_half2(byte_pair(w[2 * p], w[2 * p + 1], i)), up, off);
+              }
+              put_pair(o, i, p, y, dp);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc[t][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(Ah[t], o.H[i], acc[t][i], 0, 0, 0);
+          acc[t][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(Al[t], o.H[i], acc[t][i], 0, 0, 0);
+          if constexpr (TYPE != PBX_F16)
+            acc[t][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(Ah[t], o.L[i], acc[t][i], 0, 0, 0);
+        }
+    }
+  }
+  const float undo = ldexpf(1.f, -15 - shift);
+  float *part = a.part + (int64_t)blockIdx.z * a.M * a.K;
+#pragma unroll
+  for (int t = 0; t < TT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int m = m0 + 32 * t + 8 * (r >> 2) + 4 * h + (r & 3);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = k0 + column_of<TYPE>(lr, i);
+        if (m >= a.M || k >= a.K) continue;
+        float *p = part + (int64_t)m * a.K + k;
+        const float x = acc[t][i][r] * undo;
+        *p = a.add ? *p + x : x;
+      }
+    }
+}
+
+// An F32 head: v_mfma_f32_32x32x2_f32, one entry for each half of the wave.
+template <int TT>
+__device__ __forceinline__ void back_f32(const BackArgs &a) {
+  const int lane = threadIdx.x, lr = lane & 31, h = lane >> 5;
+  const int k0 = blockIdx.x * 128, m0 = blockIdx.y * (32 * TT);
+  const int b0 = (int)((int64_t)a.blocks * blockIdx.z / a.KS), b1 = (int)((int64_t)a.blocks * (blockIdx.z + 1) / a.KS);
+  const floatx16 zero = {};
+  floatx16 acc[TT][4];
+#pragma unroll
+  for (int t = 0; t < TT; ++t)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[t][i] = zero;
+  const int kc = min(k0 + 4 * lr, a.K - 4);
+  const float *W = reinterpret_cast<const float *>(a.qs);
+  for (int b = b0; b < b1; ++b) {
+#pragma unroll 4
+    for (int j = 0; j < 32; j += 2) {
+      const int64_t v = 32 * b + j + h;
+      const float4 w = *reinterpret_cast<const float4 *>(W + min(v, (int64_t)a.rows - 1) * a.K + kc);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const float g = a.G32[v * a.Mpad + m0 + 32 * t + lr];
+        acc[t][0] = __builtin_amdgcn_mfma_f32_32x32x2f32(g, w.x, acc[t][0], 0, 0, 0);
+        acc[t][1] = __builtin_amdgcn_mfma_f32_32x32x2f32(g, w.y, acc[t][1], 0, 0, 0);
+        acc[t][2] = __builtin_amdgcn_mfma_f32_32x32x2f32(g, w.z, acc[t][2], 0, 0, 0);
+        acc[t][3] = __builtin_amdgcn_mfma_f32_32x32x2f32(g, w.w, acc[t][3], 0, 0, 0);
+      }
+    }
+  }
+  float *part = a.part + (int64_t)blockIdx.z * a.M * a.K;
+#pragma unroll
+  for (int t = 0; t < TT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int m = m0 + 32 * t + 8 * (r >> 2) + 4 * h + (r & 3), k = k0 + 4 * lr;
+      if (m >= a.M || k >= a.K) continue;
+      float4 *p = reinterpret_cast<float4 *>(part + (int64_t)m * a.K + k);
+      float4 x = make_float4(acc[t][0][r], acc[t][1][r], acc[t][2][r], acc[t][3][r]);
+      if (a.add) x.x += p->x, x.y += p->y, x.z += p->z, x.w += p->w;
+      *p = x;
+    }
+}
+
+}  // namespace
+
+#define HEAD_BACK(TAG, TYPE)                                                                                     \
+  extern "C" __global__ void __launch_bounds__(64) pbx_head_back_##TAG##_1(BackArgs a) { back_body<TYPE, 1>(a); } \
+  extern "C" __global__ void __launch_bounds__(64) pbx_head_back_##TAG##_2(BackArgs a) { back_body<TYPE, 2>(a); }
+HEAD_BACK(q4, PBX_Q4)
+HEAD_BACK(q41, PBX_Q41)
+HEAD_BACK(q8, PBX_Q8)
+HEAD_BACK(q6k, PBX_Q6K)
+HEAD_BACK(f16, PBX_F16)
+extern "C" __global__ void __launch_bounds__(64) pbx_head_back_f32_1(BackArgs a) { back_f32<1>(a); }
+extern "C" __global__ void __launch_bounds__(64) pbx_head_back_f32_2(BackArgs a) { back_f32<2>(a); }
+
+// dX = grad * (the partial sums together), rows without a target 0: workgroup (16
+// float4s of a row), the partials over 16 threads each.
+extern "C" __global__ void __launch_bounds__(256)
+pbx_head_reduce(const float *part, int KS, int M, int K, const int *targets, int vocab, const float *grad, float *dX) {
+  __shared__ float4 sum[16][17];
+  const int64_t row = blockIdx.y, MK4 = (int64_t)M * K / 4;
+  const int c = threadIdx.x % 16, j = threadIdx.x / 16, k4 = blockIdx.x * 16 + c;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (k4 < K / 4)
+    for (int i = j; i < KS; i += 16) {
+      const float4 p = reinterpret_cast<const float4 *>(part)[i * MK4 + row * (K / 4) + k4];
+      s.x += p.x, s.y += p.y, s.z += p.z, s.w += p.w;
+    }
+  sum[j][c] = s;
+  __syncthreads();
+  if (j || k4 >= K / 4) return;
+  for (int i = 1; i < 16; ++i) s.x += sum[i][c].x, s.y += sum[i][c].y, s.z += sum[i][c].z, s.w += sum[i][c].w;
+  const int t = targets[row];
+  const float g = grad[row];
+  float4 *out = reinterpret_cast<float4 *>(dX) + row * (K / 4) + k4;
+  *out = t >= 0 && t < vocab ? make_float4(g * s.x, g * s.y, g * s.z, g * s.w) : make_float4(0.f, 0.f, 0.f, 0.f);
+}

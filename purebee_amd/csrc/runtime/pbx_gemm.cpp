@@ -90,59 +90,54 @@ int launch_reduce(pbx_ctx *c, float *part, const float *dBias, float *dY, int M,
 // F32 weights: fp32 MFMA.  M > 32: the LDS-DMA 128 x 128 kernel; otherwise
 // wave tile 16*MT x 16*NT (MT 1 / 2 for M <= 16 / <= 32), K split for about
 // eight waves per CU.
+struct F32Plan {
+  int MT = 0, NT = 0, mtiles = 0, nwg = 0, KS = 1;  // MT 0: the 128 x 128 kernel
+  size_t part(int M, int N) const { return KS > 1 ? (size_t)KS * M * N * 4 : 0; }
+};
+F32Plan plan_f32(const pbx_ctx *c, const pbx_weight *w, int M) {
+  const int N = (int)w->N, B = (int)w->B;
+  F32Plan p;
+  if (M > 32) {
+    // K split (16-k steps) for about one workgroup per CU
+    p.nwg = (N + 127) / 128;
+    p.mtiles = (M + 127) / 128;
+    const int wgs = p.nwg * p.mtiles;
+    if (wgs < c->cu_count) p.KS = std::min({2 * B, 8, (c->cu_count + wgs - 1) / wgs});
+    return p;
+  }
+  p.MT = M <= 16 ? 1 : 2;
+  p.mtiles = (M + 16 * p.MT - 1) / (16 * p.MT);
+  if (p.MT == 1)
+    p.NT = ((N + 255) / 256) * p.mtiles >= 2 * c->cu_count ? 4
+           : ((N + 127) / 128) * p.mtiles >= 2 * c->cu_count ? 2 : 1;
+  else
+    p.NT = 2;
+  p.nwg = (N + 64 * p.NT - 1) / (64 * p.NT);
+  const int waves = p.nwg * p.mtiles * 4;
+  if (waves < 8 * c->cu_count) p.KS = std::min({B, 8, (8 * c->cu_count + waves - 1) / waves});
+  return p;
+}
 int launch_f32(pbx_ctx *c, const pbx_weight *w, const float *dX, int M, const float *dBias,
                float *dY, int accumulate, hipStream_t stream, const pbx_workspace *ws) {
   const int N = (int)w->N, B = (int)w->B;
-  if (M > 32) {
-    // 128 x 128 tiles on the LDS-DMA kernel, K split (16-k steps) for about
-    // one workgroup per CU
-    const int nwg = (N + 127) / 128, mtiles = (M + 127) / 128, wgs = nwg * mtiles;
-    int KS = 1;
-    if (wgs < c->cu_count) KS = std::min({2 * B, 8, (c->cu_count + wgs - 1) / wgs});
-    float *part = nullptr;
-    if (KS > 1) {
-      char *p = nullptr;
-      int rc = workspace(c, ws, (size_t)KS * M * N * 4, &p);
-      if (rc) return rc;
-      part = (float *)p;
-    }
-    hipFunction_t fg = pbx_kernel_by_name(c, "pbx_gemm_f32_big");
-    if (!fg) return pbx_fail(c, PBX_ELOAD, "pbx_gemm: kernel pbx_gemm_f32_big missing");
-    GemmF32ArgsHost g{w->qs, dX, KS == 1 ? dBias : nullptr, KS == 1 ? dY : part,
-                      M, N, (int)w->Npad, B, KS, KS == 1 ? accumulate : 0};
-    void *args[] = {&g};
-    int rc = pbx_launch_fn(c, fg, "pbx_gemm_f32_big", dim3(nwg, mtiles, KS), dim3(256), args, stream);
-    if (rc || KS == 1) return rc;
-    return launch_reduce(c, part, dBias, dY, M, N, KS, accumulate, stream);
-  }
-  const int MT = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-  const int mtiles = (M + 16 * MT - 1) / (16 * MT);
-  int NT;
-  if (MT == 1)
-    NT = ((N + 255) / 256) * mtiles >= 2 * c->cu_count ? 4
-         : ((N + 127) / 128) * mtiles >= 2 * c->cu_count ? 2 : 1;
-  else
-    NT = MT == 2 ? 2 : 4;
-  const int nwg = (N + 64 * NT - 1) / (64 * NT);
-  int KS = 1;
-  const int waves = nwg * mtiles * 4;
-  if (waves < 8 * c->cu_count) KS = std::min({B, 8, (8 * c->cu_count + waves - 1) / waves});
+  const F32Plan p = plan_f32(c, w, M);
   float *part = nullptr;
-  if (KS > 1) {
-    char *p = nullptr;
-    int rc = workspace(c, ws, (size_t)KS * M * N * 4, &p);
+  if (p.KS > 1) {
+    char *ptr = nullptr;
+    int rc = workspace(c, ws, p.part(M, N), &ptr);
     if (rc) return rc;
-    part = (float *)p;
+    part = (float *)ptr;
   }
-  const std::string name = "pbx_gemm_f32_m" + std::to_string(MT) + "_n" + std::to_string(NT);
+  const std::string name =
+      p.MT ? "pbx_gemm_f32_m" + std::to_string(p.MT) + "_n" + std::to_string(p.NT) : "pbx_gemm_f32_big";
   hipFunction_t fg = pbx_kernel_by_name(c, name);
   if (!fg) return pbx_fail(c, PBX_ELOAD, "pbx_gemm: kernel %s missing", name.c_str());
-  GemmF32ArgsHost g{w->qs, dX, KS == 1 ? dBias : nullptr, KS == 1 ? dY : part,
-                    M, N, (int)w->Npad, B, KS, KS == 1 ? accumulate : 0};
+  GemmF32ArgsHost g{w->qs, dX, p.KS == 1 ? dBias : nullptr, p.KS == 1 ? dY : part,
+                    M, N, (int)w->Npad, B, p.KS, p.KS == 1 ? accumulate : 0};
   void *args[] = {&g};
-  int rc = pbx_launch_fn(c, fg, name.c_str(), dim3(nwg, mtiles, KS), dim3(256), args, stream);
-  if (rc || KS == 1) return rc;
-  return launch_reduce(c, part, dBias, dY, M, N, KS, accumulate, stream);
+  int rc = pbx_launch_fn(c, fg, name.c_str(), dim3(p.nwg, p.mtiles, p.KS), dim3(256), args, stream);
+  if (rc || p.KS == 1) return rc;
+  return launch_reduce(c, part, dBias, dY, M, N, p.KS, accumulate, stream);
 }
 
 // Few activation rows, one launch: 16 * MT rows of X and 16 * NT rows of W a
@@ -279,6 +274,31 @@ int pbx_gemm_run(pbx_ctx *c, const pbx_weight *w, const pbx_gemm_plan &p, const 
   return pbx_launch_fn(c, fg, p.name.c_str(), dim3(p.nwg, p.mtiles, p.KS), dim3(256), args, stream);
 }
 
+// The prepared GEMM that M rows of w take; p->M stays 0 for the one-launch kernel.
+static int prepared_plan(pbx_ctx *c, const pbx_weight *w, int M, pbx_gemm_plan *p) {
+  if (few_columns(c, w, M)) {
+    p->M = M;
+    p->Mpad = 16;
+    p->mtiles = 1;
+    p->nwg = ((int)w->N + 63) / 64;
+    p->KS = 8;  // the tiles alone are a wave each for at most half of the CUs
+    p->name = std::string("pbx_gemm_") + gemm_tag(w->type) + "_p16";
+  } else if (M > PBX_GEMM_ROWS_M || many_columns(c, w, M)) {
+    return pbx_gemm_make_plan(c, w, M, p);
+  }
+  return PBX_OK;
+}
+
+size_t pbx_linear_space(pbx_ctx *c, const pbx_weight *w, int M) {
+  if (M < PBX_GEMM_MIN_M || w->type == PBX_TYPE_Q6_K) return 0;
+  if (w->type == PBX_TYPE_F32) return plan_f32(c, w, M).part(M, (int)w->N);
+  pbx_gemm_plan p;
+  if (prepared_plan(c, w, M, &p)) return 0;
+  // (the one-launch kernel asks a caller's workspace for its rows' fp16 pair)
+  if (!p.M) return (size_t)(M <= 16 ? 16 : 32) * w->K * 4;
+  return gemm_space(p, (int)w->N, (int)w->K).total();
+}
+
 int pbx_gemm_launch(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M64,
                     const float *dBias, float *dY, int accumulate, hipStream_t stream,
                     const pbx_workspace *wsp) {
@@ -296,17 +316,7 @@ int pbx_gemm_launch(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M6
   const int M = (int)M64, N = (int)w->N, K = (int)w->B * 32;
   pbx_gemm_plan p;
   int rc;
-  if (few_columns(c, w, M)) {
-    p.M = M;
-    p.Mpad = 16;
-    p.mtiles = 1;
-    p.nwg = (N + 63) / 64;
-    p.KS = 8;  // the tiles alone are a wave each for at most half of the CUs
-    p.name = std::string("pbx_gemm_") + gemm_tag(w->type) + "_p16";
-  } else if ((M > PBX_GEMM_ROWS_M || many_columns(c, w, M)) &&
-             (rc = pbx_gemm_make_plan(c, w, M, &p))) {
-    return rc;
-  }
+  if ((rc = prepared_plan(c, w, M, &p))) return rc;
   if (!p.M) {
     // One launch on the fp32 rows: no workspace is used.  A caller that brings
     // one is still refused a K whose fp16 pair it could not hold: its limit

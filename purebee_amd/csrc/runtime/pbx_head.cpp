@@ -1,0 +1,210 @@
+// pbx_head.cpp -- log probabilities of rows straight from a head's weights and their
+// gradient (include/pbx.h): pieces of the vocabulary, workspace and launches.
+
+#include "pbx_internal.h"
+
+#include <algorithm>
+#include <string>
+
+namespace {
+
+struct BackArgsHost {  // BackArgs in pbx_head.hip
+  const void *qs, *dsc, *msc, *hi, *lo, *G32, *peaks;
+  float *part;
+  int M, Mpad, K, B, blocks, rows, KS, add;
+};
+
+#define HEAD_SHARE 8192          // of pbx_head.hip, too
+#define HEAD_PEAKS 256           // likewise
+#define HEAD_PIECE (64u << 20)   // bytes of a piece's logits at most
+
+// The head's rows from v0 on (a multiple of 128), n of them.
+pbx_weight rows_of(const pbx_weight &w, int64_t v0, int64_t n) {
+  pbx_weight v = w;
+  const size_t scales = w.type == PBX_TYPE_Q6_K ? w.K / 256 : w.B;
+  const size_t row = w.type == PBX_TYPE_F32    ? w.K * 4
+                     : w.type == PBX_TYPE_F16  ? w.K * 2
+                     : w.type == PBX_TYPE_Q6_K ? scales * 208
+                     : w.type == PBX_TYPE_Q8_0 ? scales * 32
+                                               : scales * 16;
+  v.qs = (char *)w.qs + v0 * row;
+  if (w.d) v.d = (char *)w.d + v0 * scales * 2;
+  if (w.m) v.m = (char *)w.m + v0 * scales * 2;
+  v.Npad = w.Npad - v0;
+  v.N = std::min(v.Npad, (n + 3) / 4 * 4);  // rows of logits begin 16-byte aligned; padding rows are zero
+  return v;
+}
+
+struct Plan {
+  int64_t piece;   // vocabulary entries of a piece, but for the last
+  int n_pieces, n_parts;
+  int Mpad, TT, KS;
+  // workspace: byte offsets
+  size_t gemm, z, parts, hit, g, peaks, part, bytes;
+};
+
+size_t padded(size_t n) { return (n + 255) / 256 * 256; }
+
+Plan make_plan(pbx_ctx *c, const pbx_weight *w, int64_t M, bool grad) {
+  Plan p{};
+  const int64_t V = w->N;
+  p.TT = M > 32 ? 2 : 1;
+  p.Mpad = (int)((M + 63) / 64 * 64);
+  const int64_t row = 4 * (grad ? p.Mpad : M);
+  p.piece = std::min<int64_t>((V + 127) / 128 * 128, std::max<int64_t>(128, HEAD_PIECE / row / 128 * 128));
+  p.n_pieces = (int)((V + p.piece - 1) / p.piece);
+  size_t at = 0;
+  auto take = [&](size_t n) {
+    const size_t from = at;
+    at += padded(n);
+    return from;
+  };
+  const int64_t last = V - (p.n_pieces - 1) * p.piece;
+  size_t gemm = 0;
+  for (int64_t n : {std::min(p.piece, V), last}) {
+    const pbx_weight part = rows_of(*w, 0, n);
+    gemm = std::max(gemm, pbx_linear_space(c, &part, (int)M));
+  }
+  auto shares = [](int64_t n) { return (int)((n + HEAD_SHARE - 1) / HEAD_SHARE); };
+  p.n_parts = (p.n_pieces - 1) * shares(p.piece) + shares(last);
+  p.gemm = take(gemm);
+  p.z = take((size_t)M * p.piece * 4);
+  if (!grad) {
+    p.parts = take((size_t)M * p.n_parts * 16);
+    p.hit = take((size_t)M * 4);
+  } else {
+    const int64_t tiles = (w->K + 127) / 128 * ((M + 32 * p.TT - 1) / (32 * p.TT));
+    // about two waves a SIMD
+    p.KS = (int)std::max<int64_t>(1, std::min<int64_t>(8 * c->cu_count / tiles, p.piece / 32));
+    p.g = take((size_t)p.Mpad * p.piece * 4);
+    p.peaks = take(HEAD_PEAKS * 4);
+    p.part = take((size_t)p.KS * M * w->K * 4);
+  }
+  p.bytes = at;
+  return p;
+}
+
+int check(pbx_ctx *c, const char *who, const pbx_weight *w, int64_t rows) {
+  if (!pbx_weight_ok(w)) return pbx_fail(c, PBX_EINVAL, "%s: not a live weight handle", who);
+  if (rows < 0) return pbx_fail(c, PBX_EINVAL, "%s: %lld rows", who, (long long)rows);
+  if (w->type == PBX_TYPE_Q8_REF) return pbx_fail(c, PBX_ENOTSUP, "%s: a Q8_REF weight", who);
+  if (rows > 65535 || w->N > (1 << 28)) return pbx_fail(c, PBX_ENOTSUP, "%s: at most 65,535 rows and 2^28 tokens", who);
+  if (w->type == PBX_TYPE_Q6_K && w->B > 512)
+    return pbx_fail(c, PBX_ENOTSUP, "%s: K=%lld exceeds the Q6_K limit of 16384", who, (long long)w->K);
+  return PBX_OK;
+}
+
+int check_work(pbx_ctx *c, const char *who, const Plan &p, const void *work, size_t bytes) {
+  if (!work || bytes < p.bytes || (uintptr_t)work % 256)
+    return pbx_fail(c, PBX_EINVAL, "%s: needs %zu bytes of 256-byte aligned workspace, got %zu", who, p.bytes, bytes);
+  if (hipSetDevice(c->device) != hipSuccess) return pbx_fail(c, PBX_EHIP, "%s: hipSetDevice failed", who);
+  return PBX_OK;
+}
+
+// Logits of the piece from v0 on, n entries.
+int piece_logits(pbx_ctx *c, const pbx_weight *w, const Plan &p, char *ws, const float *dX, int64_t M, int64_t v0,
+                 int64_t n, pbx_weight *rows) {
+  *rows = rows_of(*w, v0, n);
+  const pbx_workspace space{ws + p.gemm, p.z - p.gemm};
+  return pbx_linear_enqueue(c, rows, dX, M, nullptr, (float *)(ws + p.z), c->stream, &space);
+}
+
+}  // namespace
+
+extern "C" int pbx_linear_logprobs_workspace(pbx_ctx *c, const pbx_weight *w, int64_t rows, int grad, size_t *bytes) {
+  const char *who = "pbx_linear_logprobs_workspace";
+  if (!c) return pbx_fail(nullptr, PBX_EINVAL, "%s: ctx is NULL", who);
+  if (!bytes) return pbx_fail(c, PBX_EINVAL, "%s: NULL argument", who);
+  const int rc = check(c, who, w, rows);
+  if (!rc) *bytes = rows ? make_plan(c, w, rows, grad != 0).bytes : 0;
+  return rc;
+}
+
+extern "C" int pbx_linear_logprobs_dev(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M,
+                                       const int32_t *dTargets, float *dLogp, float *dEntropy, float *dLse, void *work,
+                                       size_t work_bytes) {
+  const char *who = "pbx_linear_logprobs_dev";
+  if (!c) return pbx_fail(nullptr, PBX_EINVAL, "%s: ctx is NULL", who);
+  int rc = check(c, who, w, M);
+  if (rc || !M) return rc;
+  if (!dX || (uintptr_t)dX % 16) return pbx_fail(c, PBX_EINVAL, "%s: dX needs a 16-byte aligned address", who);
+  if (!dTargets != !dLogp) return pbx_fail(c, PBX_EINVAL, "%s: dTargets and dLogp go together", who);
+  const Plan p = make_plan(c, w, M, false);
+  if ((rc = check_work(c, who, p, work, work_bytes))) return rc;
+  char *ws = (char *)work;
+  float *z = (float *)(ws + p.z), *hit = (float *)(ws + p.hit);
+  void *parts = ws + p.parts;
+  int n_parts = p.n_parts, part0 = 0;
+  for (int64_t v0 = 0; v0 < w->N; v0 += p.piece) {
+    pbx_weight rows;
+    int n = (int)std::min(p.piece, w->N - v0), at = (int)v0;
+    if ((rc = piece_logits(c, w, p, ws, dX, M, v0, n, &rows))) return rc;
+    const int here = (n + HEAD_SHARE - 1) / HEAD_SHARE;
+    int64_t stride = rows.N;
+    float *h = dLogp ? hit : nullptr;
+    void *args[] = {&z, &stride, &n, &at, (void *)&dTargets, &parts, &n_parts, &part0, &h};
+    if ((rc = pbx_launch(c, PBX_K_HEAD_STATS, dim3(here, (unsigned)M), dim3(256), args))) return rc;
+    part0 += here;
+  }
+  int vocab = (int)w->N;
+  void *args[] = {&parts, &n_parts, (void *)&dTargets, &vocab, &hit, &dLogp, &dEntropy, &dLse};
+  return pbx_launch(c, PBX_K_HEAD_JOIN, dim3((unsigned)M), dim3(256), args);
+}
+
+extern "C" int pbx_linear_logprobs_grad_dev(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M,
+                                            const int32_t *dTargets, const float *dLse, const float *dGradLogp,
+                                            float *dGradX, void *work, size_t work_bytes) {
+  const char *who = "pbx_linear_logprobs_grad_dev";
+  if (!c) return pbx_fail(nullptr, PBX_EINVAL, "%s: ctx is NULL", who);
+  int rc = check(c, who, w, M);
+  if (rc || !M) return rc;
+  if (!dX || !dGradX || (uintptr_t)dX % 16 || (uintptr_t)dGradX % 16)
+    return pbx_fail(c, PBX_EINVAL, "%s: dX and dGradX need 16-byte aligned addresses", who);
+  if (dGradX == dX) return pbx_fail(c, PBX_EINVAL, "%s: dGradX is dX itself", who);
+  if (!dTargets || !dLse || !dGradLogp) return pbx_fail(c, PBX_EINVAL, "%s: NULL argument", who);
+  const Plan p = make_plan(c, w, M, true);
+  if ((rc = check_work(c, who, p, work, work_bytes))) return rc;
+  const bool f32 = w->type == PBX_TYPE_F32;
+  const char *tag = f32                         ? "f32"
+                    : w->type == PBX_TYPE_F16   ? "f16"
+                    : w->type == PBX_TYPE_Q8_0  ? "q8"
+                    : w->type == PBX_TYPE_Q4_0  ? "q4"
+                    : w->type == PBX_TYPE_Q4_1  ? "q41"
+                                                : "q6k";
+  const std::string name = std::string("pbx_head_back_") + tag + "_" + std::to_string(p.TT);
+  hipFunction_t back = pbx_kernel_by_name(c, name);
+  if (!back) return pbx_fail(c, PBX_ELOAD, "%s: kernel %s missing", who, name.c_str());
+  char *ws = (char *)work;
+  float *z = (float *)(ws + p.z), *part = (float *)(ws + p.part);
+  void *peaks = ws + p.peaks;
+  if (w->d) {
+    int64_t n8 = w->Npad * (w->type == PBX_TYPE_Q6_K ? w->K / 256 : w->B) / 8 * (w->m ? 2 : 1);
+    void *args[] = {(void *)&w->d, &n8, &peaks};
+    if ((rc = pbx_launch(c, PBX_K_HEAD_SCALE, dim3(HEAD_PEAKS), dim3(256), args))) return rc;
+  }
+  int m = (int)M, k = (int)w->K, vocab = (int)w->N, Mpad = p.Mpad, KS = p.KS;
+  for (int64_t v0 = 0; v0 < w->N; v0 += p.piece) {
+    pbx_weight rows;
+    int n = (int)std::min(p.piece, w->N - v0), at = (int)v0;
+    if ((rc = piece_logits(c, w, p, ws, dX, M, v0, n, &rows))) return rc;
+    const int blocks = (n + 31) / 32;
+    int64_t stride = rows.N;
+    void *hi = ws + p.g, *lo = ws + p.g + (size_t)blocks * 32 * Mpad * 2;
+    if (f32) {
+      void *args[] = {&z, &stride, &n, &at, (void *)&dLse, (void *)&dTargets, &vocab, &m, &Mpad, &hi};
+      rc = pbx_launch(c, PBX_K_HEAD_G32, dim3(blocks, Mpad / 64), dim3(256), args);
+    } else {
+      void *args[] = {&z, &stride, &n, &at, (void *)&dLse, (void *)&dTargets, &vocab, &m, &Mpad, &hi, &lo};
+      rc = pbx_launch(c, PBX_K_HEAD_G, dim3(blocks, Mpad / 64), dim3(256), args);
+    }
+    if (rc) return rc;
+    BackArgsHost b{rows.qs, rows.d, rows.m, hi, lo, hi, peaks, part, m, Mpad, k, (int)w->B, blocks, (int)rows.Npad, KS,
+                   v0 > 0};
+    void *args[] = {&b};
+    if ((rc = pbx_launch_fn(c, back, name.c_str(), dim3((k + 127) / 128, (m + 32 * p.TT - 1) / (32 * p.TT), KS),
+                            dim3(64), args, c->stream)))
+      return rc;
+  }
+  void *args[] = {&part, &KS, &m, &k, (void *)&dTargets, &vocab, (void *)&dGradLogp, &dGradX};
+  return pbx_launch(c, PBX_K_HEAD_REDUCE, dim3((k / 4 + 15) / 16, (unsigned)M), dim3(256), args);
+}

@@ -16,6 +16,12 @@
   X(PBX_K_LOGPROBS_PART_512, "pbx_logprobs_part_512")        \
   X(PBX_K_LOGPROBS_JOIN, "pbx_logprobs_join")                \
   X(PBX_K_KV_ROPE_TABLE, "pbx_kv_rope_table")                \
+  X(PBX_K_HEAD_STATS, "pbx_head_stats")                      \
+  X(PBX_K_HEAD_JOIN, "pbx_head_join")                        \
+  X(PBX_K_HEAD_SCALE, "pbx_head_scale")                      \
+  X(PBX_K_HEAD_G, "pbx_head_g")                              \
+  X(PBX_K_HEAD_G32, "pbx_head_g32")                          \
+  X(PBX_K_HEAD_REDUCE, "pbx_head_reduce")                    \
   X(PBX_K_KV_COPY, "pbx_kv_copy")                            \
   X(PBX_K_REPACK_Q4_0, "pbx_repack_q4_0")                    \
   X(PBX_K_REPACK_Q8_0, "pbx_repack_q8_0")                    \
@@ -175,6 +181,10 @@ struct pbx_workspace {
 int pbx_linear_enqueue(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M,
                        const float *dBias, float *dY, hipStream_t stream,
                        const pbx_workspace *ws = nullptr);
+// Bytes of workspace that pbx_linear_enqueue asks of ws for M rows of w.
+size_t pbx_linear_space(pbx_ctx *c, const pbx_weight *w, int M);
+// Whether w is a live weight handle.
+bool pbx_weight_ok(const pbx_weight *w);
 // Bytes of the static device workspace (pbx_scratch.hip) and the lookup of
 // its address on the context's device (call with that device current).
 #define PBX_SCRATCH_BYTES ((size_t)PBX_NOALLOC_WORKSPACE_BYTES)

@@ -51,7 +51,8 @@ static const char *const kKernelNames[PBX_K_COUNT] = {
 // Code objects built from purebee_amd/csrc/kernels/*.hip, found next to this
 // library (or in the directory named by PBX_KERNEL_DIR).
 static const char *const kModuleFiles[] = {"pbx_gemv.hsaco", "pbx_decode.hsaco", "pbx_gemm.hsaco",
-                                          "pbx_prefill.hsaco", "pbx_kv.hsaco", "pbx_logprobs.hsaco"};
+                                          "pbx_prefill.hsaco", "pbx_kv.hsaco", "pbx_logprobs.hsaco",
+                                          "pbx_head.hsaco"};
 static const int kModuleCount = (int)(sizeof kModuleFiles / sizeof kModuleFiles[0]);
 
 static std::string code_object_dir() {
@@ -351,6 +352,7 @@ size_t pbx_type_row_bytes(int type, int64_t K) {
 }
 
 static bool weight_ok(const pbx_weight *w) { return w && w->magic == PBX_WEIGHT_MAGIC; }
+bool pbx_weight_ok(const pbx_weight *w) { return weight_ok(w); }
 
 static bool upload_type(int type) {
   return type == PBX_TYPE_Q4_0 || type == PBX_TYPE_Q4_1 || type == PBX_TYPE_Q8_0 ||

@@ -49,6 +49,7 @@ EXPORTS = (
     "pbx_kv_fork", "pbx_kv_compact",
     "pbx_kv_batch_create", "pbx_kv_batch_free", "pbx_kv_batch_set", "pbx_kv_batch_rows",
     "pbx_kv_append_dev", "pbx_kv_attention_dev", "pbx_kv_read_dev",
+    "pbx_linear_logprobs_workspace", "pbx_linear_logprobs_dev", "pbx_linear_logprobs_grad_dev",
     "pbx_logprobs_workspace", "pbx_logprobs_dev", "pbx_model_logprobs", "pbx_model_forward_kv",
 )
 
@@ -224,6 +225,12 @@ def load_library():
                                                   ctypes.POINTER(ctypes.c_size_t)]),
         "pbx_logprobs_dev": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i64, _vp, ctypes.c_int, _vp, _vp,
                                             _vp, _vp, _vp, ctypes.c_size_t]),
+        "pbx_linear_logprobs_workspace": (ctypes.c_int, [_vp, _vp, _i64, ctypes.c_int,
+                                                         ctypes.POINTER(ctypes.c_size_t)]),
+        "pbx_linear_logprobs_dev": (ctypes.c_int, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp,
+                                                   ctypes.c_size_t]),
+        "pbx_linear_logprobs_grad_dev": (ctypes.c_int, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp,
+                                                        ctypes.c_size_t]),
         "pbx_model_logprobs": (ctypes.c_int, [_vp, _vp, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int,
                                               _vp, _vp, _vp, _vp]),
         "pbx_model_forward_kv": (ctypes.c_int, [_vp, _vp, _vp, ctypes.c_int, _vp, _vp, _vp,
@@ -448,6 +455,25 @@ class Context:
         most likely tokens of rows of f32 logits on the device."""
         self._call("pbx_logprobs_dev", self._p, dLogits, stride, rows, vocab, dTargets, top, dLogp,
                    dEntropy, dTopIds, dTopLogp, dWork, work_bytes)
+
+    def linear_logprobs_workspace(self, w, rows, grad=False):
+        """Bytes of device workspace that linear_logprobs_dev (grad: linear_logprobs_grad_dev)
+        needs for this head and as many rows."""
+        b = ctypes.c_size_t()
+        self._call("pbx_linear_logprobs_workspace", self._p, w.ptr, rows, 1 if grad else 0, ctypes.byref(b))
+        return b.value
+
+    def linear_logprobs_dev(self, w, dX, rows, dTargets, dLogp, dEntropy, dLse, dWork, work_bytes):
+        """pbx_linear_logprobs_dev: log probabilities of dTargets, entropy and log of the
+        summed exponentials of the logits X . W^T, which are not kept."""
+        self._call("pbx_linear_logprobs_dev", self._p, w.ptr, dX, rows, dTargets, dLogp, dEntropy, dLse, dWork,
+                   work_bytes)
+
+    def linear_logprobs_grad_dev(self, w, dX, rows, dTargets, dLse, dGradLogp, dGradX, dWork, work_bytes):
+        """pbx_linear_logprobs_grad_dev: the gradient of the rows dX, from dLse of
+        linear_logprobs_dev and the gradient of the log probabilities."""
+        self._call("pbx_linear_logprobs_grad_dev", self._p, w.ptr, dX, rows, dTargets, dLse, dGradLogp, dGradX,
+                   dWork, work_bytes)
 
     def alloc(self, nbytes):
         return DeviceBuffer(self, nbytes)
