@@ -331,9 +331,12 @@ __device__ __forceinline__ void read_body(const KvArgs &a, const BlockItem *item
   }
 }
 
-// kv_pack_item and kv_page_copy of pbx_kv_plan.h
+// kv_pack_item, kv_pack_row and kv_page_copy of pbx_kv_plan.h
 struct PackItem {
-  int page, sub, pos0, rows, at, tab, raw, pad;
+  int page, sub, pos0, rows, at, raw, pad[2];
+};
+struct PackRow {
+  int page, pos;
 };
 struct PageCopy {
   int from, to, blocks, pad;
@@ -343,7 +346,7 @@ struct KvPack {
   float *scales;
   int64_t layer_codes, layer_scales;
   const void *items;
-  const int *positions, *table;
+  const PackRow *rows;
   int n_items, kv_heads, head_dim, page_shift;  // (copying: head_dim is a block's bytes)
 };
 
@@ -353,16 +356,28 @@ __device__ __forceinline__ int64_t block_index(const KvPack &a, int page, int he
 
 // Compaction: workgroup (layer, block of new rows, KV head).  A block's rows come from
 // up to 32 old blocks; each code stands for code * s (exact in 64 bits), keys turn back
-// by the distance that they move down, and the block is coded as a new one is.  Rows'
-// codes are fetched one by one: keys as pairs of dims, values byte by byte, as they lie
-// 64 bytes apart for consecutive dims.
+// by the distance that they move down, and the block is coded as a new one is.
+// A row's keys lie side by side and are fetched as they are.  Its values lie 64 bytes
+// apart for consecutive dims, so one row takes as many cache lines as the whole block:
+// the blocks' values are fetched whole, PACK_BLOCKS at a time, into LDS, where the 64
+// bytes of a dim take 68, so that dims fall in banks of their own.
+// (Fetched byte by byte the values bounded it: half of 31,000 positions, 8 heads of
+// 128, two layers 140 us.)
+constexpr int PACK_BLOCKS = 4;
+__device__ __forceinline__ int spread_byte(int key, int dim) {
+  const int slot = 8 * ((key >> 2) & 3) + 4 * (key >> 4) + (key & 3);
+  return (dim >> 5) * 1088 + (dim & 15) * 68 + (slot >> 3) * 16 + ((dim >> 4) & 1) * 8 + (slot & 7);
+}
+
 template <int HDP>
 __device__ __forceinline__ void pack_body(const KvPack &a, const KvRope &r) {
   constexpr int T = append_threads(HDP), UNITS = BLK * HDP / 4 / T, BYTES = 2 * BLK * HDP;
+  constexpr int SPREAD = HDP / 32 * 1088;  // a block's values in LDS
   __shared__ __attribute__((aligned(16))) uint8_t img[BYTES];
+  __shared__ __attribute__((aligned(16))) unsigned val[PACK_BLOCKS * SPREAD / 4];
   __shared__ uint64_t red_k[T / 64], red_v[T / 64];
-  __shared__ int64_t src[BLK];  // the rows' old blocks
-  __shared__ int key_of[BLK], down[BLK];
+  __shared__ int64_t src[BLK], of[BLK];  // the rows' old blocks; the different ones among them
+  __shared__ int key_of[BLK], down[BLK], nth[BLK];  // (nth: which of the different ones)
   __shared__ float sk[BLK], sv[BLK];
   const int units = a.head_dim / 4, tid = threadIdx.x;
   const int per_layer = a.n_items * a.kv_heads;
@@ -372,56 +387,87 @@ __device__ __forceinline__ void pack_body(const KvPack &a, const KvRope &r) {
   uint8_t *codes = a.codes + layer * a.layer_codes;
   float *scales = a.scales + layer * a.layer_scales;
   const int64_t bi = block_index(a, it.page, head, it.sub);
-  const int block_mask = (1 << a.page_shift) - 1;
-  if (it.raw) {
-    const int blk = it.pos0 / BLK;
-    const int64_t from = block_index(a, a.table[it.tab + (blk >> a.page_shift)], head, blk & block_mask);
+  if (it.raw >= 0) {
+    const int64_t from = block_index(a, it.raw, head, it.sub);
     for (int i = tid; i < BYTES / 16; i += T)
       reinterpret_cast<uintx4 *>(codes + bi * BYTES)[i] = reinterpret_cast<const uintx4 *>(codes + from * BYTES)[i];
     if (tid == 0) *reinterpret_cast<float2 *>(scales + 2 * bi) = *reinterpret_cast<const float2 *>(scales + 2 * from);
     return;
   }
-  if (tid < it.rows) {
-    const int pos = a.positions[it.at + tid], blk = pos / BLK;
-    const int64_t from = block_index(a, a.table[it.tab + (blk >> a.page_shift)], head, blk & block_mask);
+  if (tid < BLK) {
+    const PackRow row = a.rows[it.at + min(tid, it.rows - 1)];  // (the last one again past the rows)
+    const int64_t from = block_index(a, row.page, head, row.pos / BLK & ((1 << a.page_shift) - 1));
+    const float2 s = *reinterpret_cast<const float2 *>(scales + 2 * from);
+    // positions rise: a row is the first of its old block where the row before is of another
+    const int blk = row.pos / BLK;
+    const bool first = tid == 0 || __shfl_up(blk, 1) != blk;
+    const unsigned firsts = (unsigned)__ballot(first);
+    const int n = __popc(firsts & (0xFFFFFFFFu >> (31 - tid))) - 1;
     src[tid] = from;
-    key_of[tid] = pos % BLK;
-    down[tid] = pos - (it.pos0 + tid);
-    sk[tid] = scales[2 * from];
-    sv[tid] = scales[2 * from + 1];
+    key_of[tid] = row.pos % BLK;
+    down[tid] = row.pos - (it.pos0 + tid);
+    sk[tid] = s.x;
+    sv[tid] = s.y;
+    nth[tid] = n;
+    if (first) of[n] = from;
   }
   if (it.rows < BLK || a.head_dim < HDP)
     for (int i = tid; i < BYTES / 4; i += T) reinterpret_cast<unsigned *>(img)[i] = 0x80808080u;
   __syncthreads();
   const int nk_units = it.rows * units, nv_units = (it.rows + 3) / 4 * a.head_dim;
+  const int blocks = nth[BLK - 1] + 1;
   double xk[UNITS][4], xv[UNITS][4];
   uint64_t pk = 0, pv = 0;
+  unsigned kc[UNITS];
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
     const int j = tid + T * i;
-    if (j < nv_units) {
-      const int row = j / a.head_dim * 4, d = j % a.head_dim;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int w = min(row + e, it.rows - 1);
-        const int code = codes[src[w] * BYTES + BLK * HDP + value_byte(key_of[w], d)];
-        xv[i][e] = (double)(code - 128) * (double)sv[w];
-        const uint64_t m = magnitude(xv[i][e]);
-        pv = m > pv ? m : pv;
-      }
-    }
     if (j < nk_units) {
       const int w = j / units, u = j % units;
       int da, db;
       unit_dims(r, u, da, db);
       const uint8_t *from = codes + src[w] * BYTES;
-      const unsigned c0 = *reinterpret_cast<const uint16_t *>(from + key_byte<HDP>(key_of[w], da));
-      const unsigned c1 = *reinterpret_cast<const uint16_t *>(from + key_byte<HDP>(key_of[w], db));
+      kc[i] = *reinterpret_cast<const uint16_t *>(from + key_byte<HDP>(key_of[w], da)) |
+              (unsigned)*reinterpret_cast<const uint16_t *>(from + key_byte<HDP>(key_of[w], db)) << 16;
+    }
+  }
+  for (int b0 = 0; b0 < blocks; b0 += PACK_BLOCKS) {
+    if (b0) __syncthreads();  // the blocks before have been read
+    const int here = min(PACK_BLOCKS, blocks - b0);
+#pragma unroll
+    for (int i = 0; i < (PACK_BLOCKS * HDP * 2 + T - 1) / T; ++i) {
+      const int c = tid + T * i, blk = c / (2 * HDP), at = c % (2 * HDP);  // 16-byte pieces
+      if (blk < here) {
+        const uintx4 x = reinterpret_cast<const uintx4 *>(codes + of[b0 + blk] * BYTES + BLK * HDP)[at];
+        unsigned *y = val + blk * (SPREAD / 4) + (at >> 6) * 272 + (at >> 2 & 15) * 17 + (at & 3) * 4;
+        y[0] = x.x, y[1] = x.y, y[2] = x.z, y[3] = x.w;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) {
+      const int j = tid + T * i;
+      if (j >= nv_units) continue;
+      const int row = j / a.head_dim * 4, d = j % a.head_dim;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int w = min(row + e, it.rows - 1), blk = nth[w] - b0;
+        if (blk < 0 || blk >= here) continue;
+        const int code = reinterpret_cast<const uint8_t *>(val)[blk * SPREAD + spread_byte(key_of[w], d)];
+        xv[i][e] = (double)(code - 128) * (double)sv[w];
+        const uint64_t m = magnitude(xv[i][e]);
+        pv = m > pv ? m : pv;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    const int j = tid + T * i;
+    if (j < nk_units) {
+      const int w = j / units, u = j % units;
       const double s = sk[w];
-      xk[i][0] = (double)((int)(c0 & 255) - 128) * s;
-      xk[i][1] = (double)((int)(c0 >> 8) - 128) * s;
-      xk[i][2] = (double)((int)(c1 & 255) - 128) * s;
-      xk[i][3] = (double)((int)(c1 >> 8) - 128) * s;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) xk[i][e] = (double)((int)(kc[i] >> (8 * e) & 255) - 128) * s;
       Angles cs = angles_of(r, u, down[w]);
       cs.p.y = -cs.p.y;
       cs.q.y = -cs.q.y;

@@ -172,6 +172,8 @@ int pbx_weight_write_rows(pbx_ctx *c, pbx_weight *w, int64_t row0, int64_t rows,
 void pbx_weight_release(pbx_weight *w);
 int pbx_ensure_dev(pbx_ctx *c, void **p, size_t *cap, size_t need);
 int pbx_ensure_pinned(pbx_ctx *c, void **p, size_t *cap, size_t need);
+// Coherent pinned memory of at least `need` bytes with a device address.
+int pbx_ensure_mapped(pbx_ctx *c, void **h, void **d, size_t *cap, size_t need);
 // Device memory a launch path may use instead of growing the context's own
 // buffers (pbx_linear_dev_noalloc); a path that would need more fails.
 struct pbx_workspace {

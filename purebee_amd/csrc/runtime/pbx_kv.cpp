@@ -23,6 +23,22 @@ struct KvRopeHost {  // KvRope in pbx_kv.hip
   int style, dim;
 };
 
+// Lists that a call makes on the host: written to coherent pinned memory, from where a
+// kernel copies them to the device, in order with the context's other work (a copy
+// operation of the runtime costs twice as much there and back).
+struct kv_lists {
+  int32_t *host = nullptr, *mapped = nullptr, *dev = nullptr;
+  size_t host_cap = 0, dev_cap = 0;
+  hipEvent_t copied = nullptr;
+
+  int make() { return hipEventCreateWithFlags(&copied, hipEventDisableTiming) == hipSuccess ? PBX_OK : PBX_EHIP; }
+  void release() {
+    if (dev) hipFree(dev);
+    if (host) hipHostFree(host);
+    if (copied) hipEventDestroy(copied);
+  }
+};
+
 struct pbx_kv {
   uint32_t magic = PBX_KV_MAGIC;
   pbx_ctx *c = nullptr;
@@ -37,10 +53,7 @@ struct pbx_kv {
   // the kernels for this head size; attention by log2 of the query tiles (4 at most)
   hipFunction_t append = nullptr, read = nullptr, pack = nullptr, attn[3] = {};
   std::vector<pbx_kv_batch *> batches;
-  // the lists of a compaction on the device, and when the host's copy of them is read
-  int32_t *lists = nullptr, *host_lists = nullptr;
-  size_t lists_cap = 0, host_lists_cap = 0;
-  hipEvent_t copied = nullptr;
+  kv_lists lists;  // of a compaction
 };
 
 struct pbx_kv_batch {
@@ -53,10 +66,9 @@ struct pbx_kv_batch {
   bool appends = false;   // appends among them
   uint64_t alone = 0;     // forks after which its rows' pages were seen to be its sequences' alone, and one
   // the plan on the device: blocks, attention items, row positions, last rows, page ids
-  int32_t *dev = nullptr, *host = nullptr;
-  size_t dev_cap = 0, host_cap = 0;
+  // and page copies
+  kv_lists lists;
   size_t at_attn = 0, at_pos = 0, at_last = 0, at_table = 0, at_copies = 0;
-  hipEvent_t copied = nullptr;
   float *part = nullptr;  // partial results of split rows
   size_t part_cap = 0;
   // [split rows][KV head][32] parts done so far (zero between launches), each count in a
@@ -86,6 +98,23 @@ static int kv_launch(pbx_ctx *c, hipFunction_t f, const char *name, int64_t grid
   return pbx_launch_fn(c, f, name, dim3((unsigned)grid), dim3(block), args, c->stream);
 }
 
+// Room for n words of lists, whose last ones the device has read.
+static int lists_room(pbx_ctx *c, kv_lists *l, size_t n, const char *who) {
+  if (hipEventSynchronize(l->copied) != hipSuccess)
+    return pbx_fail(c, PBX_EHIP, "%s: waiting for the last lists failed", who);
+  const size_t bytes = (n * 4 + 15) / 16 * 16;
+  const int rc = pbx_ensure_mapped(c, (void **)&l->host, (void **)&l->mapped, &l->host_cap, bytes);
+  return rc ? rc : pbx_ensure_dev(c, (void **)&l->dev, &l->dev_cap, bytes);
+}
+static int lists_send(pbx_ctx *c, kv_lists *l, size_t n, const char *who) {
+  int64_t n16 = (int64_t)(n + 3) / 4;
+  void *args[] = {&l->mapped, &l->dev, &n16};
+  const int rc = pbx_launch(c, PBX_K_COPY16, dim3((unsigned)std::min<int64_t>((n16 + 255) / 256, 1024)), dim3(256), args);
+  if (rc) return rc;
+  return hipEventRecord(l->copied, c->stream) == hipSuccess ? PBX_OK
+                                                            : pbx_fail(c, PBX_EHIP, "%s: event record failed", who);
+}
+
 bool pbx_capturing(pbx_ctx *c) {
   hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
   return hipStreamIsCapturing(c->stream, &st) != hipSuccess || st != hipStreamCaptureStatusNone;
@@ -97,21 +126,18 @@ int pbx_not_capturing(pbx_ctx *c, const char *who) {
 }
 
 static void batch_release(pbx_kv_batch *b) {
-  if (b->dev) hipFree(b->dev);
-  if (b->host) hipHostFree(b->host);
+  b->lists.release();
   if (b->part) hipFree(b->part);
   if (b->arrived) hipFree(b->arrived);
-  if (b->copied) hipEventDestroy(b->copied);
   b->magic = 0;
   delete b;
 }
 
 static void kv_release(pbx_kv *kv) {
   for (pbx_kv_batch *b : kv->batches) batch_release(b);
-  for (void *p : {(void *)kv->codes, (void *)kv->scales, (void *)kv->rope, (void *)kv->lists})
+  for (void *p : {(void *)kv->codes, (void *)kv->scales, (void *)kv->rope})
     if (p) hipFree(p);
-  if (kv->host_lists) hipHostFree(kv->host_lists);
-  if (kv->copied) hipEventDestroy(kv->copied);
+  kv->lists.release();
   kv->magic = 0;
   delete kv;
 }
@@ -188,7 +214,7 @@ static int kv_make(pbx_ctx *c, const pbx_kv_config &g, pbx_kv *kv) {
     found = found && kv->attn[k];
   }
   if (!found) return pbx_fail(c, PBX_ELOAD, "pbx_kv_create: kernels for head_dim %d not found", g.head_dim);
-  if (hipEventCreateWithFlags(&kv->copied, hipEventDisableTiming) != hipSuccess)
+  if (kv->lists.make())
     return pbx_fail(c, PBX_EHIP, "pbx_kv_create: event creation failed");
   double *dfreq = nullptr;
   if (hipMalloc((void **)&kv->codes, codes) != hipSuccess ||
@@ -314,7 +340,7 @@ struct KvPackHost {  // KvPack in pbx_kv.hip
   uint8_t *codes;
   float *scales;
   int64_t layer_codes, layer_scales;  // from one layer to the next
-  const int32_t *items, *positions, *table;
+  const int32_t *items, *rows;
   int n_items, kv_heads, head_dim, page_shift;
 };
 
@@ -335,26 +361,19 @@ extern "C" int pbx_kv_compact(pbx_kv *kv, int n, const int32_t *seqs, const int3
     int rc = kv_plan_pack(&kv->pages, n, seqs, counts, positions, &p, &why);
     if (rc) return pbx_fail(c, rc, "%s: %s", who, why.c_str());
     const size_t n_items = p.items.size() * sizeof(kv_pack_item) / 4;
-    const size_t at_table = n_items + p.positions.size(), words = at_table + p.table.size();
+    const size_t words = n_items + p.rows.size() * sizeof(kv_pack_row) / 4;
     if (words) {
-      if (hipEventSynchronize(kv->copied) != hipSuccess)
-        rc = pbx_fail(c, PBX_EHIP, "%s: waiting for the last lists failed", who);
-      if (!rc) rc = pbx_ensure_pinned(c, (void **)&kv->host_lists, &kv->host_lists_cap, words * 4);
-      if (!rc) rc = pbx_ensure_dev(c, (void **)&kv->lists, &kv->lists_cap, words * 4);
-      if (!rc) {
-        memcpy(kv->host_lists, p.items.data(), n_items * 4);
-        memcpy(kv->host_lists + n_items, p.positions.data(), p.positions.size() * 4);
-        memcpy(kv->host_lists + at_table, p.table.data(), p.table.size() * 4);
-        if (hipMemcpyAsync(kv->lists, kv->host_lists, words * 4, hipMemcpyHostToDevice, c->stream) != hipSuccess ||
-            hipEventRecord(kv->copied, c->stream) != hipSuccess)
-          rc = pbx_fail(c, PBX_EHIP, "%s: copy failed", who);
+      kv_lists &l = kv->lists;
+      if (!(rc = lists_room(c, &l, words, who))) {
+        memcpy(l.host, p.items.data(), n_items * 4);
+        memcpy(l.host + n_items, p.rows.data(), p.rows.size() * sizeof(kv_pack_row));
+        rc = lists_send(c, &l, words, who);
       }
       KvRopeHost r{kv->rope, g.rope_style, g.rope_dim};
-      const int32_t *items = kv->lists;
+      const int32_t *items = l.dev;
       for (size_t k = 0; k < p.launches.size() && !rc; ++k) {
         KvPackHost a{kv->codes, kv->scales, (int64_t)kv->layer_codes, (int64_t)kv->layer_scales, items,
-                     kv->lists + n_items, kv->lists + at_table, p.launches[k], g.n_kv_heads, g.head_dim,
-                     kv->page_shift};
+                     l.dev + n_items, p.launches[k], g.n_kv_heads, g.head_dim, kv->page_shift};
         void *args[] = {&a, &r};
         rc = kv_launch(c, kv->pack, "pbx_kv_pack", (int64_t)p.launches[k] * g.n_kv_heads * g.n_layers,
                        kv_threads(kv->hdp), args);
@@ -384,8 +403,7 @@ extern "C" int pbx_kv_batch_create(pbx_kv *kv, pbx_kv_batch **out) {
     kv->batches.reserve(kv->batches.size() + 1);
     pbx_kv_batch *b = new pbx_kv_batch();
     b->kv = kv;
-    if (hipSetDevice(kv->c->device) != hipSuccess ||
-        hipEventCreateWithFlags(&b->copied, hipEventDisableTiming) != hipSuccess) {
+    if (hipSetDevice(kv->c->device) != hipSuccess || b->lists.make()) {
       delete b;
       return pbx_fail(kv->c, PBX_EHIP, "pbx_kv_batch_create: event creation failed");
     }
@@ -429,19 +447,18 @@ static int batch_upload(pbx_kv_batch *b) {
   b->at_copies = b->at_table + p.table.size();
   const size_t n = b->at_copies + p.copies.size() * sizeof(kv_page_copy) / 4;
   if (!n) return PBX_OK;
-  if (hipEventSynchronize(b->copied) != hipSuccess)
-    return pbx_fail(c, PBX_EHIP, "pbx_kv_batch_set: waiting for the last set-up failed");
-  int rc;
-  if ((rc = pbx_ensure_pinned(c, (void **)&b->host, &b->host_cap, n * 4)) ||
-      (rc = pbx_ensure_dev(c, (void **)&b->dev, &b->dev_cap, n * 4)))
-    return rc;
-  memcpy(b->host, p.blocks.data(), n_blocks * 4);
-  memcpy(b->host + b->at_attn, p.attn.data(), p.attn.size() * sizeof(kv_attn_item));
-  memcpy(b->host + b->at_pos, p.row_pos.data(), p.row_pos.size() * 4);
-  memcpy(b->host + b->at_last, p.last_rows.data(), p.last_rows.size() * 4);
-  memcpy(b->host + b->at_table, p.table.data(), p.table.size() * 4);
-  if (!p.copies.empty())
-    memcpy(b->host + b->at_copies, p.copies.data(), p.copies.size() * sizeof(kv_page_copy));
+  int rc = lists_room(c, &b->lists, n, "pbx_kv_batch_set");
+  if (rc) return rc;
+  int32_t *host = b->lists.host;
+  auto put = [&](size_t at, const void *from, size_t bytes) {
+    if (bytes) memcpy(host + at, from, bytes);
+  };
+  put(0, p.blocks.data(), n_blocks * 4);
+  put(b->at_attn, p.attn.data(), p.attn.size() * sizeof(kv_attn_item));
+  put(b->at_pos, p.row_pos.data(), p.row_pos.size() * 4);
+  put(b->at_last, p.last_rows.data(), p.last_rows.size() * 4);
+  put(b->at_table, p.table.data(), p.table.size() * 4);
+  put(b->at_copies, p.copies.data(), p.copies.size() * sizeof(kv_page_copy));
   // per slot and KV head: 16 rows of hdp sums, then their maxima and weights
   const size_t part = (size_t)p.n_slots * kv->cfg.n_kv_heads * 16 * (kv->hdp + 2) * 4;
   const size_t joins = (size_t)p.n_joins * kv->cfg.n_kv_heads * 128, joins_had = b->arrived_cap;
@@ -454,10 +471,7 @@ static int batch_upload(pbx_kv_batch *b) {
     b->arrived_cap = 0;
     return pbx_fail(c, PBX_EHIP, "pbx_kv_batch_set: clearing the counts failed");
   }
-  if (hipMemcpyAsync(b->dev, b->host, n * 4, hipMemcpyHostToDevice, c->stream) != hipSuccess ||
-      hipEventRecord(b->copied, c->stream) != hipSuccess)
-    return pbx_fail(c, PBX_EHIP, "pbx_kv_batch_set: copy failed");
-  return PBX_OK;
+  return lists_send(c, &b->lists, n, "pbx_kv_batch_set");
 }
 
 // Pages that the batch's sequences shared, copied for them.  Other batches that run
@@ -473,9 +487,9 @@ static int batch_own_pages(pbx_kv_batch *b) {
     if (o->captured && knows(o))
       return pbx_fail(c, PBX_EINVAL, "pbx_kv_batch_set: a captured graph runs over pages that a sequence shares and "
                       "would leave");
-  const int32_t *copies = b->dev + b->at_copies;
+  const int32_t *copies = b->lists.dev + b->at_copies;
   const pbx_kv_config &g = kv->cfg;
-  KvPackHost a{kv->codes, kv->scales, (int64_t)kv->layer_codes, (int64_t)kv->layer_scales, copies, nullptr, nullptr,
+  KvPackHost a{kv->codes, kv->scales, (int64_t)kv->layer_codes, (int64_t)kv->layer_scales, copies, nullptr,
                (int)p.copies.size(), g.n_kv_heads, 2 * PBX_KV_BLOCK * kv->hdp, kv->page_shift};
   void *args[] = {&a};
   const int rc = kv_launch(c, c->fn[PBX_K_KV_COPY], "pbx_kv_copy", (int64_t)p.copies.size() * g.n_kv_heads * g.n_layers,
@@ -506,6 +520,7 @@ extern "C" int pbx_kv_batch_set(pbx_kv_batch *b, int n, const int32_t *seqs, con
     b->set = false;
     try {
       std::swap(b->plan, plan);
+      b->plan.take_lists(&plan);
       kv_plan_work(kv->pages, kv->cfg.n_heads / kv->cfg.n_kv_heads, kv->cfg.n_kv_heads, kv_max_tiles(kv->hdp),
                    2 * c->cu_count, &b->plan);
       rc = batch_upload(b);
@@ -556,7 +571,7 @@ static int batch_begin(pbx_kv_batch *b, const char *who, int layer, KvArgsHost *
 int pbx_kv_batch_look(const pbx_kv_batch *b, pbx_kv_batch_view *out) {
   if (!batch_ok(b)) return pbx_fail(nullptr, PBX_EINVAL, "not a live batch");
   if (!b->set) return pbx_fail(b->kv->c, PBX_EINVAL, "the batch is not set");
-  *out = {b->kv->c, &b->kv->cfg, b->plan.n_rows, (int)b->plan.last_rows.size(), b->dev + b->at_last};
+  *out = {b->kv->c, &b->kv->cfg, b->plan.n_rows, (int)b->plan.last_rows.size(), b->lists.dev + b->at_last};
   return PBX_OK;
 }
 
@@ -611,7 +626,7 @@ extern "C" int pbx_kv_append_dev(pbx_kv_batch *b, int layer, const float *dQ, in
       return pbx_fail(c, PBX_EINVAL, "%s: queries rotated in place need one stride", who);
   }
   KvRopeHost r{kv->rope, g.rope_style, g.rope_dim};
-  const int32_t *items = b->dev, *pos = b->dev + b->at_pos;
+  const int32_t *items = b->lists.dev, *pos = b->lists.dev + b->at_pos;
   const int n_blocks = (int)b->plan.blocks.size();
   void *args[] = {&a, &r, &items, (void *)&n_blocks, &pos, &dK, &k_stride, &dV, &v_stride, &dQ, &q_stride,
                   &dQout, &qout_stride};
@@ -636,7 +651,7 @@ extern "C" int pbx_kv_attention_dev(pbx_kv_batch *b, int layer, const float *dQ,
   if (dQ == dOut && q_stride != out_stride)
     return pbx_fail(c, PBX_EINVAL, "%s: attention in place needs one stride", who);
   if (scale == 0.f) scale = (float)(1.0 / sqrt((double)g.head_dim));
-  const int32_t *items = b->dev + b->at_attn, *table = b->dev + b->at_table;
+  const int32_t *items = b->lists.dev + b->at_attn, *table = b->lists.dev + b->at_table;
   for (int k = 0; k < 3; ++k) {
     const int n = b->plan.n_attn[k];
     if (!n) continue;
@@ -660,7 +675,7 @@ extern "C" int pbx_kv_read_dev(pbx_kv_batch *b, int layer, float *dK, int64_t k_
   if ((dK && (rc = rows_check(c, who, "dK", dK, &k_stride, g.n_kv_heads, g.head_dim))) ||
       (dV && (rc = rows_check(c, who, "dV", dV, &v_stride, g.n_kv_heads, g.head_dim))))
     return rc;
-  const int32_t *items = b->dev;
+  const int32_t *items = b->lists.dev;
   void *args[] = {&a, &items, &dK, &k_stride, &dV, &v_stride};
   return batch_launch(b, kv->read, "pbx_kv_read", (int64_t)b->plan.blocks.size() * g.n_kv_heads,
                       kv_threads(kv->hdp), args);

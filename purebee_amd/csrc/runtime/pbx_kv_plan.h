@@ -163,6 +163,15 @@ struct kv_batch_plan {
   std::vector<int32_t> table;    // page ids, sequence by sequence
   int n_attn[4] = {0, 0, 0, 0};
   int n_slots = 0, n_joins = 0;
+
+  // the memory of another plan's lists, to be filled again
+  void take_lists(kv_batch_plan *p) {
+    blocks.swap(p->blocks);
+    attn.swap(p->attn);
+    row_pos.swap(p->row_pos);
+    last_rows.swap(p->last_rows);
+    table.swap(p->table);
+  }
 };
 
 // Checks a batch and, if it holds, takes its pages and fills the plan; refused
@@ -239,7 +248,6 @@ inline int kv_plan_rows(kv_pages *kv, int n, const int32_t *seqs, const int32_t 
     s.pages.reserve(kv->pages_of(q.starts[i] + counts[i]));
   }
   q.n_rows = (int)rows;
-  q.row_pos.reserve(rows);
   q.copies.reserve(q.owned.size());
   // nothing below allocates on behalf of a sequence: the pages change hands whole
   for (const kv_own_page &o : q.owned) {
@@ -279,14 +287,17 @@ inline void kv_plan_undo(kv_pages *kv, const kv_batch_plan &p) {
 struct kv_pack_item {
   int32_t page, sub;   // where it goes
   int32_t pos0, rows;  // its first (new) position, and its rows
-  int32_t at;          // the old positions of its rows, from here on in the list
-  int32_t tab;         // the sequence's old pages, from here on in the list
-  int32_t raw, pad;
+  int32_t at;          // its rows, from here on in the list
+  int32_t raw;         // the page of the old block to be copied as it is, or -1
+  int32_t pad[2];
+};
+struct kv_pack_row {
+  int32_t page, pos;  // a row's old page and position
 };
 struct kv_pack_plan {
   std::vector<kv_pack_item> items;
   std::vector<int32_t> launches;  // items of each launch: later ones fill pages that earlier ones emptied
-  std::vector<int32_t> positions, table;
+  std::vector<kv_pack_row> rows;
   std::vector<int32_t> seqs;
   std::vector<int32_t> log;  // pages taken (p) and given back (-1 - p), in order
   std::vector<kv_seq> was;
@@ -352,8 +363,7 @@ inline int kv_plan_pack(kv_pages *kv, int n, const int32_t *seqs, const int32_t 
   p->log.reserve(2 * all + 2);
   p->launches.reserve(all + 1);
   p->items.reserve(all * per_page);
-  p->positions.reserve(rows);
-  p->table.reserve(all);
+  p->rows.reserve(rows);
   std::vector<std::vector<int32_t>> made(n);
   std::vector<int> first(n), read(n);  // first page that is replaced, and old pages that are given back
   std::vector<int> from(n);            // positions from which rows or pages move
@@ -384,12 +394,10 @@ inline int kv_plan_pack(kv_pages *kv, int n, const int32_t *seqs, const int32_t 
   std::vector<int> need(n, 0);  // old pages that the pages planned so far have read for good
   for (int i = 0; i < n; ++i) {
     const std::vector<int32_t> &old = p->was[i].pages;
-    const int tab = (int)p->table.size(), list = (int)p->positions.size(), base = first[i] * T;
+    const int list = (int)p->rows.size(), base = first[i] * T;
     made[i].assign(old.begin(), old.begin() + first[i]);
-    if (first[i] < kv->pages_of(counts[i])) {
-      p->table.insert(p->table.end(), old.begin(), old.end());
-      p->positions.insert(p->positions.end(), positions + at + base, positions + at + counts[i]);
-    }
+    for (int64_t j = at + base; j < at + counts[i]; ++j)
+      p->rows.push_back({old[(unsigned)positions[j] / (unsigned)T], positions[j]});
     need[i] = first[i];
     for (int j = first[i]; j < kv->pages_of(counts[i]); ++j) {
       if (kv->free_list.empty()) {
@@ -409,8 +417,8 @@ inline int kv_plan_pack(kv_pages *kv, int n, const int32_t *seqs, const int32_t 
       made[i].push_back(page);
       for (int b = 0; b < per_page && j * T + b * PBX_KV_BLOCK < counts[i]; ++b) {
         const int pos0 = j * T + b * PBX_KV_BLOCK, m = std::min(PBX_KV_BLOCK, counts[i] - pos0);
-        p->items.push_back({page, b, pos0, m, list + pos0 - base, tab,
-                            positions[at + pos0 + m - 1] == pos0 + m - 1, 0});
+        const bool stays = positions[at + pos0 + m - 1] == pos0 + m - 1;
+        p->items.push_back({page, b, pos0, m, list + pos0 - base, stays ? old[j] : -1, {0, 0}});
       }
       const int next = (j + 1) * T;
       need[i] = next < counts[i] ? positions[at + next] / T : (int)old.size();
@@ -443,6 +451,7 @@ inline void kv_plan_work(const kv_pages &kv, int groups, int kv_heads, int max_u
   p->last_rows.clear();
   p->table.clear();
   p->n_slots = p->n_joins = 0;
+  for (int &x : p->n_attn) x = 0;
   p->last = true;
   // log2 u of each sequence: the narrowest kernel that holds its rows, or the
   // widest there is
@@ -454,9 +463,9 @@ inline void kv_plan_work(const kv_pages &kv, int groups, int kv_heads, int max_u
     return (int)(((int64_t)p->counts[i] * groups + t - 1) / t);
   };
   auto blocks_of = [&](int i, int tile) {  // visible to the tile's last row
-    const int64_t rows = (int64_t)p->counts[i] * groups;
-    const int64_t last = std::min<int64_t>(rows, (16 << width[i]) * ((int64_t)tile + 1)) - 1;
-    return (int)((p->starts[i] + last / groups) / PBX_KV_BLOCK + 1);
+    const unsigned rows = (unsigned)p->counts[i] * groups;  // (at most 2^20 rows of 2^10 heads)
+    const unsigned last = std::min(rows, (unsigned)(16 << width[i]) * (tile + 1u)) - 1;
+    return (int)((p->starts[i] + last / (unsigned)groups) / PBX_KV_BLOCK + 1);
   };
   // Where the tiles are few (one and a half a CU: `want` is two), narrower ones:
   // half as many rows a workgroup make twice as many workgroups (one sequence of
@@ -478,15 +487,19 @@ inline void kv_plan_work(const kv_pages &kv, int groups, int kv_heads, int max_u
     int wider = 4;
     for (int i = 0; i < n; ++i) {
       if (width[i] > w && p->counts[i]) wider = std::min(wider, width[i]);
-      for (int t = 0; width[i] == w && t < tiles_of(i); ++t) here += blocks_of(i, t);
+      for (int t = 0, tiles = width[i] == w ? tiles_of(i) : 0; t < tiles; ++t) here += blocks_of(i, t);
     }
     if (wider == 4 || here * kv_heads >= least * want) continue;
     for (int i = 0; i < n; ++i)
       if (width[i] == w) width[i] = wider;
   }
   int64_t total = 0;  // blocks that the tiles visit
+  std::vector<int32_t> seen;  // by each
   for (int i = 0; i < n; ++i)
-    for (int t = 0; t < tiles_of(i); ++t) total += blocks_of(i, t);
+    for (int t = 0, tiles = tiles_of(i); t < tiles; ++t) {
+      seen.push_back(blocks_of(i, t));
+      total += seen.back();
+    }
   // an item: at least 16 blocks (four a wave), and about `want` workgroups in all;
   // wide tiles that fill the GPU as they are, longest first, are split only where
   // one is far longer than that: their partial results cost more than the
@@ -494,8 +507,53 @@ inline void kv_plan_work(const kv_pages &kv, int groups, int kv_heads, int max_u
   const int64_t even = std::max<int64_t>(least, (total * kv_heads + want - 1) / want);
   const int64_t wide = workgroups() < want / 2 ? even : 4 * even;
   const int per_page = kv.page_tokens / PBX_KV_BLOCK;
-  std::vector<kv_attn_item> by_u[4];
-  int row0 = 0;
+  // Items in order of log2 u, then the ones with the most blocks first (so that none of
+  // them is the last to start), else as they come: counted by u and length, then each
+  // written to its place.
+  const unsigned chunks[2] = {(unsigned)std::min<int64_t>(even, 1 << 20), (unsigned)std::min<int64_t>(wide, 1 << 20)};
+  auto parts_of = [&](int nb, int lu) {  // (a sequence has 2^15 blocks at most)
+    const unsigned chunk = chunks[lu > 0];
+    return nb <= (int)chunk ? 1 : (int)std::min<unsigned>(KV_MAX_PARTS, (nb + chunk - 1) / chunk);
+  };
+  int most = 0;
+  int64_t n_blocks = 0, n_table = 0;
+  for (int i = 0; i < n; ++i) {
+    if (!p->counts[i]) continue;
+    const int end = p->starts[i] + p->counts[i];
+    most = std::max(most, (end - 1) / PBX_KV_BLOCK + 1);
+    n_blocks += (end - 1) / PBX_KV_BLOCK + 1 - p->starts[i] / PBX_KV_BLOCK;
+    n_table += kv.pages_of(end);
+  }
+  std::vector<int32_t> place((size_t)4 * (most + 1), 0);  // [u][most - length]
+  const int32_t *nbs = seen.data();
+  for (int i = 0; i < n; ++i) {
+    const int lu = width[i], tiles = tiles_of(i);
+    int32_t *at = place.data() + (size_t)lu * (most + 1) + most;
+    for (int t = 0; t < tiles; ++t) {
+      const int nb = *nbs++, parts = parts_of(nb, lu);
+      p->n_attn[lu] += parts;
+      if (parts == 1) {
+        ++at[-nb];
+        continue;
+      }
+      const int each = nb / parts, more = nb % parts;  // lengths differ by one at most
+      at[-each] += parts - more;
+      if (more) at[-each - 1] += more;
+    }
+  }
+  int32_t sum = 0;
+  for (int32_t &x : place) {
+    const int32_t here = x;
+    x = sum;
+    sum += here;
+  }
+  p->attn.resize(sum);
+  p->blocks.reserve(n_blocks);
+  p->table.reserve(n_table);
+  p->row_pos.resize(p->n_rows);
+  int row0 = 0, page_shift = 0;
+  while (1 << page_shift < per_page) ++page_shift;
+  nbs = seen.data();
   for (int i = 0; i < n; ++i) {
     const kv_seq &s = kv.seqs[p->seqs[i]];
     const int start = p->starts[i], count = p->counts[i], tab = (int)p->table.size(), lu = width[i];
@@ -505,16 +563,18 @@ inline void kv_plan_work(const kv_pages &kv, int groups, int kv_heads, int max_u
     p->table.insert(p->table.end(), s.pages.begin(), s.pages.begin() + used);
     for (int b = start / PBX_KV_BLOCK; b * PBX_KV_BLOCK < start + count; ++b)
       p->blocks.push_back({s.pages[b / per_page], b % per_page, b * PBX_KV_BLOCK, start, count, row0, {0, 0}});
-    for (int t = 0; t < count; ++t) p->row_pos.push_back(start + t);
-    for (int t = 0; t < tiles_of(i); ++t) {
-      const int nb = blocks_of(i, t);
-      const int64_t chunk = lu ? wide : even;
-      const int parts = (int)std::min<int64_t>(KV_MAX_PARTS, (nb + chunk - 1) / chunk);
-      for (int k = 0; k < parts; ++k) {
-        kv_attn_item x = {start, count, row0, t, (int)((int64_t)nb * k / parts), (int)((int64_t)nb * (k + 1) / parts),
-                          tab, k, parts, p->n_slots, p->n_joins, 0, {0, 0, 0, 0}};
-        for (int j = 0; j < 4; ++j) x.pages[j] = s.pages[std::min(x.blk0 / per_page + j, (x.blk1 - 1) / per_page)];
-        by_u[lu].push_back(x);
+    for (int t = 0; t < count; ++t) p->row_pos[row0 + t] = start + t;
+    int32_t *at = place.data() + (size_t)lu * (most + 1) + most;
+    const int tiles = tiles_of(i);
+    for (int t = 0; t < tiles; ++t) {
+      const int nb = *nbs++, parts = parts_of(nb, lu);
+      for (int k = 0, blk0 = 0; k < parts; ++k) {
+        const int blk1 = parts == 1 ? nb : nb * (k + 1) / parts;
+        const int first = blk0 >> page_shift, last = (blk1 - 1) >> page_shift;
+        kv_attn_item &x = p->attn[at[blk0 - blk1]++];
+        x = {start, count, row0, t, blk0, blk1, tab, k, parts, p->n_slots, p->n_joins, 0, {0, 0, 0, 0}};
+        for (int j = 0; j < 4; ++j) x.pages[j] = s.pages[std::min(first + j, last)];
+        blk0 = blk1;
       }
       if (parts > 1) {
         p->n_slots += parts << lu;
@@ -523,14 +583,6 @@ inline void kv_plan_work(const kv_pages &kv, int groups, int kv_heads, int max_u
     }
     row0 += count;
     p->last_rows.push_back(row0 - 1);
-  }
-  for (int c = 0; c < 4; ++c) {
-    // the items with the most blocks first, so that none of them is the last to start
-    std::stable_sort(by_u[c].begin(), by_u[c].end(), [](const kv_attn_item &x, const kv_attn_item &y) {
-      return x.blk1 - x.blk0 > y.blk1 - y.blk0;
-    });
-    p->attn.insert(p->attn.end(), by_u[c].begin(), by_u[c].end());
-    p->n_attn[c] = (int)by_u[c].size();
   }
 }
 

@@ -674,7 +674,7 @@ extern "C" int pbx_workspace_info(const pbx_ctx *c, size_t *grown_bytes, size_t 
 extern "C" void *pbx_ctx_stream(const pbx_ctx *c) { return c ? (void *)c->stream : nullptr; }
 
 // Coherent pinned memory of at least `need` bytes with a device address.
-static int ensure_mapped(pbx_ctx *c, void **h, void **d, size_t *cap, size_t need) {
+int pbx_ensure_mapped(pbx_ctx *c, void **h, void **d, size_t *cap, size_t need) {
   if (*cap >= need) return PBX_OK;
   if (*h) {
     HIPCHK(c, hipStreamSynchronize(c->stream));
@@ -711,8 +711,8 @@ extern "C" int pbx_linear(pbx_ctx *c, const pbx_weight *w, const float *X, int64
   if ((rc = pbx_ensure_dev(c, &c->d_x, &c->d_x_cap, xb + bpad))) return rc;
   if (bias && (rc = pbx_ensure_dev(c, &c->d_b, &c->d_b_cap, bb))) return rc;
   if (direct) {
-    if ((rc = ensure_mapped(c, &c->h_x, &c->d_hx, &c->h_x_cap, xb + bpad)) ||
-        (rc = ensure_mapped(c, &c->h_y, &c->d_hy, &c->h_y_cap, yb)))
+    if ((rc = pbx_ensure_mapped(c, &c->h_x, &c->d_hx, &c->h_x_cap, xb + bpad)) ||
+        (rc = pbx_ensure_mapped(c, &c->h_y, &c->d_hy, &c->h_y_cap, yb)))
       return rc;
     memcpy(c->h_x, X, xb);
     if (bias) memcpy((char *)c->h_x + xb, bias, bb);

@@ -143,13 +143,11 @@ int main() {
             for (int32_t i = 0; i < m; ++i, ++k) {
               const kv_pack_item &x = p.items[k];
               CHECK(x.rows > 0 && x.rows <= PBX_KV_BLOCK && x.pos0 % PBX_KV_BLOCK == 0);
-              CHECK(x.at >= 0 && x.at + x.rows <= (int)p.positions.size());
+              CHECK(x.at >= 0 && x.at + x.rows <= (int)p.rows.size());
               for (int t = 0; t < x.rows; ++t) {
-                const int pos = p.positions[x.at + t];
-                CHECK(x.tab + pos / page < (int)p.table.size());
-                const int from = p.table[x.tab + pos / page];
-                CHECK(!written[from]);
-                if (x.raw) CHECK(pos == x.pos0 + t);
+                const int pos = p.rows[x.at + t].pos, from = p.rows[x.at + t].page;
+                CHECK(from >= 0 && from < w.n_pages && !written[from]);
+                CHECK(pos >= x.pos0 + t && (x.raw < 0 || (x.raw == from && pos == x.pos0 + t)));
                 w.pool[x.page][x.sub * PBX_KV_BLOCK + t] = before[from][pos % page];
               }
             }
