@@ -354,32 +354,46 @@ __device__ __forceinline__ int64_t block_index(const KvPack &a, int page, int he
   return (((int64_t)page * a.kv_heads + head) << a.page_shift) + sub;
 }
 
-// Compaction: workgroup (layer, block of new rows, KV head).  A block's rows come from
-// up to 32 old blocks; each code stands for code * s (exact in 64 bits), keys turn back
-// by the distance that they move down, and the block is coded as a new one is.
+// Compaction: workgroup (layer, block of new rows, some KV heads).  A block's rows come
+// from up to 32 old blocks; each code stands for code * s, keys turn back by the distance
+// that they move down, and the block is coded as a new one is, quotients and largest
+// magnitude as in 64 bits.  Both are looked for in f32 first: a magnitude is off by less
+// than 2^-18 of the largest, a quotient of at most 127 by less than 10^-4, so only what
+// comes as near to the largest, or to a border between codes, is computed in 64 bits.
 // A row's keys lie side by side and are fetched as they are.  Its values lie 64 bytes
 // apart for consecutive dims, so one row takes as many cache lines as the whole block:
 // the blocks' values are fetched whole, PACK_BLOCKS at a time, into LDS, where the 64
 // bytes of a dim take 68, so that dims fall in banks of their own.
-// (Fetched byte by byte the values bounded it: half of 31,000 positions, 8 heads of
-// 128, two layers 140 us.)
 constexpr int PACK_BLOCKS = 4;
 __device__ __forceinline__ int spread_byte(int key, int dim) {
   const int slot = 8 * ((key >> 2) & 3) + 4 * (key >> 4) + (key & 3);
   return (dim >> 5) * 1088 + (dim & 15) * 68 + (slot >> 3) * 16 + ((dim >> 4) & 1) * 8 + (slot & 7);
 }
+constexpr float NEAR_LARGEST = 1.f - 0x1p-17f, NEAR_BORDER = 2e-4f;
+
+// y / s rounded half to even from q, which is it in f32 to 10^-4: where q is near the
+// border k + 1/2, by 2 |y| against (2 k + 1) s, which are exact.
+__device__ __forceinline__ float border_code(double y, float s, float q) {
+  const float k = floorf(fabsf(q));
+  if (fabsf(fabsf(q) - k - 0.5f) >= NEAR_BORDER) return rintf(q);
+  const double t = (double)(2.f * k + 1.f) * (double)s, z = 2.0 * fabs(y);
+  const float up = k + 1.f, r = z > t ? up : z < t ? k : ((int)k & 1 ? up : k);
+  return copysignf(r, q);
+}
 
 template <int HDP>
 __device__ __forceinline__ void pack_body(const KvPack &a, const KvRope &r) {
-  constexpr int T = append_threads(HDP), UNITS = BLK * HDP / 4 / T, BYTES = 2 * BLK * HDP;
+  constexpr int T = append_threads(HDP), UNITS = BLK * HDP / 4 / T, BYTES = 2 * BLK * HDP, QUADS = HDP / 4;
   constexpr int SPREAD = HDP / 32 * 1088;  // a block's values in LDS
   __shared__ __attribute__((aligned(16))) uint8_t img[BYTES];
   __shared__ __attribute__((aligned(16))) unsigned val[PACK_BLOCKS * SPREAD / 4];
-  __shared__ uint64_t red_k[T / 64], red_v[T / 64];
+  __shared__ float red[2][T / 64];
+  __shared__ uint64_t red_exact[2];
   __shared__ int64_t src[BLK], of[BLK];  // the rows' old blocks; the different ones among them
-  __shared__ int key_of[BLK], down[BLK], nth[BLK];  // (nth: which of the different ones)
+  __shared__ int val_at[BLK], nth[BLK];  // a row's place in an old block's values; which of the different ones
   __shared__ float sk[BLK], sv[BLK];
-  const int units = a.head_dim / 4, tid = threadIdx.x;
+  __shared__ unsigned bads;  // rows of blocks that read as NaN: 1 keys, 2 values
+  const int tid = threadIdx.x;
   const int per_layer = a.n_items * a.kv_heads;
   const int layer = blockIdx.x / per_layer, in_layer = blockIdx.x % per_layer;
   const PackItem it = reinterpret_cast<const PackItem *>(a.items)[in_layer / a.kv_heads];
@@ -394,43 +408,66 @@ __device__ __forceinline__ void pack_body(const KvPack &a, const KvRope &r) {
     if (tid == 0) *reinterpret_cast<float2 *>(scales + 2 * bi) = *reinterpret_cast<const float2 *>(scales + 2 * from);
     return;
   }
+  // unit i of a thread: 4 dims of row kw (keys), 4 rows from vw on at dim vd (values)
+  auto kw = [&](int i) { return (tid + T * i) / QUADS; };
+  auto ku = [&](int i) { return (tid + T * i) % QUADS; };
+  auto vw = [&](int i) { return (tid + T * i) / HDP * 4; };
+  auto vd = [&](int i) { return (tid + T * i) % HDP; };
+  int pos[UNITS];
+  bool kon[UNITS], von[UNITS];
+  float cs[UNITS][4];  // cos and sin of the unit's two pairs
+  auto angles = [&](int i) {
+    KvRope q = r;
+    asm volatile("" : "+s"(q.table));  // read again where they are needed, not kept in registers
+    Angles x = angles_of(q, ku(i), pos[i] - (it.pos0 + kw(i)));
+    x.p.y = -x.p.y;
+    x.q.y = -x.q.y;
+    return x;
+  };
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    kon[i] = kw(i) < it.rows && 4 * ku(i) < a.head_dim;
+    von[i] = vw(i) < it.rows && vd(i) < a.head_dim;
+    pos[i] = 0;
+    if (!kon[i]) continue;
+    pos[i] = a.rows[it.at + kw(i)].pos;
+    const Angles x = angles(i);
+    cs[i][0] = (float)x.p.x, cs[i][1] = (float)x.p.y, cs[i][2] = (float)x.q.x, cs[i][3] = (float)x.q.y;
+  }
   if (tid < BLK) {
     const PackRow row = a.rows[it.at + min(tid, it.rows - 1)];  // (the last one again past the rows)
     const int64_t from = block_index(a, row.page, head, row.pos / BLK & ((1 << a.page_shift) - 1));
-    const float2 s = *reinterpret_cast<const float2 *>(scales + 2 * from);
     // positions rise: a row is the first of its old block where the row before is of another
     const int blk = row.pos / BLK;
     const bool first = tid == 0 || __shfl_up(blk, 1) != blk;
     const unsigned firsts = (unsigned)__ballot(first);
     const int n = __popc(firsts & (0xFFFFFFFFu >> (31 - tid))) - 1;
     src[tid] = from;
-    key_of[tid] = row.pos % BLK;
-    down[tid] = row.pos - (it.pos0 + tid);
+    nth[tid] = n;
+    val_at[tid] = spread_byte(row.pos % BLK, 0) + n % PACK_BLOCKS * SPREAD;
+    if (first) of[n] = from;
+    const float2 s = *reinterpret_cast<const float2 *>(scales + 2 * from);
     sk[tid] = s.x;
     sv[tid] = s.y;
-    nth[tid] = n;
-    if (first) of[n] = from;
+    const unsigned any = (__ballot(!(s.x < INFINITY)) ? 1u : 0u) | (__ballot(!(s.y < INFINITY)) ? 2u : 0u);
+    if (tid == 0) bads = any;
   }
-  if (it.rows < BLK || a.head_dim < HDP)
-    for (int i = tid; i < BYTES / 4; i += T) reinterpret_cast<unsigned *>(img)[i] = 0x80808080u;
+  if (tid < 2) red_exact[tid] = 0;
   __syncthreads();
-  const int nk_units = it.rows * units, nv_units = (it.rows + 3) / 4 * a.head_dim;
-  const int blocks = nth[BLK - 1] + 1;
-  double xk[UNITS][4], xv[UNITS][4];
-  uint64_t pk = 0, pv = 0;
   unsigned kc[UNITS];
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
-    const int j = tid + T * i;
-    if (j < nk_units) {
-      const int w = j / units, u = j % units;
-      int da, db;
-      unit_dims(r, u, da, db);
-      const uint8_t *from = codes + src[w] * BYTES;
-      kc[i] = *reinterpret_cast<const uint16_t *>(from + key_byte<HDP>(key_of[w], da)) |
-              (unsigned)*reinterpret_cast<const uint16_t *>(from + key_byte<HDP>(key_of[w], db)) << 16;
-    }
+    if (!kon[i]) continue;
+    const uint8_t *from = codes + src[kw(i)] * BYTES;
+    int da, db;
+    unit_dims(r, ku(i), da, db);
+    kc[i] = *reinterpret_cast<const uint16_t *>(from + key_byte<HDP>(pos[i] % BLK, da)) |
+            (unsigned)*reinterpret_cast<const uint16_t *>(from + key_byte<HDP>(pos[i] % BLK, db)) << 16;
   }
+  if (it.rows < BLK || a.head_dim < HDP)
+    for (int i = tid; i < BYTES / 4; i += T) reinterpret_cast<unsigned *>(img)[i] = 0x80808080u;
+  const int blocks = nth[BLK - 1] + 1;
+  float vc[UNITS][4];  // codes
   for (int b0 = 0; b0 < blocks; b0 += PACK_BLOCKS) {
     if (b0) __syncthreads();  // the blocks before have been read
     const int here = min(PACK_BLOCKS, blocks - b0);
@@ -446,72 +483,129 @@ __device__ __forceinline__ void pack_body(const KvPack &a, const KvRope &r) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < UNITS; ++i) {
-      const int j = tid + T * i;
-      if (j >= nv_units) continue;
-      const int row = j / a.head_dim * 4, d = j % a.head_dim;
+      const uint8_t *at = reinterpret_cast<const uint8_t *>(val) + spread_byte(0, vd(i));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int w = min(row + e, it.rows - 1), blk = nth[w] - b0;
-        if (blk < 0 || blk >= here) continue;
-        const int code = reinterpret_cast<const uint8_t *>(val)[blk * SPREAD + spread_byte(key_of[w], d)];
-        xv[i][e] = (double)(code - 128) * (double)sv[w];
-        const uint64_t m = magnitude(xv[i][e]);
-        pv = m > pv ? m : pv;
+        const int w = vw(i) + e;
+        const float c = (float)at[val_at[w]] - 128.f;
+        if (blocks <= PACK_BLOCKS || (nth[w] >= b0 && nth[w] < b0 + PACK_BLOCKS)) vc[i][e] = c;
       }
     }
   }
+  // largest magnitudes in f32 (of numbers: a row of a block that reads as NaN is seen to below)
+  float xk[UNITS][4], pk[UNITS], pv[UNITS], mk = 0.f, mv = 0.f;
+  auto most4 = [](const float x[4]) { return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))); };
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
-    const int j = tid + T * i;
-    if (j < nk_units) {
-      const int w = j / units, u = j % units;
-      const double s = sk[w];
+    pk[i] = pv[i] = 0.f;
+    if (kon[i]) {
+      const float c0 = (float)(kc[i] & 255) - 128.f, c1 = (float)(kc[i] >> 8 & 255) - 128.f;
+      const float c2 = (float)(kc[i] >> 16 & 255) - 128.f, c3 = (float)(kc[i] >> 24) - 128.f, s = sk[kw(i)];
+      // the pairs are (0, 2) and (1, 3) where halves turn, else (0, 1) and (2, 3)
+      const bool halves = r.style == 2;
+      const float d1 = halves ? c2 : c1, d2 = halves ? c1 : c2;
+      const float y0 = (c0 * cs[i][0] - d1 * cs[i][1]) * s, y1 = (c0 * cs[i][1] + d1 * cs[i][0]) * s;
+      const float y2 = (d2 * cs[i][2] - c3 * cs[i][3]) * s, y3 = (d2 * cs[i][3] + c3 * cs[i][2]) * s;
+      xk[i][0] = y0, xk[i][1] = halves ? y2 : y1, xk[i][2] = halves ? y1 : y2, xk[i][3] = y3;
+      pk[i] = most4(xk[i]);
+      mk = fmaxf(mk, pk[i]);
+    }
+    if (von[i]) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) xk[i][e] = (double)((int)(kc[i] >> (8 * e) & 255) - 128) * s;
-      Angles cs = angles_of(r, u, down[w]);
-      cs.p.y = -cs.p.y;
-      cs.q.y = -cs.q.y;
-      turn(r, u, cs, xk[i]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint64_t m = magnitude(xk[i][e]);
-        pk = m > pk ? m : pk;
-      }
+      for (int e = 0; e < 4; ++e) vc[i][e] *= sv[vw(i) + e];  // (from here on values, to a rounding)
+      pv[i] = most4(vc[i]);
+      mv = fmaxf(mv, pv[i]);
     }
   }
-  pk = wave_max_u64(pk);
-  pv = wave_max_u64(pv);
+  mk = wave_max(mk);
+  mv = wave_max(mv);
   if ((tid & 63) == 0) {
-    red_k[tid >> 6] = pk;
-    red_v[tid >> 6] = pv;
+    red[0][tid >> 6] = mk;
+    red[1][tid >> 6] = mv;
   }
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < T / 64; ++w) {
-    pk = red_k[w] > pk ? red_k[w] : pk;
-    pv = red_v[w] > pv ? red_v[w] : pv;
+    mk = fmaxf(mk, red[0][w]);
+    mv = fmaxf(mv, red[1][w]);
   }
-  const float nk = scale_of(pk), nv = scale_of(pv);
-  const float ik = 1.f / nk, iv = 1.f / nv;
+  auto exact_keys = [&](int i, double x[4]) {
+    const double s = sk[kw(i)];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = (double)((int)(kc[i] >> (8 * e) & 255) - 128) * s;
+    turn(r, ku(i), angles(i), x);
+  };
+  // (the code again, as a product of at most 127 and s is off by a rounding)
+  auto exact_value = [&](int i, int e) {
+    const float s = sv[vw(i) + e];
+    return s > 0.f ? (double)rintf(vc[i][e] / s) * (double)s : 0.0;
+  };
+  // what may be the largest, in 64 bits
+  const float near_k = mk * NEAR_LARGEST, near_v = mv * NEAR_LARGEST;
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
-    const int j = tid + T * i;
-    if (j < nk_units) {
-      const int w = j / units, u = j % units;
-      int da, db;
-      unit_dims(r, u, da, db);
-      unsigned c = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) c |= (unsigned)(code_of(xk[i][e], nk, ik) + 128) << (8 * e);
-      *reinterpret_cast<uint16_t *>(img + key_byte<HDP>(w, da)) = (uint16_t)c;
-      *reinterpret_cast<uint16_t *>(img + key_byte<HDP>(w, db)) = (uint16_t)(c >> 16);
+    if (mk > 0.f && pk[i] >= near_k) {
+      double x[4];
+      exact_keys(i, x);
+      atomicMax((unsigned long long *)&red_exact[0],
+                magnitude(fmax(fmax(fabs(x[0]), fabs(x[1])), fmax(fabs(x[2]), fabs(x[3])))));
     }
-    if (j < nv_units) {
-      const int row = j / a.head_dim * 4, d = j % a.head_dim;
-      uint8_t *at = img + BLK * HDP + value_byte(row, d);
+    if (mv > 0.f && pv[i] >= near_v) {
+      double x = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (row + e < it.rows) at[e] = (uint8_t)(code_of(xv[i][e], nv, iv) + 128);
+      for (int e = 0; e < 4; ++e) x = fmax(x, fabs(exact_value(i, e)));
+      atomicMax((unsigned long long *)&red_exact[1], magnitude(x));
+    }
+  }
+  __syncthreads();
+  const float none = __uint_as_float(0x7fc00000u);
+  const float nk = bads & 1 ? none : scale_of(red_exact[0]), nv = bads & 2 ? none : scale_of(red_exact[1]);
+  const bool ok_k = nk > 0.f && nk < INFINITY, ok_v = nv > 0.f && nv < INFINITY;  // else codes are 0
+  const float ik = ok_k ? 1.f / nk : 0.f, iv = ok_v ? 1.f / nv : 0.f;
+  // codes of 4 quotients + 128; how far the nearest one is from a border
+  auto code4 = [](const float x[4], float inv, unsigned &w) {
+    float gap = 1.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float q = x[e] * inv;
+      gap = fminf(gap, fabsf(__builtin_amdgcn_fractf(q) - 0.5f));
+      w = __builtin_amdgcn_cvt_pk_u8_f32(rintf(q) + 128.f, e, w);
+    }
+    return gap;
+  };
+  auto mend = [](unsigned w, int e, float code) {
+    return (w & ~(255u << (8 * e))) | (unsigned)((int)code + 128) << (8 * e);
+  };
+#pragma unroll
+  for (int i = 0; i < UNITS; ++i) {
+    if (kon[i]) {
+      unsigned w = 0;
+      // (past f32's range nothing above holds)
+      if (code4(xk[i], ik, w) < NEAR_BORDER || !(mk < INFINITY)) {
+        double x[4];
+        exact_keys(i, x);
+#pragma unroll 1
+        for (int e = 0; e < 4; ++e) {
+          const double y = e == 0 ? x[0] : e == 1 ? x[1] : e == 2 ? x[2] : x[3];
+          w = mend(w, e, (float)rint(y / (double)nk));
+        }
+      }
+      if (!ok_k) w = 0x80808080u;
+      int da, db;
+      unit_dims(r, ku(i), da, db);
+      *reinterpret_cast<uint16_t *>(img + key_byte<HDP>(kw(i), da)) = (uint16_t)w;
+      *reinterpret_cast<uint16_t *>(img + key_byte<HDP>(kw(i), db)) = (uint16_t)(w >> 16);
+    }
+    if (von[i]) {
+      unsigned w = 0;
+      if (code4(vc[i], iv, w) < NEAR_BORDER) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w = mend(w, e, border_code(exact_value(i, e), nv, vc[i][e] * iv));
+      }
+      if (!ok_v) w = 0x80808080u;
+      const int rest = it.rows - vw(i);  // positions past the rows hold code 0
+      if (rest < 4) w = (w & ((1u << (8 * rest)) - 1)) | 0x80808080u << (8 * rest);
+      *reinterpret_cast<unsigned *>(img + BLK * HDP + value_byte(vw(i), vd(i))) = w;
     }
   }
   __syncthreads();
