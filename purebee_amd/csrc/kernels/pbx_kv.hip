@@ -365,6 +365,7 @@ __device__ __forceinline__ int64_t block_index(const KvPack &a, int page, int he
 // the blocks' values are fetched whole, PACK_BLOCKS at a time, into LDS, where the 64
 // bytes of a dim take 68, so that dims fall in banks of their own.
 constexpr int PACK_BLOCKS = 4;
+constexpr int pack_threads(int hdp) { return hdp <= 64 ? 256 : 2 * hdp; }
 __device__ __forceinline__ int spread_byte(int key, int dim) {
   const int slot = 8 * ((key >> 2) & 3) + 4 * (key >> 4) + (key & 3);
   return (dim >> 5) * 1088 + (dim & 15) * 68 + (slot >> 3) * 16 + ((dim >> 4) & 1) * 8 + (slot & 7);
@@ -383,7 +384,7 @@ __device__ __forceinline__ float border_code(double y, float s, float q) {
 
 template <int HDP>
 __device__ __forceinline__ void pack_body(const KvPack &a, const KvRope &r) {
-  constexpr int T = append_threads(HDP), UNITS = BLK * HDP / 4 / T, BYTES = 2 * BLK * HDP, QUADS = HDP / 4;
+  constexpr int T = pack_threads(HDP), UNITS = BLK * HDP / 4 / T, BYTES = 2 * BLK * HDP, QUADS = HDP / 4;
   constexpr int SPREAD = HDP / 32 * 1088;  // a block's values in LDS
   __shared__ __attribute__((aligned(16))) uint8_t img[BYTES];
   __shared__ __attribute__((aligned(16))) unsigned val[PACK_BLOCKS * SPREAD / 4];
@@ -1181,7 +1182,7 @@ extern "C" __global__ void __launch_bounds__(256) pbx_kv_copy(KvPack a) {
       pbx_kv_read_##HDP(KvArgs a, const BlockItem *items, float *K, int64_t ks, float *V, int64_t vs) {            \
     read_body<HDP>(a, items, K, ks, V, vs);                                                                        \
   }                                                                                                                \
-  extern "C" __global__ void __launch_bounds__(append_threads(HDP)) pbx_kv_pack_##HDP(KvPack a, KvRope r) {        \
+  extern "C" __global__ void __launch_bounds__(pack_threads(HDP)) pbx_kv_pack_##HDP(KvPack a, KvRope r) {        \
     pack_body<HDP>(a, r);                                                                                          \
   }
 #define PBX_KV_ATTN(HDP, U, NQ, KW, RING, WAVES)                                                                   \

@@ -90,6 +90,8 @@ static int kv_padded(int hd) {
 // Threads of the append and read workgroups (append_threads of pbx_kv.hip).
 static int kv_threads(int hdp) { return hdp <= 64 ? 256 : 4 * hdp; }
 
+static int pack_threads(int hdp) { return hdp <= 64 ? 256 : 2 * hdp; }  // likewise
+
 // 16-row query tiles of the widest attention kernel for a head size.
 static int kv_max_tiles(int hdp) { return hdp <= 64 ? 4 : 2; }
 
@@ -376,7 +378,7 @@ extern "C" int pbx_kv_compact(pbx_kv *kv, int n, const int32_t *seqs, const int3
                      l.dev + n_items, p.launches[k], g.n_kv_heads, g.head_dim, kv->page_shift};
         void *args[] = {&a, &r};
         rc = kv_launch(c, kv->pack, "pbx_kv_pack", (int64_t)p.launches[k] * g.n_kv_heads * g.n_layers,
-                       kv_threads(kv->hdp), args);
+                       pack_threads(kv->hdp), args);
         // (the first launch writes pages that were free: the sequences are whole until the second)
         if (rc && k) return rc;
         items += (size_t)p.launches[k] * sizeof(kv_pack_item) / 4;
