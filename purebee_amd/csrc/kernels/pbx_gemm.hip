@@ -581,6 +581,100 @@ __device__ __forceinline__ void store_tiles(const GemmArgs &a, const floatx16 (&
     }
 }
 
+// What becomes of a tile of a head's logits that are not kept (gemm_dma, gemm_dma64;
+// a.N: entries of this piece of the vocabulary, which starts at v0).
+#define HEAD_NONE 0
+#define HEAD_SUMS 1  // their sums, as pbx_head_stats gives them for a part of 8192
+#define HEAD_G 2     // the rows' gradient's first factor, as pbx_head_g gives it
+struct HeadArgs {
+  const int *targets;
+  float4 *parts;  // [M][n_parts]
+  int n_parts;
+  float *hit;     // or null
+  const float *lse;
+  _Float16 *hi, *lo;  // [blocks of 32 entries][Mpad][32]
+  int Mpad, v0, vocab;
+};
+
+// The workgroup's MT x 128 tile by way of LDS (Z, rows of 132 floats, so that 8 rows'
+// 16-byte reads fall in different banks): 256 / MT threads a row.
+template <int MT, int EPI, int TT>
+__device__ __forceinline__ void head_tile(const GemmArgs &a, const HeadArgs &e, float *Z,
+                                          const floatx16 (&acc)[TT][2], int mblk, int mw, int wn, int lr, int h) {
+  constexpr int PITCH = 132, TR = 256 / MT, C = 128 / TR;
+  __syncthreads();  // every wave has read its last operands, and no DMA is under way
+#pragma unroll
+  for (int t = 0; t < TT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int m = mw + 32 * t + 8 * (r >> 2) + 4 * h + (r & 3);
+      const float iv = a.inv[mblk + m];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) Z[m * PITCH + wn * 64 + 32 * u + lr] = acc[t][u][r] * iv;
+    }
+  __syncthreads();
+  const int row = threadIdx.x / TR, part = threadIdx.x % TR, m = mblk + row;
+  const int col0 = C * part, n = blockIdx.x * 128 + col0;  // the thread's first column
+  const float *z = Z + row * PITCH + col0;
+  if constexpr (EPI == HEAD_SUMS) {
+    float x[C], top = -3.402823466e38f, sum = 0.f, spread = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; c += 4) *reinterpret_cast<float4 *>(x + c) = *reinterpret_cast<const float4 *>(z + c);
+    if (n + C > a.N) {
+#pragma unroll
+      for (int c = 0; c < C; ++c) x[c] = n + c < a.N ? x[c] : -INFINITY;
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) top = fmaxf(top, x[c]);
+#pragma unroll
+    for (int off = 1; off < TR; off *= 2) top = fmaxf(top, __shfl_xor(top, off));
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      // (the bound hides a NaN: a NaN logit has to reach the sum)
+      const float d = fmaxf(x[c] - top, -200.f), f = __builtin_amdgcn_exp2f(d * 1.44269504f);
+      sum += x[c] != x[c] ? x[c] : f;
+      spread = fmaf(d, f, spread);
+    }
+#pragma unroll
+    for (int off = 1; off < TR; off *= 2) {
+      sum += __shfl_xor(sum, off);
+      spread += __shfl_xor(spread, off);
+    }
+    if (part == 0 && m < a.M) {
+      e.parts[(size_t)m * e.n_parts + blockIdx.x] = make_float4(top, sum, spread, 0.f);
+      if (e.hit) {
+        const int t = e.targets[m] - blockIdx.x * 128;
+        if (t >= 0 && t < 128 && e.targets[m] < a.N) e.hit[m] = z[t];
+      }
+    }
+  } else {
+    if (m >= e.Mpad) return;
+    const int t = m < a.M ? e.targets[m] : -1;
+    const bool on = t >= 0 && t < e.vocab;
+    const float s = on ? e.lse[m] : 0.f;
+#pragma unroll
+    for (int c = 0; c < C; c += 8) {
+      const float4 x0 = *reinterpret_cast<const float4 *>(z + c), x1 = *reinterpret_cast<const float4 *>(z + c + 4);
+      const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+      half8 H, L;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float d = x[i] - s;
+        float g = on && n + c + i < a.N ? -expf(d) : 0.f;
+        if (on && e.v0 + n + c + i == t) g = -expm1f(d);
+        g *= 32768.f;
+        H[i] = (_Float16)g;
+        L[i] = (_Float16)(g - (float)H[i]);
+      }
+      if (n + c < (a.N + 31) / 32 * 32) {
+        const size_t at = ((size_t)((n + c) >> 5) * e.Mpad + m) * 32 + ((n + c) & 31);
+        *reinterpret_cast<half8 *>(e.hi + at) = H;
+        *reinterpret_cast<half8 *>(e.lo + at) = L;
+      }
+    }
+  }
+}
+
 // A weight group: 64 bytes of every row, i.e. SB consecutive blocks (Q4_0 /
 // Q4_1 four of 16 code bytes, Q8_0 two of 32, F16 one of 64), and their
 // scales (and Q4_1 mins) as in the planes, [32 four-row groups][SB][4].
@@ -608,8 +702,8 @@ template <int TYPE> struct DmaW {
 // constant, 205); F16 8192 x 2048 at 512 60 -> 54 us.  What is left is LDS
 // traffic (36 KB read and 18.7 written a block), 108 vector operations to 16
 // MFMAs, and the clock under both.
-template <int TYPE, bool SW = false>
-__device__ __forceinline__ void gemm_dma(const GemmArgs &a) {
+template <int TYPE, bool SW = false, int EPI = HEAD_NONE>
+__device__ __forceinline__ void gemm_dma(const GemmArgs &a, const HeadArgs &e = HeadArgs()) {
   constexpr int MT = 128;
   typedef DmaW<TYPE> W;
   constexpr int NA = MT / 64;                 // activation chunks a wave and plane
@@ -619,6 +713,7 @@ __device__ __forceinline__ void gemm_dma(const GemmArgs &a) {
   constexpr int SB = W::SB;
   constexpr int WOFF = 3 * STAGE;             // the ring of three weight groups
   __shared__ __attribute__((aligned(1024))) uint8_t S[3 * (STAGE + W::BYTES)];
+  static_assert(sizeof S >= MT * 132 * 4, "a head's tile fits");
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // uniform: SGPR bases
   const int lr = lane & 31, h = lane >> 5;
@@ -918,7 +1013,10 @@ __device__ __forceinline__ void gemm_dma(const GemmArgs &a) {
     wait_vm<0>();
   }
 
-  store_tiles<SW, TT>(a, acc, mblk + m0, n0, wn, lr, h);
+  if constexpr (EPI)
+    head_tile<MT, EPI, TT>(a, e, reinterpret_cast<float *>(S), acc, mblk, m0, wn, lr, h);
+  else
+    store_tiles<SW, TT>(a, acc, mblk + m0, n0, wn, lr, h);
 }
 
 // 64-row tiles: a ring of NS LDS stages, each [hi/lo][64 rows][4 chunks of 8
@@ -934,8 +1032,8 @@ template <int TYPE> struct DmaB {
   static constexpr int WD = TYPE == PBX_Q8 || TYPE == PBX_F16 ? 2 : 1;      // weight DMAs a wave
 };
 
-template <int TYPE, bool SW = false>
-__device__ __forceinline__ void gemm_dma64(const GemmArgs &a) {
+template <int TYPE, bool SW = false, int EPI = HEAD_NONE>
+__device__ __forceinline__ void gemm_dma64(const GemmArgs &a, const HeadArgs &e = HeadArgs()) {
   constexpr int MT = 64, NS = 3;
   typedef DmaB<TYPE> W;
   constexpr int NA = MT / 64;                                     // activation chunks a wave and plane
@@ -944,7 +1042,8 @@ __device__ __forceinline__ void gemm_dma64(const GemmArgs &a) {
   constexpr int ASTAGE = 2 * PS;                                  // bytes
   constexpr int STAGE = ASTAGE + W::CODES + 256 * W::NSC;         // bytes
   constexpr int PER = 2 * NA + W::WD;                             // DMA instructions a wave and block
-  __shared__ __attribute__((aligned(1024))) uint8_t S[NS * STAGE];
+  constexpr int BYTES = EPI && NS * STAGE < MT * 132 * 4 ? MT * 132 * 4 : NS * STAGE;
+  __shared__ __attribute__((aligned(1024))) uint8_t S[BYTES];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // uniform: SGPR bases
   const int lr = lane & 31, h = lane >> 5;
@@ -1148,7 +1247,10 @@ __device__ __forceinline__ void gemm_dma64(const GemmArgs &a) {
     wait_vm<0>();
   }
 
-  store_tiles<SW, TT>(a, acc, mblk + m0, n0, wn, lr, h);
+  if constexpr (EPI)
+    head_tile<MT, EPI, TT>(a, e, reinterpret_cast<float *>(S), acc, mblk, m0, wn, lr, h);
+  else
+    store_tiles<SW, TT>(a, acc, mblk + m0, n0, wn, lr, h);
 }
 
 extern "C" __global__ void __launch_bounds__(256) pbx_gemm_q4_big(GemmArgs a) { gemm_dma<PBX_Q4>(a); }
@@ -1171,6 +1273,25 @@ extern "C" __global__ void __launch_bounds__(256) pbx_gemm_q4_b64_sw(GemmArgs a)
 extern "C" __global__ void __launch_bounds__(256) pbx_gemm_q8_b64_sw(GemmArgs a) { gemm_dma64<PBX_Q8, true>(a); }
 extern "C" __global__ void __launch_bounds__(256) pbx_gemm_q41_b64_sw(GemmArgs a) { gemm_dma64<PBX_Q41, true>(a); }
 extern "C" __global__ void __launch_bounds__(256) pbx_gemm_f16_b64_sw(GemmArgs a) { gemm_dma64<PBX_F16, true>(a); }
+
+// a head's logits that are not kept
+#define HEAD_KERNELS(TAG, TYPE)                                                                                      \
+  extern "C" __global__ void __launch_bounds__(256) pbx_gemm_##TAG##_big_sums(GemmArgs a, HeadArgs e) {              \
+    gemm_dma<TYPE, false, HEAD_SUMS>(a, e);                                                                          \
+  }                                                                                                                  \
+  extern "C" __global__ void __launch_bounds__(256) pbx_gemm_##TAG##_b64_sums(GemmArgs a, HeadArgs e) {              \
+    gemm_dma64<TYPE, false, HEAD_SUMS>(a, e);                                                                        \
+  }                                                                                                                  \
+  extern "C" __global__ void __launch_bounds__(256) pbx_gemm_##TAG##_big_g(GemmArgs a, HeadArgs e) {                 \
+    gemm_dma<TYPE, false, HEAD_G>(a, e);                                                                             \
+  }                                                                                                                  \
+  extern "C" __global__ void __launch_bounds__(256) pbx_gemm_##TAG##_b64_g(GemmArgs a, HeadArgs e) {                 \
+    gemm_dma64<TYPE, false, HEAD_G>(a, e);                                                                           \
+  }
+HEAD_KERNELS(q4, PBX_Q4)
+HEAD_KERNELS(q8, PBX_Q8)
+HEAD_KERNELS(q41, PBX_Q41)
+HEAD_KERNELS(f16, PBX_F16)
 
 // Row scaling to fp16: one workgroup per (padded) row.  The scale is
 // 2^(15 - e) with 2^(e-1) <= max|x| < 2^e, so every scaled value is below

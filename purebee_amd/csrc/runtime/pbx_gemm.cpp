@@ -349,6 +349,45 @@ int pbx_gemm_launch(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M6
   return PBX_OK;
 }
 
+bool pbx_gemm_has_head(const pbx_weight *w, int64_t M) {
+  return M > PBX_GEMM_ROWS_M && w->type != PBX_TYPE_F32 && gemm_tag(w->type);
+}
+
+size_t pbx_gemm_head_space(const pbx_weight *w, int M) {
+  pbx_gemm_plan p;
+  p.M = M;
+  p.Mpad = (M + 127) / 128 * 128;
+  return gemm_space(p, (int)w->N, (int)w->K).total();
+}
+
+int pbx_gemm_head(pbx_ctx *c, const pbx_weight *w, const float *dX, int M, bool prep, void *space,
+                  const pbx_head_epilogue &e) {
+  pbx_gemm_plan p;
+  p.M = M;
+  p.Mpad = (M + 127) / 128 * 128;
+  p.nwg = ((int)w->N + 127) / 128;
+  // 128-row tiles, but where 64-row tiles leave out a half-empty one of at most eight
+  const bool b64 = (M + 63) / 64 % 2 && M <= 960;
+  p.mtiles = b64 ? (M + 63) / 64 : p.Mpad / 128;
+  p.name = std::string("pbx_gemm_") + gemm_tag(w->type) + (b64 ? "_b64" : "_big") + (e.lse ? "_g" : "_sums");
+  const GemmSpace sp = gemm_space(p, (int)w->N, (int)w->K);
+  void *x16 = space, *x16lo = (char *)space + sp.x16;
+  float *inv = (float *)((char *)space + 2 * sp.x16);
+  hipFunction_t f = pbx_kernel_by_name(c, p.name), fprep = pbx_kernel_by_name(c, "pbx_gemm_prep_x");
+  if (!f || !fprep) return pbx_fail(c, PBX_ELOAD, "pbx_gemm: kernel %s missing", p.name.c_str());
+  int rc;
+  if (prep) {
+    int m = M, k = (int)w->K;
+    void *args[] = {(void *)&dX, &x16, &x16lo, &inv, &m, &k};
+    if ((rc = pbx_launch_fn(c, fprep, "pbx_gemm_prep_x", dim3(p.Mpad), dim3(256), args, c->stream))) return rc;
+  }
+  GemmArgsHost g{w->qs, w->d, x16, x16lo, inv, nullptr, nullptr,
+                 M, (int)w->N, (int)w->Npad, (int)w->B, 1, 0, w->m, p.Mpad};
+  pbx_head_epilogue he = e;
+  void *args[] = {&g, &he};
+  return pbx_launch_fn(c, f, p.name.c_str(), dim3(p.nwg, p.mtiles), dim3(256), args, c->stream);
+}
+
 int pbx_gemm_enqueue(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M,
                      const float *dBias, float *dY, hipStream_t stream, const pbx_workspace *ws) {
   return pbx_gemm_launch(c, w, dX, M, dBias, dY, 0, stream, ws);

@@ -36,6 +36,7 @@ pbx_weight rows_of(const pbx_weight &w, int64_t v0, int64_t n) {
 }
 
 struct Plan {
+  bool fused;      // logits leave the GEMM as sums or as the gradient's factor, not as such
   int64_t piece;   // vocabulary entries of a piece, but for the last
   int n_pieces, n_parts;
   int Mpad, TT, KS;
@@ -50,8 +51,11 @@ Plan make_plan(pbx_ctx *c, const pbx_weight *w, int64_t M, bool grad) {
   const int64_t V = w->N;
   p.TT = M > 32 ? 2 : 1;
   p.Mpad = (int)((M + 63) / 64 * 64);
+  p.fused = pbx_gemm_has_head(w, M);
+  if (p.fused && grad) p.Mpad = (int)((M + 127) / 128 * 128);
   const int64_t row = 4 * (grad ? p.Mpad : M);
   p.piece = std::min<int64_t>((V + 127) / 128 * 128, std::max<int64_t>(128, HEAD_PIECE / row / 128 * 128));
+  if (p.fused && !grad) p.piece = (V + 127) / 128 * 128;
   p.n_pieces = (int)((V + p.piece - 1) / p.piece);
   size_t at = 0;
   auto take = [&](size_t n) {
@@ -61,14 +65,17 @@ Plan make_plan(pbx_ctx *c, const pbx_weight *w, int64_t M, bool grad) {
   };
   const int64_t last = V - (p.n_pieces - 1) * p.piece;
   size_t gemm = 0;
-  for (int64_t n : {std::min(p.piece, V), last}) {
-    const pbx_weight part = rows_of(*w, 0, n);
-    gemm = std::max(gemm, pbx_linear_space(c, &part, (int)M));
-  }
+  if (p.fused)
+    gemm = pbx_gemm_head_space(w, (int)M);
+  else
+    for (int64_t n : {std::min(p.piece, V), last}) {
+      const pbx_weight part = rows_of(*w, 0, n);
+      gemm = std::max(gemm, pbx_linear_space(c, &part, (int)M));
+    }
   auto shares = [](int64_t n) { return (int)((n + HEAD_SHARE - 1) / HEAD_SHARE); };
-  p.n_parts = (p.n_pieces - 1) * shares(p.piece) + shares(last);
+  p.n_parts = p.fused ? (int)((V + 127) / 128) : (p.n_pieces - 1) * shares(p.piece) + shares(last);
   p.gemm = take(gemm);
-  p.z = take((size_t)M * p.piece * 4);
+  p.z = take(p.fused ? 0 : (size_t)M * p.piece * 4);
   if (!grad) {
     p.parts = take((size_t)M * p.n_parts * 16);
     p.hit = take((size_t)M * 4);
@@ -135,7 +142,11 @@ extern "C" int pbx_linear_logprobs_dev(pbx_ctx *c, const pbx_weight *w, const fl
   float *z = (float *)(ws + p.z), *hit = (float *)(ws + p.hit);
   void *parts = ws + p.parts;
   int n_parts = p.n_parts, part0 = 0;
-  for (int64_t v0 = 0; v0 < w->N; v0 += p.piece) {
+  if (p.fused) {
+    const pbx_head_epilogue e{dTargets, parts, n_parts, dLogp ? hit : nullptr, nullptr, nullptr, nullptr, 0, 0, (int)w->N};
+    if ((rc = pbx_gemm_head(c, w, dX, (int)M, true, ws + p.gemm, e))) return rc;
+  }
+  for (int64_t v0 = 0; v0 < w->N && !p.fused; v0 += p.piece) {
     pbx_weight rows;
     int n = (int)std::min(p.piece, w->N - v0), at = (int)v0;
     if ((rc = piece_logits(c, w, p, ws, dX, M, v0, n, &rows))) return rc;
@@ -186,11 +197,16 @@ extern "C" int pbx_linear_logprobs_grad_dev(pbx_ctx *c, const pbx_weight *w, con
   for (int64_t v0 = 0; v0 < w->N; v0 += p.piece) {
     pbx_weight rows;
     int n = (int)std::min(p.piece, w->N - v0), at = (int)v0;
-    if ((rc = piece_logits(c, w, p, ws, dX, M, v0, n, &rows))) return rc;
+    if (!p.fused && (rc = piece_logits(c, w, p, ws, dX, M, v0, n, &rows))) return rc;
     const int blocks = (n + 31) / 32;
     int64_t stride = rows.N;
     void *hi = ws + p.g, *lo = ws + p.g + (size_t)blocks * 32 * Mpad * 2;
-    if (f32) {
+    if (p.fused) {
+      rows = rows_of(*w, v0, n);
+      rows.N = n;
+      const pbx_head_epilogue e{dTargets, nullptr, 0, nullptr, dLse, hi, lo, Mpad, at, vocab};
+      rc = pbx_gemm_head(c, &rows, dX, m, v0 == 0, ws + p.gemm, e);
+    } else if (f32) {
       void *args[] = {&z, &stride, &n, &at, (void *)&dLse, (void *)&dTargets, &vocab, &m, &Mpad, &hi};
       rc = pbx_launch(c, PBX_K_HEAD_G32, dim3(blocks, Mpad / 64), dim3(256), args);
     } else {
