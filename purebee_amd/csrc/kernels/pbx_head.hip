@@ -227,38 +227,11 @@ struct BackArgs {
 
 namespace {
 
-// hi and lo of 4 columns of weights at 8 consecutive vocabulary entries: column i's
-// operand is H[i], L[i].  Products of a code and its scale are exact as the pair
-// (19 bits at most); Q4_1 and Q6_K values are rounded to f32 first.
-struct Operand {
-  half8 H[4], L[4];
-};
 __device__ __forceinline__ half2t as_half2(unsigned x) { return __builtin_bit_cast(half2t, x); }
 // Byte i of x and of y, as two halves u * 2^-24 (the bits of a half of exponent 0).
 __device__ __forceinline__ unsigned byte_pair(unsigned x, unsigned y, int i) {
   return __builtin_amdgcn_perm(y, x, 0x0c000c00u | (unsigned)i | (unsigned)(4 + i) << 16);
 }
-__device__ __forceinline__ void put_pair(Operand &o, int i, int p, half2t y, half2t d) {
-  const half2t h = y * d;
-  const half2t l = __builtin_elementwise_fma(y, d, -h);
-  o.H[i][2 * p] = h[0];
-  o.H[i][2 * p + 1] = h[1];
-  o.L[i][2 * p] = l[0];
-  o.L[i][2 * p + 1] = l[1];
-}
-__device__ __forceinline__ void put_value(Operand &o, int i, int e, float w) {
-  o.H[i][e] = (_Float16)w;
-  o.L[i][e] = (_Float16)(w - (float)o.H[i][e]);
-}
-
-template <int TYPE> struct HeadRaw {  // of one row
-  unsigned w;
-};
-template <> struct HeadRaw<PBX_F16> { uint2 w; };
-template <> struct HeadRaw<PBX_Q6K> {
-  unsigned ql0, ql1, qh, d;
-  uint2 sc;
-};
 
 // Column of the wave's 128 that lane lr's tile i holds.
 template <int TYPE>
@@ -268,10 +241,26 @@ __device__ __forceinline__ int column_of(int lr, int i) {
   return 4 * lr + i;
 }
 
-// TT: 32-row tiles.
+// What 16 entries' part of a wave's operands is made of, as loaded.
+template <int TYPE, int TT>
+struct BackRaw {
+  static constexpr int NW = TYPE == PBX_F16 ? 16 : TYPE == PBX_Q6K ? 24 : 8;
+  unsigned w[NW];
+  uint2 d[TYPE == PBX_Q6K ? 8 : 2], mn[TYPE == PBX_Q41 ? 2 : 1];
+  unsigned ds[TYPE == PBX_Q6K ? 8 : 1];
+  half8 Ah[TT], Al[TT];
+};
+
+// Workgroup = 32 TT rows of G, 128 columns of the head and a share of its entries, whose
+// blocks four waves take in turn; their sums meet in LDS.  A step is 16 entries: a lane
+// loads 4 columns (as they lie in a row's bytes) of 8 rows, so that the operands, 8
+// entries of a column, are put together in registers, byte by byte with no trip through
+// LDS, while the next step's loads are under way.
 template <int TYPE, int TT>
 __device__ __forceinline__ void back_body(const BackArgs &a) {
-  const int lane = threadIdx.x, lr = lane & 31, h = lane >> 5;
+  __shared__ float red[2][TT * 4 * 16 * 64];
+  const int lane = threadIdx.x & 63, lr = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int k0 = blockIdx.x * 128, m0 = blockIdx.y * (32 * TT);
   const int b0 = (int)((int64_t)a.blocks * blockIdx.z / a.KS), b1 = (int)((int64_t)a.blocks * (blockIdx.z + 1) / a.KS);
   constexpr bool NIB = TYPE == PBX_Q4 || TYPE == PBX_Q41;
@@ -289,109 +278,159 @@ __device__ __forceinline__ void back_body(const BackArgs &a) {
   const float fs = ldexpf(1.f, shift);
   // past the row's end columns repeat the last ones (and are not stored)
   const int kc = min(k0 + 4 * lr, a.K - 4), kb = min((k0 >> 5) + (lr >> 3), a.B - 1);
-  for (int b = b0; b < b1; ++b) {
+  const int SB = a.B >> 3, sb = min(k0 >> 8, SB - 1), hf = (k0 >> 7) & 1;
+  // a row's bytes, and the lane's first byte in the rows 8 h on
+  const size_t row = TYPE == PBX_F16 ? (size_t)a.K * 2 : TYPE == PBX_Q8 ? a.K : TYPE == PBX_Q6K ? (size_t)SB * PBX_Q6K_BYTES
+                                                                                           : (size_t)a.B * 16;
+  const size_t woff = 8 * h * row + (TYPE == PBX_F16   ? 2 * kc
+                                     : TYPE == PBX_Q8  ? kc
+                                     : TYPE == PBX_Q6K ? sb * PBX_Q6K_BYTES
+                                                       : kb * 16 + 2 * (lr & 7));
+  const int scols = TYPE == PBX_Q6K ? SB : a.B;                      // scales of a row
+  const size_t doff = ((size_t)2 * h * scols + (TYPE == PBX_Q6K ? sb : kb)) * 8;
+  const size_t aoff = (size_t)(m0 + lr) * 64 + 16 * h;
+  // rows of the piece reach past its last block (they are padded to 64), so no step reads
+  // beyond them
+  auto load = [&](int step, BackRaw<TYPE, TT> &q) {
+    const uint8_t *w = a.qs + (size_t)step * 16 * row;
+    const uint8_t *d = reinterpret_cast<const uint8_t *>(a.dsc) + (size_t)step * 4 * scols * 8;
+    const uint8_t *mn = reinterpret_cast<const uint8_t *>(a.msc) + (size_t)step * 4 * scols * 8;
+    if constexpr (TYPE == PBX_Q6K) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int v = 32 * b + 16 * half + 8 * h;
-      half8 Ah[TT], Al[TT];
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        const int64_t at = ((int64_t)b * a.Mpad + m0 + 32 * t + lr) * 32 + 16 * half + 8 * h;
-        Ah[t] = *reinterpret_cast<const half8 *>(a.hi + at);
-        Al[t] = *reinterpret_cast<const half8 *>(a.lo + at);
+      for (int e = 0; e < 8; ++e) {
+        const uint8_t *blk = w + e * row + woff;
+        q.w[3 * e] = blk[64 * hf + lr];
+        q.w[3 * e + 1] = blk[64 * hf + 32 + lr];
+        q.w[3 * e + 2] = blk[128 + 32 * hf + lr];
+        q.d[e] = *reinterpret_cast<const uint2 *>(blk + 192 + 8 * hf);
+        q.ds[e] = *reinterpret_cast<const uint16_t *>(d + (size_t)(e >> 2) * scols * 8 + doff + 2 * (e & 3));
       }
-      Operand o;
-      if constexpr (TYPE == PBX_F16) {
-        uint2 w[8];
+    } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          w[e] = *reinterpret_cast<const uint2 *>(a.qs + ((int64_t)min(v + e, a.rows - 1) * a.K + kc) * 2);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int p = 0; p < 4; ++p) {
-            const unsigned x = i < 2 ? w[2 * p].x : w[2 * p].y, y = i < 2 ? w[2 * p + 1].x : w[2 * p + 1].y;
-            const half2t z = as_half2(__builtin_amdgcn_perm(y, x, i & 1 ? 0x07060302u : 0x05040100u));
-            o.H[i][2 * p] = z[0];
-            o.H[i][2 * p + 1] = z[1];
-          }
-      } else if constexpr (TYPE == PBX_Q6K) {
-        // 4 tiles are the four 32-code groups of half a superblock
-        const int SB = a.B >> 3, sb = min(k0 >> 8, SB - 1), hf = (k0 >> 7) & 1;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int n = min(v + e, a.rows - 1);
-          const uint8_t *blk = a.qs + ((int64_t)n * SB + sb) * PBX_Q6K_BYTES;
-          const unsigned l0 = blk[64 * hf + lr], l1 = blk[64 * hf + 32 + lr], q = blk[128 + 32 * hf + lr];
-          const uint2 sc = *reinterpret_cast<const uint2 *>(blk + 192 + 8 * hf);
-          const float d = f16_bits_to_f32(a.dsc[dsc_index(n, sb, SB)]) * fs;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const unsigned s8 = ((i < 2 ? sc.x : sc.y) >> (16 * (i & 1) + 8 * (lr >> 4))) & 255u;
-            const int code = (int)(((i & 1 ? l1 : l0) >> (4 * (i >> 1)) & 15u) | ((q >> (2 * i) & 3u) << 4)) - 32;
-            put_value(o, i, e, d * (float)(int8_t)s8 * (float)code);
-          }
+      for (int e = 0; e < 8; ++e) {
+        const uint8_t *p = w + e * row + woff;
+        if constexpr (TYPE == PBX_F16) {
+          const uint2 x = *reinterpret_cast<const uint2 *>(p);
+          q.w[2 * e] = x.x;
+          q.w[2 * e + 1] = x.y;
+        } else if constexpr (NIB) {
+          q.w[e] = *reinterpret_cast<const uint16_t *>(p);
+        } else {
+          q.w[e] = *reinterpret_cast<const unsigned *>(p);
         }
-      } else {
-        unsigned w[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int64_t n = min(v + e, a.rows - 1);
-          if constexpr (NIB)
-            w[e] = *reinterpret_cast<const uint16_t *>(a.qs + (n * a.B + kb) * 16 + 2 * (lr & 7));
-          else
-            w[e] = *reinterpret_cast<const unsigned *>(a.qs + n * a.K + kc) ^ 0x80808080u;
-        }
-        // scales of rows v .. v + 7: two groups of four (their rows are padded to 64)
-        uint2 d[2], mn[2];
+      }
+      if constexpr (TYPE != PBX_F16) {
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          const int n = min(v + 4 * g, a.rows - 4);
-          d[g] = *reinterpret_cast<const uint2 *>(a.dsc + dsc_index(n, kb, a.B));
-          mn[g] = TYPE == PBX_Q41 ? *reinterpret_cast<const uint2 *>(a.msc + dsc_index(n, kb, a.B)) : make_uint2(0, 0);
-        }
-        if constexpr (TYPE == PBX_Q41) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const unsigned dw = e & 2 ? d[e >> 2].y : d[e >> 2].x, mw = e & 2 ? mn[e >> 2].y : mn[e >> 2].x;
-            const float df = f16_bits_to_f32(dw >> (16 * (e & 1))) * fs, mf = f16_bits_to_f32(mw >> (16 * (e & 1))) * fs;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              put_value(o, i, e, fmaf((float)(w[e] >> (8 * (i & 1) + 4 * (i >> 1)) & 15u), df, mf));
-          }
-        } else {
-#pragma unroll
-          for (int p = 0; p < 4; ++p) {
-            const half2t dp = as_half2(p & 1 ? d[p >> 1].y : d[p >> 1].x) * f1 * f2;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              half2t y;
-              if constexpr (TYPE == PBX_Q4) {
-                const unsigned x = byte_pair(w[2 * p], w[2 * p + 1], i & 1);
-                const half2t off = {(_Float16)-0.015625f, (_Float16)-0.015625f};  // -8 2^-9
-                const _Float16 up = i < 2 ? (_Float16)32768.f : (_Float16)2048.f;
-                y = __builtin_elementwise_fma(as_half2(x & (i < 2 ? 0x000F000Fu : 0x00F000F0u)), half2t{up, up}, off);
-              } else {
-                const half2t off = {(_Float16)-0.25f, (_Float16)-0.25f};  // -128 2^-9
-                const half2t up = {(_Float16)32768.f, (_Float16)32768.f};
-                y = __builtin_elementwise_fma(as_half2(byte_pair(w[2 * p], w[2 * p + 1], i)), up, off);
-              }
-              put_pair(o, i, p, y, dp);
-            }
-          }
+          q.d[g] = *reinterpret_cast<const uint2 *>(d + (size_t)g * scols * 8 + doff);
+          if constexpr (TYPE == PBX_Q41) q.mn[g] = *reinterpret_cast<const uint2 *>(mn + (size_t)g * scols * 8 + doff);
         }
       }
+    }
+    const size_t at = (size_t)(step >> 1) * a.Mpad * 64 + 32 * (step & 1);
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      q.Ah[t] = *reinterpret_cast<const half8 *>(reinterpret_cast<const uint8_t *>(a.hi) + at + 2048 * t + aoff);
+      q.Al[t] = *reinterpret_cast<const half8 *>(reinterpret_cast<const uint8_t *>(a.lo) + at + 2048 * t + aoff);
+    }
+  };
+  auto multiply = [&](const BackRaw<TYPE, TT> &q) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      half8 H, L = {};
+      if constexpr (TYPE == PBX_F16) {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const half2t z = as_half2(__builtin_amdgcn_perm(q.w[4 * p + 2 + (i >> 1)], q.w[4 * p + (i >> 1)],
+                                                          i & 1 ? 0x07060302u : 0x05040100u));
+          H[2 * p] = z[0];
+          H[2 * p + 1] = z[1];
+        }
+      } else if constexpr (TYPE == PBX_Q6K || TYPE == PBX_Q41) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float v;
+          if constexpr (TYPE == PBX_Q6K) {
+            // tile i is the i-th 32-code group of half a superblock
+            const unsigned s8 = ((i < 2 ? q.d[e].x : q.d[e].y) >> (16 * (i & 1) + 8 * (lr >> 4))) & 255u;
+            const int code = (int)((q.w[3 * e + (i & 1)] >> (4 * (i >> 1)) & 15u) | ((q.w[3 * e + 2] >> (2 * i) & 3u) << 4)) - 32;
+            v = f16_bits_to_f32(q.ds[e]) * fs * (float)(int8_t)s8 * (float)code;
+          } else {
+            const unsigned dw = e & 2 ? q.d[e >> 2].y : q.d[e >> 2].x, mw = e & 2 ? q.mn[e >> 2].y : q.mn[e >> 2].x;
+            v = fmaf((float)(q.w[e] >> (8 * (i & 1) + 4 * (i >> 1)) & 15u), f16_bits_to_f32(dw >> (16 * (e & 1))) * fs,
+                     f16_bits_to_f32(mw >> (16 * (e & 1))) * fs);
+          }
+          H[e] = (_Float16)v;
+          L[e] = (_Float16)(v - (float)H[e]);
+        }
+      } else {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const half2t d = as_half2(p & 1 ? q.d[p >> 1].y : q.d[p >> 1].x) * f1 * f2;
+          half2t y;
+          if constexpr (TYPE == PBX_Q4) {
+            const unsigned x = byte_pair(q.w[2 * p], q.w[2 * p + 1], i & 1);
+            const half2t off = {(_Float16)-0.015625f, (_Float16)-0.015625f};  // -8 2^-9
+            const _Float16 up = i < 2 ? (_Float16)32768.f : (_Float16)2048.f;
+            y = __builtin_elementwise_fma(as_half2(x & (i < 2 ? 0x000F000Fu : 0x00F000F0u)), half2t{up, up}, off);
+          } else {
+            const half2t off = {(_Float16)-0.25f, (_Float16)-0.25f};  // -128 2^-9
+            const half2t up = {(_Float16)32768.f, (_Float16)32768.f};
+            y = __builtin_elementwise_fma(as_half2(byte_pair(q.w[2 * p] ^ 0x80808080u, q.w[2 * p + 1] ^ 0x80808080u, i)), up, off);
+          }
+          const half2t hi = y * d, lo = __builtin_elementwise_fma(y, d, -hi);
+          H[2 * p] = hi[0];
+          H[2 * p + 1] = hi[1];
+          L[2 * p] = lo[0];
+          L[2 * p + 1] = lo[1];
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < TT; ++t) acc[t][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q.Ah[t], H, acc[t][i], 0, 0, 0);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) acc[t][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q.Al[t], H, acc[t][i], 0, 0, 0);
+      if constexpr (TYPE != PBX_F16) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t) acc[t][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(q.Ah[t], L, acc[t][i], 0, 0, 0);
+      }
+    }
+  };
+  if (b0 + wave < b1) {
+    BackRaw<TYPE, TT> q, n;
+    load(2 * (b0 + wave), q);
+    for (int b = b0 + wave; b < b1; b += 4) {
+      load(2 * b + 1, n);
+      multiply(q);
+      load(2 * min(b + 4, b1 - 1), q);  // (the last step loads its block again)
+      multiply(n);
+    }
+  }
+  // the waves' sums, in a fixed order: (0 + 2) + (1 + 3)
+  float *mine = red[wave & 1];
+#pragma unroll
+  for (int way = 0; way < 2; ++way) {
+    const int from = way ? 1 : 2;  // waves from .. 2 from - 1 hand theirs to those `from` below
+    if (wave >= from && wave < 2 * from) {
 #pragma unroll
       for (int t = 0; t < TT; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          acc[t][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(Ah[t], o.H[i], acc[t][i], 0, 0, 0);
-          acc[t][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(Al[t], o.H[i], acc[t][i], 0, 0, 0);
-          if constexpr (TYPE != PBX_F16)
-            acc[t][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(Ah[t], o.L[i], acc[t][i], 0, 0, 0);
-        }
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) mine[((t * 4 + i) * 16 + r) * 64 + lane] = acc[t][i][r];
     }
+    __syncthreads();
+    if (wave < from) {
+      const float *theirs = red[way ? 1 : wave];
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[t][i][r] += theirs[((t * 4 + i) * 16 + r) * 64 + lane];
+    }
+    __syncthreads();
   }
+  if (wave) return;
   const float undo = ldexpf(1.f, -15 - shift);
   float *part = a.part + (int64_t)blockIdx.z * a.M * a.K;
 #pragma unroll
@@ -456,8 +495,8 @@ __device__ __forceinline__ void back_f32(const BackArgs &a) {
 }  // namespace
 
 #define HEAD_BACK(TAG, TYPE)                                                                                     \
-  extern "C" __global__ void __launch_bounds__(64) pbx_head_back_##TAG##_1(BackArgs a) { back_body<TYPE, 1>(a); } \
-  extern "C" __global__ void __launch_bounds__(64) pbx_head_back_##TAG##_2(BackArgs a) { back_body<TYPE, 2>(a); }
+  extern "C" __global__ void __launch_bounds__(256, 2) pbx_head_back_##TAG##_1(BackArgs a) { back_body<TYPE, 1>(a); } \
+  extern "C" __global__ void __launch_bounds__(256, 2) pbx_head_back_##TAG##_2(BackArgs a) { back_body<TYPE, 2>(a); }
 HEAD_BACK(q4, PBX_Q4)
 HEAD_BACK(q41, PBX_Q41)
 HEAD_BACK(q8, PBX_Q8)

@@ -81,8 +81,9 @@ Plan make_plan(pbx_ctx *c, const pbx_weight *w, int64_t M, bool grad) {
     p.hit = take((size_t)M * 4);
   } else {
     const int64_t tiles = (w->K + 127) / 128 * ((M + 32 * p.TT - 1) / (32 * p.TT));
-    // about two waves a SIMD
-    p.KS = (int)std::max<int64_t>(1, std::min<int64_t>(8 * c->cu_count / tiles, p.piece / 32));
+    // about two waves a SIMD (an F32 head's workgroups are one wave, the others' four)
+    const int waves = w->type == PBX_TYPE_F32 ? 1 : 4;
+    p.KS = (int)std::max<int64_t>(1, std::min<int64_t>(8 / waves * c->cu_count / tiles, p.piece / (32 * waves)));
     p.g = take((size_t)p.Mpad * p.piece * 4);
     p.peaks = take(HEAD_PEAKS * 4);
     p.part = take((size_t)p.KS * M * w->K * 4);
@@ -218,7 +219,7 @@ extern "C" int pbx_linear_logprobs_grad_dev(pbx_ctx *c, const pbx_weight *w, con
                    v0 > 0};
     void *args[] = {&b};
     if ((rc = pbx_launch_fn(c, back, name.c_str(), dim3((k + 127) / 128, (m + 32 * p.TT - 1) / (32 * p.TT), KS),
-                            dim3(64), args, c->stream)))
+                            dim3(f32 ? 64 : 256), args, c->stream)))
       return rc;
   }
   void *args[] = {&part, &KS, &m, &k, (void *)&dTargets, &vocab, (void *)&dGradLogp, &dGradX};
