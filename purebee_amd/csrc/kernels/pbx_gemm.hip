@@ -598,9 +598,9 @@ struct HeadArgs {
 
 // The workgroup's MT x 128 tile by way of LDS (Z, rows of 132 floats, so that 8 rows'
 // 16-byte reads fall in different banks): 256 / MT threads a row.
-template <int MT, int EPI, int TT>
+template <int MT, int EPI, int TT, int UU>
 __device__ __forceinline__ void head_tile(const GemmArgs &a, const HeadArgs &e, float *Z,
-                                          const floatx16 (&acc)[TT][2], int mblk, int mw, int wn, int lr, int h) {
+                                          const floatx16 (&acc)[TT][UU], int mblk, int mw, int wn, int lr, int h) {
   constexpr int PITCH = 132, TR = 256 / MT, C = 128 / TR;
   __syncthreads();  // every wave has read its last operands, and no DMA is under way
 #pragma unroll
@@ -610,7 +610,7 @@ __device__ __forceinline__ void head_tile(const GemmArgs &a, const HeadArgs &e, 
       const int m = mw + 32 * t + 8 * (r >> 2) + 4 * h + (r & 3);
       const float iv = a.inv[mblk + m];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) Z[m * PITCH + wn * 64 + 32 * u + lr] = acc[t][u][r] * iv;
+      for (int u = 0; u < UU; ++u) Z[m * PITCH + 32 * (UU * wn + u) + lr] = acc[t][u][r] * iv;
     }
   __syncthreads();
   const int row = threadIdx.x / TR, part = threadIdx.x % TR, m = mblk + row;
@@ -1014,7 +1014,7 @@ __device__ __forceinline__ void gemm_dma(const GemmArgs &a, const HeadArgs &e = 
   }
 
   if constexpr (EPI)
-    head_tile<MT, EPI, TT>(a, e, reinterpret_cast<float *>(S), acc, mblk, m0, wn, lr, h);
+    head_tile<MT, EPI>(a, e, reinterpret_cast<float *>(S), acc, mblk, m0, wn, lr, h);
   else
     store_tiles<SW, TT>(a, acc, mblk + m0, n0, wn, lr, h);
 }
@@ -1032,35 +1032,38 @@ template <int TYPE> struct DmaB {
   static constexpr int WD = TYPE == PBX_Q8 || TYPE == PBX_F16 ? 2 : 1;      // weight DMAs a wave
 };
 
-template <int TYPE, bool SW = false, int EPI = HEAD_NONE>
+// MT = 32 (a head's logits that are not kept, up to 32 rows): the four waves side by
+// side, 32 x 32 each; waves 0, 1 fetch the activations' hi plane, 2, 3 lo.
+template <int TYPE, bool SW = false, int EPI = HEAD_NONE, int MT = 64>
 __device__ __forceinline__ void gemm_dma64(const GemmArgs &a, const HeadArgs &e = HeadArgs()) {
-  constexpr int MT = 64, NS = 3;
+  static_assert(MT == 64 || (MT == 32 && EPI), "64 rows, or 32 of a head");
+  constexpr int NS = 3, UU = MT / 32;                             // UU: 32-column tiles of a wave
   typedef DmaB<TYPE> W;
-  constexpr int NA = MT / 64;                                     // activation chunks a wave and plane
-  constexpr int TT = MT / 64;                                     // 32-row MFMA tiles a wave
+  constexpr int NA = 1;                                           // activation chunks a wave and plane
+  constexpr int TT = 1;                                           // 32-row MFMA tiles a wave
   constexpr int PS = MT * 32 * 2;                                 // bytes of a stage's hi (or lo) plane
   constexpr int ASTAGE = 2 * PS;                                  // bytes
   constexpr int STAGE = ASTAGE + W::CODES + 256 * W::NSC;         // bytes
-  constexpr int PER = 2 * NA + W::WD;                             // DMA instructions a wave and block
+  constexpr int PER = (MT == 64 ? 2 : 1) * NA + W::WD;            // DMA instructions a wave and block
   constexpr int BYTES = EPI && NS * STAGE < MT * 132 * 4 ? MT * 132 * 4 : NS * STAGE;
   __shared__ __attribute__((aligned(1024))) uint8_t S[BYTES];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // uniform: SGPR bases
   const int lr = lane & 31, h = lane >> 5;
-  const int wm = wave >> 1, wn = wave & 1;
-  const int n0 = blockIdx.x * 128 + wn * 64;
+  const int wm = MT == 64 ? wave >> 1 : 0, wn = MT == 64 ? wave & 1 : wave;
+  const int n0 = blockIdx.x * 128 + wn * (32 * UU);
   const int mblk = blockIdx.y * MT;
-  const int m0 = wm * (MT / 2);
+  const int m0 = 32 * wm;
   const int per = (a.B + a.KS - 1) / a.KS;
   const int b0 = blockIdx.z * per;
   const int b1 = min(a.B, b0 + per);
   const floatx16 zero16 = {};
 
-  floatx16 acc[TT][2];
+  floatx16 acc[TT][UU];
 #pragma unroll
   for (int t = 0; t < TT; ++t)
 #pragma unroll
-    for (int u = 0; u < 2; ++u) acc[t][u] = zero16;
+    for (int u = 0; u < UU; ++u) acc[t][u] = zero16;
 
   if (b0 < b1) {
     // activation DMA i (i < NA) of this wave and plane: LDS chunks
@@ -1068,7 +1071,7 @@ __device__ __forceinline__ void gemm_dma64(const GemmArgs &a, const HeadArgs &e 
     unsigned avoff[NA];
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
-      const int c = (4 * i + wave) * 64 + lane;  // plane 0 chunk (same offsets in plane 1)
+      const int c = (4 * i + (MT == 64 ? wave : wave & 1)) * 64 + lane;  // plane 0 chunk (same offsets in plane 1)
       const int r = c >> 2, q = (c & 3) ^ a_swz(r);
       avoff[i] = (unsigned)((r * 32 + q * 8) * 2);
     }
@@ -1137,17 +1140,20 @@ __device__ __forceinline__ void gemm_dma64(const GemmArgs &a, const HeadArgs &e 
       code_dma(1, 2 * wave + 1);
     }
     const unsigned lbase = lds_addr(&S[0]);
-    const unsigned lds0 = __builtin_amdgcn_readfirstlane(lbase + wave * 1024);
+    const unsigned lds0 = __builtin_amdgcn_readfirstlane(lbase + wave * 1024);  // (MT 32: planes of 2 KB)
+    const uint8_t *xmine = MT == 64 || wave < 2 ? xhi : xlo;
     unsigned ldw[2];
 #pragma unroll
     for (int k = 0; k < W::WD; ++k) ldw[k] = __builtin_amdgcn_readfirstlane(lbase + wl[k]);
     auto dma = [&](int b, int stage) {
       const unsigned so = stage * STAGE;
 #pragma unroll
-      for (int i = 0; i < NA; ++i) dma_to_lds_s<16>(xhi + b * xstep, avoff[i], lds0 + so + 4096 * i);
+      for (int i = 0; i < NA; ++i) dma_to_lds_s<16>(xmine + b * xstep, avoff[i], lds0 + so + 4096 * i);
+      if constexpr (MT == 64) {
 #pragma unroll
-      for (int i = 0; i < NA; ++i)
-        dma_to_lds_s<16>(xlo + b * xstep, avoff[i], lds0 + so + PS + 4096 * i);
+        for (int i = 0; i < NA; ++i)
+          dma_to_lds_s<16>(xlo + b * xstep, avoff[i], lds0 + so + PS + 4096 * i);
+      }
 #pragma unroll
       for (int k = 0; k < W::WD; ++k) {
         if (wsz[k] == 16)
@@ -1166,9 +1172,9 @@ __device__ __forceinline__ void gemm_dma64(const GemmArgs &a, const HeadArgs &e 
         const int r = m0 + 32 * t + lr;
         aoff[t][j] = (r * 32 + (((2 * j + h) ^ a_swz(r)) * 8)) * 2;
       }
-    int sofs[2];
+    int sofs[UU];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) sofs[u] = ASTAGE + W::CODES + (wn * 64 + 32 * u + lr) * 2;
+    for (int u = 0; u < UU; ++u) sofs[u] = ASTAGE + W::CODES + (32 * (UU * wn + u) + lr) * 2;
 
 #pragma unroll
     for (int s = 0; s < NS - 1; ++s) dma(min(b0 + s, b1 - 1), s);
@@ -1182,11 +1188,11 @@ __device__ __forceinline__ void gemm_dma64(const GemmArgs &a, const HeadArgs &e 
         lds_barrier();
         dma(min(b + NS - 1, b1 - 1), s == 0 ? NS - 1 : s - 1);
         const uint8_t *sb = rbase + s * STAGE;
-        half8 B0[2], B1[2];
-        float d[2], mn[2];
+        half8 B0[UU], B1[UU];
+        float d[UU], mn[UU];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint8_t *wr = sb + ASTAGE + (wn * 64 + 32 * u + lr) * W::CB;
+        for (int u = 0; u < UU; ++u) {
+          const uint8_t *wr = sb + ASTAGE + (32 * (UU * wn + u) + lr) * W::CB;
           if constexpr (TYPE == PBX_F16) {
             B0[u] = *reinterpret_cast<const half8 *>(wr + 16 * h);
             B1[u] = *reinterpret_cast<const half8 *>(wr + 32 + 16 * h);
@@ -1223,7 +1229,7 @@ __device__ __forceinline__ void gemm_dma64(const GemmArgs &a, const HeadArgs &e 
             xs = __builtin_amdgcn_mfma_f32_32x32x16_f16(Al1, ones, xs, 0, 0, 0);
           }
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
+          for (int u = 0; u < UU; ++u) {
             if constexpr (TYPE == PBX_F16) {
               acc[t][u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(Ah0, B0[u], acc[t][u], 0, 0, 0);
               acc[t][u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(Al0, B0[u], acc[t][u], 0, 0, 0);
@@ -1248,7 +1254,7 @@ __device__ __forceinline__ void gemm_dma64(const GemmArgs &a, const HeadArgs &e 
   }
 
   if constexpr (EPI)
-    head_tile<MT, EPI, TT>(a, e, reinterpret_cast<float *>(S), acc, mblk, m0, wn, lr, h);
+    head_tile<MT, EPI>(a, e, reinterpret_cast<float *>(S), acc, mblk, m0, wn, lr, h);
   else
     store_tiles<SW, TT>(a, acc, mblk + m0, n0, wn, lr, h);
 }
@@ -1281,6 +1287,12 @@ extern "C" __global__ void __launch_bounds__(256) pbx_gemm_f16_b64_sw(GemmArgs a
   }                                                                                                                  \
   extern "C" __global__ void __launch_bounds__(256) pbx_gemm_##TAG##_b64_sums(GemmArgs a, HeadArgs e) {              \
     gemm_dma64<TYPE, false, HEAD_SUMS>(a, e);                                                                        \
+  }                                                                                                                  \
+  extern "C" __global__ void __launch_bounds__(256) pbx_gemm_##TAG##_b32_sums(GemmArgs a, HeadArgs e) {              \
+    gemm_dma64<TYPE, false, HEAD_SUMS, 32>(a, e);                                                                    \
+  }                                                                                                                  \
+  extern "C" __global__ void __launch_bounds__(256) pbx_gemm_##TAG##_b32_g(GemmArgs a, HeadArgs e) {                 \
+    gemm_dma64<TYPE, false, HEAD_G, 32>(a, e);                                                                       \
   }                                                                                                                  \
   extern "C" __global__ void __launch_bounds__(256) pbx_gemm_##TAG##_big_g(GemmArgs a, HeadArgs e) {                 \
     gemm_dma<TYPE, false, HEAD_G>(a, e);                                                                             \

@@ -125,6 +125,185 @@ pbx_head_join(const float4 *parts, int n_parts, const int *targets, int vocab, c
   }
 }
 
+// ---- one to three rows of a Q6_K head ------------------------------------------------
+
+namespace {
+
+// The value of the lane that differs in bit OFF, by moves that need no trip through LDS.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+template <int OFF>
+__device__ __forceinline__ float partner(float v, int lane) {
+  if constexpr (OFF == 1) return dpp<0xB1>(v);              // quad_perm 1 0 3 2
+  else if constexpr (OFF == 2) return dpp<0x4E>(v);         // quad_perm 2 3 0 1
+  else if constexpr (OFF == 4) return dpp<0x1B>(dpp<0x141>(v));  // row_half_mirror, quad_perm 3 2 1 0
+  else if constexpr (OFF == 8) return dpp<0x128>(v);        // row_ror 8
+  else {
+    const unsigned u = __float_as_uint(v);
+    const auto r = OFF == 16 ? __builtin_amdgcn_permlane16_swap(u, u, false, false)
+                             : __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __uint_as_float(lane & OFF ? r[0] : r[1]);
+  }
+}
+
+struct SixArgs {
+  const uint8_t *qs;
+  const uint16_t *dsc;
+  const float *X;  // [M][K]
+  int N, SB;
+  // the answer's sums [M][n_parts] (a part is a workgroup) and the targets' logits, or (Z)
+  // the logits [M][stride]
+  const int *targets;
+  float4 *parts;
+  int n_parts;
+  float *hit, *Z;
+  int64_t stride;
+};
+
+// Logits of M rows, 24-bit activations, f32 sums.  A lane takes 16 bytes of low nibbles:
+// the 16 codes of one 32-code group of half a superblock and the 16 of the group two
+// further on, whose high bits lie in 16 bytes that it shares with one other lane; eight lanes a
+// superblock, so a row of 2,048 is one wave's (of the plain GEMV a lane takes a 32-code
+// block, 64 bytes for 24 of its own: 128,256 x 2,048 70 us).  A step is four rows
+// (whose superblock scales are one load) for each group of LANES lanes, the next step's
+// in flight; the lanes' sums of four rows are added in 7 steps instead of 24, halving what
+// each lane holds.  Bound by bytes.
+template <int M, int LANES>
+__device__ __forceinline__ void six_body(const SixArgs &a) {
+  constexpr int SLOTS = 64 / LANES;
+  __shared__ float buf[4][4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int slot = lane / LANES, sb0 = lane % LANES / 8, c = lane & 3, half = lane >> 2 & 1;
+  const int step = (int)gridDim.x * 4 * SLOTS, groups = (a.N + 3) / 4;
+  const int its = (a.SB + LANES / 8 - 1) / (LANES / 8);
+  struct Raw {
+    uint4 l[4], h[4];
+    uint2 sc[4], d;
+  };
+  // (a slot or superblock past the end reads the last one, and adds nothing)
+  auto load = [&](int g, int it, Raw &q) {
+    const int n = 4 * min(g, groups - 1), sb = min(sb0 + it * (LANES / 8), a.SB - 1);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const uint8_t *blk = a.qs + ((int64_t)(n + r) * a.SB + sb) * PBX_Q6K_BYTES;
+      q.l[r] = ld_stream(blk + 64 * half + 16 * c);
+      q.h[r] = ld_stream(blk + 128 + 32 * half + 16 * (c & 1));
+      q.sc[r] = *reinterpret_cast<const uint2 *>(blk + 192 + 8 * half);
+    }
+    q.d = *reinterpret_cast<const uint2 *>(a.dsc + dsc_index(n, sb, a.SB));
+  };
+  float x[M][32];
+  auto load_x = [&](int it) {
+    const int sb = sb0 + it * (LANES / 8);
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float4 v = sb < a.SB ? *reinterpret_cast<const float4 *>(a.X + ((int64_t)m * a.SB + sb) * 256 + 128 * half +
+                                                                       16 * c + 64 * (j >> 2) + 4 * (j & 3))
+                                   : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[m][4 * j] = v.x, x[m][4 * j + 1] = v.y, x[m][4 * j + 2] = v.z, x[m][4 * j + 3] = v.w;
+      }
+  };
+  float z[M][4];
+  auto add = [&](const Raw &q) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float d = f16_bits_to_f32((r & 2 ? q.d.y : q.d.x) >> (16 * (r & 1)));
+      const float d0 = d * (float)(int8_t)(q.sc[r].x >> (8 * c)), d1 = d * (float)(int8_t)(q.sc[r].y >> (8 * c));
+      const unsigned l[4] = {q.l[r].x, q.l[r].y, q.l[r].z, q.l[r].w}, h[4] = {q.h[r].x, q.h[r].y, q.h[r].z, q.h[r].w};
+      float s0[M], s1[M];
+#pragma unroll
+      for (int m = 0; m < M; ++m) s0[m] = s1[m] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned hi = h[j] >> (c & 2);  // groups 0, 2 or 1, 3
+        const unsigned q0 = (l[j] & 0x0F0F0F0Fu) | (hi << 4 & 0x30303030u);
+        const unsigned q1 = (l[j] >> 4 & 0x0F0F0F0Fu) | (hi & 0x30303030u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float c0 = (float)(q0 >> (8 * e) & 255u) - 32.f, c1 = (float)(q1 >> (8 * e) & 255u) - 32.f;
+#pragma unroll
+          for (int m = 0; m < M; ++m) {
+            s0[m] = fmaf(x[m][4 * j + e], c0, s0[m]);
+            s1[m] = fmaf(x[m][16 + 4 * j + e], c1, s1[m]);
+          }
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < M; ++m) z[m][r] = fmaf(d0, s0[m], fmaf(d1, s1[m], z[m][r]));
+    }
+  };
+  Sums sum[M];
+#pragma unroll
+  for (int m = 0; m < M; ++m) sum[m] = {LOWEST, 0.f, 0.f};
+  const int first = ((int)blockIdx.x * 4 + wave) * SLOTS + slot;
+  // every lane of a wave runs as many steps as its first slot
+  const int g0 = ((int)blockIdx.x * 4 + wave) * SLOTS;
+  Raw q, next;
+  if (its == 1) load_x(0);
+  load(first, 0, q);
+  for (int g = first, w = g0; w < groups; g += step, w += step) {
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) z[m][r] = 0.f;
+    for (int it = 0; it < its; ++it) {
+      if (its > 1) load_x(it);
+      const bool more = it + 1 < its;
+      load(more ? g : g + step, more ? it + 1 : 0, next);
+      add(q);
+      q = next;
+    }
+    // row r of the four is left in the lanes whose bits 0 and 1 are r
+    const int r = lane & 3, n = 4 * g + r;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const bool b0 = lane & 1, b1 = lane & 2;
+      float u = (b0 ? z[m][1] : z[m][0]) + partner<1>(b0 ? z[m][0] : z[m][1], lane);
+      const float v = (b0 ? z[m][3] : z[m][2]) + partner<1>(b0 ? z[m][2] : z[m][3], lane);
+      u = (b1 ? v : u) + partner<2>(b1 ? u : v, lane);
+      u += partner<4>(u, lane);
+      if constexpr (LANES > 8) u += partner<8>(u, lane);
+      if constexpr (LANES > 16) u += partner<16>(u, lane);
+      if constexpr (LANES > 32) u += partner<32>(u, lane);
+      if (n < a.N && g < groups) {
+        if (a.Z) {
+          if (lane % LANES < 4) a.Z[m * a.stride + n] = u;
+        } else {
+          const float top = fmaxf(sum[m].m, u);
+          sum[m] = moved(sum[m], top);
+          const float d = bounded(u - top), f = exp_of(d);
+          sum[m].s += u != u ? u : f;
+          sum[m].t = fmaf(d, f, sum[m].t);
+          if (a.hit && lane % LANES < 4 && a.targets[m] == n) a.hit[m] = u;
+        }
+      }
+    }
+  }
+  if (a.Z) return;
+#pragma unroll
+  for (int m = 0; m < M; ++m) {
+    if (lane % LANES >= 4) sum[m] = {LOWEST, 0.f, 0.f};  // the same rows again
+    const Sums all = join_threads(sum[m], buf);
+    if (threadIdx.x == 0) a.parts[(int64_t)m * a.n_parts + blockIdx.x] = make_float4(all.m, all.s, all.t, 0.f);
+    __syncthreads();
+  }
+}
+
+}  // namespace
+
+#define HEAD_SIX(M)                                                                                                   \
+  extern "C" __global__ void __launch_bounds__(256) pbx_head_q6k_##M##_8(SixArgs a) { six_body<M, 8>(a); }            \
+  extern "C" __global__ void __launch_bounds__(256) pbx_head_q6k_##M##_16(SixArgs a) { six_body<M, 16>(a); }          \
+  extern "C" __global__ void __launch_bounds__(256) pbx_head_q6k_##M##_32(SixArgs a) { six_body<M, 32>(a); }          \
+  extern "C" __global__ void __launch_bounds__(256) pbx_head_q6k_##M##_64(SixArgs a) { six_body<M, 64>(a); }
+HEAD_SIX(1)
+HEAD_SIX(2)
+HEAD_SIX(3)
+
 // ---- the gradient --------------------------------------------------------------------
 
 // The largest scale of a quantised head: a workgroup's largest magnitude of its share of

@@ -349,8 +349,31 @@ int pbx_gemm_launch(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M6
   return PBX_OK;
 }
 
-bool pbx_gemm_has_head(const pbx_weight *w, int64_t M) {
-  return M > PBX_GEMM_ROWS_M && w->type != PBX_TYPE_F32 && gemm_tag(w->type);
+// Workgroups of the GEMM whose epilogue takes a head's logits: 32 rows, or 128, or 64
+// where those leave out a half-empty 128 of at most eight; by 128 columns.
+static int head_rows(int M) { return M <= 32 ? 32 : (M + 63) / 64 % 2 && M <= 960 ? 64 : 128; }
+
+// Where it is faster than the linear's own kernels and a pass over their logits.  Its
+// time for a tile is that of K (8 us and 9 for each 1,000 columns of 32 rows), since K
+// is not split, so it wants enough tiles (us, it / they):
+// * more than 32 rows: 3000 x 2048 Q8_0 40 rows (24 workgroups) 36 / 28, 130 (72) 38 / 36,
+//   300 (120) 39 / 42; 8000 x 2048 Q4_0 40 rows (63) 33 / 35; 1000 x 512 (8) 16 / 19.
+// * 3 to 32 rows: 16000 x 2048 Q8_0 (125) 8 rows 28 / 24, 32 rows 28 / 40; 24000 x 2048
+//   Q4_0 (188) 3 rows 27 / 25, 8 rows 27 / 38; 128256 x 2048 Q8_0 4 rows 87 / 92, 32 rows
+//   89 / 119; short K from less on: 8000 x 512 Q4_0 (63) 8 rows 12.6 / 13.0, 32 rows 12.9 / 16.6.
+// * one and two rows, which the linear takes one by one at the rate of memory: an F16 head,
+//   whose GEMV is slower (32003 x 2048 one row 28 / 44), and two rows of many
+//   tiles (128256 x 2048 Q8_0 88 / 102, 49152 x 576 Q4_0 15 / 19; Q4_0 of 2048 71 / 59).
+bool pbx_gemm_has_head(const pbx_ctx *c, const pbx_weight *w, int64_t M) {
+  if (w->type == PBX_TYPE_F32 || !gemm_tag(w->type) || M > 65535) return false;
+  const int64_t K = w->K, tiles = (w->N + 127) / 128;
+  if (M > 32) {
+    const int rows = head_rows((int)M);
+    return K <= 1024 || tiles * ((M + rows - 1) / rows) >= c->cu_count / 4 - 4;
+  }
+  if (w->type == PBX_TYPE_F16) return tiles >= 100;
+  if (M >= 3) return K <= 512 ? tiles >= 60 : tiles >= 100 && tiles * M >= 1200;
+  return M == 2 && tiles >= 192 && (K <= 1024 || w->type == PBX_TYPE_Q8_0);
 }
 
 size_t pbx_gemm_head_space(const pbx_weight *w, int M) {
@@ -366,10 +389,10 @@ int pbx_gemm_head(pbx_ctx *c, const pbx_weight *w, const float *dX, int M, bool 
   p.M = M;
   p.Mpad = (M + 127) / 128 * 128;
   p.nwg = ((int)w->N + 127) / 128;
-  // 128-row tiles, but where 64-row tiles leave out a half-empty one of at most eight
-  const bool b64 = (M + 63) / 64 % 2 && M <= 960;
-  p.mtiles = b64 ? (M + 63) / 64 : p.Mpad / 128;
-  p.name = std::string("pbx_gemm_") + gemm_tag(w->type) + (b64 ? "_b64" : "_big") + (e.lse ? "_g" : "_sums");
+  const int rows = head_rows(M);
+  p.mtiles = (M + rows - 1) / rows;
+  p.name = std::string("pbx_gemm_") + gemm_tag(w->type) + (rows == 32 ? "_b32" : rows == 64 ? "_b64" : "_big") +
+           (e.lse ? "_g" : "_sums");
   const GemmSpace sp = gemm_space(p, (int)w->N, (int)w->K);
   void *x16 = space, *x16lo = (char *)space + sp.x16;
   float *inv = (float *)((char *)space + 2 * sp.x16);

@@ -14,6 +14,17 @@ struct BackArgsHost {  // BackArgs in pbx_head.hip
   int M, Mpad, K, B, blocks, rows, KS, add;
 };
 
+struct SixArgsHost {  // SixArgs in pbx_head.hip
+  const void *qs, *dsc;
+  const float *X;
+  int N, SB;
+  const int32_t *targets;
+  void *parts;
+  int n_parts;
+  float *hit, *Z;
+  int64_t stride;
+};
+
 #define HEAD_SHARE 8192          // of pbx_head.hip, too
 #define HEAD_PEAKS 256           // likewise
 #define HEAD_PIECE (64u << 20)   // bytes of a piece's logits at most
@@ -35,6 +46,19 @@ pbx_weight rows_of(const pbx_weight &w, int64_t v0, int64_t n) {
   return v;
 }
 
+// One to three rows of a Q6_K head have a kernel of their own: lanes of a row (eight a
+// superblock, 64 at most) and workgroups, up to three a CU.
+bool six(const pbx_weight *w, int64_t M) { return w->type == PBX_TYPE_Q6_K && M <= 3; }
+int six_lanes(const pbx_weight *w) {
+  int lanes = 8;
+  while (lanes < 64 && lanes < w->K / 32) lanes *= 2;
+  return lanes;
+}
+int six_groups(const pbx_ctx *c, const pbx_weight *w) {
+  const int64_t steps = ((w->N + 3) / 4 * six_lanes(w) + 63) / 64;  // of a wave
+  return (int)std::min<int64_t>(3 * c->cu_count, (steps + 3) / 4);
+}
+
 struct Plan {
   bool fused;      // logits leave the GEMM as sums or as the gradient's factor, not as such
   int64_t piece;   // vocabulary entries of a piece, but for the last
@@ -51,7 +75,7 @@ Plan make_plan(pbx_ctx *c, const pbx_weight *w, int64_t M, bool grad) {
   const int64_t V = w->N;
   p.TT = M > 32 ? 2 : 1;
   p.Mpad = (int)((M + 63) / 64 * 64);
-  p.fused = pbx_gemm_has_head(w, M);
+  p.fused = pbx_gemm_has_head(c, w, M);
   if (p.fused && grad) p.Mpad = (int)((M + 127) / 128 * 128);
   const int64_t row = 4 * (grad ? p.Mpad : M);
   p.piece = std::min<int64_t>((V + 127) / 128 * 128, std::max<int64_t>(128, HEAD_PIECE / row / 128 * 128));
@@ -73,7 +97,8 @@ Plan make_plan(pbx_ctx *c, const pbx_weight *w, int64_t M, bool grad) {
       gemm = std::max(gemm, pbx_linear_space(c, &part, (int)M));
     }
   auto shares = [](int64_t n) { return (int)((n + HEAD_SHARE - 1) / HEAD_SHARE); };
-  p.n_parts = p.fused ? (int)((V + 127) / 128) : (p.n_pieces - 1) * shares(p.piece) + shares(last);
+  if (six(w, M)) gemm = 0;
+  p.n_parts = six(w, M) ? six_groups(c, w) : p.fused ? (int)((V + 127) / 128) : (p.n_pieces - 1) * shares(p.piece) + shares(last);
   p.gemm = take(gemm);
   p.z = take(p.fused ? 0 : (size_t)M * p.piece * 4);
   if (!grad) {
@@ -109,10 +134,21 @@ int check_work(pbx_ctx *c, const char *who, const Plan &p, const void *work, siz
   return PBX_OK;
 }
 
+int launch_six(pbx_ctx *c, const pbx_weight *w, int M, SixArgsHost a) {
+  const std::string name = "pbx_head_q6k_" + std::to_string(M) + "_" + std::to_string(six_lanes(w));
+  hipFunction_t f = pbx_kernel_by_name(c, name);
+  if (!f) return pbx_fail(c, PBX_ELOAD, "pbx_linear_logprobs: kernel %s missing", name.c_str());
+  void *args[] = {&a};
+  return pbx_launch_fn(c, f, name.c_str(), dim3(six_groups(c, w)), dim3(256), args, c->stream);
+}
+
 // Logits of the piece from v0 on, n entries.
 int piece_logits(pbx_ctx *c, const pbx_weight *w, const Plan &p, char *ws, const float *dX, int64_t M, int64_t v0,
                  int64_t n, pbx_weight *rows) {
   *rows = rows_of(*w, v0, n);
+  if (six(w, M))
+    return launch_six(c, rows, (int)M, {rows->qs, rows->d, dX, (int)rows->N, (int)(rows->K / 256), nullptr, nullptr, 0,
+                                        nullptr, (float *)(ws + p.z), rows->N});
   const pbx_workspace space{ws + p.gemm, p.z - p.gemm};
   return pbx_linear_enqueue(c, rows, dX, M, nullptr, (float *)(ws + p.z), c->stream, &space);
 }
@@ -147,7 +183,11 @@ extern "C" int pbx_linear_logprobs_dev(pbx_ctx *c, const pbx_weight *w, const fl
     const pbx_head_epilogue e{dTargets, parts, n_parts, dLogp ? hit : nullptr, nullptr, nullptr, nullptr, 0, 0, (int)w->N};
     if ((rc = pbx_gemm_head(c, w, dX, (int)M, true, ws + p.gemm, e))) return rc;
   }
-  for (int64_t v0 = 0; v0 < w->N && !p.fused; v0 += p.piece) {
+  if (six(w, M) &&
+      (rc = launch_six(c, w, (int)M, {w->qs, w->d, dX, (int)w->N, (int)(w->K / 256), dTargets, parts, n_parts,
+                                      dLogp ? hit : nullptr, nullptr, 0})))
+    return rc;
+  for (int64_t v0 = 0; v0 < w->N && !p.fused && !six(w, M); v0 += p.piece) {
     pbx_weight rows;
     int n = (int)std::min(p.piece, w->N - v0), at = (int)v0;
     if ((rc = piece_logits(c, w, p, ws, dX, M, v0, n, &rows))) return rc;

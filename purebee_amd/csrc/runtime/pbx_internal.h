@@ -208,7 +208,7 @@ int pbx_gemm_make_plan(pbx_ctx *c, const pbx_weight *w, int M, pbx_gemm_plan *p,
 int pbx_gemm_run(pbx_ctx *c, const pbx_weight *w, const pbx_gemm_plan &p, const void *x16,
                  const void *x16lo, const float *inv, const float *dBias, float *out,
                  int accumulate, hipStream_t stream);
-// The GEMM of M > 32 rows of a quantised or F16 head whose logits go into sums of each
+// The GEMM of M rows of a quantised or F16 head whose logits go into sums of each
 // 128 columns (lse == nullptr) or the gradient's first factor (pbx_head.cpp).
 // prep: X16, X16lo and inv (of pbx_head_space bytes) are filled from dX first.
 struct pbx_head_epilogue {  // HeadArgs in pbx_gemm.hip
@@ -220,7 +220,7 @@ struct pbx_head_epilogue {  // HeadArgs in pbx_gemm.hip
   void *hi, *lo;
   int Mpad, v0, vocab;
 };
-bool pbx_gemm_has_head(const pbx_weight *w, int64_t M);
+bool pbx_gemm_has_head(const pbx_ctx *c, const pbx_weight *w, int64_t M);
 size_t pbx_gemm_head_space(const pbx_weight *w, int M);
 int pbx_gemm_head(pbx_ctx *c, const pbx_weight *w, const float *dX, int M, bool prep, void *space,
                   const pbx_head_epilogue &e);

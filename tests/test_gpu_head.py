@@ -104,6 +104,24 @@ def test_scores_and_gradient(ctx, kind, M, V, K):
     head.free()
 
 
+# few rows of large vocabularies, where the GEMM's epilogue takes the logits
+WIDE = [(1, 13001, 32), (2, 24705, 64), (3, 7999, 32), (17, 8001, 288), (32, 16005, 64), (5, 25000, 1056), (31, 7777, 512)]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("M,V,K", WIDE)
+def test_few_rows_of_large_vocabularies(ctx, kind, M, V, K):
+    test_scores_and_gradient(ctx, kind, M, V, K)
+
+
+@pytest.mark.parametrize("M", [1, 2, 3])
+@pytest.mark.parametrize("V,K", [(1, 256), (3, 512), (4097, 768), (999, 1024), (514, 1280), (131, 2048), (70, 2304),
+                                 (13, 4096), (37, 16384), (13000, 256)])
+def test_few_rows_of_q6_k(ctx, M, V, K):
+    """Superblocks that fill an eighth of a wave to eight passes of it."""
+    test_scores_and_gradient(ctx, "q6_k", M, V, K)
+
+
 @pytest.mark.parametrize("kind", ["q8_0", "f16", "f32", "q6_k"])
 def test_many_pieces(ctx, kind):
     """A vocabulary of several pieces and a ragged last one."""
