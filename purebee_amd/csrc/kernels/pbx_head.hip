@@ -162,22 +162,27 @@ struct SixArgs {
   int64_t stride;
 };
 
-// Logits of M rows, 24-bit activations, f32 sums.  A lane takes 16 bytes of low nibbles:
+// Logits of M rows.  A lane takes 16 bytes of low nibbles:
 // the 16 codes of one 32-code group of half a superblock and the 16 of the group two
 // further on, whose high bits lie in 16 bytes that it shares with one other lane; eight lanes a
 // superblock, so a row of 2,048 is one wave's (of the plain GEMV a lane takes a 32-code
 // block, 64 bytes for 24 of its own: 128,256 x 2,048 70 us).  A step is four rows
 // (whose superblock scales are one load) for each group of LANES lanes, the next step's
 // in flight; the lanes' sums of four rows are added in 7 steps instead of 24, halving what
-// each lane holds.  Bound by bytes.
-template <int M, int LANES>
+// each lane holds.
+// Up to 2,048 columns (one pass of the lanes) the lane keeps its activations as integers
+// of up to 8,355,711 in three signed bytes (0.5 / 2^22 of the row's largest is what they
+// may be off), so that v_dot4 sums four products with codes exactly; 32 times the bytes'
+// sums, for codes less 32, is taken off as an integer.  Longer rows: f32.
+// 128,256 x 2,048: 56 us with f32 products, 207 vector instructions a row (43 us of them).
+template <int M, int LANES, bool WHOLE>
 __device__ __forceinline__ void six_body(const SixArgs &a) {
   constexpr int SLOTS = 64 / LANES;
   __shared__ float buf[4][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int slot = lane / LANES, sb0 = lane % LANES / 8, c = lane & 3, half = lane >> 2 & 1;
   const int step = (int)gridDim.x * 4 * SLOTS, groups = (a.N + 3) / 4;
-  const int its = (a.SB + LANES / 8 - 1) / (LANES / 8);
+  const int its = WHOLE ? 1 : (a.SB + LANES / 8 - 1) / (LANES / 8);
   struct Raw {
     uint4 l[4], h[4];
     uint2 sc[4], d;
@@ -194,7 +199,58 @@ __device__ __forceinline__ void six_body(const SixArgs &a) {
     }
     q.d = *reinterpret_cast<const uint2 *>(a.dsc + dsc_index(n, sb, a.SB));
   };
-  float x[M][32];
+  float x[M][WHOLE ? 1 : 32];
+  // [byte 0 .. 2 of an activation][group][4 activations each dword], and 32 times their sums
+  int limb[M][3][8], offset[M][2][3];
+  float unit[M];
+  auto split_x = [&]() {
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      float v[32], most = 0.f;
+      bool odd = false;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float4 t = sb0 < a.SB ? *reinterpret_cast<const float4 *>(a.X + ((int64_t)m * a.SB + sb0) * 256 + 128 * half +
+                                                                        16 * c + 64 * (j >> 2) + 4 * (j & 3))
+                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[4 * j] = t.x, v[4 * j + 1] = t.y, v[4 * j + 2] = t.z, v[4 * j + 3] = t.w;
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        most = fmaxf(most, fabsf(v[j]));
+        odd = odd || !(fabsf(v[j]) < INFINITY);
+      }
+      most = wave_max(most);  // (slots hold the same row)
+      int e = 0;
+      if (most > 0.f && most < INFINITY) frexpf(most, &e);
+      e = max(e, -100);
+      float up = ldexpf(1.f, 23 - e);
+      if (most * up > 8355711.f) up *= 0.5f;
+      // a row with a NaN or an infinity has no logits
+      unit[m] = __ballot(odd) ? __uint_as_float(0x7fc00000u) : 1.f / up;
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int l = 0; l < 3; ++l) offset[m][g][l] = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        unsigned w[3] = {0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int q = (int)rintf(fminf(fmaxf(v[4 * j + i] * up, -8355711.f), 8355711.f));
+          const int q0 = (int)(int8_t)q, q1 = (int)(int8_t)((q - q0) >> 8), q2 = (q - q0 - 256 * q1) >> 16;
+          w[0] |= (unsigned)(q0 & 255) << (8 * i);
+          w[1] |= (unsigned)(q1 & 255) << (8 * i);
+          w[2] |= (unsigned)(q2 & 255) << (8 * i);
+          offset[m][j >> 2][0] += 32 * q0;
+          offset[m][j >> 2][1] += 32 * q1;
+          offset[m][j >> 2][2] += 32 * q2;
+        }
+#pragma unroll
+        for (int l = 0; l < 3; ++l) limb[m][l][j] = (int)w[l];
+      }
+    }
+  };
   auto load_x = [&](int it) {
     const int sb = sb0 + it * (LANES / 8);
 #pragma unroll
@@ -204,7 +260,7 @@ __device__ __forceinline__ void six_body(const SixArgs &a) {
         const float4 v = sb < a.SB ? *reinterpret_cast<const float4 *>(a.X + ((int64_t)m * a.SB + sb) * 256 + 128 * half +
                                                                        16 * c + 64 * (j >> 2) + 4 * (j & 3))
                                    : make_float4(0.f, 0.f, 0.f, 0.f);
-        x[m][4 * j] = v.x, x[m][4 * j + 1] = v.y, x[m][4 * j + 2] = v.z, x[m][4 * j + 3] = v.w;
+        if constexpr (!WHOLE) x[m][4 * j] = v.x, x[m][4 * j + 1] = v.y, x[m][4 * j + 2] = v.z, x[m][4 * j + 3] = v.w;
       }
   };
   float z[M][4];
@@ -214,6 +270,35 @@ __device__ __forceinline__ void six_body(const SixArgs &a) {
       const float d = f16_bits_to_f32((r & 2 ? q.d.y : q.d.x) >> (16 * (r & 1)));
       const float d0 = d * (float)(int8_t)(q.sc[r].x >> (8 * c)), d1 = d * (float)(int8_t)(q.sc[r].y >> (8 * c));
       const unsigned l[4] = {q.l[r].x, q.l[r].y, q.l[r].z, q.l[r].w}, h[4] = {q.h[r].x, q.h[r].y, q.h[r].z, q.h[r].w};
+      if constexpr (WHOLE) {
+        int t[M][2][3];
+#pragma unroll
+        for (int m = 0; m < M; ++m)
+#pragma unroll
+          for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int k = 0; k < 3; ++k) t[m][g][k] = -offset[m][g][k];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const unsigned hi = h[j] >> (c & 2);  // groups 0, 2 or 1, 3
+          const int q0 = (int)((l[j] & 0x0F0F0F0Fu) | (hi << 4 & 0x30303030u));
+          const int q1 = (int)((l[j] >> 4 & 0x0F0F0F0Fu) | (hi & 0x30303030u));
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+              t[m][0][k] = __builtin_amdgcn_sdot4(limb[m][k][j], q0, t[m][0][k], false);
+              t[m][1][k] = __builtin_amdgcn_sdot4(limb[m][k][4 + j], q1, t[m][1][k], false);
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          const float s0 = fmaf((float)t[m][0][2], 65536.f, fmaf((float)t[m][0][1], 256.f, (float)t[m][0][0]));
+          const float s1 = fmaf((float)t[m][1][2], 65536.f, fmaf((float)t[m][1][1], 256.f, (float)t[m][1][0]));
+          z[m][r] = fmaf(d0, s0, fmaf(d1, s1, z[m][r]));
+        }
+        continue;
+      }
       float s0[M], s1[M];
 #pragma unroll
       for (int m = 0; m < M; ++m) s0[m] = s1[m] = 0.f;
@@ -227,8 +312,8 @@ __device__ __forceinline__ void six_body(const SixArgs &a) {
           const float c0 = (float)(q0 >> (8 * e) & 255u) - 32.f, c1 = (float)(q1 >> (8 * e) & 255u) - 32.f;
 #pragma unroll
           for (int m = 0; m < M; ++m) {
-            s0[m] = fmaf(x[m][4 * j + e], c0, s0[m]);
-            s1[m] = fmaf(x[m][16 + 4 * j + e], c1, s1[m]);
+            s0[m] = fmaf(x[m][WHOLE ? 0 : 4 * j + e], c0, s0[m]);
+            s1[m] = fmaf(x[m][WHOLE ? 0 : 16 + 4 * j + e], c1, s1[m]);
           }
         }
       }
@@ -243,15 +328,15 @@ __device__ __forceinline__ void six_body(const SixArgs &a) {
   // every lane of a wave runs as many steps as its first slot
   const int g0 = ((int)blockIdx.x * 4 + wave) * SLOTS;
   Raw q, next;
-  if (its == 1) load_x(0);
   load(first, 0, q);
+  if constexpr (WHOLE) split_x();
   for (int g = first, w = g0; w < groups; g += step, w += step) {
 #pragma unroll
     for (int m = 0; m < M; ++m)
 #pragma unroll
       for (int r = 0; r < 4; ++r) z[m][r] = 0.f;
     for (int it = 0; it < its; ++it) {
-      if (its > 1) load_x(it);
+      if constexpr (!WHOLE) load_x(it);
       const bool more = it + 1 < its;
       load(more ? g : g + step, more ? it + 1 : 0, next);
       add(q);
@@ -266,6 +351,7 @@ __device__ __forceinline__ void six_body(const SixArgs &a) {
       const float v = (b0 ? z[m][3] : z[m][2]) + partner<1>(b0 ? z[m][2] : z[m][3], lane);
       u = (b1 ? v : u) + partner<2>(b1 ? u : v, lane);
       u += partner<4>(u, lane);
+      if constexpr (WHOLE) u *= unit[m];
       if constexpr (LANES > 8) u += partner<8>(u, lane);
       if constexpr (LANES > 16) u += partner<16>(u, lane);
       if constexpr (LANES > 32) u += partner<32>(u, lane);
@@ -295,11 +381,14 @@ __device__ __forceinline__ void six_body(const SixArgs &a) {
 
 }  // namespace
 
-#define HEAD_SIX(M)                                                                                                   \
-  extern "C" __global__ void __launch_bounds__(256) pbx_head_q6k_##M##_8(SixArgs a) { six_body<M, 8>(a); }            \
-  extern "C" __global__ void __launch_bounds__(256) pbx_head_q6k_##M##_16(SixArgs a) { six_body<M, 16>(a); }          \
-  extern "C" __global__ void __launch_bounds__(256) pbx_head_q6k_##M##_32(SixArgs a) { six_body<M, 32>(a); }          \
-  extern "C" __global__ void __launch_bounds__(256) pbx_head_q6k_##M##_64(SixArgs a) { six_body<M, 64>(a); }
+#define HEAD_SIX_KERNEL(M, TAG, LANES, WHOLE)                                                                        \
+  extern "C" __global__ void __launch_bounds__(256) pbx_head_q6k_##M##_##TAG(SixArgs a) { six_body<M, LANES, WHOLE>(a); }
+#define HEAD_SIX(M)                  \
+  HEAD_SIX_KERNEL(M, 8, 8, true)     \
+  HEAD_SIX_KERNEL(M, 16, 16, true)   \
+  HEAD_SIX_KERNEL(M, 32, 32, true)   \
+  HEAD_SIX_KERNEL(M, 64, 64, true)   \
+  HEAD_SIX_KERNEL(M, long, 64, false)
 HEAD_SIX(1)
 HEAD_SIX(2)
 HEAD_SIX(3)

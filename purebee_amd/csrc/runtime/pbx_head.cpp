@@ -135,7 +135,7 @@ int check_work(pbx_ctx *c, const char *who, const Plan &p, const void *work, siz
 }
 
 int launch_six(pbx_ctx *c, const pbx_weight *w, int M, SixArgsHost a) {
-  const std::string name = "pbx_head_q6k_" + std::to_string(M) + "_" + std::to_string(six_lanes(w));
+  const std::string name = "pbx_head_q6k_" + std::to_string(M) + "_" + (w->K > 2048 ? "long" : std::to_string(six_lanes(w)));
   hipFunction_t f = pbx_kernel_by_name(c, name);
   if (!f) return pbx_fail(c, PBX_ELOAD, "pbx_linear_logprobs: kernel %s missing", name.c_str());
   void *args[] = {&a};
