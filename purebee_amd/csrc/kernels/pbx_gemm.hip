@@ -29,7 +29,7 @@
 // decode path's logits, against a 2e-3 tolerance.  Accumulation is fp32;
 // the power of two is undone exactly in the epilogue.
 
-#include "pbx_gemv_impl.h"
+#include "pbx_head_peaks.h"
 
 using namespace pbx;
 
@@ -1403,8 +1403,7 @@ __device__ __forceinline__ void rms_row(float4 (&v)[PREP_R], const float *w, int
   }
 }
 
-extern "C" __global__ void __launch_bounds__(256)
-pbx_gemm_prep_x(const float *X, _Float16 *X16, _Float16 *X16lo, float *inv, int M, int K) {
+__device__ __forceinline__ void prep_x(const float *X, _Float16 *X16, _Float16 *X16lo, float *inv, int M, int K) {
   __shared__ float red[4];
   const int m = blockIdx.x, K4 = K / 4;  // K is a multiple of 32, at most 1024 * PREP_R
   _Float16 *dst = X16 + (size_t)m * 32, *lo = X16lo + (size_t)m * 32;
@@ -1437,6 +1436,21 @@ pbx_gemm_prep_x(const float *X, _Float16 *X16, _Float16 *X16lo, float *inv, int 
   float4 v[PREP_R];
   load_row(X + (size_t)m * K, K4, v);
   prep_split_row(v, K4, dst, lo, inv + m, red);
+}
+
+extern "C" __global__ void __launch_bounds__(256)
+pbx_gemm_prep_x(const float *X, _Float16 *X16, _Float16 *X16lo, float *inv, int M, int K) {
+  prep_x(X, X16, X16lo, inv, M, K);
+}
+
+// The same, and beside it (blockIdx.y > 0, at least HEAD_PEAKS workgroups) a head's
+// largest scales for its gradient.
+extern "C" __global__ void __launch_bounds__(256)
+pbx_gemm_prep_head(const float *X, _Float16 *X16, _Float16 *X16lo, float *inv, int M, int K, const uint16_t *scales,
+                   int64_t n8, unsigned *peaks) {
+  if (blockIdx.y == 0) return prep_x(X, X16, X16lo, inv, M, K);
+  const int part = (blockIdx.y - 1) * gridDim.x + blockIdx.x;
+  if (part < HEAD_PEAKS) head_peaks(scales, n8, peaks, part);
 }
 
 // X16 rows of RMSNorm(x) * w (K <= 1024 * PREP_R).

@@ -7,7 +7,7 @@
 //   S = S1 e^(m1 - m) + S2 e^(m2 - m),  T = sum (Ti + (mi - m) Si) e^(mi - m);
 // and d log p_t / dx = W_t - sum_v p_v W_v = sum_v G_v W_v with G = (v == t) - e^(l - lse).
 
-#include "pbx_gemv_impl.h"
+#include "pbx_head_peaks.h"
 
 using namespace pbx;
 
@@ -395,26 +395,6 @@ HEAD_SIX(3)
 
 // ---- the gradient --------------------------------------------------------------------
 
-// The largest scale of a quantised head: a workgroup's largest magnitude of its share of
-// the plane's halves, as bits.
-extern "C" __global__ void __launch_bounds__(256)
-pbx_head_scale(const uint16_t *plane, int64_t n8, unsigned *peaks) {  // n8 groups of 8 halves
-  __shared__ unsigned red[4];
-  unsigned m = 0;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n8; i += (int64_t)gridDim.x * 256) {
-    const uint4 v = reinterpret_cast<const uint4 *>(plane)[i];
-    const unsigned w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) m = max(m, max(w[e] & 0x7fffu, (w[e] >> 16) & 0x7fffu));
-  }
-#pragma unroll
-  for (int off = 32; off >= 1; off /= 2) m = max(m, (unsigned)__shfl_xor((int)m, off, 64));
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) peaks[blockIdx.x] = max(max(red[0], red[1]), max(red[2], red[3]));
-}
-
-#define HEAD_PEAKS 256  // workgroups of pbx_head_scale
 
 namespace {
 
@@ -436,10 +416,15 @@ template <int TYPE> struct HeadTarget { static constexpr int value = TYPE == PBX
 
 // G of a piece as fp16 pairs times 2^15, [n / 32][Mpad][32]: workgroup (block of 32
 // vocabulary entries, 64 rows); zeros past the vocabulary, the rows, and in rows
-// without a target.
+// without a target.  Workgroups past the blocks (HEAD_PEAKS of them where there are any)
+// look for the head's largest scales.
 extern "C" __global__ void __launch_bounds__(256)
 pbx_head_g(const float *Z, int64_t stride, int n, int v0, const float *lse, const int *targets, int vocab, int M,
-           int Mpad, _Float16 *hi, _Float16 *lo) {
+           int Mpad, _Float16 *hi, _Float16 *lo, int blocks, const uint16_t *scales, int64_t n8, unsigned *peaks) {
+  if ((int)blockIdx.x >= blocks) {
+    if (blockIdx.y == 0) head_peaks(scales, n8, peaks, blockIdx.x - blocks);
+    return;
+  }
   const int row = blockIdx.y * 64 + threadIdx.x / 4, v = blockIdx.x * 32 + 8 * (threadIdx.x % 4);
   if (row >= Mpad) return;
   half8 H = {}, L = {};

@@ -1,0 +1,28 @@
+// pbx_head_peaks.h -- the largest scale of a quantised head, which its gradient's products
+// are scaled by (pbx_head.hip, pbx_gemm.hip).
+#ifndef PBX_HEAD_PEAKS_H
+#define PBX_HEAD_PEAKS_H
+
+#include "pbx_gemv_impl.h"
+
+#define HEAD_PEAKS 256  // shares of the plane (pbx_head.cpp, too)
+
+// Share `part` of a plane of halves (n8 groups of 8): its largest magnitude's bits.
+// A workgroup of 256 threads.
+__device__ __forceinline__ void head_peaks(const uint16_t *plane, int64_t n8, unsigned *peaks, int part) {
+  __shared__ unsigned red[4];
+  unsigned m = 0;
+  for (int64_t i = (int64_t)part * 256 + threadIdx.x; i < n8; i += HEAD_PEAKS * 256) {
+    const uint4 v = reinterpret_cast<const uint4 *>(plane)[i];
+    const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m = max(m, max(w[e] & 0x7fffu, (w[e] >> 16) & 0x7fffu));
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off /= 2) m = max(m, (unsigned)__shfl_xor((int)m, off, 64));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) peaks[part] = max(max(red[0], red[1]), max(red[2], red[3]));
+}
+
+#endif

@@ -384,7 +384,7 @@ size_t pbx_gemm_head_space(const pbx_weight *w, int M) {
 }
 
 int pbx_gemm_head(pbx_ctx *c, const pbx_weight *w, const float *dX, int M, bool prep, void *space,
-                  const pbx_head_epilogue &e) {
+                  const pbx_head_epilogue &e, const pbx_head_scales &scales) {
   pbx_gemm_plan p;
   p.M = M;
   p.Mpad = (M + 127) / 128 * 128;
@@ -396,13 +396,15 @@ int pbx_gemm_head(pbx_ctx *c, const pbx_weight *w, const float *dX, int M, bool 
   const GemmSpace sp = gemm_space(p, (int)w->N, (int)w->K);
   void *x16 = space, *x16lo = (char *)space + sp.x16;
   float *inv = (float *)((char *)space + 2 * sp.x16);
-  hipFunction_t f = pbx_kernel_by_name(c, p.name), fprep = pbx_kernel_by_name(c, "pbx_gemm_prep_x");
+  hipFunction_t f = pbx_kernel_by_name(c, p.name), fprep = pbx_kernel_by_name(c, "pbx_gemm_prep_head");
   if (!f || !fprep) return pbx_fail(c, PBX_ELOAD, "pbx_gemm: kernel %s missing", p.name.c_str());
   int rc;
   if (prep) {
     int m = M, k = (int)w->K;
-    void *args[] = {(void *)&dX, &x16, &x16lo, &inv, &m, &k};
-    if ((rc = pbx_launch_fn(c, fprep, "pbx_gemm_prep_x", dim3(p.Mpad), dim3(256), args, c->stream))) return rc;
+    pbx_head_scales sc = scales;
+    void *args[] = {(void *)&dX, &x16, &x16lo, &inv, &m, &k, &sc.scales, &sc.n8, &sc.peaks};
+    const dim3 grid(p.Mpad, sc.peaks ? 1 + (PBX_HEAD_PEAKS + p.Mpad - 1) / p.Mpad : 1);
+    if ((rc = pbx_launch_fn(c, fprep, "pbx_gemm_prep_head", grid, dim3(256), args, c->stream))) return rc;
   }
   GemmArgsHost g{w->qs, w->d, x16, x16lo, inv, nullptr, nullptr,
                  M, (int)w->N, (int)w->Npad, (int)w->B, 1, 0, w->m, p.Mpad};

@@ -26,7 +26,6 @@ struct SixArgsHost {  // SixArgs in pbx_head.hip
 };
 
 #define HEAD_SHARE 8192          // of pbx_head.hip, too
-#define HEAD_PEAKS 256           // likewise
 #define HEAD_PIECE (64u << 20)   // bytes of a piece's logits at most
 
 // The head's rows from v0 on (a multiple of 128), n of them.
@@ -110,7 +109,7 @@ Plan make_plan(pbx_ctx *c, const pbx_weight *w, int64_t M, bool grad) {
     const int waves = w->type == PBX_TYPE_F32 ? 1 : 4;
     p.KS = (int)std::max<int64_t>(1, std::min<int64_t>(8 / waves * c->cu_count / tiles, p.piece / (32 * waves)));
     p.g = take((size_t)p.Mpad * p.piece * 4);
-    p.peaks = take(HEAD_PEAKS * 4);
+    p.peaks = take(PBX_HEAD_PEAKS * 4);
     p.part = take((size_t)p.KS * M * w->K * 4);
   }
   p.bytes = at;
@@ -229,11 +228,9 @@ extern "C" int pbx_linear_logprobs_grad_dev(pbx_ctx *c, const pbx_weight *w, con
   char *ws = (char *)work;
   float *z = (float *)(ws + p.z), *part = (float *)(ws + p.part);
   void *peaks = ws + p.peaks;
-  if (w->d) {
-    int64_t n8 = w->Npad * (w->type == PBX_TYPE_Q6_K ? w->K / 256 : w->B) / 8 * (w->m ? 2 : 1);
-    void *args[] = {(void *)&w->d, &n8, &peaks};
-    if ((rc = pbx_launch(c, PBX_K_HEAD_SCALE, dim3(HEAD_PEAKS), dim3(256), args))) return rc;
-  }
+  pbx_head_scales scales{};
+  if (w->d)
+    scales = {w->d, w->Npad * (w->type == PBX_TYPE_Q6_K ? w->K / 256 : w->B) / 8 * (w->m ? 2 : 1), peaks};
   int m = (int)M, k = (int)w->K, vocab = (int)w->N, Mpad = p.Mpad, KS = p.KS;
   for (int64_t v0 = 0; v0 < w->N; v0 += p.piece) {
     pbx_weight rows;
@@ -246,13 +243,15 @@ extern "C" int pbx_linear_logprobs_grad_dev(pbx_ctx *c, const pbx_weight *w, con
       rows = rows_of(*w, v0, n);
       rows.N = n;
       const pbx_head_epilogue e{dTargets, nullptr, 0, nullptr, dLse, hi, lo, Mpad, at, vocab};
-      rc = pbx_gemm_head(c, &rows, dX, m, v0 == 0, ws + p.gemm, e);
+      rc = pbx_gemm_head(c, &rows, dX, m, v0 == 0, ws + p.gemm, e, scales);
     } else if (f32) {
       void *args[] = {&z, &stride, &n, &at, (void *)&dLse, (void *)&dTargets, &vocab, &m, &Mpad, &hi};
       rc = pbx_launch(c, PBX_K_HEAD_G32, dim3(blocks, Mpad / 64), dim3(256), args);
     } else {
-      void *args[] = {&z, &stride, &n, &at, (void *)&dLse, (void *)&dTargets, &vocab, &m, &Mpad, &hi, &lo};
-      rc = pbx_launch(c, PBX_K_HEAD_G, dim3(blocks, Mpad / 64), dim3(256), args);
+      int here = blocks;
+      void *args[] = {&z, &stride, &n, &at, (void *)&dLse, (void *)&dTargets, &vocab, &m, &Mpad, &hi, &lo,
+                      &here, &scales.scales, &scales.n8, &peaks};
+      rc = pbx_launch(c, PBX_K_HEAD_G, dim3(blocks + (w->d && !v0 ? PBX_HEAD_PEAKS : 0), Mpad / 64), dim3(256), args);
     }
     if (rc) return rc;
     BackArgsHost b{rows.qs, rows.d, rows.m, hi, lo, hi, peaks, part, m, Mpad, k, (int)w->B, blocks, (int)rows.Npad, KS,

@@ -18,7 +18,6 @@
   X(PBX_K_KV_ROPE_TABLE, "pbx_kv_rope_table")                \
   X(PBX_K_HEAD_STATS, "pbx_head_stats")                      \
   X(PBX_K_HEAD_JOIN, "pbx_head_join")                        \
-  X(PBX_K_HEAD_SCALE, "pbx_head_scale")                      \
   X(PBX_K_HEAD_G, "pbx_head_g")                              \
   X(PBX_K_HEAD_G32, "pbx_head_g32")                          \
   X(PBX_K_HEAD_REDUCE, "pbx_head_reduce")                    \
@@ -210,7 +209,14 @@ int pbx_gemm_run(pbx_ctx *c, const pbx_weight *w, const pbx_gemm_plan &p, const 
                  int accumulate, hipStream_t stream);
 // The GEMM of M rows of a quantised or F16 head whose logits go into sums of each
 // 128 columns (lse == nullptr) or the gradient's first factor (pbx_head.cpp).
-// prep: X16, X16lo and inv (of pbx_head_space bytes) are filled from dX first.
+// prep: X16, X16lo and inv (in space, of pbx_gemm_head_space bytes) are filled from dX
+// first, and peaks (if not NULL) from the n8 groups of 8 halves at scales.
+struct pbx_head_scales {
+  const void *scales;
+  int64_t n8;
+  void *peaks;
+};
+#define PBX_HEAD_PEAKS 256
 struct pbx_head_epilogue {  // HeadArgs in pbx_gemm.hip
   const int32_t *targets;
   void *parts;
@@ -223,7 +229,7 @@ struct pbx_head_epilogue {  // HeadArgs in pbx_gemm.hip
 bool pbx_gemm_has_head(const pbx_ctx *c, const pbx_weight *w, int64_t M);
 size_t pbx_gemm_head_space(const pbx_weight *w, int M);
 int pbx_gemm_head(pbx_ctx *c, const pbx_weight *w, const float *dX, int M, bool prep, void *space,
-                  const pbx_head_epilogue &e);
+                  const pbx_head_epilogue &e, const pbx_head_scales &scales = {});
 int pbx_gemm_enqueue(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M,
                      const float *dBias, float *dY, hipStream_t stream,
                      const pbx_workspace *ws = nullptr);
