@@ -480,6 +480,8 @@ struct BackArgs {
 
 namespace {
 
+// 2^e, -126 <= e <= 127.
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 __device__ __forceinline__ half2t as_half2(unsigned x) { return __builtin_bit_cast(half2t, x); }
 // Byte i of x and of y, as two halves u * 2^-24 (the bits of a half of exponent 0).
 __device__ __forceinline__ unsigned byte_pair(unsigned x, unsigned y, int i) {
@@ -504,6 +506,8 @@ struct BackRaw {
   half8 Ah[TT], Al[TT];
 };
 
+#define BACK_DEPTH(TYPE, TT) ((TYPE) == PBX_Q6K || (TT) == 2 ? 2 : 4)
+
 // Workgroup = 32 TT rows of G, 128 columns of the head and a share of its entries, whose
 // blocks four waves take in turn; their sums meet in LDS.  A step is 16 entries: a lane
 // loads 4 columns (as they lie in a row's bytes) of 8 rows, so that the operands, 8
@@ -515,7 +519,9 @@ __device__ __forceinline__ void back_body(const BackArgs &a) {
   const int lane = threadIdx.x & 63, lr = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int k0 = blockIdx.x * 128, m0 = blockIdx.y * (32 * TT);
-  const int b0 = (int)((int64_t)a.blocks * blockIdx.z / a.KS), b1 = (int)((int64_t)a.blocks * (blockIdx.z + 1) / a.KS);
+  // (fewer than 2^14 blocks and 2^12 shares)
+  const int b0 = (int)((unsigned)a.blocks * blockIdx.z / (unsigned)a.KS);
+  const int b1 = (int)((unsigned)a.blocks * (blockIdx.z + 1) / (unsigned)a.KS);
   constexpr bool NIB = TYPE == PBX_Q4 || TYPE == PBX_Q41;
   const floatx16 zero = {};
   floatx16 acc[TT][4];
@@ -523,71 +529,79 @@ __device__ __forceinline__ void back_body(const BackArgs &a) {
   for (int t = 0; t < TT; ++t)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[t][i] = zero;
-  const int shift = TYPE == PBX_F16 ? 0 : head_shift(a.peaks, HeadTarget<TYPE>::value);
-  // codes enter as u 2^-9, so their scales take 2^9 more; by two factors, either of
-  // which a half holds
-  const int both = shift + 9, s1 = min(15, max(-14, both));
-  const _Float16 f1 = (_Float16)ldexpf(1.f, s1), f2 = (_Float16)ldexpf(1.f, both - s1);
-  const float fs = ldexpf(1.f, shift);
   // past the row's end columns repeat the last ones (and are not stored)
   const int kc = min(k0 + 4 * lr, a.K - 4), kb = min((k0 >> 5) + (lr >> 3), a.B - 1);
   const int SB = a.B >> 3, sb = min(k0 >> 8, SB - 1), hf = (k0 >> 7) & 1;
   // a row's bytes, and the lane's first byte in the rows 8 h on
-  const size_t row = TYPE == PBX_F16 ? (size_t)a.K * 2 : TYPE == PBX_Q8 ? a.K : TYPE == PBX_Q6K ? (size_t)SB * PBX_Q6K_BYTES
-                                                                                           : (size_t)a.B * 16;
-  const size_t woff = 8 * h * row + (TYPE == PBX_F16   ? 2 * kc
-                                     : TYPE == PBX_Q8  ? kc
-                                     : TYPE == PBX_Q6K ? sb * PBX_Q6K_BYTES
-                                                       : kb * 16 + 2 * (lr & 7));
-  const int scols = TYPE == PBX_Q6K ? SB : a.B;                      // scales of a row
-  const size_t doff = ((size_t)2 * h * scols + (TYPE == PBX_Q6K ? sb : kb)) * 8;
-  const size_t aoff = (size_t)(m0 + lr) * 64 + 16 * h;
-  // rows of the piece reach past its last block (they are padded to 64), so no step reads
-  // beyond them
-  auto load = [&](int step, BackRaw<TYPE, TT> &q) {
-    const uint8_t *w = a.qs + (size_t)step * 16 * row;
-    const uint8_t *d = reinterpret_cast<const uint8_t *>(a.dsc) + (size_t)step * 4 * scols * 8;
-    const uint8_t *mn = reinterpret_cast<const uint8_t *>(a.msc) + (size_t)step * 4 * scols * 8;
+  const unsigned row = TYPE == PBX_F16   ? a.K * 2
+                       : TYPE == PBX_Q8  ? a.K
+                       : TYPE == PBX_Q6K ? SB * PBX_Q6K_BYTES
+                                         : a.B * 16;
+  const unsigned woff = 8 * h * row + (TYPE == PBX_F16   ? 2 * kc
+                                       : TYPE == PBX_Q8  ? kc
+                                       : TYPE == PBX_Q6K ? sb * PBX_Q6K_BYTES + 64 * hf
+                                                         : kb * 16 + 2 * (lr & 7));
+  const unsigned srow = 8 * (TYPE == PBX_Q6K ? SB : a.B);  // bytes of the scales of four rows
+  const unsigned doff = 2 * h * srow + (TYPE == PBX_Q6K ? sb : kb) * 8;
+  const unsigned aoff = (m0 + lr) * 64 + 16 * h, astep = a.Mpad * 64;
+  // Buffers from the share's first block on: a load's address is a buffer's, a scalar
+  // and a lane's offset, with no vector arithmetic; the host sees to it that a share is
+  // under 2 GB.  The rows of a piece reach past its last block (they are padded to 64),
+  // so no step reads beyond them.
+  const int64_t shared_rows = (int64_t)(b1 - b0) * 32;
+  auto buffer = [](const void *p, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, (int)bytes, 0x00020000);
+  };
+  const auto wbuf = buffer(a.qs + (int64_t)b0 * 32 * row, shared_rows * row);
+  const auto dbuf = buffer(TYPE == PBX_F16 ? (const uint8_t *)a.hi : reinterpret_cast<const uint8_t *>(a.dsc) + (int64_t)b0 * 8 * srow,
+                           TYPE == PBX_F16 ? 0 : shared_rows / 4 * srow);
+  const auto mbuf = buffer(TYPE == PBX_Q41 ? reinterpret_cast<const uint8_t *>(a.msc) + (int64_t)b0 * 8 * srow : (const uint8_t *)a.hi,
+                           TYPE == PBX_Q41 ? shared_rows / 4 * srow : 0);
+  const auto hbuf = buffer(reinterpret_cast<const uint8_t *>(a.hi) + (int64_t)b0 * astep, (int64_t)(b1 - b0) * astep);
+  const auto lbuf = buffer(reinterpret_cast<const uint8_t *>(a.lo) + (int64_t)b0 * astep, (int64_t)(b1 - b0) * astep);
+  auto load = [&](int step, BackRaw<TYPE, TT> &q) {  // (step: from the share's first block on)
+    const unsigned w = step * 16 * row, d = step * 4 * srow;
     if constexpr (TYPE == PBX_Q6K) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const uint8_t *blk = w + e * row + woff;
-        q.w[3 * e] = blk[64 * hf + lr];
-        q.w[3 * e + 1] = blk[64 * hf + 32 + lr];
-        q.w[3 * e + 2] = blk[128 + 32 * hf + lr];
-        q.d[e] = *reinterpret_cast<const uint2 *>(blk + 192 + 8 * hf);
-        q.ds[e] = *reinterpret_cast<const uint16_t *>(d + (size_t)(e >> 2) * scols * 8 + doff + 2 * (e & 3));
+        const unsigned s = w + e * row;
+        q.w[3 * e] = __builtin_amdgcn_raw_buffer_load_b8(wbuf, woff + lr, s, 0);
+        q.w[3 * e + 1] = __builtin_amdgcn_raw_buffer_load_b8(wbuf, woff + lr + 32, s, 0);
+        q.w[3 * e + 2] = __builtin_amdgcn_raw_buffer_load_b8(wbuf, woff + lr + 128 - 32 * hf, s, 0);
+        q.d[e] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(wbuf, woff + 192 - 56 * hf, s, 0));
+        q.ds[e] = __builtin_amdgcn_raw_buffer_load_b16(dbuf, doff + 2 * (e & 3), d + (e >> 2) * srow, 0);
       }
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const uint8_t *p = w + e * row + woff;
+        const unsigned s = w + e * row;
         if constexpr (TYPE == PBX_F16) {
-          const uint2 x = *reinterpret_cast<const uint2 *>(p);
+          const uint2 x = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(wbuf, woff, s, 0));
           q.w[2 * e] = x.x;
           q.w[2 * e + 1] = x.y;
         } else if constexpr (NIB) {
-          q.w[e] = *reinterpret_cast<const uint16_t *>(p);
+          q.w[e] = __builtin_amdgcn_raw_buffer_load_b16(wbuf, woff, s, 0);
         } else {
-          q.w[e] = *reinterpret_cast<const unsigned *>(p);
+          q.w[e] = __builtin_amdgcn_raw_buffer_load_b32(wbuf, woff, s, 0);
         }
       }
       if constexpr (TYPE != PBX_F16) {
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
-          q.d[g] = *reinterpret_cast<const uint2 *>(d + (size_t)g * scols * 8 + doff);
-          if constexpr (TYPE == PBX_Q41) q.mn[g] = *reinterpret_cast<const uint2 *>(mn + (size_t)g * scols * 8 + doff);
+          q.d[g] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(dbuf, doff, d + g * srow, 0));
+          if constexpr (TYPE == PBX_Q41)
+            q.mn[g] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(mbuf, doff, d + g * srow, 0));
         }
       }
     }
-    const size_t at = (size_t)(step >> 1) * a.Mpad * 64 + 32 * (step & 1);
+    const unsigned at = (step >> 1) * astep + 32 * (step & 1);
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
-      q.Ah[t] = *reinterpret_cast<const half8 *>(reinterpret_cast<const uint8_t *>(a.hi) + at + 2048 * t + aoff);
-      q.Al[t] = *reinterpret_cast<const half8 *>(reinterpret_cast<const uint8_t *>(a.lo) + at + 2048 * t + aoff);
+      q.Ah[t] = __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(hbuf, aoff + 2048 * t, at, 0));
+      q.Al[t] = __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(lbuf, aoff + 2048 * t, at, 0));
     }
   };
-  auto multiply = [&](const BackRaw<TYPE, TT> &q) {
+  auto multiply = [&](const BackRaw<TYPE, TT> &q, _Float16 f1, _Float16 f2, float fs) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       half8 H, L = {};
@@ -648,16 +662,37 @@ __device__ __forceinline__ void back_body(const BackArgs &a) {
       }
     }
   };
-  if (b0 + wave < b1) {
-    BackRaw<TYPE, TT> q, n;
-    load(2 * (b0 + wave), q);
-    for (int b = b0 + wave; b < b1; b += 4) {
-      load(2 * b + 1, n);
-      multiply(q);
-      load(2 * min(b + 4, b1 - 1), q);  // (the last step loads its block again)
-      multiply(n);
+  // step j of the wave: half of its block j / 2; D - 1 steps are under way beside the one
+  // that is multiplied
+  constexpr int D = BACK_DEPTH(TYPE, TT);
+  const int steps = b0 + wave < b1 ? 2 * ((b1 - b0 - wave + 3) / 4) : 0;
+  auto step_of = [&](int j) {  // (past the end: the last one again)
+    const int i = min(j, steps - 1);
+    return 2 * (wave + 4 * (i >> 1)) + (i & 1);
+  };
+  BackRaw<TYPE, TT> q[D];
+  if (steps) {
+#pragma unroll
+    for (int j = 0; j < D - 1; ++j) load(step_of(j), q[j]);
+  }
+  const int shift = TYPE == PBX_F16 ? 0 : head_shift(a.peaks, HeadTarget<TYPE>::value);
+  // codes enter as u 2^-9, so their scales take 2^9 more; by two factors, either of
+  // which a half holds
+  const int both = shift + 9, s1 = min(15, max(-14, both));
+  const _Float16 f1 = (_Float16)power_of_two(s1), f2 = (_Float16)power_of_two(both - s1);
+  const float fs = power_of_two(shift);
+  int j = 0;
+  for (; j + D <= steps; j += D) {
+#pragma unroll
+    for (int s = 0; s < D; ++s) {
+      load(step_of(j + s + D - 1), q[(s + D - 1) % D]);
+      __builtin_amdgcn_sched_barrier(0);  // (the loads stay ahead of the products)
+      multiply(q[s], f1, f2, fs);
     }
   }
+#pragma unroll
+  for (int s = 0; s < D - 1; ++s)
+    if (j + s < steps) multiply(q[s], f1, f2, fs);
   // the waves' sums, in a fixed order: (0 + 2) + (1 + 3)
   float *mine = red[wave & 1];
 #pragma unroll
@@ -684,7 +719,7 @@ __device__ __forceinline__ void back_body(const BackArgs &a) {
     __syncthreads();
   }
   if (wave) return;
-  const float undo = ldexpf(1.f, -15 - shift);
+  const float undo = power_of_two(-15 - shift);
   float *part = a.part + (int64_t)blockIdx.z * a.M * a.K;
 #pragma unroll
   for (int t = 0; t < TT; ++t)
@@ -707,7 +742,9 @@ template <int TT>
 __device__ __forceinline__ void back_f32(const BackArgs &a) {
   const int lane = threadIdx.x, lr = lane & 31, h = lane >> 5;
   const int k0 = blockIdx.x * 128, m0 = blockIdx.y * (32 * TT);
-  const int b0 = (int)((int64_t)a.blocks * blockIdx.z / a.KS), b1 = (int)((int64_t)a.blocks * (blockIdx.z + 1) / a.KS);
+  // (fewer than 2^14 blocks and 2^12 shares)
+  const int b0 = (int)((unsigned)a.blocks * blockIdx.z / (unsigned)a.KS);
+  const int b1 = (int)((unsigned)a.blocks * (blockIdx.z + 1) / (unsigned)a.KS);
   const floatx16 zero = {};
   floatx16 acc[TT][4];
 #pragma unroll

@@ -73,12 +73,13 @@ Plan make_plan(pbx_ctx *c, const pbx_weight *w, int64_t M, bool grad) {
   Plan p{};
   const int64_t V = w->N;
   p.TT = M > 32 ? 2 : 1;
-  p.Mpad = (int)((M + 63) / 64 * 64);
+  p.Mpad = M <= 32 ? 32 : (int)((M + 63) / 64 * 64);
   p.fused = pbx_gemm_has_head(c, w, M);
-  if (p.fused && grad) p.Mpad = (int)((M + 127) / 128 * 128);
   const int64_t row = 4 * (grad ? p.Mpad : M);
-  p.piece = std::min<int64_t>((V + 127) / 128 * 128, std::max<int64_t>(128, HEAD_PIECE / row / 128 * 128));
+  p.piece = std::min<int64_t>((V + 127) / 128 * 128, std::max<int64_t>(128, HEAD_PIECE / std::max<int64_t>(row, 256) / 128 * 128));
   if (p.fused && !grad) p.piece = (V + 127) / 128 * 128;
+  // (the gradient's kernels address a piece's weights by 31 bits)
+  if (grad) p.piece = std::min<int64_t>(p.piece, std::max<int64_t>(128, (int64_t)(1u << 31) / (2 * w->K) / 128 * 128 - 128));
   p.n_pieces = (int)((V + p.piece - 1) / p.piece);
   size_t at = 0;
   auto take = [&](size_t n) {
@@ -246,12 +247,12 @@ extern "C" int pbx_linear_logprobs_grad_dev(pbx_ctx *c, const pbx_weight *w, con
       rc = pbx_gemm_head(c, &rows, dX, m, v0 == 0, ws + p.gemm, e, scales);
     } else if (f32) {
       void *args[] = {&z, &stride, &n, &at, (void *)&dLse, (void *)&dTargets, &vocab, &m, &Mpad, &hi};
-      rc = pbx_launch(c, PBX_K_HEAD_G32, dim3(blocks, Mpad / 64), dim3(256), args);
+      rc = pbx_launch(c, PBX_K_HEAD_G32, dim3(blocks, (Mpad + 63) / 64), dim3(256), args);
     } else {
       int here = blocks;
       void *args[] = {&z, &stride, &n, &at, (void *)&dLse, (void *)&dTargets, &vocab, &m, &Mpad, &hi, &lo,
                       &here, &scales.scales, &scales.n8, &peaks};
-      rc = pbx_launch(c, PBX_K_HEAD_G, dim3(blocks + (w->d && !v0 ? PBX_HEAD_PEAKS : 0), Mpad / 64), dim3(256), args);
+      rc = pbx_launch(c, PBX_K_HEAD_G, dim3(blocks + (w->d && !v0 ? PBX_HEAD_PEAKS : 0), (Mpad + 63) / 64), dim3(256), args);
     }
     if (rc) return rc;
     BackArgsHost b{rows.qs, rows.d, rows.m, hi, lo, hi, peaks, part, m, Mpad, k, (int)w->B, blocks, (int)rows.Npad, KS,
