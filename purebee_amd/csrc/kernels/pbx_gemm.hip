@@ -588,12 +588,15 @@ __device__ __forceinline__ void store_tiles(const GemmArgs &a, const floatx16 (&
 #define HEAD_G 2     // the rows' gradient's first factor, as pbx_head_g gives it
 struct HeadArgs {
   const int *targets;
-  float4 *parts;  // [M][n_parts]
-  int n_parts;
+  float4 *parts;  // [M][n_parts], from part0 on
+  int n_parts, part0;
   float *hit;     // or null
   const float *lse;
   _Float16 *hi, *lo;  // [blocks of 32 entries][Mpad][32]
   int Mpad, v0, vocab;
+  const int *f;        // or null: column n's products are 2^-f[n] of a logit
+  const int *f_peaks;  // the largest f of parts of them
+  int n_f_peaks;
 };
 
 // The workgroup's MT x 128 tile by way of LDS (Z, rows of 132 floats, so that 8 rows'
@@ -602,6 +605,14 @@ template <int MT, int EPI, int TT, int UU>
 __device__ __forceinline__ void head_tile(const GemmArgs &a, const HeadArgs &e, float *Z,
                                           const floatx16 (&acc)[TT][UU], int mblk, int mw, int wn, int lr, int h) {
   constexpr int PITCH = 132, TR = 256 / MT, C = 128 / TR;
+  // the columns' powers of two (times a row's before the product: either alone may leave
+  // f32's range where the logit does not)
+  float up[UU];
+#pragma unroll
+  for (int u = 0; u < UU; ++u) {
+    const int col = blockIdx.x * 128 + 32 * (UU * wn + u) + lr;
+    up[u] = e.f ? __uint_as_float((unsigned)(max(e.f[min(col, a.N - 1)], -126) + 127) << 23) : 1.f;
+  }
   __syncthreads();  // every wave has read its last operands, and no DMA is under way
 #pragma unroll
   for (int t = 0; t < TT; ++t)
@@ -610,7 +621,7 @@ __device__ __forceinline__ void head_tile(const GemmArgs &a, const HeadArgs &e, 
       const int m = mw + 32 * t + 8 * (r >> 2) + 4 * h + (r & 3);
       const float iv = a.inv[mblk + m];
 #pragma unroll
-      for (int u = 0; u < UU; ++u) Z[m * PITCH + 32 * (UU * wn + u) + lr] = acc[t][u][r] * iv;
+      for (int u = 0; u < UU; ++u) Z[m * PITCH + 32 * (UU * wn + u) + lr] = acc[t][u][r] * (iv * up[u]);
     }
   __syncthreads();
   const int row = threadIdx.x / TR, part = threadIdx.x % TR, m = mblk + row;
@@ -641,13 +652,14 @@ __device__ __forceinline__ void head_tile(const GemmArgs &a, const HeadArgs &e, 
       spread += __shfl_xor(spread, off);
     }
     if (part == 0 && m < a.M) {
-      e.parts[(size_t)m * e.n_parts + blockIdx.x] = make_float4(top, sum, spread, 0.f);
-      if (e.hit) {
-        const int t = e.targets[m] - blockIdx.x * 128;
-        if (t >= 0 && t < 128 && e.targets[m] < a.N) e.hit[m] = z[t];
-      }
+      e.parts[(size_t)m * e.n_parts + e.part0 + blockIdx.x] = make_float4(top, sum, spread, 0.f);
+    }
+    if (e.hit && m < a.M) {
+      const int64_t t = (int64_t)e.targets[m] - e.v0;
+      if (t >= n && t < n + C && t < a.N) e.hit[m] = z[t - n];
     }
   } else {
+    const int peak = e.f ? head_f_peak(e.f_peaks, e.n_f_peaks) : 0;
     if (m >= e.Mpad) return;
     const int t = m < a.M ? e.targets[m] : -1;
     const bool on = t >= 0 && t < e.vocab;
@@ -663,6 +675,7 @@ __device__ __forceinline__ void head_tile(const GemmArgs &a, const HeadArgs &e, 
         float g = on && n + c + i < a.N ? -expf(d) : 0.f;
         if (on && e.v0 + n + c + i == t) g = -expm1f(d);
         g *= 32768.f;
+        if (e.f) g = ldexpf(g, e.f[min(n + c + i, a.N - 1)] - peak);
         H[i] = (_Float16)g;
         L[i] = (_Float16)(g - (float)H[i]);
       }

@@ -393,6 +393,133 @@ HEAD_SIX(1)
 HEAD_SIX(2)
 HEAD_SIX(3)
 
+// ---- F32 and Q6_K heads as pairs of halves --------------------------------------------
+
+namespace {
+
+// Row n of a piece as halves [hi of K | lo of K], scaled by 2^-f[n] so that its largest
+// magnitude (Q6_K: what its scales allow) is below 2^15.  A wave's row; returns its f.
+// Rows past the piece's last one are zeros.
+template <int TYPE>
+__device__ __forceinline__ int pairs_row(const uint8_t *qs, const uint16_t *dsc, int K, int n, _Float16 *out, int *f,
+                                         int row) {
+  typedef _Float16 half4t __attribute__((ext_vector_type(4)));
+  const int lane = threadIdx.x & 63;
+  _Float16 *hi = out + (int64_t)row * 2 * K, *lo = hi + K;
+  if (row >= n) {
+    for (int k = 8 * lane; k < K; k += 512) {
+      *reinterpret_cast<half8 *>(hi + k) = half8{};
+      *reinterpret_cast<half8 *>(lo + k) = half8{};
+    }
+    if (lane == 0) f[row] = -200;
+    return -200;
+  }
+  const float4 *w4 = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(qs) + (int64_t)row * K);
+  const int SB = K >> 8;
+  const uint8_t *six = qs + (int64_t)row * SB * PBX_Q6K_BYTES;
+  float most = 0.f;
+  if constexpr (TYPE == PBX_F32) {
+    for (int k = lane; k < K / 4; k += 64) {
+      const float4 v = w4[k];
+      most = fmaxf(most, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+    }
+  } else {
+    for (int i = lane; i < SB * 16; i += 64) {
+      const float d = f16_bits_to_f32(dsc[dsc_index(row, i >> 4, SB)]);
+      most = fmaxf(most, fabsf(d * (float)(int8_t)six[(int64_t)(i >> 4) * PBX_Q6K_BYTES + 192 + (i & 15)]) * 32.f);
+    }
+  }
+  most = wave_max(most);
+  int e = -185;
+  if (most > 0.f && most < INFINITY) frexpf(most, &e);
+  e = max(e, -110);  // (2^(15 - e) stays a normal number)
+  const float up = __uint_as_float((unsigned)(15 - e + 127) << 23);
+  if (lane == 0) f[row] = e - 15;
+  auto split = [&](float v, _Float16 &h, _Float16 &l) {
+    h = (_Float16)v;
+    l = (_Float16)(v - (float)h);
+  };
+  if constexpr (TYPE == PBX_F32) {
+    for (int k = lane; k < K / 4; k += 64) {
+      const float4 v = w4[k];
+      half4t h, l;
+      _Float16 a, b;
+      split(v.x * up, a, b), h[0] = a, l[0] = b;
+      split(v.y * up, a, b), h[1] = a, l[1] = b;
+      split(v.z * up, a, b), h[2] = a, l[2] = b;
+      split(v.w * up, a, b), h[3] = a, l[3] = b;
+      reinterpret_cast<half4t *>(hi)[k] = h;
+      reinterpret_cast<half4t *>(lo)[k] = l;
+    }
+  } else {
+    // eight lanes a superblock, as in six_body
+    for (int i = lane; i < SB * 8; i += 64) {
+      const int sb = i >> 3, half = i >> 2 & 1, c = i & 3;
+      const uint8_t *blk = six + (int64_t)sb * PBX_Q6K_BYTES;
+      const uint4 l4 = ld_stream(blk + 64 * half + 16 * c), h4 = ld_stream(blk + 128 + 32 * half + 16 * (c & 1));
+      const float d = f16_bits_to_f32(dsc[dsc_index(row, sb, SB)]) * up;
+      const float d0 = d * (float)(int8_t)blk[192 + 8 * half + c], d1 = d * (float)(int8_t)blk[196 + 8 * half + c];
+      const unsigned ql[4] = {l4.x, l4.y, l4.z, l4.w}, qh[4] = {h4.x, h4.y, h4.z, h4.w};
+      const int64_t at = 256 * sb + 128 * half + 16 * c;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          half8 h, l;
+#pragma unroll
+          for (int t = 0; t < 8; ++t) {
+            const unsigned x = ql[j + (t >> 2)] >> (4 * g), y = qh[j + (t >> 2)] >> ((c & 2) + 4 * g);
+            const int code = (int)((x >> (8 * (t & 3)) & 15u) | (y >> (8 * (t & 3)) & 3u) << 4) - 32;
+            _Float16 a, b;
+            split((g ? d1 : d0) * (float)code, a, b);
+            h[t] = a;
+            l[t] = b;
+          }
+          *reinterpret_cast<half8 *>(hi + at + 64 * g + 4 * j) = h;
+          *reinterpret_cast<half8 *>(lo + at + 64 * g + 4 * j) = l;
+        }
+      }
+    }
+  }
+  return e - 15;
+}
+
+// All rows, `rows` with those past the last one, a wave each in turn; peaks[workgroup]:
+// the largest f of its rows.  Bound by bytes, 4 written for every value.
+template <int TYPE>
+__device__ __forceinline__ void pairs_body(const uint8_t *qs, const uint16_t *dsc, int K, int n, int rows, _Float16 *out,
+                                           int *f, int *peaks) {
+  __shared__ int most[4];
+  const int wave = threadIdx.x >> 6;
+  int top = -200;
+  for (int row = blockIdx.x * 4 + wave; row < rows; row += gridDim.x * 4)
+    top = max(top, pairs_row<TYPE>(qs, dsc, K, n, out, f, row));
+  if ((threadIdx.x & 63) == 0) most[wave] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) peaks[blockIdx.x] = max(max(most[0], most[1]), max(most[2], most[3]));
+}
+
+}  // namespace
+
+extern "C" __global__ void __launch_bounds__(256)
+pbx_head_pairs_f32(const uint8_t *qs, const uint16_t *dsc, int K, int n, int rows, _Float16 *out, int *f, int *peaks) {
+  pairs_body<PBX_F32>(qs, dsc, K, n, rows, out, f, peaks);
+}
+extern "C" __global__ void __launch_bounds__(256)
+pbx_head_pairs_q6k(const uint8_t *qs, const uint16_t *dsc, int K, int n, int rows, _Float16 *out, int *f, int *peaks) {
+  pairs_body<PBX_Q6K>(qs, dsc, K, n, rows, out, f, peaks);
+}
+
+// The other factor: the prepared rows' hi plane again and zeros beside it (n16 times 16
+// bytes of each), for the products with the low halves.
+extern "C" __global__ void __launch_bounds__(256)
+pbx_head_twice(uint4 *hi, uint4 *lo, int64_t n16) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n16) return;
+  hi[n16 + i] = hi[i];
+  lo[n16 + i] = make_uint4(0, 0, 0, 0);
+}
+
 // ---- the gradient --------------------------------------------------------------------
 
 
@@ -472,6 +599,8 @@ struct BackArgs {
   const _Float16 *hi, *lo;  // G
   const float *G32;
   const unsigned *peaks;
+  const int *f_peaks;  // F16 as pairs: the largest f of parts of the piece (the products are 2^(-15 - f) of theirs)
+  int n_f_peaks;
   float *part;         // [KS][M][K]
   int M, Mpad, K, B;   // B: 32-wide blocks of a row
   int blocks, rows;    // blocks of 32 entries of the piece, and weight rows that may be read
@@ -719,7 +848,8 @@ __device__ __forceinline__ void back_body(const BackArgs &a) {
     __syncthreads();
   }
   if (wave) return;
-  const float undo = power_of_two(-15 - shift);
+  const float undo = power_of_two(min(127, max(-126, TYPE == PBX_F16 && a.n_f_peaks ? head_f_peak(a.f_peaks, a.n_f_peaks) - 15
+                                                                          : -15 - shift)));
   float *part = a.part + (int64_t)blockIdx.z * a.M * a.K;
 #pragma unroll
   for (int t = 0; t < TT; ++t)
@@ -796,16 +926,19 @@ extern "C" __global__ void __launch_bounds__(64) pbx_head_back_f32_1(BackArgs a)
 extern "C" __global__ void __launch_bounds__(64) pbx_head_back_f32_2(BackArgs a) { back_f32<2>(a); }
 
 // dX = grad * (the partial sums together), rows without a target 0: workgroup (16
-// float4s of a row), the partials over 16 threads each.
+// float4s of a row), the partials over 16 threads each.  folds 2: the partial sums have
+// 2 K columns, of the head's high halves and of its low ones.
 extern "C" __global__ void __launch_bounds__(256)
-pbx_head_reduce(const float *part, int KS, int M, int K, const int *targets, int vocab, const float *grad, float *dX) {
+pbx_head_reduce(const float *part, int KS, int M, int K, int folds, const int *targets, int vocab, const float *grad,
+                float *dX) {
   __shared__ float4 sum[16][17];
-  const int64_t row = blockIdx.y, MK4 = (int64_t)M * K / 4;
+  const int64_t row = blockIdx.y, MK4 = (int64_t)M * K / 4 * folds;
   const int c = threadIdx.x % 16, j = threadIdx.x / 16, k4 = blockIdx.x * 16 + c;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (k4 < K / 4)
-    for (int i = j; i < KS; i += 16) {
-      const float4 p = reinterpret_cast<const float4 *>(part)[i * MK4 + row * (K / 4) + k4];
+    for (int i = j; i < KS * folds; i += 16) {
+      const int64_t at = i / folds * MK4 + row * folds * (K / 4) + i % folds * (K / 4) + k4;
+      const float4 p = reinterpret_cast<const float4 *>(part)[at];
       s.x += p.x, s.y += p.y, s.z += p.z, s.w += p.w;
     }
   sum[j][c] = s;

@@ -25,4 +25,13 @@ __device__ __forceinline__ void head_peaks(const uint16_t *plane, int64_t n8, un
   if (threadIdx.x == 0) peaks[part] = max(max(red[0], red[1]), max(red[2], red[3]));
 }
 
+// The largest of n exponents; by every wave for itself.
+__device__ __forceinline__ int head_f_peak(const int *peaks, int n) {
+  int m = -200;
+  for (int i = threadIdx.x & 63; i < n; i += 64) m = max(m, peaks[i]);
+#pragma unroll
+  for (int off = 32; off >= 1; off /= 2) m = max(m, __shfl_xor(m, off, 64));
+  return m;
+}
+
 #endif

@@ -383,34 +383,39 @@ size_t pbx_gemm_head_space(const pbx_weight *w, int M) {
   return gemm_space(p, (int)w->N, (int)w->K).total();
 }
 
-int pbx_gemm_head(pbx_ctx *c, const pbx_weight *w, const float *dX, int M, bool prep, void *space,
-                  const pbx_head_epilogue &e, const pbx_head_scales &scales) {
+pbx_head_rows pbx_gemm_head_rows(const pbx_weight *w, int M, void *space) {
   pbx_gemm_plan p;
   p.M = M;
   p.Mpad = (M + 127) / 128 * 128;
-  p.nwg = ((int)w->N + 127) / 128;
-  const int rows = head_rows(M);
-  p.mtiles = (M + rows - 1) / rows;
-  p.name = std::string("pbx_gemm_") + gemm_tag(w->type) + (rows == 32 ? "_b32" : rows == 64 ? "_b64" : "_big") +
-           (e.lse ? "_g" : "_sums");
   const GemmSpace sp = gemm_space(p, (int)w->N, (int)w->K);
-  void *x16 = space, *x16lo = (char *)space + sp.x16;
-  float *inv = (float *)((char *)space + 2 * sp.x16);
-  hipFunction_t f = pbx_kernel_by_name(c, p.name), fprep = pbx_kernel_by_name(c, "pbx_gemm_prep_head");
-  if (!f || !fprep) return pbx_fail(c, PBX_ELOAD, "pbx_gemm: kernel %s missing", p.name.c_str());
-  int rc;
-  if (prep) {
-    int m = M, k = (int)w->K;
-    pbx_head_scales sc = scales;
-    void *args[] = {(void *)&dX, &x16, &x16lo, &inv, &m, &k, &sc.scales, &sc.n8, &sc.peaks};
-    const dim3 grid(p.Mpad, sc.peaks ? 1 + (PBX_HEAD_PEAKS + p.Mpad - 1) / p.Mpad : 1);
-    if ((rc = pbx_launch_fn(c, fprep, "pbx_gemm_prep_head", grid, dim3(256), args, c->stream))) return rc;
-  }
-  GemmArgsHost g{w->qs, w->d, x16, x16lo, inv, nullptr, nullptr,
-                 M, (int)w->N, (int)w->Npad, (int)w->B, 1, 0, w->m, p.Mpad};
+  char *s = (char *)space;
+  return {s, s + sp.x16, (float *)(s + 2 * sp.x16), sp.x16};
+}
+
+int pbx_gemm_head_prep(pbx_ctx *c, const float *dX, int M, int K, void *x16, void *x16lo, float *inv,
+                       const pbx_head_scales &scales) {
+  hipFunction_t f = pbx_kernel_by_name(c, "pbx_gemm_prep_head");
+  if (!f) return pbx_fail(c, PBX_ELOAD, "pbx_gemm: kernel pbx_gemm_prep_head missing");
+  const int Mpad = (M + 127) / 128 * 128;
+  pbx_head_scales sc = scales;
+  void *args[] = {(void *)&dX, &x16, &x16lo, &inv, &M, &K, &sc.scales, &sc.n8, &sc.peaks};
+  const dim3 grid(Mpad, sc.peaks ? 1 + (PBX_HEAD_PEAKS + Mpad - 1) / Mpad : 1);
+  return pbx_launch_fn(c, f, "pbx_gemm_prep_head", grid, dim3(256), args, c->stream);
+}
+
+int pbx_gemm_head(pbx_ctx *c, const pbx_weight *w, int M, void *space, const pbx_head_epilogue &e) {
+  const int rows = head_rows(M);
+  const std::string name = std::string("pbx_gemm_") + gemm_tag(w->type) +
+                           (rows == 32 ? "_b32" : rows == 64 ? "_b64" : "_big") + (e.lse ? "_g" : "_sums");
+  hipFunction_t f = pbx_kernel_by_name(c, name);
+  if (!f) return pbx_fail(c, PBX_ELOAD, "pbx_gemm: kernel %s missing", name.c_str());
+  const pbx_head_rows x = pbx_gemm_head_rows(w, M, space);
+  GemmArgsHost g{w->qs, w->d, x.x16, x.x16lo, x.inv, nullptr, nullptr,
+                 M, (int)w->N, (int)w->Npad, (int)w->B, 1, 0, w->m, (M + 127) / 128 * 128};
   pbx_head_epilogue he = e;
   void *args[] = {&g, &he};
-  return pbx_launch_fn(c, f, p.name.c_str(), dim3(p.nwg, p.mtiles), dim3(256), args, c->stream);
+  return pbx_launch_fn(c, f, name.c_str(), dim3(((int)w->N + 127) / 128, (M + rows - 1) / rows), dim3(256), args,
+                       c->stream);
 }
 
 int pbx_gemm_enqueue(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M,

@@ -18,6 +18,9 @@
   X(PBX_K_KV_ROPE_TABLE, "pbx_kv_rope_table")                \
   X(PBX_K_HEAD_STATS, "pbx_head_stats")                      \
   X(PBX_K_HEAD_JOIN, "pbx_head_join")                        \
+  X(PBX_K_HEAD_PAIRS_F32, "pbx_head_pairs_f32")              \
+  X(PBX_K_HEAD_PAIRS_Q6K, "pbx_head_pairs_q6k")              \
+  X(PBX_K_HEAD_TWICE, "pbx_head_twice")                      \
   X(PBX_K_HEAD_G, "pbx_head_g")                              \
   X(PBX_K_HEAD_G32, "pbx_head_g32")                          \
   X(PBX_K_HEAD_REDUCE, "pbx_head_reduce")                    \
@@ -208,9 +211,9 @@ int pbx_gemm_run(pbx_ctx *c, const pbx_weight *w, const pbx_gemm_plan &p, const 
                  const void *x16lo, const float *inv, const float *dBias, float *out,
                  int accumulate, hipStream_t stream);
 // The GEMM of M rows of a quantised or F16 head whose logits go into sums of each
-// 128 columns (lse == nullptr) or the gradient's first factor (pbx_head.cpp).
-// prep: X16, X16lo and inv (in space, of pbx_gemm_head_space bytes) are filled from dX
-// first, and peaks (if not NULL) from the n8 groups of 8 halves at scales.
+// 128 columns (lse == nullptr) or the gradient's first factor (pbx_head.cpp), in two
+// steps: X16, X16lo and inv (in space, of pbx_gemm_head_space bytes) are filled from dX,
+// and peaks (if not NULL) from the n8 groups of 8 halves at scales; then the products.
 struct pbx_head_scales {
   const void *scales;
   int64_t n8;
@@ -218,18 +221,28 @@ struct pbx_head_scales {
 };
 #define PBX_HEAD_PEAKS 256
 struct pbx_head_epilogue {  // HeadArgs in pbx_gemm.hip
-  const int32_t *targets;
-  void *parts;
-  int n_parts;
-  float *hit;
-  const float *lse;
-  void *hi, *lo;
-  int Mpad, v0, vocab;
+  const int32_t *targets = nullptr;
+  void *parts = nullptr;
+  int n_parts = 0, part0 = 0;
+  float *hit = nullptr;
+  const float *lse = nullptr;
+  void *hi = nullptr, *lo = nullptr;
+  int Mpad = 0, v0 = 0, vocab = 0;
+  const int32_t *f = nullptr, *f_peaks = nullptr;
+  int n_f_peaks = 0;
 };
 bool pbx_gemm_has_head(const pbx_ctx *c, const pbx_weight *w, int64_t M);
 size_t pbx_gemm_head_space(const pbx_weight *w, int M);
-int pbx_gemm_head(pbx_ctx *c, const pbx_weight *w, const float *dX, int M, bool prep, void *space,
-                  const pbx_head_epilogue &e, const pbx_head_scales &scales = {});
+int pbx_gemm_head_prep(pbx_ctx *c, const float *dX, int M, int K, void *x16, void *x16lo, float *inv,
+                       const pbx_head_scales &scales = {});
+// Where pbx_gemm_head finds them in its space.
+struct pbx_head_rows {
+  void *x16, *x16lo;
+  float *inv;
+  size_t plane;  // bytes of x16, and of x16lo
+};
+pbx_head_rows pbx_gemm_head_rows(const pbx_weight *w, int M, void *space);
+int pbx_gemm_head(pbx_ctx *c, const pbx_weight *w, int M, void *space, const pbx_head_epilogue &e);
 int pbx_gemm_enqueue(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M,
                      const float *dBias, float *dY, hipStream_t stream,
                      const pbx_workspace *ws = nullptr);

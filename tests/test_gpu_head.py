@@ -122,6 +122,29 @@ def test_few_rows_of_q6_k(ctx, M, V, K):
     test_scores_and_gradient(ctx, "q6_k", M, V, K)
 
 
+# heads that become pairs of halves on the way
+@pytest.mark.parametrize("kind,M,V,K", [("f32", 2, 20011, 512), ("f32", 40, 20011, 512), ("f32", 33, 19999, 544),
+                                        ("f32", 130, 5000, 2048), ("f32", 700, 999, 1024), ("q6_k", 100, 20011, 512),
+                                        ("q6_k", 33, 16001, 768), ("q6_k", 330, 9001, 2304), ("f32", 2, 70001, 512),
+                                        ("q6_k", 96, 70001, 512)])
+def test_heads_as_pairs(ctx, kind, M, V, K):
+    test_scores_and_gradient(ctx, kind, M, V, K)
+
+
+@pytest.mark.parametrize("kind", ["f32", "q6_k"])
+def test_rows_of_very_different_size_as_pairs(ctx, kind):
+    """Every vocabulary entry keeps its bits, however small its weights; rows of zeros; huge and tiny heads."""
+    rng = np.random.default_rng(6)
+    w = rng.standard_normal((13000, 1024)).astype(np.float32)
+    w *= np.logspace(-4, 0, 13000)[rng.permutation(13000)][:, None].astype(np.float32)
+    w[::97] = 0
+    for scale in (0.05, 3e-5 if kind == "q6_k" else 1e-20, 50.0 if kind == "q6_k" else 1e15) + \
+            ((1e-28,) if kind == "f32" else ()):
+        head = Head(ctx, kind, scale * w)
+        check(head, rows_of(100, 1024, size=0.05 / scale), targets_of(100, 13000), np.ones(100))
+        head.free()
+
+
 @pytest.mark.parametrize("kind", ["q8_0", "f16", "f32", "q6_k"])
 def test_many_pieces(ctx, kind):
     """A vocabulary of several pieces and a ragged last one."""
