@@ -900,15 +900,20 @@ __device__ __forceinline__ void gemm_dma(const GemmArgs &a, const HeadArgs &e = 
     // block b + 1's operands are read from LDS and its codes unpacked, and the
     // scale FMAs of a pair of 32 x 32 products run under the next pair's
     // MFMAs (pend: the products not yet scaled).
+    // F16 goes on in one sum.  A head's products do not: a sum of its own for each block, as
+    // the other types have it, takes the scores of 200 rows of 31,424 x 2,272 from 2.8e-7 off
+    // to 1.1e-7 and their gradient from 7e-7 to 3.5e-7, for 9% (1,000 rows of 64,000 x 2,048:
+    // 576 -> 630 us) or less.
+    constexpr bool ONE_SUM = TYPE == PBX_F16 && EPI == 0;
     floatx16 pend[2] = {zero16, zero16};
     float pd[2] = {0.f, 0.f};
     auto scale_pending = [&](int t) {
-      if constexpr (TYPE != PBX_F16) {
+      if constexpr (!ONE_SUM) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            acc[t][u][r] = fmaf(pend[u][r], pd[u], acc[t][u][r]);
+            acc[t][u][r] = TYPE == PBX_F16 ? acc[t][u][r] + pend[u][r] : fmaf(pend[u][r], pd[u], acc[t][u][r]);
           }
       }
     };
@@ -967,7 +972,7 @@ __device__ __forceinline__ void gemm_dma(const GemmArgs &a, const HeadArgs &e = 
         }
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
-          if constexpr (TYPE == PBX_F16) {
+          if constexpr (ONE_SUM) {
 #pragma unroll
             for (int q = 0; q < 4; ++q)
 #pragma unroll
@@ -1191,6 +1196,7 @@ __device__ __forceinline__ void gemm_dma64(const GemmArgs &a, const HeadArgs &e 
 
 #pragma unroll
     for (int s = 0; s < NS - 1; ++s) dma(min(b0 + s, b1 - 1), s);
+    constexpr bool ONE_SUM = TYPE == PBX_F16 && EPI == 0;  // (as in gemm_dma)
 
     for (int kb = b0; kb < b1; kb += NS) {
 #pragma unroll
@@ -1243,7 +1249,7 @@ __device__ __forceinline__ void gemm_dma64(const GemmArgs &a, const HeadArgs &e 
           }
 #pragma unroll
           for (int u = 0; u < UU; ++u) {
-            if constexpr (TYPE == PBX_F16) {
+            if constexpr (ONE_SUM) {
               acc[t][u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(Ah0, B0[u], acc[t][u], 0, 0, 0);
               acc[t][u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(Al0, B0[u], acc[t][u], 0, 0, 0);
               acc[t][u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(Ah1, B1[u], acc[t][u], 0, 0, 0);
@@ -1255,7 +1261,7 @@ __device__ __forceinline__ void gemm_dma64(const GemmArgs &a, const HeadArgs &e 
               blk = __builtin_amdgcn_mfma_f32_32x32x16_f16(Al1, B1[u], blk, 0, 0, 0);
 #pragma unroll
               for (int r = 0; r < 16; ++r) {
-                acc[t][u][r] = fmaf(blk[r], d[u], acc[t][u][r]);
+                acc[t][u][r] = TYPE == PBX_F16 ? acc[t][u][r] + blk[r] : fmaf(blk[r], d[u], acc[t][u][r]);
                 if constexpr (TYPE == PBX_Q41) acc[t][u][r] = fmaf(xs[r], mn[u], acc[t][u][r]);
               }
             }
