@@ -566,11 +566,13 @@ int pbx_logprobs_dev(pbx_ctx *ctx, const float *dLogits, int64_t stride, int64_t
  *                NULL, like dTargets, to leave it out
  *   dEntropy[r]  -sum p log p, in nats; or NULL
  *   dLse[r]      log of the sum of all e^logit, which the gradient needs; or NULL
- * A row without a distribution (see above) answers with NaN.  Activations enter the
- * logits with 22 bits at least, as in pbx_linear, and so do the weights of an F32 head
- * (2^-22 of each, 2^-39 of its row's largest); sums are held in f32.  Only enqueues on the context's stream.  work: device memory of the size
- * that pbx_linear_logprobs_workspace gives (grad 1: for the gradient), 256-byte aligned,
- * any content, for this call alone until it has run.  No reference counterpart. */
+ * A row without a distribution (see above) answers with NaN; weights are finite.
+ * Activations enter the logits with 22 bits at least, as in pbx_linear, and so do the
+ * weights of an F32 head (2^-22 of each, 2^-39 of its row's largest); sums are held in
+ * f32.  Only enqueues on the context's stream.  work: device memory of the size that
+ * pbx_linear_logprobs_workspace gives (grad 1: for the gradient), 256-byte aligned, any
+ * content, for this call alone until it has run (graphs that may run side by side need
+ * one each).  No reference counterpart. */
 int pbx_linear_logprobs_workspace(pbx_ctx *ctx, const pbx_weight *W, int64_t rows, int grad, size_t *bytes);
 int pbx_linear_logprobs_dev(pbx_ctx *ctx, const pbx_weight *W, const float *dX, int64_t rows,
                             const int32_t *dTargets, float *dLogp, float *dEntropy, float *dLse,
@@ -581,7 +583,8 @@ int pbx_linear_logprobs_dev(pbx_ctx *ctx, const pbx_weight *W, const float *dX, 
  * not dX itself.  dLse as pbx_linear_logprobs_dev gave it for these rows.  Logits are
  * computed again; probabilities and weights enter the second product with 22 bits
  * (weights 2^-26 of the largest that the head's largest scale allows at least), sums are
- * held in f32 and come out the same in every call.  The weights stay as they are: they have no gradient. */
+ * held in f32 and come out the same in every call.  The weights stay as they are: they
+ * have no gradient. */
 int pbx_linear_logprobs_grad_dev(pbx_ctx *ctx, const pbx_weight *W, const float *dX, int64_t rows,
                                  const int32_t *dTargets, const float *dLse, const float *dGradLogp,
                                  float *dGradX, void *work, size_t work_bytes);

@@ -55,7 +55,8 @@ __device__ __forceinline__ Sums join_threads(Sums a, float (*buf)[4]) {
 
 // Sums of a piece's logits Z [M][stride] (n of a row count; it starts at vocabulary
 // entry v0): workgroup (part of 8192, row) -> parts[row][part0 + part], and the targets'
-// logits.
+// logits.  One pass, a running maximum a thread; heads whose products the GEMM's epilogue
+// does not take (there the logits are never written).
 extern "C" __global__ void __launch_bounds__(256)
 pbx_head_stats(const float *Z, int64_t stride, int n, int v0, const int *targets, float4 *parts, int n_parts,
                int part0, float *hit) {
@@ -98,7 +99,7 @@ pbx_head_stats(const float *Z, int64_t stride, int n, int v0, const int *targets
   }
 }
 
-// A row's parts joined: workgroup = row.
+// A row's parts joined: workgroup = row.  1,000 rows of 1,002 parts 6.5 us.
 extern "C" __global__ void __launch_bounds__(256)
 pbx_head_join(const float4 *parts, int n_parts, const int *targets, int vocab, const float *hit, float *logp,
               float *entropy, float *lse) {
@@ -485,7 +486,8 @@ __device__ __forceinline__ int pairs_row(const uint8_t *qs, const uint16_t *dsc,
 }
 
 // All rows, `rows` with those past the last one, a wave each in turn; peaks[workgroup]:
-// the largest f of its rows.  Bound by bytes, 4 written for every value.
+// the largest f of its rows.  Bound by bytes, 4 written for every value: 20,000 x 2,048
+// F32 60 us, Q6_K 40.
 template <int TYPE>
 __device__ __forceinline__ void pairs_body(const uint8_t *qs, const uint16_t *dsc, int K, int n, int rows, _Float16 *out,
                                            int *f, int *peaks) {
@@ -544,7 +546,8 @@ template <int TYPE> struct HeadTarget { static constexpr int value = TYPE == PBX
 // G of a piece as fp16 pairs times 2^15, [n / 32][Mpad][32]: workgroup (block of 32
 // vocabulary entries, 64 rows); zeros past the vocabulary, the rows, and in rows
 // without a target.  Workgroups past the blocks (HEAD_PEAKS of them where there are any)
-// look for the head's largest scales.
+// look for the head's largest scales.  Few rows, where the GEMM's epilogue does not take
+// the head: a pass over the piece's logits, bound by bytes.
 extern "C" __global__ void __launch_bounds__(256)
 pbx_head_g(const float *Z, int64_t stride, int n, int v0, const float *lse, const int *targets, int vocab, int M,
            int Mpad, _Float16 *hi, _Float16 *lo, int blocks, const uint16_t *scales, int64_t n8, unsigned *peaks) {
@@ -635,13 +638,19 @@ struct BackRaw {
   half8 Ah[TT], Al[TT];
 };
 
+// Steps whose loads are under way: four where the registers allow it (few rows, which
+// wait for memory: 5 rows of 49,152 x 576 Q4_0 17 us), else two.
 #define BACK_DEPTH(TYPE, TT) ((TYPE) == PBX_Q6K || (TT) == 2 ? 2 : 4)
 
 // Workgroup = 32 TT rows of G, 128 columns of the head and a share of its entries, whose
 // blocks four waves take in turn; their sums meet in LDS.  A step is 16 entries: a lane
 // loads 4 columns (as they lie in a row's bytes) of 8 rows, so that the operands, 8
 // entries of a column, are put together in registers, byte by byte with no trip through
-// LDS, while the next step's loads are under way.
+// LDS, while the next step's loads are under way.  Codes times scales are pairs of fp16
+// (three products with G's pair; F16 weights two).  Many rows are bound by the matrix
+// instructions: 512 rows of 32,768 x 2,048 Q8_0 205 us (1,000 TFLOP/s of products), 37
+// rows of 32,003 x 2,048 F16 37 us.  Splitting over the entries, and joining, instead of
+// more rows a workgroup: a head has few columns, and G is small beside it.
 template <int TYPE, int TT>
 __device__ __forceinline__ void back_body(const BackArgs &a) {
   __shared__ float red[2][TT * 4 * 16 * 64];

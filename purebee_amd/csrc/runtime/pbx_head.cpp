@@ -4,6 +4,7 @@
 #include "pbx_internal.h"
 
 #include <algorithm>
+#include <new>
 #include <string>
 
 namespace {
@@ -246,7 +247,7 @@ extern "C" int pbx_linear_logprobs_workspace(pbx_ctx *c, const pbx_weight *w, in
 
 extern "C" int pbx_linear_logprobs_dev(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M,
                                        const int32_t *dTargets, float *dLogp, float *dEntropy, float *dLse, void *work,
-                                       size_t work_bytes) {
+                                       size_t work_bytes) try {
   const char *who = "pbx_linear_logprobs_dev";
   if (!c) return pbx_fail(nullptr, PBX_EINVAL, "%s: ctx is NULL", who);
   int rc = check(c, who, w, M);
@@ -300,11 +301,13 @@ extern "C" int pbx_linear_logprobs_dev(pbx_ctx *c, const pbx_weight *w, const fl
   int vocab = (int)w->N;
   void *args[] = {&parts, &n_parts, (void *)&dTargets, &vocab, &hit, &dLogp, &dEntropy, &dLse};
   return pbx_launch(c, PBX_K_HEAD_JOIN, dim3((unsigned)M), dim3(256), args);
+} catch (const std::bad_alloc &) {
+  return pbx_fail(c, PBX_ENOMEM, "pbx_linear_logprobs_dev: out of host memory");
 }
 
 extern "C" int pbx_linear_logprobs_grad_dev(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M,
                                             const int32_t *dTargets, const float *dLse, const float *dGradLogp,
-                                            float *dGradX, void *work, size_t work_bytes) {
+                                            float *dGradX, void *work, size_t work_bytes) try {
   const char *who = "pbx_linear_logprobs_grad_dev";
   if (!c) return pbx_fail(nullptr, PBX_EINVAL, "%s: ctx is NULL", who);
   int rc = check(c, who, w, M);
@@ -316,12 +319,12 @@ extern "C" int pbx_linear_logprobs_grad_dev(pbx_ctx *c, const pbx_weight *w, con
   const Plan p = make_plan(c, w, M, true);
   if ((rc = check_work(c, who, p, work, work_bytes))) return rc;
   const bool f32 = w->type == PBX_TYPE_F32 && !p.pairs;
-  const char *tag = f32                                    ? "f32"
-                    : w->type == PBX_TYPE_F16 || p.pairs   ? "f16"
-                    : w->type == PBX_TYPE_Q8_0  ? "q8"
-                    : w->type == PBX_TYPE_Q4_0  ? "q4"
-                    : w->type == PBX_TYPE_Q4_1  ? "q41"
-                                                : "q6k";
+  const char *tag = f32                                  ? "f32"
+                    : w->type == PBX_TYPE_F16 || p.pairs ? "f16"
+                    : w->type == PBX_TYPE_Q8_0           ? "q8"
+                    : w->type == PBX_TYPE_Q4_0           ? "q4"
+                    : w->type == PBX_TYPE_Q4_1           ? "q41"
+                                                         : "q6k";
   const std::string name = std::string("pbx_head_back_") + tag + "_" + std::to_string(p.TT);
   hipFunction_t back = pbx_kernel_by_name(c, name);
   if (!back) return pbx_fail(c, PBX_ELOAD, "%s: kernel %s missing", who, name.c_str());
@@ -382,4 +385,6 @@ extern "C" int pbx_linear_logprobs_grad_dev(pbx_ctx *c, const pbx_weight *w, con
   }
   void *args[] = {&part, &KS, &m, &k, &folds, (void *)&dTargets, &vocab, (void *)&dGradLogp, &dGradX};
   return pbx_launch(c, PBX_K_HEAD_REDUCE, dim3((k / 4 + 15) / 16, (unsigned)M), dim3(256), args);
+} catch (const std::bad_alloc &) {
+  return pbx_fail(c, PBX_ENOMEM, "pbx_linear_logprobs_grad_dev: out of host memory");
 }
