@@ -53,7 +53,8 @@ struct pbx_kv {
   // the kernels for this head size; attention by log2 of the query tiles (4 at most)
   hipFunction_t append = nullptr, read = nullptr, pack = nullptr, attn[3] = {};
   std::vector<pbx_kv_batch *> batches;
-  kv_lists lists;  // of a compaction
+  kv_lists lists;        // of a compaction
+  kv_pack_plan packing;  // the last one, whose memory the next one uses
 };
 
 struct pbx_kv_batch {
@@ -359,7 +360,7 @@ extern "C" int pbx_kv_compact(pbx_kv *kv, int n, const int32_t *seqs, const int3
   const pbx_kv_config &g = kv->cfg;
   try {
     std::string why;
-    kv_pack_plan p;
+    kv_pack_plan &p = kv->packing;
     int rc = kv_plan_pack(&kv->pages, n, seqs, counts, positions, &p, &why);
     if (rc) return pbx_fail(c, rc, "%s: %s", who, why.c_str());
     const size_t n_items = p.items.size() * sizeof(kv_pack_item) / 4;

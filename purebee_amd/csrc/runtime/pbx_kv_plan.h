@@ -339,10 +339,14 @@ inline int kv_plan_pack(kv_pages *kv, int n, const int32_t *seqs, const int32_t 
       snprintf(buf, sizeof buf, "sequence %d twice", s);
     else if (counts[i] < 0 || counts[i] > len)
       snprintf(buf, sizeof buf, "sequence %d holds %d positions, %d are to stay", s, len, counts[i]);
-    for (int j = 0; !buf[0] && j < counts[i]; ++j)
-      if (positions[at + j] < (j ? positions[at + j - 1] + 1 : 0) || positions[at + j] >= len)
+    const int32_t *pos = positions + at;
+    bool rise = true;  // (all of them, without a branch, and the first that does not only then)
+    for (int j = 1; !buf[0] && j < counts[i]; ++j) rise &= pos[j] > pos[j - 1];
+    if (!buf[0] && counts[i]) rise &= pos[0] >= 0 && pos[counts[i] - 1] < len;
+    for (int j = 0; !buf[0] && !rise && j < counts[i]; ++j)
+      if (pos[j] < 0 || pos[j] >= len || (j && pos[j] <= pos[j - 1]))
         snprintf(buf, sizeof buf, "sequence %d: positions have to rise within [0, %d) (%d at place %d)", s, len,
-                 positions[at + j], j);
+                 pos[j], j);
     if (buf[0]) {
       *why = buf;
       return PBX_EINVAL;
@@ -357,13 +361,17 @@ inline int kv_plan_pack(kv_pages *kv, int n, const int32_t *seqs, const int32_t 
     return PBX_ENOTSUP;
   }
   const int T = kv->page_tokens, per_page = T / PBX_KV_BLOCK;
-  // everything that may throw comes first (the log and the lists cannot grow past these)
+  // everything that may throw comes first (the log and the lists cannot grow past these);
+  // a plan that was used before gives its memory
+  p->log.clear();
+  p->launches.clear();
+  p->items.clear();
   p->seqs.assign(seqs, seqs + n);
   p->was.resize(n);
   p->log.reserve(2 * all + 2);
   p->launches.reserve(all + 1);
   p->items.reserve(all * per_page);
-  p->rows.reserve(rows);
+  p->rows.resize(rows);
   std::vector<std::vector<int32_t>> made(n);
   std::vector<int> first(n), read(n);  // first page that is replaced, and old pages that are given back
   std::vector<int> from(n);            // positions from which rows or pages move
@@ -390,14 +398,18 @@ inline int kv_plan_pack(kv_pages *kv, int n, const int32_t *seqs, const int32_t 
     }
   };
   at = 0;
+  int shift = 0, listed = 0;
+  while (1 << shift < T) ++shift;  // (pages are a power of two)
   int done = 0;  // sequences whose old pages were given back
   std::vector<int> need(n, 0);  // old pages that the pages planned so far have read for good
   for (int i = 0; i < n; ++i) {
     const std::vector<int32_t> &old = p->was[i].pages;
-    const int list = (int)p->rows.size(), base = first[i] * T;
+    const int base = first[i] * T, list = listed;
     made[i].assign(old.begin(), old.begin() + first[i]);
-    for (int64_t j = at + base; j < at + counts[i]; ++j)
-      p->rows.push_back({old[(unsigned)positions[j] / (unsigned)T], positions[j]});
+    const int32_t *pages = old.data(), *pos = positions + at;
+    kv_pack_row *out = p->rows.data() + listed;
+    for (int j = base; j < counts[i]; ++j) out[j - base] = {pages[(unsigned)pos[j] >> shift], pos[j]};
+    listed += std::max(0, counts[i] - base);
     need[i] = first[i];
     for (int j = first[i]; j < kv->pages_of(counts[i]); ++j) {
       if (kv->free_list.empty()) {
@@ -425,6 +437,7 @@ inline int kv_plan_pack(kv_pages *kv, int n, const int32_t *seqs, const int32_t 
     }
     at += counts[i];
   }
+  p->rows.resize(listed);
   if (p->items.size() > launched) p->launches.push_back((int32_t)(p->items.size() - launched));
   for (int i = 0; i < n; ++i) give(i, (int)p->was[i].pages.size());
   for (int i = 0; i < n; ++i) {

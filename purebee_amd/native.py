@@ -505,10 +505,13 @@ class Context:
         return ms.value
 
 
+_INT32 = np.dtype(np.int32)
+
+
 def _i32(a):
     """1-D int32 of a's whole numbers; OverflowError for one past 32 bits."""
-    if isinstance(a, np.ndarray) and a.dtype == np.int32 and a.ndim == 1:
-        return np.ascontiguousarray(a)
+    if type(a) is np.ndarray and a.dtype == _INT32 and a.ndim == 1:
+        return a if a.flags.c_contiguous else np.ascontiguousarray(a)
     return np.ascontiguousarray(list(a), np.int32)
 
 
