@@ -101,6 +101,12 @@ static int kv_launch(pbx_ctx *c, hipFunction_t f, const char *name, int64_t grid
   return pbx_launch_fn(c, f, name, dim3((unsigned)grid), dim3(block), args, c->stream);
 }
 
+// Items of a launch at most, where each is a workgroup (of up to 512 threads) a layer and
+// KV head: a grid holds less than 2^32 threads.
+static int kv_items_a_launch(const pbx_kv_config &g) {
+  return (int)std::max<int64_t>(1, (1 << 22) / ((int64_t)g.n_kv_heads * g.n_layers));
+}
+
 // Room for n words of lists, whose last ones the device has read.
 static int lists_room(pbx_ctx *c, kv_lists *l, size_t n, const char *who) {
   if (hipEventSynchronize(l->copied) != hipSuccess)
@@ -374,16 +380,19 @@ extern "C" int pbx_kv_compact(pbx_kv *kv, int n, const int32_t *seqs, const int3
       }
       KvRopeHost r{kv->rope, g.rope_style, g.rope_dim};
       const int32_t *items = l.dev;
-      for (size_t k = 0; k < p.launches.size() && !rc; ++k) {
-        KvPackHost a{kv->codes, kv->scales, (int64_t)kv->layer_codes, (int64_t)kv->layer_scales, items,
-                     l.dev + n_items, p.launches[k], g.n_kv_heads, g.head_dim, kv->page_shift};
-        void *args[] = {&a, &r};
-        rc = kv_launch(c, kv->pack, "pbx_kv_pack", (int64_t)p.launches[k] * g.n_kv_heads * g.n_layers,
-                       pack_threads(kv->hdp), args);
-        // (the first launch writes pages that were free: the sequences are whole until the second)
-        if (rc && k) return rc;
-        items += (size_t)p.launches[k] * sizeof(kv_pack_item) / 4;
-      }
+      const int most = kv_items_a_launch(g);
+      for (size_t k = 0; k < p.launches.size() && !rc; ++k)
+        for (int at = 0; at < p.launches[k] && !rc; at += most) {
+          const int here = std::min(most, p.launches[k] - at);
+          KvPackHost a{kv->codes, kv->scales, (int64_t)kv->layer_codes, (int64_t)kv->layer_scales, items,
+                       l.dev + n_items, here, g.n_kv_heads, g.head_dim, kv->page_shift};
+          void *args[] = {&a, &r};
+          rc = kv_launch(c, kv->pack, "pbx_kv_pack", (int64_t)here * g.n_kv_heads * g.n_layers, pack_threads(kv->hdp),
+                         args);
+          // (the first ones write pages that were free: the sequences are whole until later ones)
+          if (rc && k) return rc;
+          items += (size_t)here * sizeof(kv_pack_item) / 4;
+        }
     }
     if (rc) {
       kv_pack_undo(&kv->pages, &p);
@@ -492,12 +501,16 @@ static int batch_own_pages(pbx_kv_batch *b) {
                       "would leave");
   const int32_t *copies = b->lists.dev + b->at_copies;
   const pbx_kv_config &g = kv->cfg;
-  KvPackHost a{kv->codes, kv->scales, (int64_t)kv->layer_codes, (int64_t)kv->layer_scales, copies, nullptr,
-               (int)p.copies.size(), g.n_kv_heads, 2 * PBX_KV_BLOCK * kv->hdp, kv->page_shift};
-  void *args[] = {&a};
-  const int rc = kv_launch(c, c->fn[PBX_K_KV_COPY], "pbx_kv_copy", (int64_t)p.copies.size() * g.n_kv_heads * g.n_layers,
-                           256, args);
-  if (rc) return rc;
+  const int most = kv_items_a_launch(g), all = (int)p.copies.size();
+  for (int at = 0; at < all; at += most) {
+    KvPackHost a{kv->codes, kv->scales, (int64_t)kv->layer_codes, (int64_t)kv->layer_scales,
+                 copies + (size_t)at * sizeof(kv_page_copy) / 4, nullptr, std::min(most, all - at), g.n_kv_heads,
+                 2 * PBX_KV_BLOCK * kv->hdp, kv->page_shift};
+    void *args[] = {&a};
+    const int rc = kv_launch(c, c->fn[PBX_K_KV_COPY], "pbx_kv_copy", (int64_t)a.n_items * g.n_kv_heads * g.n_layers, 256,
+                             args);
+    if (rc) return rc;
+  }
   for (pbx_kv_batch *o : kv->batches)
     if (knows(o)) o->stale = true;
   return PBX_OK;

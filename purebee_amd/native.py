@@ -512,7 +512,14 @@ def _i32(a):
     """1-D int32 of a's whole numbers; OverflowError for one past 32 bits."""
     if type(a) is np.ndarray and a.dtype == _INT32 and a.ndim == 1:
         return a if a.flags.c_contiguous else np.ascontiguousarray(a)
-    return np.ascontiguousarray(list(a), np.int32)
+    if isinstance(a, np.ndarray) and a.dtype.kind in "iu" and a.ndim == 1:
+        if a.size and not -2**31 <= int(a.min()) <= int(a.max()) < 2**31:
+            raise OverflowError("a number past 32 bits")
+        return np.ascontiguousarray(a, np.int32)
+    out = np.ascontiguousarray(list(a), np.int32)
+    if out.ndim != 1:
+        raise ValueError(f"one row of numbers, not {out.ndim} dimensions")
+    return out
 
 
 def _int32(v):

@@ -431,3 +431,32 @@ def test_long_moves(ctx):
         p.compact([0], [np.r_[:4, 5:p.ref.length(0)]])
     p.check_values()
     p.free()
+
+
+def test_more_blocks_than_a_launch_takes(ctx):
+    """A launch takes 2^22 blocks over all layers and heads: here 10 sequences of 210 blocks of 4,096 layers, compacted
+    and branched; the last layer's values are looked at, and the first one's, which nobody wrote."""
+    layers, n = 4096, 6700
+    p = BranchPair(ctx, 1, 1, 32, seqs=20, n_pages=20 * 7 + 80, page=1024, max_seq=8192, layers=layers, seed=4)
+    for s in range(10):
+        q, k, v = p.rows(n)
+        b = p.cache.batch([s], [n])
+        dk, dv = Rows(ctx, n, 32, k), Rows(ctx, n, 32, v)
+        b.append_dev(layers - 1, None, dk.ptr, dv.ptr, None)
+        ctx.sync()
+        p.ref.append([s], [n], q, k, v)
+        for x in (dk, dv, b):
+            x.free()
+    p.compact(list(range(10)), [np.r_[1:n]] * 10)
+    p.check_values(range(10), layer=layers - 1)
+    p.fork(list(range(10, 20)), list(range(10)))
+    p.append(list(range(10, 20)), [1] * 10, layer=layers - 1)
+    p.check_values(layer=layers - 1)
+    got = Rows(ctx, 1, 32)
+    b = p.cache.batch([3], [1], [5000])
+    b.read_dev(0, got.ptr, None)
+    ctx.sync()
+    assert not got.get().any()
+    got.free()
+    b.free()
+    p.free()

@@ -4,6 +4,7 @@ import os
 import shutil
 import subprocess
 
+import numpy as np
 import pytest
 
 from purebee_amd import native
@@ -35,3 +36,19 @@ def test_null_handles_are_refused():
     for rc in (L.pbx_kv_fork(None, 0, None, None, None), L.pbx_kv_compact(None, 0, None, None, None)):
         assert rc == -1
         assert b"not a live cache" in L.pbx_last_error(None)
+
+
+def test_lists_of_numbers():
+    """What sequences and positions may be given as."""
+    for a in ([3, 1, 2**31 - 1], (3, 1, 2**31 - 1), np.array([3, 1, 2**31 - 1]), np.array([3, 1, 2**31 - 1], np.uint32),
+              np.array([3, 0, 1, 0, 2**31 - 1, 0], np.int32)[::2]):
+        got = native._i32(a)
+        assert got.dtype == np.int32 and got.flags.c_contiguous and got.tolist() == [3, 1, 2**31 - 1]
+    for empty in ([], np.zeros(0, np.int64), np.zeros(0, np.int32), range(0)):
+        assert native._i32(empty).shape == (0,)
+    for a in ([2**31], np.array([-2**31 - 1]), np.array([2**31], np.uint32), np.array([2**63], np.uint64)):
+        with pytest.raises(OverflowError):
+            native._i32(a)
+    for a in ([[1, 2], [3, 4]], np.ones((2, 2), np.int32), np.ones((2, 2), np.int64)):
+        with pytest.raises(ValueError):
+            native._i32(a)
