@@ -352,12 +352,18 @@ int pbx_gemm_launch(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M6
 // Workgroups of the GEMM whose epilogue takes a head's logits: 32 rows, or 128, or 64
 // where those leave out a half-empty 128 of at most eight; by 128 columns.
 static int head_rows(int M) { return M <= 32 ? 32 : (M + 63) / 64 % 2 && M <= 960 ? 64 : 128; }
+// 33 to 64 rows are two workgroups of 32 where as many of 64 would leave half of the CUs
+// without one (us, 32 / 64: 50 rows of 16000 x 2048 Q4_0 (125 tiles) 29 / 35, 8000 x 2048 28 / 34;
+// 37 rows of 32003 x 2048 F16 (251) 51 / 39, 64 of Q8_0 49 / 42).
+static int head_rows(const pbx_ctx *c, int N, int M) {
+  return M <= 64 && 2 * ((N + 127) / 128) <= c->cu_count ? 32 : head_rows(M);
+}
 
 // Where it is faster than the linear's own kernels and a pass over their logits.  Its
 // time for a tile is that of K (8 us and 9 for each 1,000 columns of 32 rows), since K
 // is not split, so it wants enough tiles (us, it / they):
 // * more than 32 rows: 3000 x 2048 Q8_0 40 rows (24 workgroups) 36 / 28, 130 (72) 38 / 36,
-//   300 (120) 39 / 42; 8000 x 2048 Q4_0 40 rows (63) 33 / 35; 1000 x 512 (8) 16 / 19.
+//   300 (120) 39 / 42; 8000 x 2048 Q4_0 40 rows (63; 126 of 32 rows) 28 / 35; 1000 x 512 (8) 16 / 19.
 // * 3 to 32 rows: 16000 x 2048 Q8_0 (125) 8 rows 28 / 24, 32 rows 28 / 40; 24000 x 2048
 //   Q4_0 (188) 3 rows 27 / 25, 8 rows 27 / 38; 128256 x 2048 Q8_0 4 rows 87 / 92, 32 rows
 //   89 / 119; short K from less on: 8000 x 512 Q4_0 (63) 8 rows 12.6 / 13.0, 32 rows 12.9 / 16.6.
@@ -404,7 +410,7 @@ int pbx_gemm_head_prep(pbx_ctx *c, const float *dX, int M, int K, void *x16, voi
 }
 
 int pbx_gemm_head(pbx_ctx *c, const pbx_weight *w, int M, void *space, const pbx_head_epilogue &e) {
-  const int rows = head_rows(M);
+  const int rows = head_rows(c, (int)w->N, M);
   const std::string name = std::string("pbx_gemm_") + gemm_tag(w->type) +
                            (rows == 32 ? "_b32" : rows == 64 ? "_b64" : "_big") + (e.lse ? "_g" : "_sums");
   hipFunction_t f = pbx_kernel_by_name(c, name);
