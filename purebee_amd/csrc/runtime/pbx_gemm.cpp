@@ -352,11 +352,14 @@ int pbx_gemm_launch(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M6
 // Workgroups of the GEMM whose epilogue takes a head's logits: 32 rows, or 128, or 64
 // where those leave out a half-empty 128 of at most eight; by 128 columns.
 static int head_rows(int M) { return M <= 32 ? 32 : (M + 63) / 64 % 2 && M <= 960 ? 64 : 128; }
-// 33 to 64 rows are two workgroups of 32 where as many of 64 would leave half of the CUs
-// without one (us, 32 / 64: 50 rows of 16000 x 2048 Q4_0 (125 tiles) 29 / 35, 8000 x 2048 28 / 34;
-// 37 rows of 32003 x 2048 F16 (251) 51 / 39, 64 of Q8_0 49 / 42).
+// Half as many rows where half of the CUs would have no workgroup (us, half / whole: 50 rows
+// of 16000 x 2048 Q4_0 (125 tiles) 29 / 35, 8000 x 2048 28 / 34, but 37 rows of 32003 x 2048
+// F16 (251) 51 / 39, 64 of Q8_0 49 / 42; 100 rows of 8000 x 2048 Q4_0 30 / 48 (35 of 64), 200 of
+// Q8_0 41 / 50, 500 of 3000 x 1024 26 / 32, 1000 of 1000 x 2048 33 / 52).
 static int head_rows(const pbx_ctx *c, int N, int M) {
-  return M <= 64 && 2 * ((N + 127) / 128) <= c->cu_count ? 32 : head_rows(M);
+  int rows = head_rows(M);
+  while (rows > 32 && 2 * (int64_t)((N + 127) / 128) * ((M + rows - 1) / rows) <= c->cu_count) rows /= 2;
+  return rows;
 }
 
 // Where it is faster than the linear's own kernels and a pass over their logits.  Its
