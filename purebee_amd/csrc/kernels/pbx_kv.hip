@@ -364,10 +364,10 @@ __device__ __forceinline__ int64_t block_index(const KvPack &a, int page, int he
 // apart for consecutive dims, so one row takes as many cache lines as the whole block:
 // the blocks' values are fetched whole, PACK_BLOCKS at a time, into LDS, where the 64
 // bytes of a dim take 68, so that dims fall in banks of their own.
-// 60,000 of 125,000 positions, 8 KV heads of 128, two layers: 109 us, where the codes
-// read and written (156 MB) take 32; rows kept singly come from nearly as many blocks, so
-// it is the chain of list, scales and codes that a workgroup waits for, and 40% of the
-// issue slots, that are left.  A cut of 2,000 positions, heads of 64: 8 us.
+// Half of 30,600 positions, kept here and there, 8 KV heads of 128, two layers: 109 us,
+// where the codes read and written (156 MB) take 32; vector instructions fill 60% of the
+// issue slots, and a workgroup waits for its chain of list, scales, codes and largest
+// magnitudes.  A window of 1,000 of 5,000 positions, heads of 64: 8 us.
 constexpr int PACK_BLOCKS = 4;
 constexpr int pack_threads(int hdp) { return hdp <= 64 ? 256 : 2 * hdp; }
 __device__ __forceinline__ int spread_byte(int key, int dim) {
