@@ -24,8 +24,8 @@ struct KvRopeHost {  // KvRope in pbx_kv.hip
 };
 
 // Lists that a call makes on the host: written to coherent pinned memory, from where a
-// kernel copies them to the device, in order with the context's other work (a copy
-// operation of the runtime costs twice as much there and back).
+// kernel copies them to the device, in order with the context's other work (setting a
+// small batch took 17.6 us with a copy operation of the runtime, 14.2 so).
 struct kv_lists {
   int32_t *host = nullptr, *mapped = nullptr, *dev = nullptr;
   size_t host_cap = 0, dev_cap = 0;
