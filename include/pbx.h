@@ -484,7 +484,9 @@ int pbx_kv_fork(pbx_kv *kv, int n, const int32_t *dsts, const int32_t *srcs, con
  * least one (PBX_ENOMEM, and nothing changed; the fewer there are, the more launches),
  * and given back; sequences that share them keep theirs.  Batches over moved positions
  * are refused from then on.  Enqueues on the context's stream, and waits for no GPU work
- * but the lists of the compaction before. */
+ * but the lists of the compaction before.  Where a launch fails (PBX_EHIP) nothing changed,
+ * or, if ones before it wrote pages that were given back, the sequences are left with the
+ * positions in pages before the first row that moves. */
 int pbx_kv_compact(pbx_kv *kv, int n, const int32_t *seqs, const int32_t *counts, const int32_t *positions);
 
 /* A batch: counts[i] rows of sequence seqs[i] (none twice) at the positions

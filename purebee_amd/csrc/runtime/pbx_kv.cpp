@@ -371,6 +371,7 @@ extern "C" int pbx_kv_compact(pbx_kv *kv, int n, const int32_t *seqs, const int3
     if (rc) return pbx_fail(c, rc, "%s: %s", who, why.c_str());
     const size_t n_items = p.items.size() * sizeof(kv_pack_item) / 4;
     const size_t words = n_items + p.rows.size() * sizeof(kv_pack_row) / 4;
+    bool lost = false;  // a launch that wrote pages given back before is under way
     if (words) {
       kv_lists &l = kv->lists;
       if (!(rc = lists_room(c, &l, words, who))) {
@@ -389,21 +390,21 @@ extern "C" int pbx_kv_compact(pbx_kv *kv, int n, const int32_t *seqs, const int3
           void *args[] = {&a, &r};
           rc = kv_launch(c, kv->pack, "pbx_kv_pack", (int64_t)here * g.n_kv_heads * g.n_layers, pack_threads(kv->hdp),
                          args);
-          // (the first ones write pages that were free: the sequences are whole until later ones)
-          if (rc && k) return rc;
+          lost = lost || (!rc && k);  // (the first ones write pages that were free)
           items += (size_t)here * sizeof(kv_pack_item) / 4;
         }
     }
-    if (rc) {
+    if (rc && !lost) {
       kv_pack_undo(&kv->pages, &p);
       return rc;
     }
+    if (rc) kv_pack_cut(&kv->pages, p);
     for (pbx_kv_batch *b : kv->batches)
       if (kv_plan_moved(kv->pages, b->plan)) b->stale = true;
+    return rc;
   } catch (const std::bad_alloc &) {
     return pbx_fail(c, PBX_ENOMEM, "%s: out of host memory", who);
   }
-  return PBX_OK;
 }
 
 extern "C" int pbx_kv_batch_create(pbx_kv *kv, pbx_kv_batch **out) {

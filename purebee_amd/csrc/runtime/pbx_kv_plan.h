@@ -319,6 +319,14 @@ inline void kv_pack_undo(kv_pages *kv, kv_pack_plan *p) {
   p->was.clear();
 }
 
+// Where a compaction ends with some of its launches missing, after others wrote pages that
+// were given back before: neither the old rows nor the new ones are whole, and the sequences
+// are cut to the positions before those that move.
+inline void kv_pack_cut(kv_pages *kv, const kv_pack_plan &p) {
+  std::string why;
+  for (int32_t s : p.seqs) kv->truncate(s, std::min(kv->seqs[s].len, kv->seqs[s].moved_at), &why);
+}
+
 // Sequence seqs[i] keeps counts[i] of its positions (rising; `positions` holds them
 // one sequence after the other), which move together to 0 .. counts[i] - 1.  Pages
 // whose rows all stay are kept; the rest goes to fresh pages, so that no block is
