@@ -487,19 +487,26 @@ static int batch_upload(pbx_kv_batch *b) {
   return lists_send(c, &b->lists, n, "pbx_kv_batch_set");
 }
 
-// Pages that the batch's sequences shared, copied for them.  Other batches that run
-// over those sequences know the old pages: they have to be set again, and a graph
-// that holds one cannot be, so then the batch is refused.
+// Whether batch o, of another plan than the last one, runs over pages that this one's
+// sequences left for copies.
+static bool knows_left(const pbx_kv *kv, const pbx_kv_batch *o) { return !o->stale && kv_plan_moved(kv->pages, o->plan); }
+
+// Other batches that run over sequences which get copies of pages know the old pages: they
+// have to be set again, and a graph that holds one cannot be, so then the batch is refused.
+static int batch_may_own(const pbx_kv_batch *b, const kv_batch_plan &p) {
+  for (const pbx_kv_batch *o : b->kv->batches)
+    if (!p.copies.empty() && o != b && o->captured && knows_left(b->kv, o))
+      return pbx_fail(b->kv->c, PBX_EINVAL, "pbx_kv_batch_set: a captured graph runs over pages that a sequence shares "
+                      "and would leave");
+  return PBX_OK;
+}
+
+// Pages that the batch's sequences shared, copied for them.
 static int batch_own_pages(pbx_kv_batch *b) {
   pbx_kv *kv = b->kv;
   pbx_ctx *c = kv->c;
   const kv_batch_plan &p = b->plan;
   if (p.copies.empty()) return PBX_OK;
-  auto knows = [&](const pbx_kv_batch *o) { return o != b && !o->stale && kv_plan_moved(kv->pages, o->plan); };
-  for (const pbx_kv_batch *o : kv->batches)
-    if (o->captured && knows(o))
-      return pbx_fail(c, PBX_EINVAL, "pbx_kv_batch_set: a captured graph runs over pages that a sequence shares and "
-                      "would leave");
   const int32_t *copies = b->lists.dev + b->at_copies;
   const pbx_kv_config &g = kv->cfg;
   const int most = kv_items_a_launch(g), all = (int)p.copies.size();
@@ -513,7 +520,7 @@ static int batch_own_pages(pbx_kv_batch *b) {
     if (rc) return rc;
   }
   for (pbx_kv_batch *o : kv->batches)
-    if (knows(o)) o->stale = true;
+    if (o != b && knows_left(kv, o)) o->stale = true;
   return PBX_OK;
 }
 
@@ -534,6 +541,10 @@ extern "C" int pbx_kv_batch_set(pbx_kv_batch *b, int n, const int32_t *seqs, con
     kv_batch_plan plan;
     int rc = kv_plan_rows(&kv->pages, n, seqs, starts, counts, &plan, &why);
     if (rc) return pbx_fail(c, rc, "pbx_kv_batch_set: %s", why.c_str());
+    if ((rc = batch_may_own(b, plan))) {
+      kv_plan_undo(&kv->pages, plan);
+      return rc;
+    }
     b->set = false;
     try {
       std::swap(b->plan, plan);

@@ -138,9 +138,33 @@ static void failed_compactions() {
   }
 }
 
+// A batch that is refused, because a captured graph reads a page that its sequence would
+// leave, stays what it was.
+static void refused_sets() {
+  Cache k(8);
+  pbx_kv_batch *b = k.batch(0, 0, 50), *reads = nullptr;
+  const int32_t one = 1, zero = 0, more = 2;
+  CHECK(pbx_kv_fork(k.kv, 1, &one, &zero, nullptr) == PBX_OK);
+  b = k.batch(1, 0, 50);
+  reads = k.batch(1, 0, 50);
+  capturing = true;
+  CHECK(read(reads) == PBX_OK);
+  CHECK(pbx_kv_batch_set(b, 1, &one, nullptr, &more) == PBX_EINVAL);  // (inside a capture none is set)
+  capturing = false;
+  int rows = 0;
+  for (int again = 0; again < 2; ++again) {
+    CHECK(pbx_kv_batch_set(b, 1, &one, nullptr, &more) == PBX_EINVAL && strstr(said, "captured graph"));
+    CHECK(k.length(1) == 50 && k.free_pages() == 6);
+    CHECK(pbx_kv_batch_rows(b, &rows) == PBX_OK && rows == 50 && read(b) == PBX_OK && read(reads) == PBX_OK);
+  }
+  CHECK(pbx_kv_batch_free(reads) == PBX_OK);
+  CHECK(pbx_kv_batch_set(b, 1, &one, nullptr, &more) == PBX_OK && k.length(1) == 52 && k.free_pages() == 5);
+}
+
 int main(int argc, char **argv) {
   const std::string what = argc > 1 ? argv[1] : "";
   if (what == "failed_compactions") failed_compactions();
+  else if (what == "refused_sets") refused_sets();
   else return 2;
   return 0;
 }

@@ -34,3 +34,8 @@ def host(tmp_path_factory):
 def test_a_compaction_that_fails_midway(host):
     """Sequences keep what had not moved, and batches over the rest are refused."""
     host("failed_compactions")
+
+
+def test_a_refused_set_changes_nothing(host):
+    """Neither the sequences nor the batch, which goes on with the rows that it had."""
+    host("refused_sets")
