@@ -374,7 +374,7 @@ __device__ __forceinline__ int spread_byte(int key, int dim) {
   const int slot = 8 * ((key >> 2) & 3) + 4 * (key >> 4) + (key & 3);
   return (dim >> 5) * 1088 + (dim & 15) * 68 + (slot >> 3) * 16 + ((dim >> 4) & 1) * 8 + (slot & 7);
 }
-constexpr float NEAR_LARGEST = 1.f - 0x1p-17f, NEAR_BORDER = 2e-4f;
+constexpr float LARGEST = 3.402823466e38f, NEAR_LARGEST = 1.f - 0x1p-17f, NEAR_BORDER = 2e-4f;
 
 // y / s rounded half to even from q, which is it in f32 to 10^-4: where q is near the
 // border k + 1/2, by 2 |y| against (2 k + 1) s, which are exact.
@@ -534,6 +534,16 @@ __device__ __forceinline__ void pack_body(const KvPack &a, const KvRope &r) {
     mk = fmaxf(mk, red[0][w]);
     mv = fmaxf(mv, red[1][w]);
   }
+  // (127 times the scale of f32's largest number rounds past it)
+  if (!(mv < INFINITY)) {
+    mv = LARGEST;
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) {
+      pv[i] = fminf(pv[i], LARGEST);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) vc[i][e] = fminf(fmaxf(vc[i][e], -LARGEST), LARGEST);
+    }
+  }
   auto exact_keys = [&](int i, double x[4]) {
     const double s = sk[kw(i)];
 #pragma unroll
@@ -546,7 +556,7 @@ __device__ __forceinline__ void pack_body(const KvPack &a, const KvRope &r) {
     return s > 0.f ? (double)rintf(vc[i][e] / s) * (double)s : 0.0;
   };
   // what may be the largest, in 64 bits
-  const float near_k = mk * NEAR_LARGEST, near_v = mv * NEAR_LARGEST;
+  const float near_k = fminf(mk, LARGEST) * NEAR_LARGEST, near_v = mv * NEAR_LARGEST;
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
     if (mk > 0.f && pk[i] >= near_k) {
