@@ -528,7 +528,8 @@ pbx_head_twice(uint4 *hi, uint4 *lo, int64_t n16) {
 namespace {
 
 // The power of two that weights enter the products with: the largest scale (or Q4_1
-// minimum) comes to just below 2^TARGET.
+// minimum) comes to just below 2^TARGET, or less: 2^21 times it, as 2^(21 + 9) is two
+// halves' product (back_body).
 __device__ __forceinline__ int head_shift(const unsigned *peaks, int target) {
   unsigned m = 0;
   for (int i = threadIdx.x & 63; i < HEAD_PEAKS; i += 64) m = max(m, peaks[i]);
@@ -537,7 +538,7 @@ __device__ __forceinline__ int head_shift(const unsigned *peaks, int target) {
   int e = 0;
   if (m) frexpf(f16_bits_to_f32(m), &e);  // 2^(e - 1) <= it < 2^e
   if (m >= 0x7c00u) e = 16;
-  return __builtin_amdgcn_readfirstlane(target - e);
+  return __builtin_amdgcn_readfirstlane(min(target - e, 21));
 }
 template <int TYPE> struct HeadTarget { static constexpr int value = TYPE == PBX_Q8 ? -5 : TYPE == PBX_Q6K ? -10 : TYPE == PBX_Q41 ? -2 : -1; };
 
