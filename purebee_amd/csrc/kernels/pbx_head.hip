@@ -858,8 +858,8 @@ __device__ __forceinline__ void back_body(const BackArgs &a) {
     __syncthreads();
   }
   if (wave) return;
-  const float undo = power_of_two(min(127, max(-126, TYPE == PBX_F16 && a.n_f_peaks ? head_f_peak(a.f_peaks, a.n_f_peaks) - 15
-                                                                          : -15 - shift)));
+  // (of pairs down to 2^-140, so no factor)
+  const int undo = TYPE == PBX_F16 && a.n_f_peaks ? head_f_peak(a.f_peaks, a.n_f_peaks) - 15 : -15 - shift;
   float *part = a.part + (int64_t)blockIdx.z * a.M * a.K;
 #pragma unroll
   for (int t = 0; t < TT; ++t)
@@ -871,7 +871,7 @@ __device__ __forceinline__ void back_body(const BackArgs &a) {
         const int k = k0 + column_of<TYPE>(lr, i);
         if (m >= a.M || k >= a.K) continue;
         float *p = part + (int64_t)m * a.K + k;
-        const float x = acc[t][i][r] * undo;
+        const float x = ldexpf(acc[t][i][r], undo);
         *p = a.add ? *p + x : x;
       }
     }

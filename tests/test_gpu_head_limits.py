@@ -29,3 +29,14 @@ def test_smallest_scales(ctx, kind, M, top):
     got, dx = check(head, x, targets_of(M, 700), np.ones(M))
     assert dx.any()
     head.free()
+
+
+@pytest.mark.parametrize("M", [2, 100])
+@pytest.mark.parametrize("scale", [1e-30, 1e-33])
+def test_tiny_weights_as_pairs(ctx, M, scale):
+    """F32 heads that become pairs of halves, all of whose weights are below 2^-97."""
+    rng = np.random.default_rng(8)
+    w = scale * rng.standard_normal((13000, 1024)) * np.logspace(-2, 0, 13000)[rng.permutation(13000)][:, None]
+    head = Head(ctx, "f32", w)
+    check(head, rows_of(M, 1024, size=0.05 / scale), targets_of(M, 13000), np.ones(M))
+    head.free()
