@@ -172,7 +172,7 @@ struct SixArgs {
 // in flight; the lanes' sums of four rows are added in 7 steps instead of 24, halving what
 // each lane holds.
 // Up to 2,048 columns (one pass of the lanes) the lane keeps its activations as integers
-// of up to 8,355,711 in three signed bytes (0.5 / 2^22 of the row's largest is what they
+// of up to 8,355,711 in three signed bytes (0.5 / 2^22 of the largest of its 32 is what they
 // may be off), so that v_dot4 sums four products with codes exactly; 32 times the bytes'
 // sums, for codes less 32, is taken off as an integer.  Longer rows: f32.
 // 128,256 x 2,048: 56 us with f32 products, 207 vector instructions a row (43 us of them).
@@ -221,7 +221,6 @@ __device__ __forceinline__ void six_body(const SixArgs &a) {
         most = fmaxf(most, fabsf(v[j]));
         odd = odd || !(fabsf(v[j]) < INFINITY);
       }
-      most = wave_max(most);  // (slots hold the same row)
       int e = 0;
       if (most > 0.f && most < INFINITY) frexpf(most, &e);
       e = max(e, -100);
@@ -296,7 +295,7 @@ __device__ __forceinline__ void six_body(const SixArgs &a) {
         for (int m = 0; m < M; ++m) {
           const float s0 = fmaf((float)t[m][0][2], 65536.f, fmaf((float)t[m][0][1], 256.f, (float)t[m][0][0]));
           const float s1 = fmaf((float)t[m][1][2], 65536.f, fmaf((float)t[m][1][1], 256.f, (float)t[m][1][0]));
-          z[m][r] = fmaf(d0, s0, fmaf(d1, s1, z[m][r]));
+          z[m][r] = unit[m] * fmaf(d0, s0, d1 * s1);
         }
         continue;
       }
@@ -352,7 +351,6 @@ __device__ __forceinline__ void six_body(const SixArgs &a) {
       const float v = (b0 ? z[m][3] : z[m][2]) + partner<1>(b0 ? z[m][2] : z[m][3], lane);
       u = (b1 ? v : u) + partner<2>(b1 ? u : v, lane);
       u += partner<4>(u, lane);
-      if constexpr (WHOLE) u *= unit[m];
       if constexpr (LANES > 8) u += partner<8>(u, lane);
       if constexpr (LANES > 16) u += partner<16>(u, lane);
       if constexpr (LANES > 32) u += partner<32>(u, lane);

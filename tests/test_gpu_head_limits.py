@@ -3,8 +3,9 @@ probabilities come to their formats' ends, on the GPU against tests/head_ref.py.
 import numpy as np
 import pytest
 
-from tests.head_ref import Head
-from tests.test_gpu_head import check, rows_of, targets_of
+from tests.head_ref import Head, forward, gradient
+from tests.kv_ref import within
+from tests.test_gpu_head import Call, check, rows_of, targets_of
 
 pytestmark = pytest.mark.gpu
 
@@ -39,4 +40,30 @@ def test_tiny_weights_as_pairs(ctx, M, scale):
     w = scale * rng.standard_normal((13000, 1024)) * np.logspace(-2, 0, 13000)[rng.permutation(13000)][:, None]
     head = Head(ctx, "f32", w)
     check(head, rows_of(M, 1024, size=0.05 / scale), targets_of(M, 13000), np.ones(M))
+    head.free()
+
+
+@pytest.mark.parametrize("M", [1, 2, 3])
+@pytest.mark.parametrize("V,K", [(700, 512), (1000, 1024), (333, 2048), (200, 2560)])
+def test_columns_far_larger_than_the_rest(ctx, M, V, K):
+    """Rows before a head have outliers: 256 columns are 10^5 times the others, which keep their bits.  Their weights
+    are zeros, so the answer is that of the rows without them."""
+    rng = np.random.default_rng(V)
+    w = 0.05 * rng.standard_normal((V, K))
+    w[:, 256:512] = 0
+    head = Head(ctx, "q6_k", w)
+    assert not head.values[:, 256:512].any()
+    x, target = rows_of(M, K, seed=K), rng.integers(0, V, M)
+    clean = x.copy()
+    x[:, 256:512] *= 1e5
+    clean[:, 256:512] = 0
+    c = Call(head, x, target)
+    c.forward()
+    c.backward()
+    got, dx = c.answers(), c.gradient()
+    want, tol, _ = forward(head.values, clean, target)
+    for n in got:
+        within(got[n], want[n], tol[n])
+    within(dx, *gradient(head.values, clean, target, np.ones(M)))
+    c.free()
     head.free()
