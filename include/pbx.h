@@ -584,8 +584,11 @@ int pbx_linear_logprobs_dev(pbx_ctx *ctx, const pbx_weight *W, const float *dX, 
  *   = dGradLogp[r] * (W[dTargets[r]] - sum_v e^(logit_v - dLse[r]) W[v]),
  * 0 where a row's target is outside the vocabulary (padding), [rows][K], 16-byte aligned,
  * not dX itself.  dLse as pbx_linear_logprobs_dev gave it for these rows.  Logits are
- * computed again; probabilities and weights enter the second product with 22 bits
- * (weights 2^-26 of the largest that the head's largest scale allows at least), sums are
+ * computed again; of a target that is likelier than not, 1 - e^(logit - dLse) is taken as
+ * the sum of the other entries' e^(logit_v - dLse), which keeps its bits however near to 1
+ * the target comes.  Probabilities enter the second product with 22 bits, or with 2^-40 of
+ * what the head's largest row would add where that is more, and weights with 22 bits
+ * (2^-26 of the largest that the head's largest scale allows at least); sums are
  * held in f32 and come out the same in every call.  The weights stay as they are: they
  * have no gradient. */
 int pbx_linear_logprobs_grad_dev(pbx_ctx *ctx, const pbx_weight *W, const float *dX, int64_t rows,

@@ -593,13 +593,15 @@ struct HeadArgs {
   const int *targets;
   float4 *parts;  // [M][n_parts], from part0 on
   int n_parts, part0;
-  float *hit;     // or null
+  float *hit;     // the targets' logits, or null; HEAD_G: less lse
   const float *lse;
   _Float16 *hi, *lo;  // [blocks of 32 entries][Mpad][32]
   int Mpad, v0, vocab;
   const int *f;        // or null: column n's products are 2^-f[n] of a logit
   const int *f_peaks;  // the largest f of parts of them
   int n_f_peaks;
+  float *others;       // [M][n_others]: sums of the other entries' e^(l - lse) by tile of a piece
+  int n_others, add;   // add: to those of the pieces before
 };
 
 // The workgroup's MT x 128 tile by way of LDS (Z, rows of 132 floats, so that 8 rows'
@@ -667,6 +669,15 @@ __device__ __forceinline__ void head_tile(const GemmArgs &a, const HeadArgs &e, 
     const int t = m < a.M ? e.targets[m] : -1;
     const bool on = t >= 0 && t < e.vocab;
     const float s = on ? e.lse[m] : 0.f;
+    // the target among the thread's columns, if it is there
+    const int64_t own = on ? (int64_t)t - e.v0 - n : -1;
+    const int hit = own >= 0 && own < C ? (int)own : -1;
+    float others = 0.f, at_hit = 0.f;
+    if (hit >= 0) {
+      const float d = z[hit] - s;
+      e.hit[m] = d;
+      at_hit = head_target_g(d);
+    }
 #pragma unroll
     for (int c = 0; c < C; c += 8) {
       const float4 x0 = *reinterpret_cast<const float4 *>(z + c), x1 = *reinterpret_cast<const float4 *>(z + c + 4);
@@ -674,10 +685,9 @@ __device__ __forceinline__ void head_tile(const GemmArgs &a, const HeadArgs &e, 
       half8 H, L;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float d = x[i] - s;
-        float g = on && n + c + i < a.N ? -expf(d) : 0.f;
-        if (on && e.v0 + n + c + i == t) g = -expm1f(d);
-        g *= 32768.f;
+        const float d = x[i] - s, q = on && n + c + i < a.N ? expf(d) : 0.f;
+        float g = (c + i == hit ? at_hit : -q) * 32768.f;
+        others += c + i == hit ? 0.f : q;
         if (e.f) g = ldexpf(g, e.f[min(n + c + i, a.N - 1)] - peak);
         H[i] = (_Float16)g;
         L[i] = (_Float16)(g - (float)H[i]);
@@ -687,6 +697,12 @@ __device__ __forceinline__ void head_tile(const GemmArgs &a, const HeadArgs &e, 
         *reinterpret_cast<half8 *>(e.hi + at) = H;
         *reinterpret_cast<half8 *>(e.lo + at) = L;
       }
+    }
+#pragma unroll
+    for (int off = 1; off < TR; off *= 2) others += __shfl_xor(others, off);
+    if (part == 0 && on) {
+      float *p = e.others + (size_t)m * e.n_others + blockIdx.x;
+      *p = e.add ? *p + others : others;
     }
   }
 }

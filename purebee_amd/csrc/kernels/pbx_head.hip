@@ -5,7 +5,8 @@
 //   lse = m + log S,  log p_t = l_t - lse,  entropy = log S - T / S,
 // where (m, S, T) of parts of the vocabulary join as
 //   S = S1 e^(m1 - m) + S2 e^(m2 - m),  T = sum (Ti + (mi - m) Si) e^(mi - m);
-// and d log p_t / dx = W_t - sum_v p_v W_v = sum_v G_v W_v with G = (v == t) - e^(l - lse).
+// and d log p_t / dx = W_t - sum_v p_v W_v = sum_v G_v W_v with G = (v == t) - e^(l - lse),
+// G_t being the sum of the others' e^(l - lse), too.
 
 #include "pbx_head_peaks.h"
 
@@ -544,12 +545,15 @@ template <int TYPE> struct HeadTarget { static constexpr int value = TYPE == PBX
 
 // G of a piece as fp16 pairs times 2^15, [n / 32][Mpad][32]: workgroup (block of 32
 // vocabulary entries, 64 rows); zeros past the vocabulary, the rows, and in rows
-// without a target.  Workgroups past the blocks (HEAD_PEAKS of them where there are any)
+// without a target; and each row's others [M][n_others], by block of a piece (add: to those
+// of the pieces before), and hit, the target's logit less lse.  Workgroups past the blocks
+// (HEAD_PEAKS of them where there are any)
 // look for the head's largest scales.  Few rows, where the GEMM's epilogue does not take
 // the head: a pass over the piece's logits, bound by bytes.
 extern "C" __global__ void __launch_bounds__(256)
 pbx_head_g(const float *Z, int64_t stride, int n, int v0, const float *lse, const int *targets, int vocab, int M,
-           int Mpad, _Float16 *hi, _Float16 *lo, int blocks, const uint16_t *scales, int64_t n8, unsigned *peaks) {
+           int Mpad, _Float16 *hi, _Float16 *lo, int blocks, const uint16_t *scales, int64_t n8, unsigned *peaks,
+           float *hit, float *others, int n_others, int add) {
   if ((int)blockIdx.x >= blocks) {
     if (blockIdx.y == 0) head_peaks(scales, n8, peaks, blockIdx.x - blocks);
     return;
@@ -558,6 +562,7 @@ pbx_head_g(const float *Z, int64_t stride, int n, int v0, const float *lse, cons
   if (row >= Mpad) return;
   half8 H = {}, L = {};
   const int t = row < M ? targets[row] : -1;
+  float sum = 0.f;
   if (t >= 0 && t < vocab) {
     const float *z = Z + (int64_t)row * stride;
     const float s = lse[row];
@@ -565,7 +570,14 @@ pbx_head_g(const float *Z, int64_t stride, int n, int v0, const float *lse, cons
     for (int e = 0; e < 8; ++e) {
       if (v + e >= n) continue;
       const float d = z[v + e] - s;
-      const float g = (v0 + v + e == t ? -expm1f(d) : -expf(d)) * 32768.f;
+      float g = -expf(d);
+      if (v0 + v + e == t) {
+        g = head_target_g(d);
+        hit[row] = d;
+      } else {
+        sum -= g;
+      }
+      g *= 32768.f;
       H[e] = (_Float16)g;
       L[e] = (_Float16)(g - (float)H[e]);
     }
@@ -573,26 +585,45 @@ pbx_head_g(const float *Z, int64_t stride, int n, int v0, const float *lse, cons
   const int64_t at = ((int64_t)blockIdx.x * Mpad + row) * 32 + 8 * (threadIdx.x % 4);
   *reinterpret_cast<half8 *>(hi + at) = H;
   *reinterpret_cast<half8 *>(lo + at) = L;
+  sum += __shfl_xor(sum, 1);
+  sum += __shfl_xor(sum, 2);
+  if (threadIdx.x % 4 == 0 && row < M) {
+    float *p = others + (int64_t)row * n_others + blockIdx.x;
+    *p = add ? *p + sum : sum;
+  }
 }
 
 // The same in f32 for an F32 head: [n][Mpad].
 extern "C" __global__ void __launch_bounds__(256)
 pbx_head_g32(const float *Z, int64_t stride, int n, int v0, const float *lse, const int *targets, int vocab, int M,
-             int Mpad, float *G) {
-  const int row = blockIdx.y * 64 + (threadIdx.x & 63), v = blockIdx.x * 32 + 8 * (threadIdx.x >> 6);
-  if (row >= Mpad) return;
+             int Mpad, float *G, float *hit, float *others, int n_others, int add) {
+  __shared__ float sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = blockIdx.y * 64 + lane, v = blockIdx.x * 32 + 8 * wave;
   const int t = row < M ? targets[row] : -1;
   const bool on = t >= 0 && t < vocab;
   const float s = on ? lse[row] : 0.f;
+  float sum = 0.f;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     float g = 0.f;
     if (on && v + e < n) {
       const float d = Z[(int64_t)row * stride + v + e] - s;
-      g = v0 + v + e == t ? -expm1f(d) : -expf(d);
+      g = -expf(d);
+      if (v0 + v + e == t) {
+        g = head_target_g(d);
+        hit[row] = d;
+      } else {
+        sum -= g;
+      }
     }
-    G[(int64_t)(v + e) * Mpad + row] = g;
+    if (row < Mpad) G[(int64_t)(v + e) * Mpad + row] = g;
   }
+  sums[wave][lane] = sum;
+  __syncthreads();
+  if (wave || row >= M) return;
+  sum = sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane];
+  float *p = others + (int64_t)row * n_others + blockIdx.x;
+  *p = add ? *p + sum : sum;
 }
 
 struct BackArgs {
@@ -933,28 +964,60 @@ HEAD_BACK(f16, PBX_F16)
 extern "C" __global__ void __launch_bounds__(64) pbx_head_back_f32_1(BackArgs a) { back_f32<1>(a); }
 extern "C" __global__ void __launch_bounds__(64) pbx_head_back_f32_2(BackArgs a) { back_f32<2>(a); }
 
+struct ReduceArgs {
+  const float *part;
+  int KS, M, K, folds;
+  const int *targets;
+  int vocab;
+  const float *grad;
+  float *dX;
+  const float *hit, *others;  // of pbx_head_g
+  int n_others;
+  // the head
+  int type;
+  const uint8_t *qs;
+  const uint16_t *dsc, *msc;
+};
+
 // dX = grad * (the partial sums together), rows without a target 0: workgroup (16
 // float4s of a row), the partials over 16 threads each.  folds 2: the partial sums have
-// 2 K columns, of the head's high halves and of its low ones.
+// 2 K columns, of the head's high halves and of its low ones.  Rows whose target is likelier
+// than not: and the others' sum times the target's weights.
 extern "C" __global__ void __launch_bounds__(256)
-pbx_head_reduce(const float *part, int KS, int M, int K, int folds, const int *targets, int vocab, const float *grad,
-                float *dX) {
+pbx_head_reduce(ReduceArgs a) {
   __shared__ float4 sum[16][17];
-  const int64_t row = blockIdx.y, MK4 = (int64_t)M * K / 4 * folds;
+  __shared__ float other[4];
+  const int64_t row = blockIdx.y, MK4 = (int64_t)a.M * a.K / 4 * a.folds;
   const int c = threadIdx.x % 16, j = threadIdx.x / 16, k4 = blockIdx.x * 16 + c;
+  const int t = a.targets[row];
+  const float d = a.hit[row], grad = a.grad[row];  // (d: anything in a row without a target)
+  const bool on = t >= 0 && t < a.vocab, likely = on && head_likely(d);
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (k4 < K / 4)
-    for (int i = j; i < KS * folds; i += 16) {
-      const int64_t at = i / folds * MK4 + row * folds * (K / 4) + i % folds * (K / 4) + k4;
-      const float4 p = reinterpret_cast<const float4 *>(part)[at];
+  if (k4 < a.K / 4)
+    for (int i = j; i < a.KS * a.folds; i += 16) {
+      const int64_t at = i / a.folds * MK4 + row * a.folds * (a.K / 4) + i % a.folds * (a.K / 4) + k4;
+      const float4 p = reinterpret_cast<const float4 *>(a.part)[at];
       s.x += p.x, s.y += p.y, s.z += p.z, s.w += p.w;
     }
   sum[j][c] = s;
+  float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (likely) {
+    if (!j && k4 < a.K / 4) {
+      auto value = [&](int e) { return row_value(a.qs, a.dsc, a.msc, a.type, t, 4 * k4 + e, a.K); };
+      w = make_float4(value(0), value(1), value(2), value(3));
+    }
+    float g = 0.f;
+    for (int i = threadIdx.x; i < a.n_others; i += 256) g += a.others[row * a.n_others + i];
+    g = wave_sum(g);
+    if ((threadIdx.x & 63) == 0) other[threadIdx.x >> 6] = g;
+  }
   __syncthreads();
-  if (j || k4 >= K / 4) return;
+  if (j || k4 >= a.K / 4) return;
   for (int i = 1; i < 16; ++i) s.x += sum[i][c].x, s.y += sum[i][c].y, s.z += sum[i][c].z, s.w += sum[i][c].w;
-  const int t = targets[row];
-  const float g = grad[row];
-  float4 *out = reinterpret_cast<float4 *>(dX) + row * (K / 4) + k4;
-  *out = t >= 0 && t < vocab ? make_float4(g * s.x, g * s.y, g * s.z, g * s.w) : make_float4(0.f, 0.f, 0.f, 0.f);
+  if (likely) {
+    const float g = other[0] + other[1] + other[2] + other[3];
+    s.x = fmaf(g, w.x, s.x), s.y = fmaf(g, w.y, s.y), s.z = fmaf(g, w.z, s.z), s.w = fmaf(g, w.w, s.w);
+  }
+  float4 *out = reinterpret_cast<float4 *>(a.dX) + row * (a.K / 4) + k4;
+  *out = on ? make_float4(grad * s.x, grad * s.y, grad * s.z, grad * s.w) : make_float4(0.f, 0.f, 0.f, 0.f);
 }

@@ -1,5 +1,6 @@
-// pbx_head_peaks.h -- the largest scale of a quantised head, which its gradient's products
-// are scaled by (pbx_head.hip, pbx_gemm.hip).
+// pbx_head_peaks.h -- what the head's kernels (pbx_head.hip) and the GEMM's epilogues for it
+// (pbx_gemm.hip) share: the largest scale of a quantised head, which its gradient's
+// products are scaled by, and the target's place in the gradient's first factor.
 #ifndef PBX_HEAD_PEAKS_H
 #define PBX_HEAD_PEAKS_H
 
@@ -33,5 +34,12 @@ __device__ __forceinline__ int head_f_peak(const int *peaks, int n) {
   for (int off = 32; off >= 1; off /= 2) m = max(m, __shfl_xor(m, off, 64));
   return m;
 }
+
+// The target's G from d = l - lse, 1 - e^d.  Where it is likelier than not, lse (rounded to
+// 2^-24 of itself, so to 10^-6 of e^lse) leaves little or nothing of 1 - e^d, while the sum of
+// the other entries' e^(l - lse), which it stands for, is off by no more than they are:
+// there G is 0 here, and pbx_head_reduce adds that sum times the target's weights.
+__device__ __forceinline__ bool head_likely(float d) { return d > -0.6931472f; }
+__device__ __forceinline__ float head_target_g(float d) { return head_likely(d) ? 0.f : -expm1f(d); }
 
 #endif

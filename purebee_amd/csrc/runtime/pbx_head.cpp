@@ -27,6 +27,18 @@ struct SixArgsHost {  // SixArgs in pbx_head.hip
   int64_t stride;
 };
 
+struct ReduceArgsHost {  // ReduceArgs in pbx_head.hip
+  const float *part;
+  int KS, M, K, folds;
+  const int32_t *targets;
+  int vocab;
+  const float *grad;
+  float *dX;
+  const float *hit, *others;
+  int n_others, type;
+  const void *qs, *dsc, *msc;
+};
+
 #define HEAD_SHARE 8192          // of pbx_head.hip, too
 #define HEAD_PIECE (64u << 20)   // bytes of a piece's logits, or factors, at most
 #define HEAD_PAIRS (128u << 20)  // bytes of a piece's weights as pairs at most
@@ -106,9 +118,9 @@ struct Plan {
   bool fused;      // logits leave the GEMM as sums or as the gradient's factor, not as such
   int64_t piece;   // vocabulary entries of a piece, but for the last
   int n_pieces, n_parts;
-  int Mpad, TT, KS;
+  int Mpad, TT, KS, n_others;
   // workspace: byte offsets
-  size_t gemm, z, parts, hit, g, peaks, part, halves, f, f_peaks, bytes;
+  size_t gemm, z, parts, hit, others, g, peaks, part, halves, f, f_peaks, bytes;
 };
 
 size_t padded(size_t n) { return (n + 255) / 256 * 256; }
@@ -152,10 +164,14 @@ Plan make_plan(pbx_ctx *c, const pbx_weight *w, int64_t M, bool grad) {
   p.n_parts = alone ? six_groups(c, w) : p.fused ? (int)((V + 127) / 128) : (p.n_pieces - 1) * shares(p.piece) + shares(last);
   p.gemm = take(gemm);
   p.z = take(p.fused ? 0 : (size_t)M * p.piece * 4);
+  p.hit = take((size_t)M * 4);
   if (!grad) {
     p.parts = take((size_t)M * p.n_parts * 16);
-    p.hit = take((size_t)M * 4);
   } else {
+    // of a piece, which the ones after it add to: by the GEMM's tiles, or pbx_head_g's blocks
+    const int64_t first = std::min(p.piece, V);
+    p.n_others = (int)(p.fused ? (first + 127) / 128 : (first + 31) / 32);
+    p.others = take((size_t)M * p.n_others * 4);
     const int64_t tiles = (K + 127) / 128 * ((M + 32 * p.TT - 1) / (32 * p.TT));
     // about two waves a SIMD (an F32 head's workgroups are one wave, the others' four)
     const int waves = w->type == PBX_TYPE_F32 && !p.pairs ? 1 : 4;
@@ -330,11 +346,13 @@ extern "C" int pbx_linear_logprobs_grad_dev(pbx_ctx *c, const pbx_weight *w, con
   if (!back) return pbx_fail(c, PBX_ELOAD, "%s: kernel %s missing", who, name.c_str());
   char *ws = (char *)work;
   float *z = (float *)(ws + p.z), *part = (float *)(ws + p.part);
+  float *hit = (float *)(ws + p.hit), *others = (float *)(ws + p.others);
   void *peaks = ws + p.peaks;
   pbx_head_scales scales{};
   if (w->d && !p.pairs)
     scales = {w->d, w->Npad * (w->type == PBX_TYPE_Q6_K ? w->K / 256 : w->B) / 8 * (w->m ? 2 : 1), peaks};
   int m = (int)M, k = (int)w->K, vocab = (int)w->N, Mpad = p.Mpad, KS = p.KS, folds = p.pairs ? 2 : 1;
+  int n_others = p.n_others;
   const int columns = k * folds;
   if (p.pairs) {
     rc = pairs_rows(c, w, p, ws, dX, M);
@@ -348,6 +366,7 @@ extern "C" int pbx_linear_logprobs_grad_dev(pbx_ctx *c, const pbx_weight *w, con
     int n = (int)std::min(p.piece, w->N - v0), at = (int)v0;
     if (!p.fused && (rc = piece_logits(c, w, p, ws, dX, M, v0, n, &rows))) return rc;
     const int blocks = (n + 31) / 32;
+    int add = v0 > 0;
     int64_t stride = rows.N;
     void *hi = ws + p.g, *lo = ws + p.g + (size_t)blocks * 32 * Mpad * 2;
     pbx_head_epilogue e;
@@ -359,6 +378,10 @@ extern "C" int pbx_linear_logprobs_grad_dev(pbx_ctx *c, const pbx_weight *w, con
       e.Mpad = Mpad;
       e.v0 = at;
       e.vocab = vocab;
+      e.hit = hit;
+      e.others = others;
+      e.n_others = n_others;
+      e.add = add;
       if (p.pairs) {
         if ((rc = pairs_piece(c, w, p, ws, v0, n, &rows, &e))) return rc;
       } else {
@@ -367,23 +390,26 @@ extern "C" int pbx_linear_logprobs_grad_dev(pbx_ctx *c, const pbx_weight *w, con
       }
       rc = pbx_gemm_head(c, &rows, m, ws + p.gemm, e);
     } else if (f32) {
-      void *args[] = {&z, &stride, &n, &at, (void *)&dLse, (void *)&dTargets, &vocab, &m, &Mpad, &hi};
+      void *args[] = {&z, &stride, &n, &at, (void *)&dLse, (void *)&dTargets, &vocab, &m, &Mpad, &hi,
+                      &hit, &others, &n_others, &add};
       rc = pbx_launch(c, PBX_K_HEAD_G32, dim3(blocks, (Mpad + 63) / 64), dim3(256), args);
     } else {
       int here = blocks;
       void *args[] = {&z, &stride, &n, &at, (void *)&dLse, (void *)&dTargets, &vocab, &m, &Mpad, &hi, &lo,
-                      &here, &scales.scales, &scales.n8, &peaks};
+                      &here, &scales.scales, &scales.n8, &peaks, &hit, &others, &n_others, &add};
       rc = pbx_launch(c, PBX_K_HEAD_G, dim3(blocks + (w->d && !v0 ? PBX_HEAD_PEAKS : 0), (Mpad + 63) / 64), dim3(256), args);
     }
     if (rc) return rc;
     BackArgsHost b{rows.qs, rows.d, rows.m, hi, lo, hi, peaks, e.f_peaks, e.n_f_peaks, part, m, Mpad, columns, (int)rows.B, blocks,
-                   (int)rows.Npad, KS, v0 > 0};
+                   (int)rows.Npad, KS, add};
     void *args[] = {&b};
     if ((rc = pbx_launch_fn(c, back, name.c_str(), dim3((columns + 127) / 128, (m + 32 * p.TT - 1) / (32 * p.TT), KS),
                             dim3(f32 ? 64 : 256), args, c->stream)))
       return rc;
   }
-  void *args[] = {&part, &KS, &m, &k, &folds, (void *)&dTargets, &vocab, (void *)&dGradLogp, &dGradX};
+  ReduceArgsHost r{part, KS, m, k, folds, dTargets, vocab, dGradLogp, dGradX, hit, others, n_others,
+                   pbx_kernel_type(w->type), w->qs, w->d, w->m};
+  void *args[] = {&r};
   return pbx_launch(c, PBX_K_HEAD_REDUCE, dim3((k / 4 + 15) / 16, (unsigned)M), dim3(256), args);
 } catch (const std::bad_alloc &) {
   return pbx_fail(c, PBX_ENOMEM, "pbx_linear_logprobs_grad_dev: out of host memory");

@@ -187,6 +187,17 @@ int pbx_linear_enqueue(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t
                        const pbx_workspace *ws = nullptr);
 // Bytes of workspace that pbx_linear_enqueue asks of ws for M rows of w.
 size_t pbx_linear_space(pbx_ctx *c, const pbx_weight *w, int M);
+// PBX_Q4 / PBX_Q8 / PBX_F32 / PBX_Q41 / PBX_F16 / PBX_Q6K of pbx_gemv_impl.h
+inline int pbx_kernel_type(int t) {
+  switch (t) {
+    case PBX_TYPE_Q4_0: return 0;
+    case PBX_TYPE_Q8_0: return 1;
+    case PBX_TYPE_Q4_1: return 3;
+    case PBX_TYPE_F16: return 4;
+    case PBX_TYPE_Q6_K: return 5;
+    default: return 2;
+  }
+}
 // Whether w is a live weight handle.
 bool pbx_weight_ok(const pbx_weight *w);
 // Bytes of the static device workspace (pbx_scratch.hip) and the lookup of
@@ -230,6 +241,8 @@ struct pbx_head_epilogue {  // HeadArgs in pbx_gemm.hip
   int Mpad = 0, v0 = 0, vocab = 0;
   const int32_t *f = nullptr, *f_peaks = nullptr;
   int n_f_peaks = 0;
+  float *others = nullptr;
+  int n_others = 0, add = 0;
 };
 bool pbx_gemm_has_head(const pbx_ctx *c, const pbx_weight *w, int64_t M);
 size_t pbx_gemm_head_space(const pbx_weight *w, int M);

@@ -171,18 +171,6 @@ const char *type_tag(int t) {
   }
 }
 
-// PBX_Q4 / PBX_Q8 / PBX_F32 / PBX_Q41 / PBX_F16 / PBX_Q6K of pbx_gemv_impl.h
-int kernel_type(int t) {
-  switch (t) {
-    case PBX_TYPE_Q4_0: return 0;
-    case PBX_TYPE_Q8_0: return 1;
-    case PBX_TYPE_Q4_1: return 3;
-    case PBX_TYPE_F16: return 4;
-    case PBX_TYPE_Q6_K: return 5;
-    default: return 2;
-  }
-}
-
 }  // namespace
 
 struct pbx_model {
@@ -659,7 +647,7 @@ static int build_ops(pbx_model *m) {
   e.block = dim3(256);
   e.role = "embed";
   e.bytes = (double)pbx_type_row_bytes(m->embd->type, g.dim) + 4.0 * g.dim;
-  e.embed = EmbedArgsHost{m->embd->qs, m->embd->d, m->x, m->state, kernel_type(m->embd->type),
+  e.embed = EmbedArgsHost{m->embd->qs, m->embd->d, m->x, m->state, pbx_kernel_type(m->embd->type),
                           g.dim, g.vocab_size, m->embd->m};
   m->embed_op = e;
   hipFunction_t fattn = pbx_kernel_by_name(c, "pbx_attention_decode");
@@ -1870,7 +1858,7 @@ static int batch_layers(pbx_model *m, const int32_t *tokens, int n, int start, i
     memcpy(toks.t, tokens, (size_t)n * 4);
     const void *qs = m->embd->qs, *dsc = m->embd->d, *msc = m->embd->m;
     float *x = m->bx;
-    int type = kernel_type(m->embd->type), dim = g.dim, vocab = g.vocab_size;
+    int type = pbx_kernel_type(m->embd->type), dim = g.dim, vocab = g.vocab_size;
     void *args[] = {(void *)&qs, (void *)&dsc, (void *)&msc, &toks, &x, &type, &dim, &vocab};
     if ((rc = launch_k(m, "pbx_embed_rows_arg", dim3((g.dim + 255) / 256, n), dim3(256), args)))
       return rc;
@@ -1883,7 +1871,7 @@ static int batch_layers(pbx_model *m, const int32_t *tokens, int n, int start, i
     const void *qs = m->embd->qs, *dsc = m->embd->d, *msc = m->embd->m;
     int *tok = m->d_tok;
     float *x = m->bx;
-    int type = kernel_type(m->embd->type), dim = g.dim, vocab = g.vocab_size;
+    int type = pbx_kernel_type(m->embd->type), dim = g.dim, vocab = g.vocab_size;
     void *args[] = {(void *)&qs, (void *)&dsc, (void *)&msc, &tok, &x, &type, &dim, &vocab};
     if ((rc = launch_k(m, "pbx_embed_rows", dim3((g.dim + 255) / 256, n), dim3(256), args))) return rc;
     if (hipEventRecord(m->tok_ev, c->stream) != hipSuccess)

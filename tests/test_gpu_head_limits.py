@@ -3,7 +3,7 @@ probabilities come to their formats' ends, on the GPU against tests/head_ref.py.
 import numpy as np
 import pytest
 
-from tests.head_ref import Head, forward, gradient
+from tests.head_ref import U, TYPES, Head, forward, gradient
 from tests.kv_ref import within
 from tests.test_gpu_head import Call, check, rows_of, targets_of
 
@@ -66,4 +66,54 @@ def test_columns_far_larger_than_the_rest(ctx, M, V, K):
         within(got[n], want[n], tol[n])
     within(dx, *gradient(head.values, clean, target, np.ones(M)))
     c.free()
+    head.free()
+
+
+def likely_gradient(W, x, target):
+    """(rows' gradient where targets are likelier than not, a bound for each value, one for each row's norm).
+
+    1 - p of the target is the sum of the others' p, so its error is theirs, p_v each_v, and the sum's (96 roundings of
+    it), however small it is.  The rest as in tests/head_ref.py: pairs of halves, 2^-40 of 1 at least, whose roundings
+    of different entries are independent (the norm: four deviations of their sum, 2^-40 / sqrt 3 each at most)."""
+    x = np.asarray(x, np.float64)
+    _, _, more = forward(W, x, target)
+    z, off, lse = more["z"], more["off"], more["lse"]
+    d = z - lse[:, None]
+    each = off + (more["tol_lse"] + 4 * U * np.abs(lse))[:, None] + (np.abs(d) + 8) * 2 * U
+    p = np.exp(d)
+    p[np.arange(len(x)), target] = 0
+    rest, aw = p.sum(1, keepdims=True), np.abs(W)
+    want = rest * W[target] - p @ W
+    off = (p * each).sum(1, keepdims=True) + 96 * U * rest
+    tol = off * aw[target] + (p * (each + 3 * 2.0 ** -22 + (len(W) / 16 + 128) * U)) @ aw \
+        + rest * 2.0 ** -26 * aw.max() + 4 * U * np.abs(want)
+    length = np.linalg.norm(tol, axis=1) + 4 * 2.0 ** -40 / 3 ** 0.5 * np.linalg.norm(W)
+    return want, tol + 2.0 ** -40 * aw.sum(0), length
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("M,V,K", [(48, 3000, 512), (2, 3000, 512), (4, 9000, 512), (48, 13000, 1024)])
+def test_all_but_certain_targets(ctx, kind, M, V, K):
+    """A row's gradient keeps its bits where the target's 1 - p comes to 10^-7: neither the target's term nor the
+    others' is lost.  (The logits' own errors, up to 10^-3 in these bounds, are what is left.)"""
+    rng = np.random.default_rng(M)
+    head = Head(ctx, kind, 0.05 * rng.standard_normal((V, K)))
+    target = rng.integers(0, V, M)
+    W = head.values[target]
+    lean = np.linspace(8, 27, M) if M > 4 else np.linspace(19, 23, M)
+    x = (rows_of(M, K, size=1.0) + lean[:, None] * W / (W ** 2).sum(1, keepdims=True)).astype(np.float32)
+    c = Call(head, x, target)
+    c.forward()
+    c.backward()
+    got, dx = c.answers(), c.gradient().astype(np.float64)
+    c.free()
+    want, tol, length = likely_gradient(head.values, x, target)
+    exact = forward(head.values, x, target)[0]["logp"]
+    likely = exact > np.log(0.5)
+    within(dx[likely], want[likely], tol[likely])
+    rows = (exact > -1e-4) & (exact < -1e-7)
+    assert rows.sum() >= min(M, 4) / 2
+    size = np.linalg.norm(want, axis=1)
+    assert (length < 0.02 * size)[rows].all()  # (so a row without its target's term, or of zeros, fails)
+    assert (np.linalg.norm(dx - want, axis=1) <= length)[rows].all()
     head.free()
