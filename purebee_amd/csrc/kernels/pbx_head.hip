@@ -986,6 +986,7 @@ struct ReduceArgs {
 extern "C" __global__ void __launch_bounds__(256)
 pbx_head_reduce(ReduceArgs a) {
   __shared__ float4 sum[16][17];
+  __shared__ __attribute__((aligned(16))) float weight[64];
   __shared__ float other[4];
   const int64_t row = blockIdx.y, MK4 = (int64_t)a.M * a.K / 4 * a.folds;
   const int c = threadIdx.x % 16, j = threadIdx.x / 16, k4 = blockIdx.x * 16 + c;
@@ -1000,12 +1001,9 @@ pbx_head_reduce(ReduceArgs a) {
       s.x += p.x, s.y += p.y, s.z += p.z, s.w += p.w;
     }
   sum[j][c] = s;
-  float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
   if (likely) {
-    if (!j && k4 < a.K / 4) {
-      auto value = [&](int e) { return row_value(a.qs, a.dsc, a.msc, a.type, t, 4 * k4 + e, a.K); };
-      w = make_float4(value(0), value(1), value(2), value(3));
-    }
+    const int col = blockIdx.x * 64 + threadIdx.x;
+    if (threadIdx.x < 64 && col < a.K) weight[threadIdx.x] = row_value(a.qs, a.dsc, a.msc, a.type, t, col, a.K);
     float g = 0.f;
     for (int i = threadIdx.x; i < a.n_others; i += 256) g += a.others[row * a.n_others + i];
     g = wave_sum(g);
@@ -1016,6 +1014,7 @@ pbx_head_reduce(ReduceArgs a) {
   for (int i = 1; i < 16; ++i) s.x += sum[i][c].x, s.y += sum[i][c].y, s.z += sum[i][c].z, s.w += sum[i][c].w;
   if (likely) {
     const float g = other[0] + other[1] + other[2] + other[3];
+    const float4 w = *reinterpret_cast<const float4 *>(weight + 4 * c);
     s.x = fmaf(g, w.x, s.x), s.y = fmaf(g, w.y, s.y), s.z = fmaf(g, w.z, s.z), s.w = fmaf(g, w.w, s.w);
   }
   float4 *out = reinterpret_cast<float4 *>(a.dX) + row * (a.K / 4) + k4;
