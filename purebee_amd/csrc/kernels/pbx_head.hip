@@ -175,8 +175,10 @@ struct SixArgs {
 // Up to 2,048 columns (one pass of the lanes) the lane keeps its activations as integers
 // of up to 8,355,711 in three signed bytes (0.5 / 2^22 of the largest of its 32 is what they
 // may be off), so that v_dot4 sums four products with codes exactly; 32 times the bytes'
-// sums, for codes less 32, is taken off as an integer.  Longer rows: f32.
-// 128,256 x 2,048: 56 us with f32 products, 207 vector instructions a row (43 us of them).
+// sums, for codes less 32, is taken off as an integer (128,256 x 2,048: 49 us, 4.4 TB/s; 56 us with
+// f32 products, 207 vector instructions a row, 43 us of them).  Longer rows: f32, 128,256 x 4,096
+// 122 us with the join, where the head's bytes take 84 at a copy's rate; integers would be made anew
+// for each pass of the lanes.
 template <int M, int LANES, bool WHOLE>
 __device__ __forceinline__ void six_body(const SixArgs &a) {
   constexpr int SLOTS = 64 / LANES;
@@ -547,9 +549,8 @@ template <int TYPE> struct HeadTarget { static constexpr int value = TYPE == PBX
 // vocabulary entries, 64 rows); zeros past the vocabulary, the rows, and in rows
 // without a target; and each row's others [M][n_others], by block of a piece (add: to those
 // of the pieces before), and hit, the target's logit less lse.  Workgroups past the blocks
-// (HEAD_PEAKS of them where there are any)
-// look for the head's largest scales.  Few rows, where the GEMM's epilogue does not take
-// the head: a pass over the piece's logits, bound by bytes.
+// (HEAD_PEAKS of them where there are any) look for the head's largest scales.  Few rows, where
+// the GEMM's epilogue does not take the head: a pass over the piece's logits, bound by bytes.
 extern "C" __global__ void __launch_bounds__(256)
 pbx_head_g(const float *Z, int64_t stride, int n, int v0, const float *lse, const int *targets, int vocab, int M,
            int Mpad, _Float16 *hi, _Float16 *lo, int blocks, const uint16_t *scales, int64_t n8, unsigned *peaks,
@@ -982,7 +983,9 @@ struct ReduceArgs {
 // dX = grad * (the partial sums together), rows without a target 0: workgroup (16
 // float4s of a row), the partials over 16 threads each.  folds 2: the partial sums have
 // 2 K columns, of the head's high halves and of its low ones.  Rows whose target is likelier
-// than not: and the others' sum times the target's weights.
+// than not: and the others' sum times the target's weights.  Few rows are a launch's own time and
+// two chains of loads (5 rows of 576 columns, 102 partials, 384 sums of others: 5.2 us, 4.8 with no
+// likely target); 512 rows of 2,048, 4 partials: 15 us.
 extern "C" __global__ void __launch_bounds__(256)
 pbx_head_reduce(ReduceArgs a) {
   __shared__ float4 sum[16][17];
