@@ -252,13 +252,15 @@ int pairs_piece(pbx_ctx *c, const pbx_weight *w, const Plan &p, char *ws, int64_
 
 }  // namespace
 
-extern "C" int pbx_linear_logprobs_workspace(pbx_ctx *c, const pbx_weight *w, int64_t rows, int grad, size_t *bytes) {
+extern "C" int pbx_linear_logprobs_workspace(pbx_ctx *c, const pbx_weight *w, int64_t rows, int grad, size_t *bytes) try {
   const char *who = "pbx_linear_logprobs_workspace";
   if (!c) return pbx_fail(nullptr, PBX_EINVAL, "%s: ctx is NULL", who);
   if (!bytes) return pbx_fail(c, PBX_EINVAL, "%s: NULL argument", who);
   const int rc = check(c, who, w, rows);
   if (!rc) *bytes = rows ? make_plan(c, w, rows, grad != 0).bytes : 0;
   return rc;
+} catch (const std::bad_alloc &) {
+  return pbx_fail(c, PBX_ENOMEM, "pbx_linear_logprobs_workspace: out of host memory");
 }
 
 extern "C" int pbx_linear_logprobs_dev(pbx_ctx *c, const pbx_weight *w, const float *dX, int64_t M,
