@@ -303,7 +303,7 @@ extern "C" int pbx_kv_length(const pbx_kv *kv, int seq, int *n) {
   return PBX_OK;
 }
 
-extern "C" int pbx_kv_truncate(pbx_kv *kv, int seq, int n) {
+extern "C" int pbx_kv_truncate(pbx_kv *kv, int seq, int n) try {
   if (!kv_ok(kv)) return pbx_fail(nullptr, PBX_EINVAL, "pbx_kv_truncate: not a live cache");
   std::string why;
   const int rc = kv->pages.truncate(seq, n, &why);
@@ -311,6 +311,8 @@ extern "C" int pbx_kv_truncate(pbx_kv *kv, int seq, int n) {
   for (pbx_kv_batch *b : kv->batches)
     if (kv_plan_reaches(b->plan, seq, n)) b->stale = true;
   return PBX_OK;
+} catch (const std::bad_alloc &) {
+  return pbx_fail(kv->c, PBX_ENOMEM, "pbx_kv_truncate: out of host memory");
 }
 
 extern "C" int pbx_kv_fork(pbx_kv *kv, int n, const int32_t *dsts, const int32_t *srcs, const int32_t *lens) {

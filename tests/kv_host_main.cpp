@@ -7,6 +7,8 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <functional>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -21,6 +23,19 @@
 static char said[512];
 static int packs = 0, refuse_pack = -1;  // launches of compactions so far, and the one that fails
 static bool capturing = false;
+
+static int left = -1;  // allocations that succeed, -1: all
+void *operator new(size_t n) {
+  if (left >= 0 && left-- == 0) {
+    left = 0;
+    throw std::bad_alloc();
+  }
+  void *p = malloc(n ? n : 1);
+  if (!p) throw std::bad_alloc();
+  return p;
+}
+void operator delete(void *p) noexcept { free(p); }
+void operator delete(void *p, size_t) noexcept { free(p); }
 
 extern "C" {
 hipError_t hipMalloc(void **p, size_t n) { return (*p = calloc(1, n ? n : 1)) ? hipSuccess : hipErrorOutOfMemory; }
@@ -161,10 +176,47 @@ static void refused_sets() {
   CHECK(pbx_kv_batch_set(b, 1, &one, nullptr, &more) == PBX_OK && k.length(1) == 52 && k.free_pages() == 5);
 }
 
+// Every call with one allocation more each time, until it succeeds: until then it changes nothing.
+static void memory_runs_out() {
+  int refused = 0;
+  Cache k(60);
+  pbx_kv_batch *grown = k.batch(3, 0, 1), *kept = k.batch(0, 0, 700);
+  auto until_done = [&](int expected, const std::function<int()> &call) {
+    for (int n = 0;; ++n) {
+      int had[4];
+      for (int s = 0; s < 4; ++s) had[s] = k.length(s);
+      const int pages = k.free_pages();
+      left = n;
+      const int rc = call();
+      left = -1;
+      if (rc == expected) break;
+      CHECK(rc == PBX_ENOMEM && n < 200);
+      ++refused;
+      for (int s = 0; s < 4; ++s) CHECK(k.length(s) == had[s]);
+      CHECK(k.free_pages() == pages && read(kept) == PBX_OK);
+    }
+  };
+  const int32_t all[] = {1, 2, 3}, from[] = {0, 0, 0}, lens[] = {700, 50, 333}, rows[] = {40, 1, 90};
+  until_done(PBX_OK, [&] { return pbx_kv_fork(k.kv, 3, all, from, lens); });
+  CHECK(k.length(2) == 50 && k.free_pages() == 60 - 22);
+  until_done(PBX_OK, [&] { return pbx_kv_batch_set(grown, 3, all, nullptr, rows); });
+  CHECK(k.length(3) == 423 && read(grown) == PBX_OK);
+  std::vector<int32_t> at = without(740, 100, 17);
+  for (int32_t p : without(423, 0, 50)) at.push_back(p);
+  const int32_t two[] = {1, 3}, counts[] = {723, 373};
+  until_done(PBX_OK, [&] { return pbx_kv_compact(k.kv, 2, two, counts, at.data()); });
+  CHECK(k.length(1) == 723 && k.length(3) == 373 && read(grown) == PBX_EINVAL);
+  until_done(PBX_EINVAL, [&] { return pbx_kv_truncate(k.kv, 1, 1000); });
+  until_done(PBX_EINVAL, [&] { return pbx_kv_truncate(k.kv, 7, 0); });
+  for (int s = 0; s < 4; ++s) CHECK(pbx_kv_truncate(k.kv, s, 0) == PBX_OK);
+  CHECK(k.free_pages() == 60 && refused > 30);
+}
+
 int main(int argc, char **argv) {
   const std::string what = argc > 1 ? argv[1] : "";
   if (what == "failed_compactions") failed_compactions();
   else if (what == "refused_sets") refused_sets();
+  else if (what == "memory_runs_out") memory_runs_out();
   else return 2;
   return 0;
 }

@@ -39,3 +39,8 @@ def test_a_compaction_that_fails_midway(host):
 def test_a_refused_set_changes_nothing(host):
     """Neither the sequences nor the batch, which goes on with the rows that it had."""
     host("refused_sets")
+
+
+def test_memory_that_runs_out_is_an_error(host):
+    """PBX_ENOMEM, nothing changed, and no exception past the C entry points."""
+    host("memory_runs_out")
