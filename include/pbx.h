@@ -569,10 +569,10 @@ int pbx_logprobs_dev(pbx_ctx *ctx, const float *dLogits, int64_t stride, int64_t
  *   dEntropy[r]  -sum p log p, in nats; or NULL
  *   dLse[r]      log of the sum of all e^logit, which the gradient needs; or NULL
  * A row without a distribution (see above) answers with NaN; weights are finite.
- * Activations enter the logits as in pbx_linear: with 22 bits each (2^-39 of their row's
- * largest at least) or with 22 bits of the largest of 32 columns, and so do the
- * weights of an F32 head (2^-22 of each, 2^-39 of its row's largest); sums are held in
- * f32.  Only enqueues on the context's stream.  work: device memory of the size that
+ * Activations enter the logits with 22 bits each (2^-39 of their row's largest at least)
+ * or with 22 bits of the largest of 32 columns, as in pbx_linear, or as they are; the
+ * weights of an F32 head with 22 bits each (2^-39 of their row's largest at least); sums
+ * are held in f32.  Only enqueues on the context's stream.  work: device memory of the size that
  * pbx_linear_logprobs_workspace gives (grad 1: for the gradient), 256-byte aligned, any
  * content, for this call alone until it has run (graphs that may run side by side need
  * one each).  No reference counterpart. */
